@@ -1116,6 +1116,43 @@ int zl_bezasun_stats(zl_bezasun_t* m, double* weight_bytes, int* kernels_per_ste
 int zl_bezasun_read_cache(zl_bezasun_t* m, int layer, int slot, int n_rows, float* a_host, float* b_host);
 /* One slot's state of a state-space layer, (heads, vdim, state) fp32 (tests). */
 int zl_bezasun_read_state(zl_bezasun_t* m, int layer, int slot, float* out_host);
+/* ------------------------------------------------------------------------------------------ *
+ * A step of new tokens (one, a few drafted ones, a portion of a prompt) over a paged key / value cache.
+ *
+ * The cache is a pool of num_pages pages of page_size rows, K and V alike: element (page, row, head, i) at page * page_stride + row * row_stride +
+ * head * head_stride + i (strides in elements, multiples of 8; both bases on 16 bytes).  page_table (seqs, >= max_pages) int32, row pitch ld_table:
+ * row r of sequence b lies in page page_table[b][r / page_size].  A page number outside the pool is not followed: it reads as rows of zeros and
+ * takes no writes.  Entries behind a sequence's rows are not looked at.
+ * ------------------------------------------------------------------------------------------ */
+/* Fused query / key / value rows (T, ldq >= (heads + 2 kv_heads) * dim) turned by positions on several axes and appended: frequency i of `half` turns
+ * pair i of every query and key head (columns (i, i + half) or (2i, 2i + 1) by `layout`; columns from 2 * half on stay) by pos[axis[i] * ld_pos + t] *
+ * inv_freq[i], cos and sin times mscale; an axis[i] outside [0, axes) does not turn.  q_out (T, heads * dim); keys and values go to row placement[t]
+ * of sequence token_seq[t], unless that row (negative: none) or sequence does not exist.  Rows of one call have different places: of two with the same
+ * place, pieces of either may stay.  The angle is taken in 64 bits. */
+int zl_qkv_axes_rope_append(const void* qkv, long long ldq, const int32_t* pos, long long ld_pos, int axes, const double* inv_freq,
+                            const int32_t* axis, int half, int layout, float mscale, const int32_t* token_seq, const int32_t* placement,
+                            const int32_t* page_table, int ld_table, int max_pages, int seqs, void* k_cache, void* v_cache, long long num_pages,
+                            int page_size, long long page_stride, long long row_stride, long long head_stride, void* q_out, int T, int heads,
+                            int kv_heads, int dim, int dtype, int pdl, zl_stream_t stream);
+/* Attention of the rows q_starts[b] .. q_starts[b + 1] - 1 (q_starts (seqs + 1) ascending) of q (rows, heads * dim) over sequence b: row i of its n rows
+ * stands at place p = seq_lens[b] - n + i and sees the keys j <= p that the sequence has, with window > 0 those with j > p - window only;
+ * out = softmax(scale q k) v, zeros where a row sees nothing.  Rows of q of no sequence: out stays as it is.  seq_lens counts the new tokens, whose
+ * keys and values are appended already.  What masked keys and values hold (infinities, NaN) does not matter.  max_new: a bound of the sequences' new
+ * tokens, which chooses the kernels; results do not depend on it.  scale > 0; dim 64 or 128; dtype fp16 or bf16. */
+size_t zl_paged_attention_workspace_bytes(int rows, int max_new, int seqs, int heads, int kv_heads, int dim);
+int zl_paged_attention(const void* q, const void* k_cache, const void* v_cache, long long num_pages, int page_size, long long page_stride,
+                       long long row_stride, long long head_stride, const int32_t* page_table, int ld_table, int max_pages,
+                       const int32_t* seq_lens, const int32_t* q_starts, int seqs, float scale, int window, void* out, int rows, int max_new,
+                       int heads, int kv_heads, int dim, void* workspace, size_t workspace_bytes, int dtype, int pdl, zl_stream_t stream);
+/* Verification of drafted tokens by given random numbers.  target: probabilities (seqs, drafts + 1, vocab) fp32, row i of sequence b at b * target_seq +
+ * i * target_row; draft likewise (seqs, drafts, vocab), NULL: every draft had probability 1.  Draft i of count[b] (NULL: `drafts`; clamped to
+ * 0 .. drafts) is taken while accept[b][i] * draft(word) < target(word); a word outside the vocabulary is refused.  The next word comes from the row of
+ * the first refused draft with weights max(target - draft, 0) (where nothing is left: target), or behind the last draft from target: the first one
+ * whose running sum passes sample[b] * (sum of the row's weights), at most the last one of positive weight.  Weights that are negative or not finite
+ * count as zero.  accepted (seqs): drafts taken; tokens (seqs, drafts + 1): those, the next word (-1: no weight at all), then -1.  64-bit sums. */
+int zl_verify_drafts(const float* target, long long target_seq, long long target_row, const float* draft, long long draft_seq, long long draft_row,
+                     const int32_t* drafted, const float* accept, const float* sample, const int32_t* count, int32_t* accepted, int32_t* tokens,
+                     int seqs, int drafts, int vocab, int pdl, zl_stream_t stream);
 #ifdef __cplusplus
 }
 #endif

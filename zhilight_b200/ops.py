@@ -1105,3 +1105,137 @@ def silu_gate_group_rmsnorm(o, z, weight, groups, eps, out_dtype):
     y = torch.empty((t, d), dtype=out_dtype, device=o.device)
     _lib.call("zl_silu_gate_group_rmsnorm", _p(o), d, _p(z), z.shape[1], _p(weight), _p(y), d, t, d, groups, eps, _dt(y), 0, _stream())
     return y
+
+
+# ------------------------------------------------------------------ a step of new tokens over a paged cache: rotation on several axes
+# with the append, attention, verification of drafts
+def rope_axis_map(sections, interleaved=False):
+    """numpy int32 (sum(sections)): the axis that turns each frequency.  sections: frequencies of every axis; one piece after the other, or
+    interleaved: the axes in turn as long as each has frequencies left, the first axis takes the rest."""
+    import numpy as np
+    out = np.repeat(np.arange(len(sections)), sections).astype(np.int32)
+    if interleaved:
+        out[:] = 0
+        for a in range(1, len(sections)):
+            at = np.arange(sections[a]) * len(sections) + a
+            if at.size and at[-1] >= out.size:
+                raise _lib.ZLError(-1, "axis %d has too many frequencies to take turns" % a)
+            out[at] = a
+    return out
+
+
+def _need(ok, what, code=-1):
+    if not ok:
+        raise _lib.ZLError(code, what)
+
+
+def _here(*tensors):
+    """All on the current device."""
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for t in tensors:
+        if t is not None:
+            _need(t.is_cuda, "zhilight_b200 ops need CUDA tensors (no CPU fallback)")
+            _need(t.device.index == dev, "tensors must be on the current device")
+
+
+def _paged_cache(k_cache, v_cache, page_table, dtype):
+    """(pages, page_size, kv_heads, dim) caches, views into larger pools or with the heads outside the rows too: -> strides of their pages, rows, heads."""
+    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "k_cache and v_cache must be (pages, page_size, kv_heads, dim)")
+    _need(k_cache.dtype == dtype and v_cache.dtype == dtype and dtype in (torch.float16, torch.bfloat16), "caches must be fp16 or bf16, like the rows", -2)
+    steps, more = ([0 if n == 1 else s for n, s in zip(c.shape, c.stride())] for c in (k_cache, v_cache))   # of one page, row or head none is taken
+    _need(steps == more and k_cache.stride(3) == 1, "k_cache and v_cache must have the same strides, heads in one piece")
+    _need(all(s > 0 or n == 1 for n, s in zip(k_cache.shape, steps)), "pages, rows and heads of a cache must not share memory")
+    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.stride(1) == 1 and page_table.numel() > 0,
+          "page_table must be (sequences, pages) int32, its rows in one piece")
+    _need(k_cache.numel() > 0 and k_cache.shape[3] > 1, "the cache is empty")
+    return steps[:3]
+
+
+def _ints(name, t, shape):
+    _need(t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous(), "%s must be contiguous int32 %s" % (name, tuple(shape)))
+
+
+def qkv_axes_rope_append(qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout=ROT_HALVES, mscale=1.0,
+                         pdl=False):
+    """qkv (T, (heads + 2 kv_heads) * dim), rows of any pitch; pos (axes, T) int32; inv_freq (half) float64 and axis (half) int32 (rope_axis_map):
+    frequency i turns pair i of queries and keys by pos[axis[i]] * inv_freq[i], cos and sin times mscale.  Keys and values go to row placement (T) int32
+    (negative: nowhere) of sequence token_seq (T) int32 in the caches (pages, page_size, kv_heads, dim) behind page_table (sequences, pages) int32;
+    the places of a call's rows differ.  -> q (T, heads * dim)."""
+    steps = _paged_cache(k_cache, v_cache, page_table, qkv.dtype)
+    pages, page_size, kv_heads, dim = k_cache.shape
+    _need(qkv.dim() == 2 and heads > 0 and qkv.shape[1] == (heads + 2 * kv_heads) * dim and qkv.stride(1) == 1,
+          "qkv must be (T, (heads + 2 kv_heads) * dim), its rows in one piece")
+    t, half = qkv.shape[0], inv_freq.numel()
+    _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and 2 * half <= dim,
+          "inv_freq must be contiguous float64, two columns of a head for each")
+    _ints("axis", axis, (half,))
+    _need(pos.dim() == 2 and pos.shape[0] > 0, "pos must be (axes, T)")
+    _ints("pos", pos, (pos.shape[0], t))
+    _ints("token_seq", token_seq, (t,))
+    _ints("placement", placement, (t,))
+    _here(qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache)
+    q = torch.empty((t, heads * dim), dtype=qkv.dtype, device=qkv.device)
+    if t == 0:
+        return q
+    _lib.call("zl_qkv_axes_rope_append", qkv.data_ptr(), qkv.stride(0) if t > 1 else qkv.shape[1], pos.data_ptr(), t, pos.shape[0],
+              ctypes.cast(inv_freq.data_ptr(), ctypes.POINTER(ctypes.c_double)), axis.data_ptr(), half, layout, float(mscale), token_seq.data_ptr(),
+              placement.data_ptr(), page_table.data_ptr(), page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1], page_table.shape[1],
+              page_table.shape[0], k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, *steps, q.data_ptr(), t, heads, kv_heads, dim,
+              _dt(qkv), int(pdl), _stream())
+    return q
+
+
+def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window=0, max_new=None, out=None, pdl=False):
+    """Attention of the new tokens of every sequence over its pages: rows q_starts[b] to q_starts[b + 1] of q (T, heads * dim) or (T, heads, dim) are
+    the last tokens of sequence b, whose seq_lens[b] keys and values (the new ones among them) are in the caches (pages, page_size, kv_heads, dim)
+    behind page_table (sequences, pages) int32.  Each sees the keys up to its own, with a window only the last `window` of them; a row that sees none
+    gives zeros.  seq_lens (sequences) and q_starts (sequences + 1), ascending, int32.  max_new: a bound of the new tokens of one sequence (None: all
+    rows), which chooses kernels and nothing else.  Rows of no sequence: out, if given, keeps what it holds there.  -> out, like q."""
+    steps = _paged_cache(k_cache, v_cache, page_table, q.dtype)
+    pages, page_size, kv_heads, dim = k_cache.shape
+    _need(q.dim() in (2, 3) and q.is_contiguous() and (q.dim() == 2 or q.shape[2] == dim), "q must be contiguous (T, heads * dim) or (T, heads, dim)")
+    t, width, seqs = q.shape[0], q.shape[1] * (dim if q.dim() == 3 else 1), page_table.shape[0]
+    _need(width > 0 and width % (kv_heads * dim) == 0, "the heads of q must be a multiple of the cache's")
+    _ints("seq_lens", seq_lens, (seqs,))
+    _ints("q_starts", q_starts, (seqs + 1,))
+    _need(out is None or (out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()), "out must be contiguous, of q's shape and type")
+    _need(max_new is None or max_new > 0, "max_new must be positive")
+    _here(q, k_cache, v_cache, page_table, seq_lens, q_starts, out)
+    if out is None:
+        out = torch.empty_like(q)
+    if t == 0:
+        return out
+    heads, most = width // dim, t if max_new is None else min(max_new, t)
+    nbytes = _lib.load().zl_paged_attention_workspace_bytes(t, most, seqs, heads, kv_heads, dim)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.call("zl_paged_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, *steps, page_table.data_ptr(),
+              page_table.stride(0) if seqs > 1 else page_table.shape[1], page_table.shape[1], seq_lens.data_ptr(), q_starts.data_ptr(), seqs, float(scale),
+              int(window), out.data_ptr(), t, most, heads, kv_heads, dim, _dp(ws), nbytes, _dt(q), int(pdl), _stream())
+    return out
+
+
+def verify_drafts(target, draft, drafted, accept, sample, count=None, pdl=False):
+    """Drafted tokens against the target's probabilities, by given random numbers in [0, 1).  target (B, K + 1, vocab) and draft (B, K, vocab) fp32
+    probabilities, rows of any pitch; draft None: every draft was certain (looked up, or the likeliest).  drafted (B, K) int32; accept (B, K) and
+    sample (B) fp32; count (B) int32: drafts of each sequence (None: K).  Draft i is taken while accept * draft(word) < target(word); the word behind
+    the last one taken is drawn by `sample` from max(target - draft, 0) of the refused draft's row, from target behind the last draft.
+    -> (accepted (B) int32, tokens (B, K + 1) int32: the drafts taken, the word drawn, then -1)."""
+    _need(target.dim() == 3 and target.dtype == torch.float32 and target.shape[1] > 0 and target.shape[2] > 0 and target.stride(2) == 1,
+          "target must be (B, K + 1, vocab) fp32, its rows in one piece")
+    b, k, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+    _need(draft is None or (tuple(draft.shape) == (b, k, vocab) and draft.dtype == torch.float32 and draft.stride(2) == 1),
+          "draft must be (B, K, vocab) fp32, its rows in one piece")
+    _ints("drafted", drafted, (b, k))
+    for name, t, shape in (("accept", accept, (b, k)), ("sample", sample, (b,))):
+        _need(t.dtype == torch.float32 and tuple(t.shape) == shape and t.is_contiguous(), "%s must be contiguous fp32 %s" % (name, shape))
+    if count is not None:
+        _ints("count", count, (b,))
+    _here(target, draft, drafted, accept, sample, count)
+    accepted = torch.empty((b,), dtype=torch.int32, device=target.device)
+    tokens = torch.empty((b, k + 1), dtype=torch.int32, device=target.device)
+    if b == 0:
+        return accepted, tokens
+    _lib.call("zl_verify_drafts", target.data_ptr(), target.stride(0), target.stride(1), _dp(draft), draft.stride(0) if draft is not None else 0,
+              draft.stride(1) if draft is not None else 0, drafted.data_ptr(), accept.data_ptr(), sample.data_ptr(), _dp(count), accepted.data_ptr(),
+              tokens.data_ptr(), b, k, vocab, int(pdl), _stream())
+    return accepted, tokens
