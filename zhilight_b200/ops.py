@@ -1206,7 +1206,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
     if t == 0:
         return out
     heads, most = width // dim, t if max_new is None else min(max_new, t)
-    nbytes = _lib.load().zl_paged_attention_workspace_bytes(t, most, seqs, heads, kv_heads, dim)
+    nbytes = _lib.load().zl_paged_attention_workspace_bytes(t, most, seqs, min(page_table.shape[1] * page_size, 2 ** 31 - 256), heads, kv_heads, dim)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _lib.call("zl_paged_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, *steps, page_table.data_ptr(),
               page_table.stride(0) if seqs > 1 else page_table.shape[1], page_table.shape[1], seq_lens.data_ptr(), q_starts.data_ptr(), seqs, float(scale),
