@@ -1,0 +1,371 @@
+// Attention of few (token, head) rows of a kv head -- single tokens, drafts of small groups -- over pages: bound by the bytes of K and V, which the CTAs
+// of the grid share out evenly, whatever the sequences' lengths are.  All tiles of 64 keys of all blocks (16 or 32 rows of one kv head of one sequence)
+// stand in one line; a CTA takes an equal stretch of it.  A block that lies in one stretch is written at once, the parts of one that is cut go to the
+// workspace, its first part to the CTA's place 1, others to its place 0, and k_paged_few_join puts them together.
+//
+// A warp has 16 keys of a tile to itself, in a ring of its own (16-byte cp.async; no barrier between the warps until a block's end):
+// S = Q K^T and O += P V by mma.sync with Q as the 16-row operand, whose accumulators are the next product's operand as they stand.  The probabilities are
+// rounded to the type of the rows, their sum is not; the reference maximum of a row follows lazily as in paged_attn_tc.cuh.
+#pragma once
+#include "paged_attn.cuh"
+
+#include <type_traits>
+
+namespace zl {
+
+constexpr int kPfWarps = 4, kPfKeys = 16 * kPfWarps, kPfStages = 3, kPfPerSm = 2;
+
+template <int D>
+struct PfCfg {
+    static constexpr int kStage = 16 * D * 2 * 2;                    // 16 rows of K, then of V
+    static constexpr int kWarp = kPfStages * kStage;
+    static constexpr int kBytes = kPfWarps * kWarp;
+    static constexpr int kPitch = D + 8;                             // floats; of a row of a warp's output in its ring
+};
+
+// Tiles of a block, at least one: a block that sees nothing is written too
+__device__ __forceinline__ int paged_few_tiles(const PagedBlock& k) { return k.hi >= 0 ? k.hi / kPfKeys - k.lo / kPfKeys + 1 : 1; }
+
+struct PfPlace {
+    int hk, off, tiles, index;   // kv head; tile within the block and how many it has; number of the block among all (token, head) blocks of a kv head
+    long long start;             // the block's place in the line
+};
+
+// Lane's share: tiles of a kv head of sequence b
+__device__ __forceinline__ int paged_few_sum(const PagedAttn& p, const PagedCache& c, int b, int size, int& blocks) {
+    PagedBlock k;
+    k.seq = b;
+    blocks = 0;
+    if (b >= c.seqs) return 0;
+    const int n = paged_new(p, b, k.first) * p.group;
+    if (n > p.few) return 0;
+    int sum = 0;
+    for (k.row0 = 0; k.row0 < n; k.row0 += size, ++blocks) {
+        k.rows = min(size, n - k.row0);
+        paged_bounds(p, c, k);
+        sum += paged_few_tiles(k);
+    }
+    return sum;
+}
+
+__device__ __forceinline__ int paged_scan(int v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+
+// Length of the line, by a warp
+__device__ __forceinline__ long long paged_few_total(const PagedAttn& p, const PagedCache& c, int kv_heads, int size) {
+    long long sum = 0;
+    int blocks;
+    for (int b0 = 0; b0 < c.seqs; b0 += 32) sum += __shfl_sync(0xffffffffu, paged_scan(paged_few_sum(p, c, b0 + (threadIdx.x & 31), size, blocks)), 31);
+    return sum * kv_heads;
+}
+
+// The block at place w of the line: sequence by sequence, in it kv head by kv head, in that block by block.  By a warp.
+__device__ __forceinline__ void paged_few_at(const PagedAttn& p, const PagedCache& c, int kv_heads, int size, long long w, PagedBlock& k, PfPlace& at) {
+    long long before = 0;
+    int blocks, first_block = 0;
+    for (int b0 = 0; b0 < c.seqs; b0 += 32) {
+        const int mine = paged_few_sum(p, c, b0 + (threadIdx.x & 31), size, blocks), upto = paged_scan(mine), blocks_upto = paged_scan(blocks);
+        const unsigned hit = __ballot_sync(0xffffffffu, before + (long long)upto * kv_heads > w);
+        if (hit) {
+            const int src = __ffs(hit) - 1, each = __shfl_sync(0xffffffffu, mine, src);
+            const long long here = before + (long long)__shfl_sync(0xffffffffu, upto - mine, src) * kv_heads;
+            int rem = (int)(w - here);
+            at.hk = rem / each;
+            rem -= at.hk * each;
+            k.seq = b0 + src;
+            at.index = first_block + __shfl_sync(0xffffffffu, blocks_upto - blocks, src);
+            const int n = paged_new(p, k.seq, k.first) * p.group;
+            for (k.row0 = 0;; k.row0 += size, ++at.index) {
+                k.rows = min(size, n - k.row0);
+                paged_bounds(p, c, k);
+                at.tiles = paged_few_tiles(k);
+                if (rem < at.tiles) break;
+                rem -= at.tiles;
+            }
+            at.off = rem;
+            at.start = w - rem;
+            return;
+        }
+        before += (long long)__shfl_sync(0xffffffffu, upto, 31) * kv_heads;
+        first_block += __shfl_sync(0xffffffffu, blocks_upto, 31);
+    }
+}
+
+__device__ __forceinline__ void pf_ldsm(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pf_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void pf_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value) mma_16816_f16(d, a, b0, b1, d);
+    else mma_16816_bf16(d, a, b0, b1, d);
+}
+__device__ __forceinline__ float pf_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pf_pack(float a, float b) {
+    T two[2] = {from_f32<T>(a), from_f32<T>(b)};
+    return *reinterpret_cast<const uint32_t*>(two);
+}
+
+// Row r of a block, D columns from `o`(e) of this lane, E neighbouring ones each: rounded and stored, or done again where it is no number
+template <typename T, int D>
+__device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedCache& c, const PagedBlock& k, int hk, int r, float l, const float (&o)[D / 32]) {
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31, row = k.row0 + r, t = row / p.group, head = hk * p.group + row - t * p.group, place = k.place0 + t;
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    T v[E];
+    bool broken = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float x = l == 0.f ? 0.f : o[e] * inv;
+        broken |= x != x;
+        v[e] = from_f32<T>(x);
+    }
+    T* dst = static_cast<T*>(p.out) + ((size_t)(k.first + t) * p.heads + head) * D + lane * E;
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
+    else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(v);
+    if (__any_sync(0xffffffffu, broken)) {
+        __syncwarp();
+        paged_row_exact<T, D>(p, c, k.seq, k.first + t, head, p.window ? max(0, place - p.window + 1) : 0, min(place, k.have - 1));
+    }
+}
+
+// grid: CTAs that share the line
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(const PagedAttn p, const PagedCache c, int kv_heads) {
+    using C = PfCfg<D>;
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr int R = 16 * MT, CH = D / 8, KS = D / 16;
+    constexpr float kTau = kHalf ? 5.f : 8.f, kUp = kHalf ? 10.f : 0.f;
+    extern __shared__ __align__(128) uint8_t pf_smem[];
+    __shared__ float2 s_ml[kPfWarps][R];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    uint8_t* ring = pf_smem + warp * C::kWarp;
+    const uint32_t ring_at = smem_u32(ring);
+    pdl_trigger();
+    pdl_wait();
+    const long long total = paged_few_total(p, c, kv_heads, R);
+    long long w = total * blockIdx.x / gridDim.x;
+    const long long end = total * (blockIdx.x + 1) / gridDim.x;
+    while (w < end) {
+        PagedBlock k;
+        PfPlace at;
+        paged_few_at(p, c, kv_heads, R, w, k, at);
+        const int count = (int)min(end - w, (long long)(at.tiles - at.off)), key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + at.off) * kPfKeys + warp * 16;
+        const long long head = (long long)at.hk * c.head_stride;
+        // copies of a stage: lane's chunk of two rows at a time; lanes 0 - 15 know where the 16 rows lie, a stage ahead
+        auto find = [&](int j) {
+            const int row = key0 + j * kPfKeys + (lane & 15);
+            return j < count && row <= k.hi ? c.row_at(k.seq, row) : -1;
+        };
+        auto copy = [&](int j, long long off) {
+            const uint32_t to = ring_at + (uint32_t)(j % kPfStages) * C::kStage;
+            const int ch = lane % CH;
+#pragma unroll
+            for (int i = 0; i < 16 * CH / 32; ++i) {
+                const int r = lane / CH + i * (32 / CH);
+                const long long o = __shfl_sync(0xffffffffu, off, r);
+                const long long from = o < 0 ? 0 : o + head + ch * 8;
+                const int bytes = o < 0 ? 0 : 16;
+                const uint32_t dst = to + (uint32_t)(r * (D * 2) + ((ch ^ (r & 7)) << 4));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(static_cast<const T*>(c.k) + from), "r"(bytes) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 16 * D * 2), "l"(static_cast<const T*>(c.v) + from), "r"(bytes) : "memory");
+            }
+        };
+        long long off = find(0);
+#pragma unroll
+        for (int j = 0; j < kPfStages - 1; ++j) {
+            if (j < count) copy(j, off);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            off = find(j + 1);
+        }
+        // rows of q: (g, g + 8) of each 16
+        uint32_t qa[MT][KS][4];
+        int hi[MT][2], lo[MT][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = m * 16 + g + u * 8;
+                const bool in = r < k.rows;
+                const int row = k.row0 + (in ? r : 0), t = row / p.group, place = k.place0 + t;
+                const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + ((size_t)(k.first + t) * p.heads + at.hk * p.group + row - t * p.group) * D);
+                hi[m][u] = in ? min(place, k.have - 1) : -1;
+                lo[m][u] = p.window ? max(0, place - p.window + 1) : 0;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) qa[m][s][u] = in ? src[s * 8 + t4] : 0u, qa[m][s][2 + u] = in ? src[s * 8 + 4 + t4] : 0u;
+            }
+        float o[MT][D / 8][4], l[MT][2], m_ref[MT][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
+            l[m][0] = l[m][1] = 0.f, m_ref[m][0] = m_ref[m][1] = -1.4426950e20f;
+        }
+        for (int j = 0; j < count; ++j) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kPfStages - 2) : "memory");
+            __syncwarp();
+            if (j + kPfStages - 1 < count) copy(j + kPfStages - 1, off);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            off = find(j + kPfStages);
+            const int kb = key0 + j * kPfKeys;
+            if (kb > k.hi || kb + 15 < k.lo) continue;
+            const uint32_t st = ring_at + (uint32_t)(j % kPfStages) * C::kStage;
+            float s[MT][2][4] = {};
+            {
+                // matrices of 8 keys x 8 columns: (keys 0-7, first 8), (0-7, next 8), (8-15, first 8), (8-15, next 8)
+                const int r = (lane & 7) + ((lane >> 4) << 3), ch0 = (lane >> 3) & 1;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    uint32_t b[4];
+                    pf_ldsm(b, st + (uint32_t)(r * (D * 2) + (((2 * i + ch0) ^ (r & 7)) << 4)));
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) pf_mma<T>(s[m][0], qa[m][i], b[0], b[1]), pf_mma<T>(s[m][1], qa[m][i], b[2], b[3]);
+                }
+            }
+            uint32_t pa[MT][4];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = kb + n * 8 + t4 * 2 + (e & 1);
+                        s[m][n][e] = key <= hi[m][e >> 1] && key >= lo[m][e >> 1] ? s[m][n][e] * p.scale : -INFINITY;
+                    }
+                bool up = false;
+                float top[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    top[u] = fmaxf(fmaxf(s[m][0][2 * u], s[m][0][2 * u + 1]), fmaxf(s[m][1][2 * u], s[m][1][2 * u + 1]));
+                    up |= top[u] > m_ref[m][u] + kTau;
+                }
+                if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
+                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
+                        const float f = top[u] > m_ref[m][u] ? pf_exp2(m_ref[m][u] - top[u]) : 1.f;
+                        m_ref[m][u] = fmaxf(m_ref[m][u], top[u]);
+                        l[m][u] *= f;
+#pragma unroll
+                        for (int n = 0; n < D / 8; ++n) o[m][n][2 * u] *= f, o[m][n][2 * u + 1] *= f;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float x = pf_exp2(s[m][n][2 * u] + (kUp - m_ref[m][u])), y = pf_exp2(s[m][n][2 * u + 1] + (kUp - m_ref[m][u]));
+                        l[m][u] += x + y;
+                        pa[m][2 * n + u] = pf_pack<T>(x, y);
+                    }
+            }
+            {
+                // transposed: (keys 0-7, first 8 columns), (keys 8-15, first 8), (0-7, next 8), (8-15, next 8)
+                const int r = (lane & 7) + (((lane >> 3) & 1) << 3), ch0 = lane >> 4;
+#pragma unroll
+                for (int n = 0; n < D / 8; n += 2) {
+                    uint32_t b[4];
+                    pf_ldsm_t(b, st + (uint32_t)(16 * D * 2 + r * (D * 2) + (((n + ch0) ^ (r & 7)) << 4)));
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) pf_mma<T>(o[m][n], pa[m], b[0], b[1]), pf_mma<T>(o[m][n + 1], pa[m], b[2], b[3]);
+                }
+            }
+        }
+        // the warps' parts, in their rings
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+        float* mine = reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = m * 16 + g + u * 8;
+                float sum = l[m][u];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (t4 == 0) s_ml[warp][r] = make_float2(m_ref[m][u], sum);
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(mine + r * C::kPitch + n * 8 + t4 * 2) = make_float2(o[m][n][2 * u], o[m][n][2 * u + 1]);
+            }
+        __syncthreads();
+        const bool whole = count == at.tiles;
+        const size_t part = ((size_t)blockIdx.x * 2 + (at.off > 0 ? 0 : 1)) * R;
+        for (int r = warp; r < k.rows; r += kPfWarps) {
+            constexpr int E = D / 32;
+            float m = s_ml[0][r].x, sum = 0.f, v[E] = {};
+#pragma unroll
+            for (int x = 1; x < kPfWarps; ++x) m = fmaxf(m, s_ml[x][r].x);
+#pragma unroll
+            for (int x = 0; x < kPfWarps; ++x) {
+                const float f = pf_exp2(s_ml[x][r].x - m);
+                sum = fmaf(s_ml[x][r].y, f, sum);
+                const float* from = reinterpret_cast<const float*>(pf_smem + x * C::kWarp) + r * C::kPitch + lane * E;
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = fmaf(from[e], f, v[e]);
+            }
+            if (whole) {
+                paged_row_out<T, D>(p, c, k, at.hk, r, sum, v);
+            } else {
+                if (lane == 0) p.ml[part + r] = make_float2(m, sum);
+                float* dst = p.part + (part + r) * D + lane * E;
+                if constexpr (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+                else *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
+            }
+        }
+        __syncthreads();   // the rings are the next block's
+        w += count;
+    }
+}
+
+// Blocks that were cut: grid (parts' CTAs).  CTA i looks at the block that begins in stretch i - and is cut - of the line: there is one at the most.
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kPfWarps * 32) k_paged_few_join(const PagedAttn p, const PagedCache c, int kv_heads) {
+    constexpr int R = 16 * MT, E = D / 32;
+    pdl_trigger();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long total = paged_few_total(p, c, kv_heads, R);
+    const long long w0 = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
+    if (w0 >= end || end == total) return;
+    PagedBlock k;
+    PfPlace at;
+    paged_few_at(p, c, kv_heads, R, end - 1, k, at);
+    if (at.start < w0 || at.start + at.tiles <= end) return;   // begins in an earlier stretch; ends in this one
+    // stretches that have a part: this one and those up to the one with the block's last tile
+    const int last = (int)(((at.start + at.tiles) * gridDim.x - 1) / total);
+    for (int r = warp; r < k.rows; r += kPfWarps) {
+        float m = -INFINITY, l = 0.f, v[E] = {};
+        for (int i = blockIdx.x; i <= last; ++i) {
+            if (total * i / gridDim.x == total * (i + 1) / gridDim.x) continue;   // an empty stretch
+            m = fmaxf(m, p.ml[((size_t)i * 2 + (i == (int)blockIdx.x)) * R + r].x);
+        }
+        for (int i = blockIdx.x; i <= last; ++i) {
+            if (total * i / gridDim.x == total * (i + 1) / gridDim.x) continue;
+            const size_t part = ((size_t)i * 2 + (i == (int)blockIdx.x)) * R + r;
+            const float2 x = p.ml[part];
+            const float f = pf_exp2(x.x - m);
+            l = fmaf(x.y, f, l);
+            const float* from = p.part + part * D + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = fmaf(from[e], f, v[e]);
+        }
+        paged_row_out<T, D>(p, c, k, at.hk, r, l, v);
+    }
+}
+
+}  // namespace zl
