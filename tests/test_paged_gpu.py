@@ -416,3 +416,78 @@ def test_same_call_same_bits(cuda):
     for _ in range(5):
         for a, b in zip(first, s.run()):
             assert torch.equal(a, b)
+
+
+# ---- the native host module and the general path ---------------------------------------------------------------------------------
+class Asked:
+    """The native module, with a note of whether it served each call or left it to the general path."""
+
+    def __init__(self, host):
+        self.host, self.served = host, []
+
+    def __getattr__(self, name):
+        def call(*args):
+            y = getattr(self.host, name)(*args)
+            self.served.append(y is not None)
+            return y
+        return call
+
+
+def both_ways(monkeypatch, f, served=True, refused=False):
+    from zhilight_b200 import _lib
+    asked, outs = Asked(_lib.host), []
+    for host in (asked, None):
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "host", host)
+            if refused:
+                with pytest.raises(_lib.ZLError):
+                    f()
+            else:
+                y = f()
+                outs.append([x.clone() for x in (y if isinstance(y, tuple) else (y,))])
+    assert asked.served == [served]
+    for x, y in zip(*outs) if outs else ():
+        assert x.dtype == y.dtype and x.shape == y.shape and torch.equal(x, y)
+
+
+class Own(torch.Tensor):
+    pass
+
+
+def test_both_ways_from_tensors_to_launches(cuda, monkeypatch):
+    s = Step(11)
+    d = dict(s.dev)
+    d["q"] = torch.randn(s.qkv.shape[0], 8 * 128, device="cuda").to(BF16)
+
+    def append(**kw):
+        e = dict(d, **kw)
+        return lambda: ops.qkv_axes_rope_append(e["qkv"], e["pos"], e["freq"], e["axis"], e["seq"], e["place"], e["table"], e["k"], e["v"], e.get("heads", 8),
+                                                layout=e.get("layout", 0), mscale=e.get("mscale", 1), pdl=e.get("pdl", False))
+
+    def attend(**kw):
+        e = dict(d, **kw)
+        return lambda: ops.paged_attention(e["q"], e["k"], e["v"], e["table"], e["lens"], e["starts"], e.get("scale", 0.1), window=e.get("window", 0),
+                                           max_new=e.get("max_new"), out=e.get("out"), pdl=e.get("pdl", False))
+
+    def verify(**kw):
+        e = dict(d, **kw)
+        return lambda: ops.verify_drafts(e["target"], e["draft"], e["words"], e["accept"], e["sample"], e.get("count"), pdl=e.get("pdl", False))
+
+    wide = torch.cat([d["qkv"], d["qkv"]], 1)[:, :12 * 128]
+    for kw in (dict(), dict(mscale=1.5), dict(layout=1, pdl=True), dict(qkv=wide), dict(qkv=torch.nn.Parameter(d["qkv"], requires_grad=False))):
+        both_ways(monkeypatch, append(**kw))
+    both_ways(monkeypatch, append(qkv=d["qkv"].as_subclass(Own)), served=False)
+    for kw in (dict(layout=2), dict(qkv=wide[:, :-1]), dict(axis=d["axis"][1:]), dict(k=d["k"].half()), dict(freq=d["freq"].float()), dict(place=d["place"].long()),
+               dict(pos=d["pos"][:, 1:]), dict(heads=7), dict(qkv=d["qkv"].cpu()), dict(table=d["table"][:, ::2])):
+        both_ways(monkeypatch, append(**kw), served="layout" in kw, refused=True)
+    out = torch.zeros_like(d["q"])
+    for kw in (dict(), dict(q=d["q"].view(-1, 8, 128)), dict(window=7, max_new=130, pdl=True), dict(out=out), dict(scale=1)):
+        both_ways(monkeypatch, attend(**kw))
+    both_ways(monkeypatch, attend(table=d["table"].as_subclass(Own)), served=False)
+    for kw in (dict(scale=-1.0), dict(window=-1), dict(q=d["q"][:, :100]), dict(lens=d["lens"][1:]), dict(max_new=0), dict(out=out.float()),
+               dict(k=d["k"][:, :, :1].expand(d["k"].shape)), dict(starts=d["starts"].long()), dict(v=d["v"].cpu())):
+        both_ways(monkeypatch, attend(**kw), served=kw.get("scale", 0) < 0 or "window" in kw, refused=True)
+    for kw in (dict(), dict(draft=None), dict(count=d["starts"][1:].clone()), dict(target=torch.cat([d["target"]] * 2, 2)[:, :, :9000])):
+        both_ways(monkeypatch, verify(**kw))
+    for kw in (dict(target=d["target"].double()), dict(draft=d["target"]), dict(words=d["words"].long()), dict(count=d["starts"]), dict(sample=d["sample"][1:])):
+        both_ways(monkeypatch, verify(**kw), served=False, refused=True)

@@ -11,10 +11,12 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <vector>
 
 #include "../../../include/zhilight_b200.h"
@@ -30,6 +32,10 @@ struct {
     decltype(&zl_w8a8_gemm) w8;
     decltype(&zl_decode_attention_workspace_bytes) attn_bytes;
     decltype(&zl_decode_attention_host) attn;
+    decltype(&zl_qkv_axes_rope_append) axes_rope;
+    decltype(&zl_paged_attention_workspace_bytes) paged_bytes;
+    decltype(&zl_paged_attention) paged;
+    decltype(&zl_verify_drafts) verify;
 } zl;
 
 struct NotPlain {};   // the general path's
@@ -226,6 +232,150 @@ PyObject* decode_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
     });
 }
 
+// ---- a step of new tokens over a paged cache: what ops.py checks of shapes, types, strides and devices has to hold here, else ops.py refuses it
+void must(bool ok) {
+    if (!ok) throw NotPlain{};
+}
+double to_double(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) {
+        PyErr_Clear();
+        throw NotPlain{};
+    }
+    return v;
+}
+// a tensor on the current device
+const at::Tensor& here(PyObject* o, bool contiguous) {
+    const at::Tensor& t = plain(o, contiguous);
+    must(t.device().index() == c10::cuda::current_device());
+    return t;
+}
+const int32_t* ints(PyObject* o, int64_t n) {   // (n)
+    const at::Tensor& t = here(o, true);
+    must(t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n);
+    return static_cast<const int32_t*>(t.data_ptr());
+}
+struct Paged {
+    void *k, *v;
+    const int32_t* table;
+    long long pages, step[3];
+    int page_size, kv_heads, dim, ld_table, max_pages, seqs;
+};
+Paged paged_cache(PyObject* k_cache, PyObject* v_cache, PyObject* page_table, at::ScalarType type) {
+    const at::Tensor &k = here(k_cache, false), &v = here(v_cache, false), &t = here(page_table, false);
+    must(k.dim() == 4 && v.sizes() == k.sizes() && k.scalar_type() == type && v.scalar_type() == type && (type == at::kHalf || type == at::kBFloat16));
+    must(k.numel() > 0 && k.size(3) > 1 && k.stride(3) == 1 && v.stride(3) == 1 && t.dim() == 2 && t.scalar_type() == at::kInt && t.numel() > 0 && t.stride(1) == 1);
+    Paged p = {k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(t.data_ptr()), k.size(0)};
+    for (int i = 0; i < 3; ++i) {
+        p.step[i] = k.size(i) == 1 ? 0 : k.stride(i);
+        must(p.step[i] == (k.size(i) == 1 ? 0 : v.stride(i)) && (p.step[i] > 0 || k.size(i) == 1));
+    }
+    must(k.size(1) < 1 << 30 && t.size(0) < 1 << 30 && t.size(1) < 1 << 30 && t.stride(0) < 1ll << 31 && k.size(2) < 1 << 16 && k.size(3) < 1 << 16);
+    p.page_size = (int)k.size(1), p.kv_heads = (int)k.size(2), p.dim = (int)k.size(3);
+    p.seqs = (int)t.size(0), p.max_pages = (int)t.size(1), p.ld_table = p.seqs > 1 ? (int)t.stride(0) : p.max_pages;
+    return p;
+}
+
+// qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout, mscale, pdl
+PyObject* qkv_axes_rope_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    return guarded([&]() -> PyObject* {
+        args(na, 13);
+        must(zl.axes_rope);
+        const at::Tensor& x = here(a[0], false);
+        const Paged c = paged_cache(a[7], a[8], a[6], x.scalar_type());
+        const int heads = to_int(a[9]), layout = to_int(a[10]), pdl = truth(a[12]);
+        const double mscale = to_double(a[11]);
+        must(x.dim() == 2 && heads > 0 && heads < 1 << 16 && x.size(1) == (int64_t)(heads + 2 * c.kv_heads) * c.dim && x.stride(1) == 1);
+        const int64_t t = x.size(0);
+        must(t > 0 && t < 1ll << 31);
+        const at::Tensor &pos = here(a[1], true), &freq = here(a[2], true);
+        must(pos.scalar_type() == at::kInt && pos.dim() == 2 && pos.size(0) > 0 && pos.size(0) < 1 << 16 && pos.size(1) == t);
+        must(freq.scalar_type() == at::kDouble && freq.dim() == 1 && 2 * freq.size(0) <= c.dim);
+        const int32_t *axis = ints(a[3], freq.size(0)), *seq = ints(a[4], t), *place = ints(a[5], t);
+        const at::Tensor q = empty(x, {t, (int64_t)heads * c.dim}, x.scalar_type());
+        const long long ld = t > 1 ? x.stride(0) : x.size(1);
+        const int dt = dtype_of(x);
+        const zl_stream_t s = stream();
+        return result(unlocked([&] {
+                          return zl.axes_rope(x.data_ptr(), ld, static_cast<const int32_t*>(pos.data_ptr()), t, (int)pos.size(0),
+                                              static_cast<const double*>(freq.data_ptr()), axis, (int)freq.size(0), layout, (float)mscale, seq, place, c.table,
+                                              c.ld_table, c.max_pages, c.seqs, c.k, c.v, c.pages, c.page_size, c.step[0], c.step[1], c.step[2], q.data_ptr(), (int)t,
+                                              heads, c.kv_heads, c.dim, dt, pdl, s);
+                      }),
+                      q);
+    });
+}
+
+// q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    return guarded([&]() -> PyObject* {
+        args(na, 11);
+        must(zl.paged && zl.paged_bytes);
+        const at::Tensor& q = here(a[0], true);
+        const Paged c = paged_cache(a[1], a[2], a[3], q.scalar_type());
+        must((q.dim() == 2 || q.dim() == 3) && (q.dim() == 2 || q.size(2) == c.dim));
+        const int64_t t = q.size(0), width = q.size(1) * (q.dim() == 3 ? c.dim : 1);
+        must(t > 0 && t < 1ll << 31 && width > 0 && width < 1 << 24 && width % ((int64_t)c.kv_heads * c.dim) == 0);
+        const int32_t *lens = ints(a[4], c.seqs), *starts = ints(a[5], (int64_t)c.seqs + 1);
+        const double scale = to_double(a[6]);
+        const int window = to_int(a[7]), most = a[8] == Py_None ? (int)t : to_int(a[8]), pdl = truth(a[10]);
+        must(most > 0);
+        if (a[9] != Py_None) {
+            const at::Tensor& o = here(a[9], true);
+            must(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type());
+        }
+        const at::Tensor out = a[9] == Py_None ? empty(q, q.sizes(), q.scalar_type()) : THPVariable_Unpack(a[9]);
+        const int heads = (int)(width / c.dim), new_ = (int)std::min<int64_t>(most, t);
+        const size_t bytes = zl.paged_bytes((int)t, new_, c.seqs, (int)std::min<long long>((long long)c.max_pages * c.page_size, (1ll << 31) - 256), heads, c.kv_heads, c.dim);
+        at::Tensor room;
+        if (bytes) room = empty(q, {(int64_t)bytes}, at::kByte);
+        void* const ws = bytes ? room.data_ptr() : nullptr;
+        const int dt = dtype_of(q);
+        const zl_stream_t s = stream();
+        return result(unlocked([&] {
+                          return zl.paged(q.data_ptr(), c.k, c.v, c.pages, c.page_size, c.step[0], c.step[1], c.step[2], c.table, c.ld_table, c.max_pages, lens, starts,
+                                          c.seqs, (float)scale, window, out.data_ptr(), (int)t, new_, heads, c.kv_heads, c.dim, ws, bytes, dt, pdl, s);
+                      }),
+                      out);
+    });
+}
+
+// target, draft, drafted, accept, sample, count, pdl: a pair of tensors
+PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    return guarded([&]() -> PyObject* {
+        args(na, 7);
+        must(zl.verify);
+        const at::Tensor &p = here(a[0], false), &words = here(a[2], true), &accept = here(a[3], true), &sample = here(a[4], true);
+        must(p.dim() == 3 && p.scalar_type() == at::kFloat && p.size(1) > 0 && p.size(2) > 0 && p.stride(2) == 1);
+        const int64_t b = p.size(0), k = p.size(1) - 1, vocab = p.size(2);
+        must(b > 0 && b < 1 << 30 && k < 1 << 30 && vocab <= 1 << 30);
+        long long d_seq = 0, d_row = 0;
+        const float* draft = nullptr;
+        if (a[1] != Py_None) {
+            const at::Tensor& d = here(a[1], false);
+            must(d.dim() == 3 && d.size(0) == b && d.size(1) == k && d.size(2) == vocab && d.scalar_type() == at::kFloat && d.stride(2) == 1);
+            draft = static_cast<const float*>(d.data_ptr()), d_seq = d.stride(0), d_row = d.stride(1);
+        }
+        must(words.scalar_type() == at::kInt && words.dim() == 2 && words.size(0) == b && words.size(1) == k);
+        must(accept.scalar_type() == at::kFloat && accept.dim() == 2 && accept.size(0) == b && accept.size(1) == k);
+        must(sample.scalar_type() == at::kFloat && sample.dim() == 1 && sample.size(0) == b);
+        const int32_t* count = a[5] == Py_None ? nullptr : ints(a[5], b);
+        const int pdl = truth(a[6]);
+        const at::Tensor accepted = empty(p, {b}, at::kInt), tokens = empty(p, {b, k + 1}, at::kInt);
+        const zl_stream_t s = stream();
+        const int rc = unlocked([&] {
+            return zl.verify(static_cast<const float*>(p.data_ptr()), p.stride(0), p.stride(1), draft, d_seq, d_row, static_cast<const int32_t*>(words.data_ptr()),
+                             static_cast<const float*>(accept.data_ptr()), static_cast<const float*>(sample.data_ptr()), count, static_cast<int32_t*>(accepted.data_ptr()),
+                             static_cast<int32_t*>(tokens.data_ptr()), (int)b, (int)k, (int)vocab, pdl, s);
+        });
+        if (rc) return PyLong_FromLong(rc);
+        PyObject *first = THPVariable_Wrap(accepted), *second = THPVariable_Wrap(tokens), *pair = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+        Py_XDECREF(first);
+        Py_XDECREF(second);
+        return pair;
+    });
+}
+
 // {name of an entry point: its address}
 PyObject* bind(PyObject*, PyObject* d) {
     if (!PyDict_Check(d)) {
@@ -243,12 +393,17 @@ PyObject* bind(PyObject*, PyObject* d) {
     set(zl.w8, "zl_w8a8_gemm");
     set(zl.attn_bytes, "zl_decode_attention_workspace_bytes");
     set(zl.attn, "zl_decode_attention_host");
+    set(zl.axes_rope, "zl_qkv_axes_rope_append");
+    set(zl.paged_bytes, "zl_paged_attention_workspace_bytes");
+    set(zl.paged, "zl_paged_attention");
+    set(zl.verify, "zl_verify_drafts");
     if (PyErr_Occurred()) return nullptr;
     Py_RETURN_NONE;
 }
 
 #define ZL_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ZL_FAST(w4a16_gemm_fused), ZL_FAST(dense_gemm_skinny), ZL_FAST(w8_linear), ZL_FAST(decode_attention),
+                         ZL_FAST(qkv_axes_rope_append), ZL_FAST(paged_attention), ZL_FAST(verify_drafts),
                          {"bind", bind, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

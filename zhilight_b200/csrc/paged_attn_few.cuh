@@ -27,76 +27,71 @@ struct PfCfg {
 __device__ __forceinline__ int paged_few_tiles(const PagedBlock& k) { return k.hi >= 0 ? k.hi / kPfKeys - k.lo / kPfKeys + 1 : 1; }
 
 struct PfPlace {
-    int hk, off, tiles, index;   // kv head; tile within the block and how many it has; number of the block among all (token, head) blocks of a kv head
-    long long start;             // the block's place in the line
+    int hk, off, tiles;   // kv head; tile within the block, and how many that has
+    int start;            // the block's place in the line
 };
 
-// Lane's share: tiles of a kv head of sequence b
-__device__ __forceinline__ int paged_few_sum(const PagedAttn& p, const PagedCache& c, int b, int size, int& blocks) {
-    PagedBlock k;
-    k.seq = b;
-    blocks = 0;
-    if (b >= c.seqs) return 0;
-    const int n = paged_new(p, b, k.first) * p.group;
-    if (n > p.few) return 0;
-    int sum = 0;
-    for (k.row0 = 0; k.row0 < n; k.row0 += size, ++blocks) {
-        k.rows = min(size, n - k.row0);
-        paged_bounds(p, c, k);
-        sum += paged_few_tiles(k);
-    }
-    return sum;
-}
+// A warp's view of the line: sequence by sequence, in it kv head by kv head, in that block by block; 32 sequences at a time, one a lane.  Everything fits
+// 32 bits, which the entry point sees to.
+struct PfLine {
+    int size, kv_heads;           // rows of a block
+    int b0, before, mine, upto;   // first sequence in view and its place; tiles of a kv head of this lane's sequence, and up to and with it
 
-__device__ __forceinline__ int paged_scan(int v) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += x;
-    }
-    return v;
-}
-
-// Length of the line, by a warp
-__device__ __forceinline__ long long paged_few_total(const PagedAttn& p, const PagedCache& c, int kv_heads, int size) {
-    long long sum = 0;
-    int blocks;
-    for (int b0 = 0; b0 < c.seqs; b0 += 32) sum += __shfl_sync(0xffffffffu, paged_scan(paged_few_sum(p, c, b0 + (threadIdx.x & 31), size, blocks)), 31);
-    return sum * kv_heads;
-}
-
-// The block at place w of the line: sequence by sequence, in it kv head by kv head, in that block by block.  By a warp.
-__device__ __forceinline__ void paged_few_at(const PagedAttn& p, const PagedCache& c, int kv_heads, int size, long long w, PagedBlock& k, PfPlace& at) {
-    long long before = 0;
-    int blocks, first_block = 0;
-    for (int b0 = 0; b0 < c.seqs; b0 += 32) {
-        const int mine = paged_few_sum(p, c, b0 + (threadIdx.x & 31), size, blocks), upto = paged_scan(mine), blocks_upto = paged_scan(blocks);
-        const unsigned hit = __ballot_sync(0xffffffffu, before + (long long)upto * kv_heads > w);
-        if (hit) {
-            const int src = __ffs(hit) - 1, each = __shfl_sync(0xffffffffu, mine, src);
-            const long long here = before + (long long)__shfl_sync(0xffffffffu, upto - mine, src) * kv_heads;
-            int rem = (int)(w - here);
-            at.hk = rem / each;
-            rem -= at.hk * each;
-            k.seq = b0 + src;
-            at.index = first_block + __shfl_sync(0xffffffffu, blocks_upto - blocks, src);
+    __device__ __forceinline__ void view(const PagedAttn& p, const PagedCache& c) {
+        PagedBlock k;
+        k.seq = b0 + (threadIdx.x & 31);
+        mine = 0;
+        if (k.seq < c.seqs) {
             const int n = paged_new(p, k.seq, k.first) * p.group;
-            for (k.row0 = 0;; k.row0 += size, ++at.index) {
-                k.rows = min(size, n - k.row0);
-                paged_bounds(p, c, k);
-                at.tiles = paged_few_tiles(k);
-                if (rem < at.tiles) break;
-                rem -= at.tiles;
-            }
-            at.off = rem;
-            at.start = w - rem;
-            return;
+            if (n <= p.few)
+                for (k.row0 = 0; k.row0 < n; k.row0 += size) {
+                    k.rows = min(size, n - k.row0);
+                    paged_bounds(p, c, k);
+                    mine += paged_few_tiles(k);
+                }
         }
-        before += (long long)__shfl_sync(0xffffffffu, upto, 31) * kv_heads;
-        first_block += __shfl_sync(0xffffffffu, blocks_upto, 31);
+        upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if ((int)(threadIdx.x & 31) >= o) upto += x;
+        }
     }
-}
+    // length of the line; the view is at its beginning then
+    __device__ __forceinline__ int begin(const PagedAttn& p, const PagedCache& c) {
+        int total = 0;
+        before = 0;
+        for (b0 = (c.seqs - 1) & ~31;; b0 -= 32) {
+            view(p, c);
+            total += __shfl_sync(0xffffffffu, upto, 31) * kv_heads;
+            if (b0 == 0) return total;
+        }
+    }
+    // the block at place w, which is in view or behind it
+    __device__ __forceinline__ void at(const PagedAttn& p, const PagedCache& c, int w, PagedBlock& k, PfPlace& place) {
+        unsigned hit;
+        while (!(hit = __ballot_sync(0xffffffffu, before + upto * kv_heads > w))) {
+            before += __shfl_sync(0xffffffffu, upto, 31) * kv_heads;
+            b0 += 32;
+            view(p, c);
+        }
+        const int src = __ffs(hit) - 1, each = __shfl_sync(0xffffffffu, mine, src);
+        int rem = w - before - __shfl_sync(0xffffffffu, upto - mine, src) * kv_heads;
+        place.hk = rem / each;
+        rem -= place.hk * each;
+        k.seq = b0 + src;
+        const int n = paged_new(p, k.seq, k.first) * p.group;
+        for (k.row0 = 0;; k.row0 += size) {
+            k.rows = min(size, n - k.row0);
+            paged_bounds(p, c, k);
+            place.tiles = paged_few_tiles(k);
+            if (rem < place.tiles) break;
+            rem -= place.tiles;
+        }
+        place.off = rem;
+        place.start = w - rem;
+    }
+};
 
 __device__ __forceinline__ void pf_ldsm(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -155,29 +150,36 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     uint8_t* ring = pf_smem + warp * C::kWarp;
     const uint32_t ring_at = smem_u32(ring);
-    pdl_trigger();
     pdl_wait();
-    const long long total = paged_few_total(p, c, kv_heads, R);
-    long long w = total * blockIdx.x / gridDim.x;
-    const long long end = total * (blockIdx.x + 1) / gridDim.x;
-    while (w < end) {
+    pdl_trigger();   // behind the wait: the join reads lengths and starts ahead of its own
+    PfLine line;
+    line.size = R, line.kv_heads = kv_heads;
+    const int total = line.begin(p, c), per = cdiv(total, (int)gridDim.x), end = min(total, per * ((int)blockIdx.x + 1));
+    for (int w = min(total, per * (int)blockIdx.x); w < end;) {
         PagedBlock k;
         PfPlace at;
-        paged_few_at(p, c, kv_heads, R, w, k, at);
-        const int count = (int)min(end - w, (long long)(at.tiles - at.off)), key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + at.off) * kPfKeys + warp * 16;
+        line.at(p, c, w, k, at);
+        const int count = min(end - w, at.tiles - at.off), key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + at.off) * kPfKeys + warp * 16;
         const long long head = (long long)at.hk * c.head_stride;
-        // copies of a stage: lane's chunk of two rows at a time; lanes 0 - 15 know where the 16 rows lie, a stage ahead
+        // Copies of a stage: each lane has a chunk of some rows.  Lanes 0 - 15 ask for the page numbers of the 16 rows a stage ahead; where pages hold whole
+        // 16s these are one page.
+        const bool one_page = c.page_size % 16 == 0;
         auto find = [&](int j) {
-            const int row = key0 + j * kPfKeys + (lane & 15);
-            return j < count && row <= k.hi ? c.row_at(k.seq, row) : -1;
+            const int row = key0 + j * kPfKeys + (lane & 15), pg = c.by_page(row);
+            return j < count && row <= k.hi && pg < c.max_pages ? c.table[(size_t)k.seq * c.ld_table + pg] : -1;
         };
-        auto copy = [&](int j, long long off) {
+        auto copy = [&](int j, int id) {
             const uint32_t to = ring_at + (uint32_t)(j % kPfStages) * C::kStage;
-            const int ch = lane % CH;
+            const int ch = lane % CH, row0 = key0 + j * kPfKeys, mine = row0 + (one_page ? 0 : lane & 15);
+            long long off = id >= 0 && id < c.num_pages ? (long long)id * c.page_stride + (long long)(mine - c.by_page(mine) * c.page_size) * c.row_stride : -1;
+            if (one_page) off = __shfl_sync(0xffffffffu, off, 0);
 #pragma unroll
             for (int i = 0; i < 16 * CH / 32; ++i) {
                 const int r = lane / CH + i * (32 / CH);
-                const long long o = __shfl_sync(0xffffffffu, off, r);
+                long long o = off;
+                if (!one_page) o = __shfl_sync(0xffffffffu, off, r);
+                else if (row0 + r > k.hi) o = -1;
+                else if (o >= 0) o += r * c.row_stride;
                 const long long from = o < 0 ? 0 : o + head + ch * 8;
                 const int bytes = o < 0 ? 0 : 16;
                 const uint32_t dst = to + (uint32_t)(r * (D * 2) + ((ch ^ (r & 7)) << 4));
@@ -185,12 +187,13 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 16 * D * 2), "l"(static_cast<const T*>(c.v) + from), "r"(bytes) : "memory");
             }
         };
-        long long off = find(0);
-#pragma unroll
+        int id = find(0);
+#pragma unroll 1
         for (int j = 0; j < kPfStages - 1; ++j) {
-            if (j < count) copy(j, off);
+            const int next = find(j + 1);
+            if (j < count) copy(j, id);
             asm volatile("cp.async.commit_group;" ::: "memory");
-            off = find(j + 1);
+            id = next;
         }
         // rows of q: (g, g + 8) of each 16
         uint32_t qa[MT][KS][4];
@@ -218,9 +221,10 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
         for (int j = 0; j < count; ++j) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kPfStages - 2) : "memory");
             __syncwarp();
-            if (j + kPfStages - 1 < count) copy(j + kPfStages - 1, off);
+            const int next = find(j + kPfStages);
+            if (j + kPfStages - 1 < count) copy(j + kPfStages - 1, id);
             asm volatile("cp.async.commit_group;" ::: "memory");
-            off = find(j + kPfStages);
+            id = next;
             const int kb = key0 + j * kPfKeys;
             if (kb > k.hi || kb + 15 < k.lo) continue;
             const uint32_t st = ring_at + (uint32_t)(j % kPfStages) * C::kStage;
@@ -332,37 +336,47 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
     }
 }
 
-// Blocks that were cut: grid (parts' CTAs).  CTA i looks at the block that begins in stretch i - and is cut - of the line: there is one at the most.
+// Blocks that were cut: grid (the parts' CTAs).  CTA i joins the block that begins in stretch i of the line and goes on behind it: there is one at the most.
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kPfWarps * 32) k_paged_few_join(const PagedAttn p, const PagedCache c, int kv_heads) {
     constexpr int R = 16 * MT, E = D / 32;
-    pdl_trigger();
-    pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long total = paged_few_total(p, c, kv_heads, R);
-    const long long w0 = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
-    if (w0 >= end || end == total) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i0 = blockIdx.x;
+    PfLine line;
+    line.size = R, line.kv_heads = kv_heads;
+    const int total = line.begin(p, c), per = cdiv(total, (int)gridDim.x), end = per * (i0 + 1);   // the first kernel has seen its predecessors end
     PagedBlock k;
     PfPlace at;
-    paged_few_at(p, c, kv_heads, R, end - 1, k, at);
-    if (at.start < w0 || at.start + at.tiles <= end) return;   // begins in an earlier stretch; ends in this one
-    // stretches that have a part: this one and those up to the one with the block's last tile
-    const int last = (int)(((at.start + at.tiles) * gridDim.x - 1) / total);
+    bool cut = end < total;
+    if (cut) {
+        line.at(p, c, end - 1, k, at);
+        cut = at.start >= per * i0 && at.start + at.tiles > end;   // else it begins in an earlier stretch, or ends here
+    }
+    pdl_trigger();
+    pdl_wait();
+    if (!cut) return;
+    const int parts = (at.start + at.tiles - 1) / per - i0 + 1;
+    auto place = [&](int s, int r) { return ((size_t)(i0 + s) * 2 + (s == 0)) * R + r; };
     for (int r = warp; r < k.rows; r += kPfWarps) {
         float m = -INFINITY, l = 0.f, v[E] = {};
-        for (int i = blockIdx.x; i <= last; ++i) {
-            if (total * i / gridDim.x == total * (i + 1) / gridDim.x) continue;   // an empty stretch
-            m = fmaxf(m, p.ml[((size_t)i * 2 + (i == (int)blockIdx.x)) * R + r].x);
-        }
-        for (int i = blockIdx.x; i <= last; ++i) {
-            if (total * i / gridDim.x == total * (i + 1) / gridDim.x) continue;
-            const size_t part = ((size_t)i * 2 + (i == (int)blockIdx.x)) * R + r;
-            const float2 x = p.ml[part];
-            const float f = pf_exp2(x.x - m);
-            l = fmaf(x.y, f, l);
-            const float* from = p.part + part * D + lane * E;
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = fmaf(from[e], f, v[e]);
+        for (int s = lane; s < parts; s += 32) m = fmaxf(m, p.ml[place(s, r)].x);
+        m = warp_max(m);
+        for (int s0 = 0; s0 < parts; s0 += 32) {
+            const float2 x = s0 + lane < parts ? p.ml[place(s0 + lane, r)] : make_float2(-INFINITY, 0.f);
+            const float f = s0 + lane < parts ? pf_exp2(x.x - m) : 0.f;
+            l += warp_sum(x.y * f);
+            const int n = min(32, parts - s0);
+#pragma unroll 8
+            for (int s = 0; s < n; ++s) {
+                const float w = __shfl_sync(0xffffffffu, f, s);
+                const float* from = p.part + place(s0 + s, r) * D + lane * E;
+                if constexpr (E == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(from);
+                    v[0] = fmaf(y.x, w, v[0]), v[1] = fmaf(y.y, w, v[1]), v[2] = fmaf(y.z, w, v[2]), v[3] = fmaf(y.w, w, v[3]);
+                } else {
+                    const float2 y = *reinterpret_cast<const float2*>(from);
+                    v[0] = fmaf(y.x, w, v[0]), v[1] = fmaf(y.y, w, v[1]);
+                }
+            }
         }
         paged_row_out<T, D>(p, c, k, at.hk, r, l, v);
     }

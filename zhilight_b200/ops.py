@@ -1161,6 +1161,10 @@ def qkv_axes_rope_append(qkv, pos, inv_freq, axis, token_seq, placement, page_ta
     frequency i turns pair i of queries and keys by pos[axis[i]] * inv_freq[i], cos and sin times mscale.  Keys and values go to row placement (T) int32
     (negative: nowhere) of sequence token_seq (T) int32 in the caches (pages, page_size, kv_heads, dim) behind page_table (sequences, pages) int32;
     the places of a call's rows differ.  -> q (T, heads * dim)."""
+    if _lib.host is not None:
+        y = _lib.host.qkv_axes_rope_append(qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout, mscale, pdl)
+        if y is not None:
+            return _done(y)
     steps = _paged_cache(k_cache, v_cache, page_table, qkv.dtype)
     pages, page_size, kv_heads, dim = k_cache.shape
     _need(qkv.dim() == 2 and heads > 0 and qkv.shape[1] == (heads + 2 * kv_heads) * dim and qkv.stride(1) == 1,
@@ -1191,6 +1195,10 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
     behind page_table (sequences, pages) int32.  Each sees the keys up to its own, with a window only the last `window` of them; a row that sees none
     gives zeros.  seq_lens (sequences) and q_starts (sequences + 1), ascending, int32.  max_new: a bound of the new tokens of one sequence (None: all
     rows), which chooses kernels and nothing else.  Rows of no sequence: out, if given, keeps what it holds there.  -> out, like q."""
+    if _lib.host is not None:
+        y = _lib.host.paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl)
+        if y is not None:
+            return _done(y)
     steps = _paged_cache(k_cache, v_cache, page_table, q.dtype)
     pages, page_size, kv_heads, dim = k_cache.shape
     _need(q.dim() in (2, 3) and q.is_contiguous() and (q.dim() == 2 or q.shape[2] == dim), "q must be contiguous (T, heads * dim) or (T, heads, dim)")
@@ -1220,6 +1228,10 @@ def verify_drafts(target, draft, drafted, accept, sample, count=None, pdl=False)
     sample (B) fp32; count (B) int32: drafts of each sequence (None: K).  Draft i is taken while accept * draft(word) < target(word); the word behind
     the last one taken is drawn by `sample` from max(target - draft, 0) of the refused draft's row, from target behind the last draft.
     -> (accepted (B) int32, tokens (B, K + 1) int32: the drafts taken, the word drawn, then -1)."""
+    if _lib.host is not None:
+        y = _lib.host.verify_drafts(target, draft, drafted, accept, sample, count, pdl)
+        if y is not None:
+            return _done(y)
     _need(target.dim() == 3 and target.dtype == torch.float32 and target.shape[1] > 0 and target.shape[2] > 0 and target.stride(2) == 1,
           "target must be (B, K + 1, vocab) fp32, its rows in one piece")
     b, k, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
