@@ -9,9 +9,51 @@
 #include "paged.cuh"
 #include "tc2_common.cuh"
 
+#include <climits>
+
 namespace zl {
 
 constexpr int kVdWarps = 16, kVdMaxCluster = 8, kVdAhead = 8;
+
+constexpr int kVdEach = kVdMaxCluster * kVdWarps / 32;   // sums of runs that a lane looks at
+
+__device__ __forceinline__ double vd_scan(double v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+
+// the weight of a word; what is not finite or not positive counts as none
+__device__ __forceinline__ double vd_weight(float a, float q) { return a > q && a < INFINITY && q > -INFINITY ? (double)a - (double)q : 0.0; }
+
+// This lane's share of the weights of lo .. hi - 1: target less draft (TWO), or target alone, less one at `skip`
+template <bool TWO>
+__device__ __forceinline__ double vd_sum(const float* __restrict__ tr, const float* __restrict__ dr, int lo, int hi, int skip) {
+    double s[2] = {0.0, 0.0};
+    int i = lo + (threadIdx.x & 31);
+    float a[kVdAhead], q[kVdAhead];
+    for (; i + 32 * (kVdAhead - 1) < hi; i += 32 * kVdAhead) {
+#pragma unroll
+        for (int u = 0; u < kVdAhead; ++u) {
+            a[u] = tr[i + 32 * u];
+            if (TWO) q[u] = dr[i + 32 * u];
+        }
+#pragma unroll
+        for (int u = 0; u < kVdAhead; ++u) s[u & 1] += vd_weight(a[u], TWO ? q[u] : i + 32 * u == skip ? 1.f : 0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < kVdAhead; ++u) {
+        a[u] = i + 32 * u < hi ? tr[i + 32 * u] : 0.f;
+        if (TWO) q[u] = i + 32 * u < hi ? dr[i + 32 * u] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kVdAhead; ++u) s[u & 1] += vd_weight(a[u], TWO ? q[u] : i + 32 * u == skip ? 1.f : 0.f);
+    return s[0] + s[1];
+}
 
 struct VerifyDrafts {
     const float *target, *draft;
@@ -25,64 +67,45 @@ struct VerifyDrafts {
 // grid (CTAs of a sequence, sequences), a cluster along x
 __global__ void __launch_bounds__(kVdWarps * 32) k_verify_drafts(const VerifyDrafts p) {
     __shared__ double part[kVdMaxCluster][kVdWarps];
-    __shared__ int s_taken;
+    __shared__ double s_sum[kVdWarps];
+    __shared__ int s_taken, s_count, s_first[kVdWarps], s_last[kVdWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, b = blockIdx.y, ctas = gridDim.x, cta = blockIdx.x;
     if (ctas > 1) cluster_arrive();   // every CTA runs before another one stores into it
     pdl_trigger();
     pdl_wait();
-    const int n = p.count ? min(max(p.count[b], 0), p.k) : p.k;
     if (warp == 0) {
-        int taken = 0;
+        int taken = 0, n = p.k;
         for (int i0 = 0; i0 < n; i0 += 32) {
             const int i = i0 + lane;
+            int x = -1;
+            float u = 0.f;
+            if (i < n) x = p.drafted[(size_t)b * p.k + i], u = p.accept[(size_t)b * p.k + i];
+            if (i0 == 0 && p.count) n = min(max(p.count[b], 0), p.k);   // beside the two above
             bool ok = false;
-            if (i < n) {
-                const int x = p.drafted[(size_t)b * p.k + i];
-                if ((unsigned)x < (unsigned)p.vocab) {
-                    const double q = p.draft ? (double)p.draft[b * p.d_seq + i * p.d_row + x] : 1.0;
-                    ok = (double)p.accept[(size_t)b * p.k + i] * q < (double)p.target[b * p.t_seq + i * p.t_row + x];
-                }
+            if (i < n && (unsigned)x < (unsigned)p.vocab) {
+                const double q = p.draft ? (double)p.draft[b * p.d_seq + i * p.d_row + x] : 1.0;
+                ok = (double)u * q < (double)p.target[b * p.t_seq + i * p.t_row + x];
             }
             const unsigned m = __ballot_sync(0xffffffffu, ok);
-            if (m != 0xffffffffu) {
-                taken += __ffs(~m) - 1;
-                break;
-            }
-            taken += 32;
+            taken += m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+            if (m != 0xffffffffu) break;
         }
-        if (lane == 0) s_taken = min(taken, n);
+        if (lane == 0) s_taken = min(taken, n), s_count = n;
     }
     __syncthreads();
     const int taken = s_taken;
-    const bool refused = taken < n;
+    const bool refused = taken < s_count;
     const float* tr = p.target + b * p.t_seq + taken * p.t_row;
     const float* dr = refused && p.draft ? p.draft + b * p.d_seq + taken * p.d_row : nullptr;
     const int skip = refused && !p.draft ? p.drafted[(size_t)b * p.k + taken] : -1;   // a draft without probabilities has all of its own on one word
     // this warp's run
     const int run = cdiv(p.vocab, ctas * kVdWarps), lo = min((cta * kVdWarps + warp) * run, p.vocab), hi = min(lo + run, p.vocab);
-    double total = 0.0, before = 0.0, mine = 0.0;
+    double total = 0.0, below = 0.0, each[kVdEach];
     bool plain = !refused;
     if (ctas > 1) cluster_wait();
-    // the weight of a word; what is not finite or not positive counts as none
-    auto weigh = [&](float a, float q, int i) {
-        const double w = plain ? (double)a : (i == skip ? (double)a - 1.0 : (double)a - (double)q);
-        return w > 0.0 && w < INFINITY ? w : 0.0;
-    };
     for (;;) {
-        const float* d2 = plain ? nullptr : dr;
-        double s[2] = {0.0, 0.0};
-        for (int i = lo + lane; i < hi; i += 32 * kVdAhead) {
-            float a[kVdAhead], q[kVdAhead];
-#pragma unroll
-            for (int u = 0; u < kVdAhead; ++u) {
-                const int at = i + 32 * u;
-                a[u] = at < hi ? tr[at] : 0.f;
-                q[u] = d2 && at < hi ? d2[at] : 0.f;
-            }
-#pragma unroll
-            for (int u = 0; u < kVdAhead; ++u) s[u & 1] += weigh(a[u], q[u], i + 32 * u);
-        }
-        mine = s[0] + s[1];
+        const double sum = plain || !dr ? vd_sum<false>(tr, nullptr, lo, hi, plain ? -1 : skip) : vd_sum<true>(tr, dr, lo, hi, -1);
+        double mine = sum;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
         if (ctas > 1) {
@@ -95,12 +118,15 @@ __global__ void __launch_bounds__(kVdWarps * 32) k_verify_drafts(const VerifyDra
             if (lane == 0) part[0][warp] = mine;
             __syncthreads();
         }
-        total = before = 0.0;
-        for (int c = 0; c < ctas; ++c)
-            for (int w = 0; w < kVdWarps; ++w) {
-                if (c == cta && w == warp) before = total;
-                total += part[c][w];
-            }
+        // sums of the runs up to and with this lane's, in order: up to four runs a lane
+#pragma unroll
+        for (int u = 0; u < kVdEach; ++u) {
+            const int e = lane * kVdEach + u;
+            each[u] = (u ? each[u - 1] : 0.0) + (e < ctas * kVdWarps ? part[e / kVdWarps][e % kVdWarps] : 0.0);
+        }
+        below = vd_scan(each[kVdEach - 1]);
+        total = __shfl_sync(0xffffffffu, below, 31);
+        below -= each[kVdEach - 1];   // for the places of the runs; which run has the word goes by these same numbers
         if (total > 0.0 || plain) break;
         plain = true;                    // nothing is left of the target: its own row decides
         if (ctas > 1) cluster_sync_all();   // the sums have been read
@@ -118,38 +144,46 @@ __global__ void __launch_bounds__(kVdWarps * 32) k_verify_drafts(const VerifyDra
     // The warp whose run holds the word: the first whose running sum passes; behind them all (u of one, or sums that round apart) the last one that has
     // a weight.  Every warp knows all sums, so each tells by itself.
     const double goal = (double)p.sample[b] * total;
-    int owner = -1, last = -1;
-    {
-        double sum = 0.0;
-        for (int c = 0; c < ctas; ++c)
-            for (int w = 0; w < kVdWarps; ++w) {
-                if (part[c][w] > 0.0) last = c * kVdWarps + w;
-                sum += part[c][w];
-                if (owner < 0 && sum > goal) owner = c * kVdWarps + w;
-            }
-    }
-    if (owner < 0) owner = last;
-    if (owner != cta * kVdWarps + warp) return;
-    double run_sum = before;
-    int word = -1;
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        const double w = i < hi ? weigh(tr[i], plain || !dr ? 0.f : dr[i], i) : 0.0;
-        double up = w;
+    int past = kVdEach, some = -1;   // of this lane's runs the first that passes, the last with a weight
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double v = __shfl_up_sync(0xffffffffu, up, o);
-            if (lane >= o) up += v;
-        }
-        const unsigned some = __ballot_sync(0xffffffffu, w > 0.0), past = __ballot_sync(0xffffffffu, w > 0.0 && run_sum + up > goal);
-        if (past) {
-            word = i0 + __ffs(past) - 1;
-            break;
-        }
-        if (some) word = i0 + 31 - __clz(some);
-        run_sum += __shfl_sync(0xffffffffu, up, 31);
+    for (int u = kVdEach - 1; u >= 0; --u) {
+        const bool weight = each[u] > (u ? each[u - 1] : 0.0);
+        if (weight && below + each[u] > goal) past = u;
+        if (weight && some < 0) some = u;
     }
-    if (lane == 0) p.tokens[(size_t)b * (p.k + 1) + taken] = word;
+    const unsigned passes = __ballot_sync(0xffffffffu, past < kVdEach), has = __ballot_sync(0xffffffffu, some >= 0);
+    const int src = passes ? __ffs(passes) - 1 : 31 - __clz(has);
+    const int owner = src * kVdEach + __shfl_sync(0xffffffffu, passes ? past : some, src);
+    if (owner / kVdWarps != cta) return;
+    // The run once more by the whole CTA: a piece of neighbouring words for every thread, then the words of the piece that passes.
+    const int u0 = owner % kVdEach, from = min(owner * run, p.vocab), to = min(from + run, p.vocab), piece = cdiv(to - from, kVdWarps * 32);
+    const int a = min(from + tid * piece, to), z = min(a + piece, to);
+    auto weight_at = [&](int i) { return vd_weight(tr[i], plain ? 0.f : dr ? dr[i] : i == skip ? 1.f : 0.f); };
+    double w = 0.0;
+#pragma unroll 4
+    for (int i = a; i < z; ++i) w += weight_at(i);
+    const double up = vd_scan(w);
+    if (lane == 31) s_sum[warp] = up;
+    __syncthreads();
+    double sum = lane < kVdWarps ? s_sum[lane] : 0.0;
+    sum = vd_scan(sum) - sum;        // of the warps before
+    sum = __shfl_sync(0xffffffffu, sum, warp) + __shfl_sync(0xffffffffu, below + (u0 ? each[u0 - 1] : 0.0), src);
+    const unsigned here = __ballot_sync(0xffffffffu, w > 0.0 && sum + up > goal), any = __ballot_sync(0xffffffffu, w > 0.0);
+    if (lane == 0) s_first[warp] = here ? tid + __ffs(here) - 1 : INT_MAX, s_last[warp] = any ? tid + 31 - __clz(any) : -1;
+    __syncthreads();
+    int first = __reduce_min_sync(0xffffffffu, lane < kVdWarps ? s_first[lane] : INT_MAX);
+    const int back = __reduce_max_sync(0xffffffffu, lane < kVdWarps ? s_last[lane] : -1);
+    if (first == INT_MAX) first = back;
+    if (tid != first) return;
+    int word = -1;
+    sum += up - w;
+    for (int i = a; i < z; ++i) {
+        const double x = weight_at(i);
+        sum += x;
+        if (x > 0.0) word = i;
+        if (x > 0.0 && sum > goal) break;
+    }
+    p.tokens[(size_t)b * (p.k + 1) + taken] = word;
 }
 
 }  // namespace zl
