@@ -1128,7 +1128,7 @@ int zl_bezasun_read_state(zl_bezasun_t* m, int layer, int slot, float* out_host)
  * pair i of every query and key head (columns (i, i + half) or (2i, 2i + 1) by `layout`; columns from 2 * half on stay) by pos[axis[i] * ld_pos + t] *
  * inv_freq[i], cos and sin times mscale; an axis[i] outside [0, axes) does not turn.  q_out (T, heads * dim); keys and values go to row placement[t]
  * of sequence token_seq[t], unless that row (negative: none) or sequence does not exist.  Rows of one call have different places: of two with the same
- * place, pieces of either may stay.  The angle is taken in 64 bits. */
+ * place, pieces of either may stay.  The angle is taken in 64 bits.  dim a multiple of 8 up to 1024, a row of up to 110000 elements. */
 int zl_qkv_axes_rope_append(const void* qkv, long long ldq, const int32_t* pos, long long ld_pos, int axes, const double* inv_freq,
                             const int32_t* axis, int half, int layout, float mscale, const int32_t* token_seq, const int32_t* placement,
                             const int32_t* page_table, int ld_table, int max_pages, int seqs, void* k_cache, void* v_cache, long long num_pages,

@@ -50,7 +50,7 @@ unsigned* zl::wait_words() {
 extern "C" void* zl_wait_words(void) { return zl::wait_words(); }
 extern "C" int zl_check_waits(void) {
     static const char* const names[zl::kWaitWords] = {"general tensor-core GEMM", "4-bit GEMM over pairs of SMs",
-                                                      "attention of prompt portions", "attention over pages"};
+                                                      "attention of prompt portions", "attention over pages", "rotation with the append to pages"};
     unsigned* words = zl::wait_words();
     if (!words) return ZL_OK;   // no kernel that would write them has been launched
     for (int i = 0; i < zl::kWaitWords; ++i) {
