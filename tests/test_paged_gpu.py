@@ -160,6 +160,15 @@ def test_attention_portions(cuda, dtype, heads, kv_heads, dim, page, order, wind
     check_attention(dtype, heads, kv_heads, dim, page, order, window, seqs)
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,window,seqs", [
+    (BF16, 16, 2, 64, 16, 0, [(3000, 1500)]), (F16, 8, 2, 128, 48, 0, [(2111, 700), (1900, 333), (1800, 1)]), (BF16, 8, 2, 128, 20, 900, [(2500, 900), (1111, 40)]),
+    (F16, 64, 8, 128, 64, 0, [(1000 + 131 * i, 1 + i % 16) for i in range(10)]), (BF16, 48, 8, 64, 32, 1000, [(2000 + 77 * i, 9 + i) for i in range(6)]),
+    (F16, 24, 8, 64, 256, 0, [(3001, 43), (2048, 30), (130, 130), (2500, 12)])])
+def test_attention_of_long_stretches(cuda, dtype, heads, kv_heads, dim, page, window, seqs):
+    """Enough keys for every CTA to go round its buffers several times, blocks of one and of two tiles, whole and cut."""
+    check_attention(dtype, heads, kv_heads, dim, page, "rows", window, seqs, max_new=max(n for _, n in seqs))
+
+
 @pytest.mark.parametrize("max_new", [1, 3, 20, 200, None])
 def test_attention_does_not_depend_on_the_bound_of_new_tokens(cuda, max_new):
     check_attention(BF16, 8, 2, 128, 16, "rows", 0, [(300, 200), (40, 1), (90, 3), (600, 18)], max_new=max_new)

@@ -33,8 +33,8 @@ struct PagedCache {
         if (id < 0 || id >= num_pages) return -1;
         return (long long)id * page_stride + (long long)(i - pg * page_size) * row_stride;
     }
-    // rows that the table has room for
-    __device__ __forceinline__ int room() const { return (int)min((long long)max_pages * page_size, 0x7fffffffll); }
+    // rows that the table has room for, as far as tiles of them are counted in 32 bits
+    __device__ __forceinline__ int room() const { return (int)min((long long)max_pages * page_size, 0x7fff0000ll); }
 };
 
 }  // namespace zl

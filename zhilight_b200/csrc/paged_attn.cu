@@ -10,9 +10,8 @@ namespace zl {
 constexpr int kFewRows = 32;   // (token, head) rows of a kv head that a sequence brings to the kernel for few rows
 
 struct PagedPlan {
-    bool tiles, few;                        // which kernels run
-    int blocks, splits;                     // of the tiles
-    int ctas, few_rows;                     // of the few rows; rows of their blocks
+    bool tiles, few;              // which kernels run
+    int ctas, few_ctas, few_rows; // their CTAs; rows of a block of the few
     size_t ml, part, few_ml, few_part, bytes;   // places in the workspace
 };
 
@@ -27,73 +26,82 @@ static PagedPlan paged_plan(int rows, int max_new, int seqs, int max_keys, int h
         s.bytes += (bytes + 255) / 256 * 256;
         return at;
     };
+    // no more CTAs than the line can be long: every sequence adds less than one block to those of the rows, each of all the keys there is room for
     if (s.tiles) {
-        // every sequence adds less than one block to those of the rows, and only those of more than kFewRows rows have any
-        const long long more = seqs > 1 ? all / (kFewRows + 1) : 1;
-        s.blocks = (int)(all / kPtRows + (more < seqs ? more : seqs));
-        const int tiles = cdiv(max_keys, kPtKeys);
-        s.splits = 1;
-        while (s.splits < 16 && 2ll * s.splits * s.blocks * kv_heads <= sms && tiles >= 8 * s.splits) s.splits *= 2;
-        if (s.splits > 1) {
-            const size_t parts = (size_t)s.blocks * s.splits * kv_heads * kPtRows;
-            s.ml = take(parts * sizeof(float2)), s.part = take(parts * dim * sizeof(float));
-        }
+        const long long turns = (all / kPtRows + seqs) * cdiv(max_keys, kPtKeys) * kv_heads;
+        s.ctas = (int)(turns < sms ? turns : sms);
+        const size_t parts = (size_t)s.ctas * 2 * kPtRows;
+        s.ml = take(parts * sizeof(float2)), s.part = take(parts * dim * sizeof(float));
     }
     if (s.few) {
         s.few_rows = most <= 16 ? 16 : 32;
-        // no more CTAs than there can be tiles: every block has the pool's rows of its sequence at the most
-        const long long blocks = all / s.few_rows + seqs, tiles = blocks * cdiv(max_keys, kPfKeys) * kv_heads;
-        s.ctas = (int)(tiles < kPfPerSm * sms ? tiles : kPfPerSm * sms);
-        const size_t parts = (size_t)s.ctas * 2 * s.few_rows;
+        const long long tiles = (all / s.few_rows + seqs) * cdiv(max_keys, kPfKeys) * kv_heads;
+        s.few_ctas = (int)(tiles < kPfPerSm * sms ? tiles : kPfPerSm * sms);
+        const size_t parts = (size_t)s.few_ctas * 2 * s.few_rows;
         s.few_ml = take(parts * sizeof(float2)), s.few_part = take(parts * dim * sizeof(float));
     }
     return s;
 }
 
-template <typename T, int D, int MT>
-static int paged_few(PagedAttn p, const PagedCache& c, const PagedPlan& s, int kv_heads, bool pdl, zl_stream_t stream) {
-    static bool attr_set[64] = {};
+// once for every device: `done` remembers
+template <typename... KArgs>
+static cudaError_t allow_smem(void (*kernel)(KArgs...), int bytes, bool (&done)[64]) {
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-        ZL_CHECK_CUDA(cudaFuncSetAttribute(k_paged_attn_few<T, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PfCfg<D>::kBytes));
-        if (dev >= 0 && dev < 64) attr_set[dev] = true;
-    }
-    ZL_CHECK_CUDA(launch(k_paged_attn_few<T, D, MT>, dim3(s.ctas), dim3(kPfWarps * 32), PfCfg<D>::kBytes, stream, pdl, p, c, kv_heads));
-    if (s.ctas > 1) ZL_CHECK_CUDA(launch(k_paged_few_join<T, D, MT>, dim3(s.ctas), dim3(kPfWarps * 32), 0, stream, true, p, c, kv_heads));
+    if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    return e;
+}
+
+template <typename T, int D, int MT>
+static int paged_few(PagedAttn p, const PagedCache& c, const PagedPlan& s, void* ws, bool pdl, zl_stream_t stream) {
+    static bool done[64] = {};
+    ZL_CHECK_CUDA(allow_smem(k_paged_attn_few<T, D, MT>, PfCfg<D>::kBytes, done));
+    p.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + s.few_ml), p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + s.few_part);
+    ZL_CHECK_CUDA(launch(k_paged_attn_few<T, D, MT>, dim3(s.few_ctas), dim3(kPfWarps * 32), PfCfg<D>::kBytes, stream, pdl, p, c));
+    if (s.few_ctas > 1)
+        ZL_CHECK_CUDA(launch(k_paged_join<T, D, PfKind<16 * MT>, false>, dim3(s.few_ctas, MT), dim3(kJoinThreads), 0, stream, true, p, c, 0, p.few));
     return ZL_OK;
 }
 
 template <typename T, int D>
-static int paged_attention(PagedAttn p, const PagedCache& c, const PagedPlan& s, int kv_heads, int pdl, zl_stream_t stream) {
-    unsigned* words = nullptr;
-    if (s.tiles) {
-        ZL_CHECK_WAITS();
-        words = wait_words();
-        ZL_CHECK_CUDA(words ? cudaSuccess : cudaErrorMemoryAllocation);
-        static bool attr_set[64] = {};
-        int dev = 0;
-        cudaGetDevice(&dev);
-        if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-            ZL_CHECK_CUDA(cudaFuncSetAttribute(k_paged_attn_tiles<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PtCfg<D>::kBytes));
-            if (dev >= 0 && dev < 64) attr_set[dev] = true;
-        }
+static int paged_tiles(PagedAttn p, const PagedCache& c, const PagedPlan& s, void* ws, bool pdl, zl_stream_t stream) {
+    static bool done[64] = {};
+    ZL_CHECK_WAITS();
+    unsigned* words = wait_words();
+    ZL_CHECK_CUDA(words ? cudaSuccess : cudaErrorMemoryAllocation);
+    ZL_CHECK_CUDA(allow_smem(k_paged_attn_tiles<T, D>, PtCfg<D>::kBytes, done));
+    p.ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(ws) + s.ml), p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + s.part);
+    // boxes: the rows that a tile and a page have in common wherever they meet
+    int box = 1;
+    while (box < kPtKeys && c.page_size % (2 * box) == 0) box *= 2;
+    CUtensorMap maps[2] = {};
+    if (box >= 8) {
+        const CUtensorMapDataType dt = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        auto step = [](long long elements, int n) { return n > 1 ? (uint64_t)elements * 2 : (uint64_t)(D * 2); };   // of one alone none is taken
+        const uint64_t dims[4] = {(uint64_t)D, (uint64_t)c.page_size, (uint64_t)p.kv_heads, (uint64_t)c.num_pages};
+        const uint64_t strides[3] = {step(c.row_stride, c.page_size), step(c.head_stride, p.kv_heads), step(c.page_stride, c.num_pages > 1 ? 2 : 1)};
+        const uint32_t rows[4] = {64, (uint32_t)box, 1, 1};
+        for (int i = 0; i < 2; ++i)
+            if (!tc_make_map_nd(&maps[i], i ? c.v : c.k, dt, 4, dims, strides, rows, CU_TENSOR_MAP_SWIZZLE_128B)) box = 0;
+    } else {
+        box = 0;
     }
-    uint8_t* ws = reinterpret_cast<uint8_t*>(p.ml);
-    p.few = !s.tiles ? INT_MAX : s.few ? kFewRows : 0;
-    if (s.few) {
-        p.ml = reinterpret_cast<float2*>(ws + s.few_ml), p.part = reinterpret_cast<float*>(ws + s.few_part);
-        const int rc = s.few_rows == 16 ? paged_few<T, D, 1>(p, c, s, kv_heads, pdl != 0, stream) : paged_few<T, D, 2>(p, c, s, kv_heads, pdl != 0, stream);
-        if (rc) return rc;
-    }
-    if (s.tiles) {
-        p.ml = reinterpret_cast<float2*>(ws + s.ml), p.part = reinterpret_cast<float*>(ws + s.part);
-        // behind the other kernels of this call it may be launched early whatever the caller's chain allows: it waits for them to end
-        ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D>, dim3(s.blocks * s.splits, kv_heads), dim3(kPtThreads), PtCfg<D>::kBytes, stream, pdl != 0 || s.few, p, c,
-                             words + kWaitAttnPaged));
-        if (s.splits > 1) ZL_CHECK_CUDA(launch(k_paged_attn_join<T, D>, dim3(s.blocks, kv_heads), dim3(256), 0, stream, true, p, c));
-    }
+    ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D>, dim3(s.ctas), dim3(kPtThreads), PtCfg<D>::kBytes, stream, pdl, p, c, maps[0], maps[1], box, words + kWaitAttnPaged));
+    if (s.ctas > 1)
+        ZL_CHECK_CUDA(launch(k_paged_join<T, D, PtKind, true>, dim3(s.ctas, kPtRows / kJoinRows), dim3(kJoinThreads), 0, stream, true, p, c, p.few, INT_MAX));
     return ZL_OK;
+}
+
+template <typename T, int D>
+static int paged_attention(PagedAttn p, const PagedCache& c, const PagedPlan& s, void* ws, bool pdl, zl_stream_t stream) {
+    p.few = !s.tiles ? INT_MAX : s.few ? kFewRows : 0;
+    int rc = ZL_OK;
+    if (s.few) rc = s.few_rows == 16 ? paged_few<T, D, 1>(p, c, s, ws, pdl, stream) : paged_few<T, D, 2>(p, c, s, ws, pdl, stream);
+    // behind the other kernels of this call it may be launched early whatever the caller's chain allows: it waits for them to end
+    if (rc == ZL_OK && s.tiles) rc = paged_tiles<T, D>(p, c, s, ws, pdl || s.few, stream);
+    return rc;
 }
 
 }  // namespace zl
@@ -122,8 +130,9 @@ extern "C" int zl_paged_attention(const void* q, const void* k_cache, const void
     ZL_CHECK_ARG(s.bytes == 0 || (workspace && workspace_bytes >= s.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0));
     const PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), num_pages, page_stride, row_stride, head_stride, page_table, ld_table, max_pages,
                           page_size, seqs, paged_divisor(page_size)};
-    const PagedAttn p = {q, out, seq_lens, q_starts, rows, heads, heads / kv_heads, window, scale * 1.4426950408889634f, 0, s.splits ? s.splits : 1,
-                         static_cast<float2*>(workspace), nullptr};
-    if (dtype == ZL_F16) return dim == 64 ? paged_attention<__half, 64>(p, c, s, kv_heads, pdl, stream) : paged_attention<__half, 128>(p, c, s, kv_heads, pdl, stream);
-    return dim == 64 ? paged_attention<__nv_bfloat16, 64>(p, c, s, kv_heads, pdl, stream) : paged_attention<__nv_bfloat16, 128>(p, c, s, kv_heads, pdl, stream);
+    const PagedAttn p = {q, out, seq_lens, q_starts, rows, heads, heads / kv_heads, window, scale * 1.4426950408889634f, 0, kv_heads, nullptr, nullptr};
+    if (dtype == ZL_F16)
+        return dim == 64 ? paged_attention<__half, 64>(p, c, s, workspace, pdl != 0, stream) : paged_attention<__half, 128>(p, c, s, workspace, pdl != 0, stream);
+    return dim == 64 ? paged_attention<__nv_bfloat16, 64>(p, c, s, workspace, pdl != 0, stream)
+                     : paged_attention<__nv_bfloat16, 128>(p, c, s, workspace, pdl != 0, stream);
 }

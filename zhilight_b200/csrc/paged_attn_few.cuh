@@ -23,74 +23,11 @@ struct PfCfg {
     static constexpr int kPitch = D + 8;                             // floats; of a row of a warp's output in its ring
 };
 
-// Tiles of a block, at least one: a block that sees nothing is written too
-__device__ __forceinline__ int paged_few_tiles(const PagedBlock& k) { return k.hi >= 0 ? k.hi / kPfKeys - k.lo / kPfKeys + 1 : 1; }
-
-struct PfPlace {
-    int hk, off, tiles;   // kv head; tile within the block, and how many that has
-    int start;            // the block's place in the line
-};
-
-// A warp's view of the line: sequence by sequence, in it kv head by kv head, in that block by block; 32 sequences at a time, one a lane.  Everything fits
-// 32 bits, which the entry point sees to.
-struct PfLine {
-    int size, kv_heads;           // rows of a block
-    int b0, before, mine, upto;   // first sequence in view and its place; tiles of a kv head of this lane's sequence, and up to and with it
-
-    __device__ __forceinline__ void view(const PagedAttn& p, const PagedCache& c) {
-        PagedBlock k;
-        k.seq = b0 + (threadIdx.x & 31);
-        mine = 0;
-        if (k.seq < c.seqs) {
-            const int n = paged_new(p, k.seq, k.first) * p.group;
-            if (n <= p.few)
-                for (k.row0 = 0; k.row0 < n; k.row0 += size) {
-                    k.rows = min(size, n - k.row0);
-                    paged_bounds(p, c, k);
-                    mine += paged_few_tiles(k);
-                }
-        }
-        upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, upto, o);
-            if ((int)(threadIdx.x & 31) >= o) upto += x;
-        }
-    }
-    // length of the line; the view is at its beginning then
-    __device__ __forceinline__ int begin(const PagedAttn& p, const PagedCache& c) {
-        int total = 0;
-        before = 0;
-        for (b0 = (c.seqs - 1) & ~31;; b0 -= 32) {
-            view(p, c);
-            total += __shfl_sync(0xffffffffu, upto, 31) * kv_heads;
-            if (b0 == 0) return total;
-        }
-    }
-    // the block at place w, which is in view or behind it
-    __device__ __forceinline__ void at(const PagedAttn& p, const PagedCache& c, int w, PagedBlock& k, PfPlace& place) {
-        unsigned hit;
-        while (!(hit = __ballot_sync(0xffffffffu, before + upto * kv_heads > w))) {
-            before += __shfl_sync(0xffffffffu, upto, 31) * kv_heads;
-            b0 += 32;
-            view(p, c);
-        }
-        const int src = __ffs(hit) - 1, each = __shfl_sync(0xffffffffu, mine, src);
-        int rem = w - before - __shfl_sync(0xffffffffu, upto - mine, src) * kv_heads;
-        place.hk = rem / each;
-        rem -= place.hk * each;
-        k.seq = b0 + src;
-        const int n = paged_new(p, k.seq, k.first) * p.group;
-        for (k.row0 = 0;; k.row0 += size) {
-            k.rows = min(size, n - k.row0);
-            paged_bounds(p, c, k);
-            place.tiles = paged_few_tiles(k);
-            if (rem < place.tiles) break;
-            rem -= place.tiles;
-        }
-        place.off = rem;
-        place.start = w - rem;
-    }
+// tiles of 64 keys; at least one: a block that sees nothing is written too
+template <int R>
+struct PfKind {
+    static constexpr int kRows = R;
+    static __device__ __forceinline__ int units(const PagedBlock& k) { return k.hi >= 0 ? k.hi / kPfKeys - k.lo / kPfKeys + 1 : 1; }
 };
 
 __device__ __forceinline__ void pf_ldsm(uint32_t (&r)[4], uint32_t addr) {
@@ -115,32 +52,9 @@ __device__ __forceinline__ uint32_t pf_pack(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(two);
 }
 
-// Row r of a block, D columns from `o`(e) of this lane, E neighbouring ones each: rounded and stored, or done again where it is no number
-template <typename T, int D>
-__device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedCache& c, const PagedBlock& k, int hk, int r, float l, const float (&o)[D / 32]) {
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31, row = k.row0 + r, t = row / p.group, head = hk * p.group + row - t * p.group, place = k.place0 + t;
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    T v[E];
-    bool broken = false;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float x = l == 0.f ? 0.f : o[e] * inv;
-        broken |= x != x;
-        v[e] = from_f32<T>(x);
-    }
-    T* dst = static_cast<T*>(p.out) + ((size_t)(k.first + t) * p.heads + head) * D + lane * E;
-    if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
-    else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(v);
-    if (__any_sync(0xffffffffu, broken)) {
-        __syncwarp();
-        paged_row_exact<T, D>(p, c, k.seq, k.first + t, head, p.window ? max(0, place - p.window + 1) : 0, min(place, k.have - 1));
-    }
-}
-
 // grid: CTAs that share the line
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(const PagedAttn p, const PagedCache c, int kv_heads) {
+__global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(const PagedAttn p, const PagedCache c) {
     using C = PfCfg<D>;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int R = 16 * MT, CH = D / 8, KS = D / 16;
@@ -152,14 +66,14 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
     const uint32_t ring_at = smem_u32(ring);
     pdl_wait();
     pdl_trigger();   // behind the wait: the join reads lengths and starts ahead of its own
-    PfLine line;
-    line.size = R, line.kv_heads = kv_heads;
+    PagedLine<PfKind<R>> line;
+    line.kv_heads = p.kv_heads, line.above = 0, line.upto_rows = p.few;
     const int total = line.begin(p, c), per = cdiv(total, (int)gridDim.x), end = min(total, per * ((int)blockIdx.x + 1));
     for (int w = min(total, per * (int)blockIdx.x); w < end;) {
         PagedBlock k;
-        PfPlace at;
+        PagedPlace at;
         line.at(p, c, w, k, at);
-        const int count = min(end - w, at.tiles - at.off), key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + at.off) * kPfKeys + warp * 16;
+        const int count = min(end - w, at.units - at.off), key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + at.off) * kPfKeys + warp * 16;
         const long long head = (long long)at.hk * c.head_stride;
         // Copies of a stage: each lane has a chunk of some rows.  Lanes 0 - 15 ask for the page numbers of the 16 rows a stage ahead; where pages hold whole
         // 16s these are one page.
@@ -307,7 +221,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(mine + r * C::kPitch + n * 8 + t4 * 2) = make_float2(o[m][n][2 * u], o[m][n][2 * u + 1]);
             }
         __syncthreads();
-        const bool whole = count == at.tiles;
+        const bool whole = count == at.units;
         const size_t part = ((size_t)blockIdx.x * 2 + (at.off > 0 ? 0 : 1)) * R;
         for (int r = warp; r < k.rows; r += kPfWarps) {
             constexpr int E = D / 32;
@@ -333,52 +247,6 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
         }
         __syncthreads();   // the rings are the next block's
         w += count;
-    }
-}
-
-// Blocks that were cut: grid (the parts' CTAs).  CTA i joins the block that begins in stretch i of the line and goes on behind it: there is one at the most.
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kPfWarps * 32) k_paged_few_join(const PagedAttn p, const PagedCache c, int kv_heads) {
-    constexpr int R = 16 * MT, E = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i0 = blockIdx.x;
-    PfLine line;
-    line.size = R, line.kv_heads = kv_heads;
-    const int total = line.begin(p, c), per = cdiv(total, (int)gridDim.x), end = per * (i0 + 1);   // the first kernel has seen its predecessors end
-    PagedBlock k;
-    PfPlace at;
-    bool cut = end < total;
-    if (cut) {
-        line.at(p, c, end - 1, k, at);
-        cut = at.start >= per * i0 && at.start + at.tiles > end;   // else it begins in an earlier stretch, or ends here
-    }
-    pdl_trigger();
-    pdl_wait();
-    if (!cut) return;
-    const int parts = (at.start + at.tiles - 1) / per - i0 + 1;
-    auto place = [&](int s, int r) { return ((size_t)(i0 + s) * 2 + (s == 0)) * R + r; };
-    for (int r = warp; r < k.rows; r += kPfWarps) {
-        float m = -INFINITY, l = 0.f, v[E] = {};
-        for (int s = lane; s < parts; s += 32) m = fmaxf(m, p.ml[place(s, r)].x);
-        m = warp_max(m);
-        for (int s0 = 0; s0 < parts; s0 += 32) {
-            const float2 x = s0 + lane < parts ? p.ml[place(s0 + lane, r)] : make_float2(-INFINITY, 0.f);
-            const float f = s0 + lane < parts ? pf_exp2(x.x - m) : 0.f;
-            l += warp_sum(x.y * f);
-            const int n = min(32, parts - s0);
-#pragma unroll 8
-            for (int s = 0; s < n; ++s) {
-                const float w = __shfl_sync(0xffffffffu, f, s);
-                const float* from = p.part + place(s0 + s, r) * D + lane * E;
-                if constexpr (E == 4) {
-                    const float4 y = *reinterpret_cast<const float4*>(from);
-                    v[0] = fmaf(y.x, w, v[0]), v[1] = fmaf(y.y, w, v[1]), v[2] = fmaf(y.z, w, v[2]), v[3] = fmaf(y.w, w, v[3]);
-                } else {
-                    const float2 y = *reinterpret_cast<const float2*>(from);
-                    v[0] = fmaf(y.x, w, v[0]), v[1] = fmaf(y.y, w, v[1]);
-                }
-            }
-        }
-        paged_row_out<T, D>(p, c, k, at.hk, r, l, v);
     }
 }
 
