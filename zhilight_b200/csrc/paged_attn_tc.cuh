@@ -4,9 +4,10 @@
 // blocks stand in one line that the CTAs, one per SM, share out evenly (paged_attn.cuh).
 //
 //   warps 0-3, 4-7  softmax of a tile each: thread = row = lane of tensor memory; running maximum and sum in 32 bits; probabilities go back over the scores
-//   warp 8          one thread issues S = Q K^T and O += P V (P from tensor memory, V as it lies: rows of keys, the B operand along n) of both tiles
-//   warp 9          K and V from the pages into a ring of tiles by TMA, a box for the rows of a tile that one page has; where that is no multiple of 8
-//                   rows, of the swizzle's period, warps 9-11 copy 16 bytes at a time
+//   warp 8          one thread issues S = Q K^T of both tiles, 64 keys at a time into two buffers each
+//   warp 9          one thread issues O += P V of both tiles (P from tensor memory, V as it lies: rows of keys, the B operand along n)
+//   warp 10         K and V from the pages into a ring of tiles by TMA, a box for the rows of a tile that one page has; where that is no multiple of 8
+//                   rows, of the swizzle's period, warps 10 and 11 copy 16 bytes at a time
 //
 // A page's rows behind the last visible key may hold anything.  Copies of 16 bytes leave them out; behind TMA the softmax's threads make those values zeros
 // before they hand the tile's probabilities on.  Rows behind a page number outside the pool are zeros either way.  Tensor memory: scores of the two tiles (128 columns each, probabilities over their first
@@ -24,7 +25,7 @@
 
 namespace zl {
 
-constexpr int kPtRows = 256, kPtKeys = 128, kPtThreads = 384, kPtWarpMma = 8, kPtWarpLoad = 9, kPtLoaders = 96;
+constexpr int kPtRows = 256, kPtKeys = 128, kPtHalf = 64, kPtThreads = 384, kPtWarpS = 8, kPtWarpO = 9, kPtWarpLoad = 10, kPtLoaders = 64;
 
 // turns of a block, at least one: a block that sees nothing is written too
 struct PtKind {
@@ -63,18 +64,18 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     constexpr int CH = D / 8;
     extern __shared__ uint8_t pt_smem[];
     uint8_t* smem = pt_smem + ((1024u - (smem_u32(pt_smem) & 1023u)) & 1023u);
-    __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2], p_full[2], o_done[2];
+    __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2][2], p_full[2][2], o_done[2][2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     volatile int* s_abort = &s_gave_up;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], box ? 1 : kPtLoaders), mbar_init(&empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_done[i], 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&s_full[i >> 1][i & 1], 1), mbar_init(&p_full[i >> 1][i & 1], 4), mbar_init(&o_done[i >> 1][i & 1], 1);
         s_gave_up = 0;
         mbar_fence_init();
     }
-    if (warp == kPtWarpMma) {
+    if (warp == kPtWarpS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "n"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -87,7 +88,9 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     PagedLine<PtKind> line;
     line.kv_heads = p.kv_heads, line.above = p.few, line.upto_rows = 0x7fffffff;
     const int total = line.begin(p, c), per = cdiv(total, (int)gridDim.x), end = min(total, per * ((int)blockIdx.x + 1));
-    int turn = 0, ring = 0;   // of the blocks before: turns, tiles of the ring
+    // Of the blocks before: turns, tiles of the ring.  Every barrier's phases are waited for by each of its waiters without a gap, or a later one cannot end
+    // before the waiter has gone on: a phase is told from its neighbours by its parity alone.
+    int turn = 0, ring = 0;
     bool ok = true;           // no wait has given up
     for (int w = min(total, per * (int)blockIdx.x), count; w < end; w += count) {
         PagedBlock k;
@@ -96,7 +99,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
         count = min(end - w, at.units - at.off);
         const bool two_rows = k.rows > kPaRows;                        // two row tiles; else two key tiles
         const int t0 = (k.hi >= 0 ? k.lo / kPtKeys : 0) + (two_rows ? at.off : 2 * at.off), items = two_rows ? 2 : 4;   // of the ring in a turn
-        if (warp < kPtWarpMma) {
+        if (warp < kPtWarpS) {
             asm volatile("bar.sync 3, 256;" ::: "memory");             // the block before has been written
             // rows of q, [64 of d][row][128 B] with the chunks xor the row; rows behind the last one are zeros
             const int ch = tid % CH;
@@ -111,7 +114,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             pa_fence_async();
-            asm volatile("bar.sync 1, 288;" ::: "memory");
+            asm volatile("bar.sync 1, 320;" ::: "memory");
             const int m = warp >> 2, r = two_rows ? tid : tid & (kPaRows - 1);   // tile; row of the block
             const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = taddr + (uint32_t)(m * 128), to = taddr + (uint32_t)(C::kO + m * D);
             constexpr float kTau = kHalf ? 5.f : 8.f, kUp = kHalf ? 10.f : 0.f;
@@ -120,36 +123,39 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             const int hi = r < k.rows ? min(place, k.have - 1) : -1, lo = r < k.rows && p.window ? max(0, place - p.window + 1) : 0;
             const int key0 = (t0 + (two_rows ? 0 : m)) * kPtKeys, step = two_rows ? kPtKeys : 2 * kPtKeys;
             float l = 0.f, m_ref = -1.4426950e20f;
-            for (int j = 0; j < count; ++j) {
-                const int h = hi - (key0 + j * step), from_ = lo - (key0 + j * step);   // this row sees from_ .. h of the tile
-                if (!tc2_wait(&s_full[m], (uint32_t)(turn + j) & 1u, s_abort, err, 0x5600 + m)) break;
+            for (int j = 0; j < 2 * count; ++j) {                      // 64 keys
+                const int b = j & 1, base = key0 + (j >> 1) * step + b * kPtHalf, h = hi - base, from_ = lo - base;   // this row sees from_ .. h of them
+                const uint32_t tb = ts + (uint32_t)(b * kPtHalf);
+                if (!tc2_wait(&s_full[m][b], (uint32_t)(turn + (j >> 1)) & 1u, s_abort, err, 0x5600 + m)) break;
                 tc_fence_after();
-                uint32_t raw[kPtKeys];
+                uint32_t raw[kPtHalf];
 #pragma unroll
-                for (int i = 0; i < kPtKeys; i += 32) pa_ld32(ts + i, raw + i);
+                for (int i = 0; i < kPtHalf; i += 32) pa_ld32(tb + i, raw + i);
                 pa_wait_ld();
-                if (!__all_sync(0xffffffffu, h >= kPtKeys - 1 && from_ <= 0)) {
+                if (!__all_sync(0xffffffffu, h >= kPtHalf - 1 && from_ <= 0)) {
                     const unsigned span = h >= from_ ? (unsigned)(h - from_) : 0u, from = h >= from_ ? (unsigned)from_ : 0x40000000u;
 #pragma unroll
-                    for (int i = 0; i < kPtKeys; ++i)
+                    for (int i = 0; i < kPtHalf; ++i)
                         if ((unsigned)i - from > span) raw[i] = 0xff800000u;
                 }
                 float mx[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(raw[i]);
 #pragma unroll
-                for (int i = 4; i < kPtKeys - 4; i += 8)
+                for (int i = 4; i < kPtHalf - 4; i += 8)
 #pragma unroll
                     for (int u = 0; u < 4; ++u) mx[u] = pa_max3(mx[u], __uint_as_float(raw[i + 2 * u]), __uint_as_float(raw[i + 2 * u + 1]));
-                mx[0] = pa_max3(mx[0], __uint_as_float(raw[kPtKeys - 4]), __uint_as_float(raw[kPtKeys - 3]));
-                mx[1] = pa_max3(mx[1], __uint_as_float(raw[kPtKeys - 2]), __uint_as_float(raw[kPtKeys - 1]));
+                mx[0] = pa_max3(mx[0], __uint_as_float(raw[kPtHalf - 4]), __uint_as_float(raw[kPtHalf - 3]));
+                mx[1] = pa_max3(mx[1], __uint_as_float(raw[kPtHalf - 2]), __uint_as_float(raw[kPtHalf - 1]));
                 const float m_tile = pa_max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * cs;
                 const bool up = m_tile > m_ref + kTau;
                 if (__any_sync(0xffffffffu, up)) {
                     const float f = up ? pa_exp2(m_ref - m_tile) : 1.f;
                     if (up) m_ref = m_tile;
                     l *= f;
-                    if (j > 0) {   // P V of the turn before has ended: these scores were issued behind it
+                    if (j > 0) {
+                        if (!tc2_wait(&o_done[m][b ^ 1], (uint32_t)(turn + ((j - 1) >> 1)) & 1u, s_abort, err, 0x5680 + m)) break;   // P V of the keys before
+                        tc_fence_after();
 #pragma unroll 1
                         for (int d0 = 0; d0 < D; d0 += 16) {
                             float v[16];
@@ -164,33 +170,33 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 const uint64_t c2 = pa_two(cs, cs), m2 = pa_two(kUp - m_ref, kUp - m_ref);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int part = 0; part < kPtKeys; part += 32) {
+                for (int part = 0; part < kPtHalf; part += 32) {
                     uint32_t x[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        float a, b;
-                        pa_split(pa_fma2(pa_two(__uint_as_float(raw[part + 2 * i]), __uint_as_float(raw[part + 2 * i + 1])), c2, m2), a, b);
+                        float a, e;
+                        pa_split(pa_fma2(pa_two(__uint_as_float(raw[part + 2 * i]), __uint_as_float(raw[part + 2 * i + 1])), c2, m2), a, e);
                         a = pa_exp2(a);
-                        b = pa_exp2(b);
-                        sum[i & 1] = pa_add2(sum[i & 1], pa_two(a, b));
+                        e = pa_exp2(e);
+                        sum[i & 1] = pa_add2(sum[i & 1], pa_two(a, e));
                         if constexpr (kHalf) {
-                            const __half2 y = __floats2half2_rn(a, b);
+                            const __half2 y = __floats2half2_rn(a, e);
                             x[i] = *reinterpret_cast<const uint32_t*>(&y);
                         } else {
-                            const __nv_bfloat162 y = __floats2bfloat162_rn(a, b);
+                            const __nv_bfloat162 y = __floats2bfloat162_rn(a, e);
                             x[i] = *reinterpret_cast<const uint32_t*>(&y);
                         }
                     }
-                    tc_st16(ts + (uint32_t)(part / 2), x);
+                    tc_st16(tb + (uint32_t)(part / 2), x);
                 }
                 float s0, s1;
                 pa_split(pa_add2(sum[0], sum[1]), s0, s1);
                 l += s0 + s1;
                 // The tile with the last visible key, where that ends within a box: values behind it become zeros.  Of two row tiles the first sees to it, whose
                 // product comes first.  The tile is there or on its way: the ring's tiles before it have been used.
-                const int behind = k.hi + 1 - (key0 + j * step);
-                if (box && behind > 0 && behind < kPtKeys && behind % box != 0 && (m == 0 || !two_rows)) {
-                    const int it = ring + j * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
+                const int behind = k.hi + 1 - base;
+                if (box && b == 0 && behind > 0 && behind < kPtKeys && behind % box != 0 && (m == 0 || !two_rows)) {
+                    const int it = ring + (j >> 1) * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
                     if (!tc2_wait(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5800 + slot)) break;
                     const int r1 = (behind + box - 1) / box * box;   // further boxes are zeros already
                     for (int x = tid & (kPaRows - 1); x < (r1 - behind) * CH; x += kPaRows) {
@@ -202,9 +208,9 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[m]);
+                if (lane == 0) mbar_arrive(&p_full[m][b]);
             }
-            tc2_wait(&o_done[m], (uint32_t)(turn + count - 1) & 1u, s_abort, err, 0x5700 + m);
+            for (int b = 0; b < 2; ++b) tc2_wait(&o_done[m][b], (uint32_t)(turn + count - 1) & 1u, s_abort, err, 0x5700 + m);
             tc_fence_after();
             if (count < at.units) {
                 // a part: {maximum, sum}, then the output as it stands
@@ -277,49 +283,56 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 }
             }
             tc_fence_before();   // the next block's products write where this one's results were read
-        } else if (warp == kPtWarpMma) {
-            asm volatile("bar.sync 1, 288;" ::: "memory");
+        } else if (warp == kPtWarpS) {
+            asm volatile("bar.sync 1, 320;" ::: "memory");
             if (tc_elect_one()) {
-                constexpr uint32_t id_s = pa_idesc(!kHalf, kPtKeys, false), id_o = pa_idesc(!kHalf, D, true);
-                auto scores = [&](int m, int j) {
-                    const int it = ring + j * items + (two_rows ? 0 : m), slot = it % C::kRing;
-                    ok = ok && tc2_wait1(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5100 + slot);
-                    if (!ok) return;
-                    pa_fence_async();
-                    tc_fence_after();
-                    const uint64_t qd = tc_desc_sw128(smem_u32(smem + (two_rows ? m : 0) * C::kQ)), kd = tc_desc_sw128(smem_u32(smem + C::kRingOff + slot * C::kTile));
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-                        pa_mma_ss(tmem + (uint32_t)(m * 128), qd + (uint64_t)((i >> 2) * (kPaRows * 128 / 16) + (i & 3) * 2),
-                                  kd + (uint64_t)((i >> 2) * (kPtKeys * 128 / 16) + (i & 3) * 2), id_s, i > 0 ? 1u : 0u);
-                    tc_commit(&s_full[m]);
-                    if (m == 1 || !two_rows) tc_commit(&empty[slot]);
-                };
-                auto values = [&](int m, int j) {
-                    const int it = ring + j * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
-                    ok = ok && tc2_wait1(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5200 + slot);
-                    ok = ok && tc2_wait1(&p_full[m], (uint32_t)(turn + j) & 1u, s_abort, err, 0x5300 + m);
-                    if (!ok) return;
-                    pa_fence_async();
-                    tc_fence_after();
-                    const uint64_t vd = pa_desc_mn(smem_u32(smem + C::kRingOff + slot * C::kTile), kPtKeys * 128);
-#pragma unroll
-                    for (int i = 0; i < kPtKeys / 16; ++i)
-                        pa_mma_ts(tmem + (uint32_t)(C::kO + m * D), tmem + (uint32_t)(m * 128 + i * 8), vd + (uint64_t)(i * (16 * 128 / 16)), id_o,
-                                  (j > 0 || i > 0) ? 1u : 0u);
-                    tc_commit(&o_done[m]);
-                    if (m == 1 || !two_rows) tc_commit(&empty[slot]);
-                };
-                scores(0, 0);
-                scores(1, 0);
-                for (int j = 0; j < count && ok; ++j)
+                constexpr uint32_t id = pa_idesc(!kHalf, kPtHalf, false);
+                const uint64_t qd = tc_desc_sw128(smem_u32(smem));
+                // The scores of 64 keys come under the softmax of the 64 before; they lie over the probabilities of those before these, which P V has to have read.
+                for (int j = 0; j < 2 * count && ok; ++j)
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
-                        values(m, j);
-                        if (j + 1 < count) {   // over the probabilities that P V has read
-                            ok = ok && tc2_wait1(&o_done[m], (uint32_t)(turn + j) & 1u, s_abort, err, 0x5400 + m);
-                            scores(m, j + 1);
+                        const int it = ring + (j >> 1) * items + (two_rows ? 0 : m), slot = it % C::kRing;
+                        if (!(j & 1) && (m == 0 || !two_rows)) {
+                            ok = ok && tc2_wait1(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5100 + slot);
+                            if (!box) pa_fence_async();
                         }
+                        if (j > 1) ok = ok && tc2_wait1(&o_done[m][j & 1], (uint32_t)(turn + (j >> 1) - 1) & 1u, s_abort, err, 0x5400 + m);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t kd = tc_desc_sw128(smem_u32(smem + C::kRingOff + slot * C::kTile + (j & 1) * (kPtHalf * 128)));
+                        const uint64_t qm = qd + (uint64_t)((two_rows ? m : 0) * (C::kQ / 16));
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i)
+                            pa_mma_ss(tmem + (uint32_t)(m * 128 + (j & 1) * kPtHalf), qm + (uint64_t)((i >> 2) * (kPaRows * 128 / 16) + (i & 3) * 2),
+                                      kd + (uint64_t)((i >> 2) * (kPtKeys * 128 / 16) + (i & 3) * 2), id, i > 0 ? 1u : 0u);
+                        tc_commit(&s_full[m][j & 1]);
+                        if ((j & 1) && (m == 1 || !two_rows)) tc_commit(&empty[slot]);
+                    }
+            }
+            __syncwarp();
+        } else if (warp == kPtWarpO) {
+            asm volatile("bar.sync 1, 320;" ::: "memory");
+            if (tc_elect_one()) {
+                constexpr uint32_t id = pa_idesc(!kHalf, D, true);
+                for (int j = 0; j < 2 * count && ok; ++j)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        const int it = ring + (j >> 1) * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
+                        if (!(j & 1) && (m == 0 || !two_rows)) {
+                            ok = ok && tc2_wait1(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5200 + slot);
+                            if (!box) pa_fence_async();
+                        }
+                        ok = ok && tc2_wait1(&p_full[m][j & 1], (uint32_t)(turn + (j >> 1)) & 1u, s_abort, err, 0x5300 + m);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t vd = pa_desc_mn(smem_u32(smem + C::kRingOff + slot * C::kTile + (j & 1) * (kPtHalf * 128)), kPtKeys * 128);
+#pragma unroll
+                        for (int i = 0; i < kPtHalf / 16; ++i)
+                            pa_mma_ts(tmem + (uint32_t)(C::kO + m * D), tmem + (uint32_t)(m * 128 + (j & 1) * kPtHalf + i * 8), vd + (uint64_t)(i * (16 * 128 / 16)), id,
+                                      (j > 0 || i > 0) ? 1u : 0u);
+                        tc_commit(&o_done[m][j & 1]);
+                        if ((j & 1) && (m == 1 || !two_rows)) tc_commit(&empty[slot]);
                     }
             }
             __syncwarp();
@@ -362,11 +375,10 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 const uint32_t to = smem_u32(smem) + (uint32_t)(C::kRingOff + slot * C::kTile + (ch >> 3) * (kPtKeys * 128));
 #pragma unroll
                 for (int u = 0; u < kPtKeys / 32; ++u)
-                    for (int x = (warp - kPtWarpLoad) * kRowsAtOnce; x < 32; x += 3 * kRowsAtOnce) {
+                    for (int x = (warp - kPtWarpLoad) * kRowsAtOnce; x < 32; x += 2 * kRowsAtOnce) {
                         const int r = x + lane / CH;
-                        const long long off = __shfl_sync(0xffffffffu, offs[u], r);   // r below 32: the step divides what is left, or lanes repeat a row
-                        if (x + lane / CH < 32)
-                            pa_cp16(to + (uint32_t)((u * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4)), from + (off < 0 ? 0 : off), off >= 0);
+                        const long long off = __shfl_sync(0xffffffffu, offs[u], r);
+                        pa_cp16(to + (uint32_t)((u * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4)), from + (off < 0 ? 0 : off), off >= 0);
                     }
                 pa_landed(&full[slot]);
             }
@@ -378,7 +390,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     tc2_drain(s_abort);
     tc_fence_before();
     __syncthreads();
-    if (warp == kPtWarpMma) {
+    if (warp == kPtWarpS) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
     }
