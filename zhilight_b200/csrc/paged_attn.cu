@@ -130,7 +130,7 @@ extern "C" int zl_paged_attention(const void* q, const void* k_cache, const void
     ZL_CHECK_ARG(s.bytes == 0 || (workspace && workspace_bytes >= s.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0));
     const PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), num_pages, page_stride, row_stride, head_stride, page_table, ld_table, max_pages,
                           page_size, seqs, paged_divisor(page_size)};
-    const PagedAttn p = {q, out, seq_lens, q_starts, rows, heads, heads / kv_heads, window, scale * 1.4426950408889634f, 0, kv_heads, nullptr, nullptr};
+    const PagedAttn p = {q, out, seq_lens, q_starts, rows, heads, heads / kv_heads, window, paged_divisor(heads / kv_heads), scale * 1.4426950408889634f, 0, kv_heads, nullptr, nullptr};
     if (dtype == ZL_F16)
         return dim == 64 ? paged_attention<__half, 64>(p, c, s, workspace, pdl != 0, stream) : paged_attention<__half, 128>(p, c, s, workspace, pdl != 0, stream);
     return dim == 64 ? paged_attention<__nv_bfloat16, 64>(p, c, s, workspace, pdl != 0, stream)

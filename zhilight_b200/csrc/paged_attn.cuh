@@ -9,6 +9,7 @@ struct PagedAttn {
     void* out;
     const int32_t *lens, *starts;
     int rows, heads, group, window;   // group: heads of a kv head
+    PagedDivisor by_group;
     float scale;                      // times log2(e)
     int few, kv_heads;                // sequences of up to so many (token, head) rows of a kv head go to the kernel for few rows
     float2* ml;                       // parts of blocks that were cut, two places for every CTA: {maximum, sum} of their rows, and the rows
@@ -32,7 +33,7 @@ __device__ __forceinline__ int paged_new(const PagedAttn& p, int b, int& first) 
 
 // What the block's rows see
 __device__ __forceinline__ void paged_sees(const PagedAttn& p, PagedBlock& k) {
-    const int t0 = k.row0 / p.group, t1 = (k.row0 + k.rows - 1) / p.group;
+    const int t0 = p.by_group(k.row0), t1 = p.by_group(k.row0 + k.rows - 1);
     k.hi = min(k.place0 + t1, k.have - 1);
     k.lo = p.window ? max(0, k.place0 + t0 - p.window + 1) : 0;
     if (k.lo > k.hi) k.hi = -1, k.lo = 0;
@@ -50,42 +51,57 @@ struct PagedPlace {
 };
 
 // A warp's view of the line that the blocks of a kernel's work stand in: sequence by sequence, in it kv head by kv head, in that block by block, each
-// block KIND::units() long.  A CTA of the grid takes an equal stretch of the line.  128 sequences are in view at a time, four to a lane.  Everything fits 32
-// bits, which the entry point sees to.
+// block KIND::units() long.  A CTA of the grid takes an equal stretch of the line.  128 sequences are in view at a time, four to a lane; the blocks of a
+// sequence that has many are looked at by the whole warp.  Everything fits 32 bits, which the entry point sees to.
 template <typename KIND>
 struct PagedLine {
+    static constexpr int kAlone = 4;   // blocks of a sequence that a lane looks at by itself
     int kv_heads, above, upto_rows;   // sequences of more than `above` and up to `upto_rows` (token, head) rows of a kv head are in it
     int b0, before, upto, cum[4];     // first sequence in view and its place; units of a kv head up to and with this lane's, and of this lane's four
 
+    // units of the blocks of a sequence from `from` on, every `step`-th
+    __device__ __forceinline__ int sum(const PagedAttn& p, PagedBlock& k, int n, int from, int step) {
+        int units = 0;
+        for (k.row0 = from * KIND::kRows; k.row0 < n; k.row0 += step * KIND::kRows) {
+            k.rows = min(KIND::kRows, n - k.row0);
+            paged_sees(p, k);
+            units += KIND::units(k);
+        }
+        return units;
+    }
     __device__ __forceinline__ void view(const PagedAttn& p, const PagedCache& c) {
-        const int b = b0 + (threadIdx.x & 31) * 4;
+        const int lane = threadIdx.x & 31, b = b0 + lane * 4;
         int at[5], len[4];
 #pragma unroll
         for (int u = 0; u < 5; ++u) at[u] = b + u <= c.seqs ? p.starts[b + u] : 0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) len[u] = b + u < c.seqs ? p.lens[b + u] : 0;
-        int sum = 0;
+        int all = 0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             PagedBlock k;
             k.first = max(at[u], 0);
-            const int n = b + u < c.seqs ? max(min(at[u + 1], p.rows) - k.first, 0) * p.group : 0;
-            if (n > above && n <= upto_rows) {
-                k.place0 = len[u] - at[u + 1] + k.first;
-                k.have = min(max(len[u], 0), c.room());
-                for (k.row0 = 0; k.row0 < n; k.row0 += KIND::kRows) {
-                    k.rows = min(KIND::kRows, n - k.row0);
-                    paged_sees(p, k);
-                    sum += KIND::units(k);
-                }
+            int n = b + u < c.seqs ? max(min(at[u + 1], p.rows) - k.first, 0) * p.group : 0;
+            if (n <= above || n > upto_rows) n = 0;
+            k.place0 = len[u] - at[u + 1] + k.first;
+            k.have = min(max(len[u], 0), c.room());
+            const bool many = n > kAlone * KIND::kRows;
+            int units = many ? 0 : sum(p, k, n, 0, 1);
+            for (unsigned left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
+                const int src = __ffs(left) - 1;
+                PagedBlock o;
+                o.place0 = __shfl_sync(0xffffffffu, k.place0, src), o.have = __shfl_sync(0xffffffffu, k.have, src);
+                const int x = __reduce_add_sync(0xffffffffu, sum(p, o, __shfl_sync(0xffffffffu, n, src), lane, 32));
+                if (lane == src) units = x;
             }
-            cum[u] = sum;
+            all += units;
+            cum[u] = all;
         }
-        upto = sum;
+        upto = all;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, upto, o);
-            if ((int)(threadIdx.x & 31) >= o) upto += x;
+            if (lane >= o) upto += x;
         }
     }
     // length of the line; the view is at its beginning then
@@ -100,6 +116,7 @@ struct PagedLine {
     }
     // the block at place w, which is in view or behind it
     __device__ __forceinline__ void at(const PagedAttn& p, const PagedCache& c, int w, PagedBlock& k, PagedPlace& place) {
+        const int lane = threadIdx.x & 31;
         unsigned hit;
         while (!(hit = __ballot_sync(0xffffffffu, before + upto * kv_heads > w))) {
             before += __shfl_sync(0xffffffffu, upto, 31) * kv_heads;
@@ -121,12 +138,31 @@ struct PagedLine {
         rem -= place.hk * each;
         k.seq = b0 + src * 4 + u;
         const int n = paged_new(p, k.seq, k.first) * p.group;
-        for (k.row0 = 0;; k.row0 += KIND::kRows) {
-            k.rows = min(KIND::kRows, n - k.row0);
-            paged_bounds(p, c, k);
-            place.units = KIND::units(k);
-            if (rem < place.units) break;
-            rem -= place.units;
+        k.row0 = 0, k.rows = min(KIND::kRows, n);
+        paged_bounds(p, c, k);
+        place.units = KIND::units(k);
+        // 32 blocks at a time
+        for (int i0 = 0; n > KIND::kRows; i0 += 32) {
+            PagedBlock o = k;
+            o.row0 = (i0 + lane) * KIND::kRows, o.rows = min(KIND::kRows, n - o.row0);
+            int mine = 0;
+            if (o.row0 < n) paged_sees(p, o), mine = KIND::units(o);
+            int up = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, up, d);
+                if (lane >= d) up += x;
+            }
+            const unsigned here = __ballot_sync(0xffffffffu, up > rem);
+            if (here) {
+                const int l = __ffs(here) - 1;
+                rem -= __shfl_sync(0xffffffffu, up - mine, l);
+                k.row0 = (i0 + l) * KIND::kRows, k.rows = min(KIND::kRows, n - k.row0);
+                paged_sees(p, k);
+                place.units = KIND::units(k);
+                break;
+            }
+            rem -= __shfl_sync(0xffffffffu, up, 31);
         }
         place.off = rem;
         place.start = w - rem;
@@ -138,7 +174,7 @@ template <typename T, int D>
 __device__ __noinline__ void paged_row_exact(const PagedAttn& p, const PagedCache& c, int seq, int t, int h, int lo, int hi) {
     constexpr int E = D / 32;
     const int lane = threadIdx.x & 31;
-    const long long head = (long long)(h / p.group) * c.head_stride + lane;
+    const long long head = (long long)p.by_group(h) * c.head_stride + lane;
     const size_t row = ((size_t)t * p.heads + h) * D + lane;
     float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -164,7 +200,7 @@ __device__ __noinline__ void paged_row_exact(const PagedAttn& p, const PagedCach
 template <typename T, int D>
 __device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedCache& c, const PagedBlock& k, int hk, int r, float l, const float (&o)[D / 32]) {
     constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31, row = k.row0 + r, t = row / p.group, head = hk * p.group + row - t * p.group, place = k.place0 + t;
+    const int lane = threadIdx.x & 31, row = k.row0 + r, t = p.by_group(row), head = hk * p.group + row - t * p.group, place = k.place0 + t;
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     T v[E];
     bool broken = false;

@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
             for (int u = 0; u < 2; ++u) {
                 const int r = m * 16 + g + u * 8;
                 const bool in = r < k.rows;
-                const int row = k.row0 + (in ? r : 0), t = row / p.group, place = k.place0 + t;
+                const int row = k.row0 + (in ? r : 0), t = p.by_group(row), place = k.place0 + t;
                 const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + ((size_t)(k.first + t) * p.heads + at.hk * p.group + row - t * p.group) * D);
                 hi[m][u] = in ? min(place, k.have - 1) : -1;
                 lo[m][u] = p.window ? max(0, place - p.window + 1) : 0;

@@ -108,7 +108,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 const int r = tid / CH + i * (256 / CH), rr = r & (kPaRows - 1);
                 if (r >= kPaRows && !two_rows) break;
                 const bool in = r < k.rows;
-                const int row = k.row0 + (in ? r : 0), t = row / p.group;
+                const int row = k.row0 + (in ? r : 0), t = p.by_group(row);
                 const T* src = static_cast<const T*>(p.q) + ((size_t)(k.first + t) * p.heads + at.hk * p.group + row - t * p.group) * D + ch * 8;
                 pa_cp16(smem_u32(smem) + (uint32_t)((r >> 7) * C::kQ + (ch >> 3) * (kPaRows * 128) + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)), src, in);
             }
@@ -119,7 +119,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = taddr + (uint32_t)(m * 128), to = taddr + (uint32_t)(C::kO + m * D);
             constexpr float kTau = kHalf ? 5.f : 8.f, kUp = kHalf ? 10.f : 0.f;
             const float cs = p.scale;
-            const int row = k.row0 + r, t = row / p.group, place = k.place0 + t;
+            const int row = k.row0 + r, t = p.by_group(row), place = k.place0 + t;
             const int hi = r < k.rows ? min(place, k.have - 1) : -1, lo = r < k.rows && p.window ? max(0, place - p.window + 1) : 0;
             const int key0 = (t0 + (two_rows ? 0 : m)) * kPtKeys, step = two_rows ? kPtKeys : 2 * kPtKeys;
             float l = 0.f, m_ref = -1.4426950e20f;
