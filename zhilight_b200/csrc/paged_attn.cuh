@@ -11,25 +11,21 @@ struct PagedAttn {
     int rows, heads, group, window;   // group: heads of a kv head
     PagedDivisor by_group;
     float scale;                      // times log2(e)
-    int few, kv_heads;                // sequences of up to so many (token, head) rows of a kv head go to the kernel for few rows
+    int kv_heads;
+    int block_rows, tile_rows;        // of a block; of one of its two tiles, 0 where blocks are one tile
     float2* ml;                       // parts of blocks that were cut, two places for every CTA: {maximum, sum} of their rows, and the rows
     float* part;
+    struct PagedCut* cuts;            // for every CTA
 };
 
 // One block of up to `size` (token, head) rows of a kv head of one sequence.
 struct PagedBlock {
-    int seq, first;      // its sequence, whose new tokens begin at row `first` of q
+    int seq, first, n;   // its sequence, whose new tokens begin at row `first` of q and make up n (token, head) rows
     int row0, rows;      // (token, head) rows of the block, token-major
     int place0;          // place of the sequence's first new token
     int have;            // keys of the sequence
     int lo, hi;          // keys that any row of the block sees; hi < 0: none
 };
-
-// The new tokens of sequence b, as far as q has them.
-__device__ __forceinline__ int paged_new(const PagedAttn& p, int b, int& first) {
-    first = max(p.starts[b], 0);
-    return max(min(p.starts[b + 1], p.rows) - first, 0);
-}
 
 // What the block's rows see
 __device__ __forceinline__ void paged_sees(const PagedAttn& p, PagedBlock& k) {
@@ -38,36 +34,30 @@ __device__ __forceinline__ void paged_sees(const PagedAttn& p, PagedBlock& k) {
     k.lo = p.window ? max(0, k.place0 + t0 - p.window + 1) : 0;
     if (k.lo > k.hi) k.hi = -1, k.lo = 0;
 }
-__device__ __forceinline__ void paged_bounds(const PagedAttn& p, const PagedCache& c, PagedBlock& k) {
-    const int len = p.lens[k.seq];
-    k.place0 = len - p.starts[k.seq + 1] + k.first;
-    k.have = min(max(len, 0), c.room());
-    paged_sees(p, k);
-}
-
 struct PagedPlace {
     int hk, off, units;   // kv head; unit within the block, and how many that has
     int start;            // the block's place in the line
 };
 
+// A block that begins in a CTA's stretch of the line and goes on in the next ones: there is one at the most
+struct PagedCut {
+    PagedBlock k;
+    int hk, parts;   // its kv head; stretches that have a part, 0: there is no such block
+};
+
 // A warp's view of the line that the blocks of a kernel's work stand in: sequence by sequence, in it kv head by kv head, in that block by block, each
-// block KIND::units() long.  A CTA of the grid takes an equal stretch of the line.  128 sequences are in view at a time, four to a lane; the blocks of a
+// KIND::units() long.  A CTA of the grid takes an equal stretch of the line.  128 sequences are in view at a time, four to a lane; the blocks of a
 // sequence that has many are looked at by the whole warp.  Everything fits 32 bits, which the entry point sees to.
 template <typename KIND>
 struct PagedLine {
     static constexpr int kAlone = 4;   // blocks of a sequence that a lane looks at by itself
-    int kv_heads, above, upto_rows;   // sequences of more than `above` and up to `upto_rows` (token, head) rows of a kv head are in it
-    int b0, before, upto, cum[4];     // first sequence in view and its place; units of a kv head up to and with this lane's, and of this lane's four
+    int total, per;                    // length of the line and of a stretch
+    int b0, before, upto, cum[4];      // first sequence in view and its place; units of a kv head up to and with this lane's, and of this lane's four
 
-    // units of the blocks of a sequence from `from` on, every `step`-th
-    __device__ __forceinline__ int sum(const PagedAttn& p, PagedBlock& k, int n, int from, int step) {
-        int units = 0;
-        for (k.row0 = from * KIND::kRows; k.row0 < n; k.row0 += step * KIND::kRows) {
-            k.rows = min(KIND::kRows, n - k.row0);
-            paged_sees(p, k);
-            units += KIND::units(k);
-        }
-        return units;
+    __device__ __forceinline__ int block(const PagedAttn& p, PagedBlock& k, int row0) {
+        k.row0 = row0, k.rows = min(p.block_rows, k.n - row0);
+        paged_sees(p, k);
+        return KIND::units(p, k);
     }
     __device__ __forceinline__ void view(const PagedAttn& p, const PagedCache& c) {
         const int lane = threadIdx.x & 31, b = b0 + lane * 4;
@@ -81,17 +71,20 @@ struct PagedLine {
         for (int u = 0; u < 4; ++u) {
             PagedBlock k;
             k.first = max(at[u], 0);
-            int n = b + u < c.seqs ? max(min(at[u + 1], p.rows) - k.first, 0) * p.group : 0;
-            if (n <= above || n > upto_rows) n = 0;
+            k.n = b + u < c.seqs ? max(min(at[u + 1], p.rows) - k.first, 0) * p.group : 0;
             k.place0 = len[u] - at[u + 1] + k.first;
             k.have = min(max(len[u], 0), c.room());
-            const bool many = n > kAlone * KIND::kRows;
-            int units = many ? 0 : sum(p, k, n, 0, 1);
+            const bool many = k.n > kAlone * p.block_rows;
+            int units = 0;
+            if (!many)
+                for (int r = 0; r < k.n; r += p.block_rows) units += block(p, k, r);
             for (unsigned left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
                 const int src = __ffs(left) - 1;
                 PagedBlock o;
-                o.place0 = __shfl_sync(0xffffffffu, k.place0, src), o.have = __shfl_sync(0xffffffffu, k.have, src);
-                const int x = __reduce_add_sync(0xffffffffu, sum(p, o, __shfl_sync(0xffffffffu, n, src), lane, 32));
+                o.place0 = __shfl_sync(0xffffffffu, k.place0, src), o.have = __shfl_sync(0xffffffffu, k.have, src), o.n = __shfl_sync(0xffffffffu, k.n, src);
+                int x = 0;
+                for (int r = lane * p.block_rows; r < o.n; r += 32 * p.block_rows) x += block(p, o, r);
+                x = __reduce_add_sync(0xffffffffu, x);
                 if (lane == src) units = x;
             }
             all += units;
@@ -104,49 +97,49 @@ struct PagedLine {
             if (lane >= o) upto += x;
         }
     }
-    // length of the line; the view is at its beginning then
-    __device__ __forceinline__ int begin(const PagedAttn& p, const PagedCache& c) {
-        int total = 0;
-        before = 0;
+    // length of the line, which `ctas` share; the view is at its beginning then
+    __device__ __forceinline__ void begin(const PagedAttn& p, const PagedCache& c, int ctas) {
+        total = before = 0;
         for (b0 = (c.seqs - 1) & ~127;; b0 -= 128) {
             view(p, c);
-            total += __shfl_sync(0xffffffffu, upto, 31) * kv_heads;
-            if (b0 == 0) return total;
+            total += __shfl_sync(0xffffffffu, upto, 31) * p.kv_heads;
+            if (b0 == 0) break;
         }
+        per = (total + ctas - 1) / ctas;
     }
     // the block at place w, which is in view or behind it
     __device__ __forceinline__ void at(const PagedAttn& p, const PagedCache& c, int w, PagedBlock& k, PagedPlace& place) {
         const int lane = threadIdx.x & 31;
         unsigned hit;
-        while (!(hit = __ballot_sync(0xffffffffu, before + upto * kv_heads > w))) {
-            before += __shfl_sync(0xffffffffu, upto, 31) * kv_heads;
+        while (!(hit = __ballot_sync(0xffffffffu, before + upto * p.kv_heads > w))) {
+            before += __shfl_sync(0xffffffffu, upto, 31) * p.kv_heads;
             b0 += 128;
             view(p, c);
         }
         const int src = __ffs(hit) - 1;
-        int rem = w - before - __shfl_sync(0xffffffffu, upto - cum[3], src) * kv_heads, each = 0, u = 0;
+        int rem = w - before - __shfl_sync(0xffffffffu, upto - cum[3], src) * p.kv_heads, each = 0, u = 0;
 #pragma unroll
         for (int v = 0, below = 0; v < 4; ++v) {
             const int x = __shfl_sync(0xffffffffu, cum[v], src) - below;   // units of this one
             if (each == 0) {
-                if (rem < x * kv_heads) each = x, u = v;
-                else rem -= x * kv_heads;
+                if (rem < x * p.kv_heads) each = x, u = v;
+                else rem -= x * p.kv_heads;
             }
             below += x;
         }
         place.hk = rem / each;
         rem -= place.hk * each;
         k.seq = b0 + src * 4 + u;
-        const int n = paged_new(p, k.seq, k.first) * p.group;
-        k.row0 = 0, k.rows = min(KIND::kRows, n);
-        paged_bounds(p, c, k);
-        place.units = KIND::units(k);
+        k.first = max(p.starts[k.seq], 0);
+        k.n = max(min(p.starts[k.seq + 1], p.rows) - k.first, 0) * p.group;
+        const int len = p.lens[k.seq];
+        k.place0 = len - p.starts[k.seq + 1] + k.first;
+        k.have = min(max(len, 0), c.room());
         // 32 blocks at a time
-        for (int i0 = 0; n > KIND::kRows; i0 += 32) {
+        int row0 = 0;
+        for (int r0 = 0; k.n > p.block_rows; r0 += 32 * p.block_rows) {
             PagedBlock o = k;
-            o.row0 = (i0 + lane) * KIND::kRows, o.rows = min(KIND::kRows, n - o.row0);
-            int mine = 0;
-            if (o.row0 < n) paged_sees(p, o), mine = KIND::units(o);
+            const int r = r0 + lane * p.block_rows, mine = r < k.n ? block(p, o, r) : 0;
             int up = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -157,15 +150,32 @@ struct PagedLine {
             if (here) {
                 const int l = __ffs(here) - 1;
                 rem -= __shfl_sync(0xffffffffu, up - mine, l);
-                k.row0 = (i0 + l) * KIND::kRows, k.rows = min(KIND::kRows, n - k.row0);
-                paged_sees(p, k);
-                place.units = KIND::units(k);
+                row0 = r0 + l * p.block_rows;
                 break;
             }
             rem -= __shfl_sync(0xffffffffu, up, 31);
         }
+        place.units = block(p, k, row0);
         place.off = rem;
         place.start = w - rem;
+    }
+    // the block behind this one, at place w
+    __device__ __forceinline__ void next(const PagedAttn& p, const PagedCache& c, int w, PagedBlock& k, PagedPlace& place) {
+        int row0 = k.row0 + p.block_rows;
+        if (row0 >= k.n) {
+            if (place.hk + 1 == p.kv_heads) return at(p, c, w, k, place);
+            row0 = 0, ++place.hk;
+        }
+        place.units = block(p, k, row0);
+        place.off = 0;
+        place.start = w;
+    }
+    // whether this block, of which `count` units are done here, is the one that CTA i's stretch cuts
+    __device__ __forceinline__ void cut(const PagedAttn& p, const PagedBlock& k, const PagedPlace& place, int count, int i) {
+        if (place.off == 0 && count < place.units) {
+            PagedCut x = {k, place.hk, (place.start + place.units - 1) / per - i + 1};
+            p.cuts[i] = x;
+        }
     }
 };
 
@@ -219,57 +229,46 @@ __device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedCac
     }
 }
 
-// Blocks that were cut.  grid (the CTAs of the first kernel, groups of kJoinRows rows): CTA i joins the block that begins in stretch i of the line and goes on
-// behind it -- there is one at the most.  Its first part lies in that CTA's place 1, the others in the place 0 of theirs.  HALVES: blocks of up to half
-// of KIND::kRows rows have two parts in a place, one behind the other.
-constexpr int kJoinRows = 16, kJoinThreads = 128;
-template <typename T, int D, typename KIND, bool HALVES>
-__global__ void __launch_bounds__(kJoinThreads) k_paged_join(const PagedAttn p, const PagedCache c, int above, int upto_rows) {
-    constexpr int R = KIND::kRows, E = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i0 = blockIdx.x;
-    PagedLine<KIND> line;
-    line.kv_heads = p.kv_heads, line.above = above, line.upto_rows = upto_rows;
-    const int total = line.begin(p, c), per = cdiv(total, (int)gridDim.x), end = per * (i0 + 1);   // the first kernel has seen its predecessors end
-    PagedBlock k;
-    PagedPlace at;
-    bool cut = end < total;
-    if (cut) {
-        line.at(p, c, end - 1, k, at);
-        cut = at.start >= per * i0 && at.start + at.units > end;   // else it begins in an earlier stretch, or ends here
-    }
+// Blocks that were cut.  grid (the CTAs of the first kernel, groups of kJoinRows rows), a warp a row: the first part of a block lies in its CTA's place 1,
+// the others in the place 0 of theirs, R rows each.  Of a block with two tiles of rows the second begins at row R / 2 of its place; one with a single tile
+// has two results in a place, the second there.
+constexpr int kJoinRows = 8;
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(kJoinRows * 32) k_paged_join(const PagedAttn p, const PagedCache c) {
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31, r = blockIdx.y * kJoinRows + (threadIdx.x >> 5);
     pdl_trigger();
     pdl_wait();
-    if (!cut) return;
-    const bool halves = HALVES && k.rows <= R / 2;
-    const int parts = ((at.start + at.units - 1) / per - i0 + 1) << (halves ? 1 : 0);
-    auto place = [&](int s, int r) {
-        const int i = halves ? s >> 1 : s;
-        return ((size_t)(i0 + i) * 2 + (i == 0)) * R + r + (halves && (s & 1) ? R / 2 : 0);
+    const PagedCut x = p.cuts[blockIdx.x];
+    if (x.parts == 0 || r >= x.k.rows) return;
+    const bool twice = p.tile_rows && x.k.rows <= p.tile_rows;
+    const int parts = twice ? 2 * x.parts : x.parts, row = p.tile_rows && r >= p.tile_rows ? r - p.tile_rows + R / 2 : r;
+    auto place = [&](int s) {
+        const int i = twice ? s >> 1 : s;
+        return ((size_t)(blockIdx.x + i) * 2 + (i == 0)) * R + row + (twice && (s & 1) ? R / 2 : 0);
     };
-    for (int r = blockIdx.y * kJoinRows + warp; r < min(k.rows, (int)(blockIdx.y + 1) * kJoinRows); r += kJoinThreads / 32) {
-        float m = -INFINITY, l = 0.f, v[E] = {};
-        for (int s = lane; s < parts; s += 32) m = fmaxf(m, p.ml[place(s, r)].x);
-        m = warp_max(m);
-        for (int s0 = 0; s0 < parts; s0 += 32) {
-            const float2 x = s0 + lane < parts ? p.ml[place(s0 + lane, r)] : make_float2(-INFINITY, 0.f);
-            const float f = s0 + lane < parts ? exp2f(x.x - m) : 0.f;
-            l += warp_sum(x.y * f);
-            const int n = min(32, parts - s0);
-#pragma unroll 4
-            for (int s = 0; s < n; ++s) {
-                const float w = __shfl_sync(0xffffffffu, f, s);
-                const float* from = p.part + place(s0 + s, r) * D + lane * E;
-                if constexpr (E == 4) {
-                    const float4 y = *reinterpret_cast<const float4*>(from);
-                    v[0] = fmaf(y.x, w, v[0]), v[1] = fmaf(y.y, w, v[1]), v[2] = fmaf(y.z, w, v[2]), v[3] = fmaf(y.w, w, v[3]);
-                } else {
-                    const float2 y = *reinterpret_cast<const float2*>(from);
-                    v[0] = fmaf(y.x, w, v[0]), v[1] = fmaf(y.y, w, v[1]);
-                }
+    float m = -INFINITY, l = 0.f, v[E] = {};
+    for (int s = lane; s < parts; s += 32) m = fmaxf(m, p.ml[place(s)].x);
+    m = warp_max(m);
+    for (int s0 = 0; s0 < parts; s0 += 32) {
+        const float2 y = s0 + lane < parts ? p.ml[place(s0 + lane)] : make_float2(-INFINITY, 0.f);
+        const float f = s0 + lane < parts ? exp2f(y.x - m) : 0.f;
+        l += warp_sum(y.y * f);
+        const int n = min(32, parts - s0);
+#pragma unroll 8
+        for (int s = 0; s < n; ++s) {
+            const float w = __shfl_sync(0xffffffffu, f, s);
+            const float* from = p.part + place(s0 + s) * D + lane * E;
+            if constexpr (E == 4) {
+                const float4 z = *reinterpret_cast<const float4*>(from);
+                v[0] = fmaf(z.x, w, v[0]), v[1] = fmaf(z.y, w, v[1]), v[2] = fmaf(z.z, w, v[2]), v[3] = fmaf(z.w, w, v[3]);
+            } else {
+                const float2 z = *reinterpret_cast<const float2*>(from);
+                v[0] = fmaf(z.x, w, v[0]), v[1] = fmaf(z.y, w, v[1]);
             }
         }
-        paged_row_out<T, D>(p, c, k, at.hk, r, l, v);
     }
+    paged_row_out<T, D>(p, c, x.k, x.hk, r, l, v);
 }
 
 }  // namespace zl

@@ -1,7 +1,7 @@
 // Attention of few (token, head) rows of a kv head -- single tokens, drafts of small groups -- over pages: bound by the bytes of K and V, which the CTAs
 // of the grid share out evenly, whatever the sequences' lengths are.  All tiles of 64 keys of all blocks (16 or 32 rows of one kv head of one sequence)
 // stand in one line; a CTA takes an equal stretch of it.  A block that lies in one stretch is written at once, the parts of one that is cut go to the
-// workspace, its first part to the CTA's place 1, others to its place 0, and k_paged_few_join puts them together.
+// workspace, its first part to the CTA's place 1, others to its place 0, and k_paged_join puts them together.
 //
 // A warp has 16 keys of a tile to itself, in a ring of its own (16-byte cp.async; no barrier between the warps until a block's end):
 // S = Q K^T and O += P V by mma.sync with Q as the 16-row operand, whose accumulators are the next product's operand as they stand.  The probabilities are
@@ -24,10 +24,8 @@ struct PfCfg {
 };
 
 // tiles of 64 keys; at least one: a block that sees nothing is written too
-template <int R>
 struct PfKind {
-    static constexpr int kRows = R;
-    static __device__ __forceinline__ int units(const PagedBlock& k) { return k.hi >= 0 ? k.hi / kPfKeys - k.lo / kPfKeys + 1 : 1; }
+    static __device__ __forceinline__ int units(const PagedAttn&, const PagedBlock& k) { return k.hi >= 0 ? k.hi / kPfKeys - k.lo / kPfKeys + 1 : 1; }
 };
 
 __device__ __forceinline__ void pf_ldsm(uint32_t (&r)[4], uint32_t addr) {
@@ -65,14 +63,16 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
     uint8_t* ring = pf_smem + warp * C::kWarp;
     const uint32_t ring_at = smem_u32(ring);
     pdl_wait();
-    pdl_trigger();   // behind the wait: the join reads lengths and starts ahead of its own
-    PagedLine<PfKind<R>> line;
-    line.kv_heads = p.kv_heads, line.above = 0, line.upto_rows = p.few;
-    const int total = line.begin(p, c), per = cdiv(total, (int)gridDim.x), end = min(total, per * ((int)blockIdx.x + 1));
-    for (int w = min(total, per * (int)blockIdx.x); w < end;) {
-        PagedBlock k;
-        PagedPlace at;
-        line.at(p, c, w, k, at);
+    pdl_trigger();
+    PagedLine<PfKind> line;
+    line.begin(p, c, (int)gridDim.x);
+    const int begin = min(line.total, line.per * (int)blockIdx.x), end = min(line.total, begin + line.per);
+    if (tid == 0) p.cuts[blockIdx.x].parts = 0;
+    PagedBlock k;
+    PagedPlace at;
+    for (int w = begin; w < end;) {
+        if (w == begin) line.at(p, c, w, k, at);
+        else line.next(p, c, w, k, at);
         const int count = min(end - w, at.units - at.off), key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + at.off) * kPfKeys + warp * 16;
         const long long head = (long long)at.hk * c.head_stride;
         // Copies of a stage: each lane has a chunk of some rows.  Lanes 0 - 15 ask for the page numbers of the 16 rows a stage ahead; where pages hold whole
@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 else *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
             }
         }
+        if (tid == 0) line.cut(p, k, at, count, (int)blockIdx.x);
         __syncthreads();   // the rings are the next block's
         w += count;
     }

@@ -1,13 +1,13 @@
-// Attention of many new tokens over pages on the 5th-generation tensor cores.  Blocks of up to 256 (token, head) rows of one kv head of one sequence, all
-// heads of the group beside one another, walk the keys of their rows in turns, two tiles of 128 rows x 128 keys a turn: the block's two row tiles over
-// the same keys, or, in a block of up to 128 rows, its one tile over two tiles of keys, whose results are joined at the end.  The turns of all
-// blocks stand in one line that the CTAs, one per SM, share out evenly (paged_attn.cuh).
+// Attention of many new tokens over pages on the 5th-generation tensor cores.  A tile is up to 128 (token, head) rows of one kv head of one sequence, whole
+// tokens with all heads of the group; blocks of one or two tiles walk the keys of their rows in turns, two tiles of 128 x 128 scores a turn: the block's two
+// row tiles over the same keys, or its one tile over two tiles of keys, whose results are joined at the end.  The turns of all blocks stand in one
+// line that the CTAs, one per SM, share out evenly (paged_attn.cuh).
 //
 //   warps 0-3, 4-7  softmax of a tile each: thread = row = lane of tensor memory; running maximum and sum in 32 bits; probabilities go back over the scores
 //   warp 8          one thread issues S = Q K^T of both tiles, 64 keys at a time into two buffers each
 //   warp 9          one thread issues O += P V of both tiles (P from tensor memory, V as it lies: rows of keys, the B operand along n)
-//   warp 10         K and V from the pages into a ring of tiles by TMA, a box for the rows of a tile that one page has; where that is no multiple of 8
-//                   rows, of the swizzle's period, warps 10 and 11 copy 16 bytes at a time
+//   warp 10         Q by TMA, once for a block; K and V from the pages into a ring of tiles by TMA, a box for the rows of a tile that one page has
+//                   (where that is no multiple of 8 rows, of the swizzle's period, warps 10 and 11 copy 16 bytes at a time)
 //
 // A page's rows behind the last visible key may hold anything.  Copies of 16 bytes leave them out; behind TMA the softmax's threads make those values zeros
 // before they hand the tile's probabilities on.  Rows behind a page number outside the pool are zeros either way.  Tensor memory: scores of the two tiles (128 columns each, probabilities over their first
@@ -29,10 +29,9 @@ constexpr int kPtRows = 256, kPtKeys = 128, kPtHalf = 64, kPtThreads = 384, kPtW
 
 // turns of a block, at least one: a block that sees nothing is written too
 struct PtKind {
-    static constexpr int kRows = kPtRows;
-    static __device__ __forceinline__ int units(const PagedBlock& k) {
+    static __device__ __forceinline__ int units(const PagedAttn& p, const PagedBlock& k) {
         const int tiles = k.hi >= 0 ? k.hi / kPtKeys - k.lo / kPtKeys + 1 : 1;
-        return k.rows > kPaRows ? tiles : (tiles + 1) >> 1;
+        return k.rows > p.tile_rows ? tiles : (tiles + 1) >> 1;
     }
 };
 
@@ -55,16 +54,29 @@ __device__ __forceinline__ void pt_load_4d(uint32_t dst, const CUtensorMap* map,
         : "memory");
 }
 
-// grid: CTAs that share the line.  box: rows of a TMA box, 0: no TMA
+__device__ __forceinline__ void pt_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
+// tc2_wait for a barrier whose phase has mostly ended by now: all lanes look once
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile int* s_abort, unsigned* err, unsigned code) {
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || tc2_wait(bar, parity, s_abort, err, code);
+}
+
+// grid: CTAs that share the line.  box: rows of a TMA box of K and V, 0: no TMA
 template <typename T, int D>
 __global__ void __launch_bounds__(kPtThreads, 1)
-k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, int box, unsigned* err) {
+k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                   const __grid_constant__ CUtensorMap v_map, int box, unsigned* err) {
     using C = PtCfg<D>;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int CH = D / 8;
     extern __shared__ uint8_t pt_smem[];
     uint8_t* smem = pt_smem + ((1024u - (smem_u32(pt_smem) & 1023u)) & 1023u);
-    __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2][2], p_full[2][2], o_done[2][2];
+    __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2][2], p_full[2][2], o_done[2][2], q_full, q_free, o_free, joined;
+    __shared__ float2 s_ml[kPaRows];
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     volatile int* s_abort = &s_gave_up;
@@ -72,6 +84,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     if (tid == 0) {
         for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], box ? 1 : kPtLoaders), mbar_init(&empty[i], 1);
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i >> 1][i & 1], 1), mbar_init(&p_full[i >> 1][i & 1], 4), mbar_init(&o_done[i >> 1][i & 1], 1);
+        mbar_init(&q_full, 1), mbar_init(&q_free, 1), mbar_init(&o_free, 8), mbar_init(&joined, 4);
         s_gave_up = 0;
         mbar_fence_init();
     }
@@ -83,50 +96,40 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     __syncthreads();
     tc_fence_after();
     pdl_wait();
-    pdl_trigger();   // behind the wait: the join reads lengths and starts ahead of its own
+    pdl_trigger();
     const uint32_t tmem = s_tmem;
     PagedLine<PtKind> line;
-    line.kv_heads = p.kv_heads, line.above = p.few, line.upto_rows = 0x7fffffff;
-    const int total = line.begin(p, c), per = cdiv(total, (int)gridDim.x), end = min(total, per * ((int)blockIdx.x + 1));
-    // Of the blocks before: turns, tiles of the ring.  Every barrier's phases are waited for by each of its waiters without a gap, or a later one cannot end
-    // before the waiter has gone on: a phase is told from its neighbours by its parity alone.
-    int turn = 0, ring = 0;
+    line.begin(p, c, (int)gridDim.x);
+    const int begin = min(line.total, line.per * (int)blockIdx.x), end = min(line.total, begin + line.per);
+    if (tid == 0) p.cuts[blockIdx.x].parts = 0;
+    // Of the blocks before: how many, their turns, their tiles of the ring.  Every barrier's phases are waited for by each of its waiters without a gap, or a
+    // later one cannot end before the waiter has gone on: a phase is told from its neighbours by its parity alone.
+    int blocks = 0, turn = 0, ring = 0;
     bool ok = true;           // no wait has given up
-    for (int w = min(total, per * (int)blockIdx.x), count; w < end; w += count) {
-        PagedBlock k;
-        PagedPlace at;
-        line.at(p, c, w, k, at);
+    PagedBlock k;
+    PagedPlace at;
+    bool was_joined = false;  // the block before had one tile of rows, and its two results met where Q lies
+    int joins_before = 0;     // blocks so far that did
+    for (int w = begin, count; w < end; w += count, ++blocks) {
+        if (w == begin) line.at(p, c, w, k, at);
+        else line.next(p, c, w, k, at);
         count = min(end - w, at.units - at.off);
-        const bool two_rows = k.rows > kPaRows;                        // two row tiles; else two key tiles
+        const bool two_rows = k.rows > p.tile_rows, joins = !two_rows && count == at.units;   // two row tiles; else two key tiles
         const int t0 = (k.hi >= 0 ? k.lo / kPtKeys : 0) + (two_rows ? at.off : 2 * at.off), items = two_rows ? 2 : 4;   // of the ring in a turn
         if (warp < kPtWarpS) {
-            asm volatile("bar.sync 3, 256;" ::: "memory");             // the block before has been written
-            // rows of q, [64 of d][row][128 B] with the chunks xor the row; rows behind the last one are zeros
-            const int ch = tid % CH;
-#pragma unroll 4
-            for (int i = 0; i < kPtRows * CH / 256; ++i) {
-                const int r = tid / CH + i * (256 / CH), rr = r & (kPaRows - 1);
-                if (r >= kPaRows && !two_rows) break;
-                const bool in = r < k.rows;
-                const int row = k.row0 + (in ? r : 0), t = p.by_group(row);
-                const T* src = static_cast<const T*>(p.q) + ((size_t)(k.first + t) * p.heads + at.hk * p.group + row - t * p.group) * D + ch * 8;
-                pa_cp16(smem_u32(smem) + (uint32_t)((r >> 7) * C::kQ + (ch >> 3) * (kPaRows * 128) + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)), src, in);
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            pa_fence_async();
-            asm volatile("bar.sync 1, 320;" ::: "memory");
-            const int m = warp >> 2, r = two_rows ? tid : tid & (kPaRows - 1);   // tile; row of the block
+            const int m = warp >> 2, rt = tid & (kPaRows - 1), r = two_rows ? m * p.tile_rows + rt : rt;   // tile; row of it and of the block
+            const bool mine = rt < p.tile_rows && r < k.rows;
             const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = taddr + (uint32_t)(m * 128), to = taddr + (uint32_t)(C::kO + m * D);
             constexpr float kTau = kHalf ? 5.f : 8.f, kUp = kHalf ? 10.f : 0.f;
             const float cs = p.scale;
-            const int row = k.row0 + r, t = p.by_group(row), place = k.place0 + t;
-            const int hi = r < k.rows ? min(place, k.have - 1) : -1, lo = r < k.rows && p.window ? max(0, place - p.window + 1) : 0;
+            const int row = k.row0 + (mine ? r : 0), t = p.by_group(row), place = k.place0 + t;
+            const int hi = mine ? min(place, k.have - 1) : -1, lo = mine && p.window ? max(0, place - p.window + 1) : 0;
             const int key0 = (t0 + (two_rows ? 0 : m)) * kPtKeys, step = two_rows ? kPtKeys : 2 * kPtKeys;
             float l = 0.f, m_ref = -1.4426950e20f;
             for (int j = 0; j < 2 * count; ++j) {                      // 64 keys
                 const int b = j & 1, base = key0 + (j >> 1) * step + b * kPtHalf, h = hi - base, from_ = lo - base;   // this row sees from_ .. h of them
                 const uint32_t tb = ts + (uint32_t)(b * kPtHalf);
-                if (!tc2_wait(&s_full[m][b], (uint32_t)(turn + (j >> 1)) & 1u, s_abort, err, 0x5600 + m)) break;
+                if (!pt_wait(&s_full[m][b], (uint32_t)(turn + (j >> 1)) & 1u, s_abort, err, 0x5600 + m)) break;
                 tc_fence_after();
                 uint32_t raw[kPtHalf];
 #pragma unroll
@@ -215,36 +218,38 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             if (count < at.units) {
                 // a part: {maximum, sum}, then the output as it stands
                 const size_t part = ((size_t)blockIdx.x * 2 + (at.off > 0 ? 0 : 1)) * kPtRows + tid;
-                if (r < k.rows) p.ml[part] = make_float2(m_ref, l);
+                if (mine) p.ml[part] = make_float2(m_ref, l);
 #pragma unroll 1
-                for (int d0 = 0; d0 < D; d0 += 16) {
-                    float v[16];
-                    tc_ld16(to + (uint32_t)d0, v);
-                    if (r < k.rows)
+                for (int d0 = 0; d0 < D; d0 += 32) {
+                    uint32_t v[32];
+                    pa_ld32(to + (uint32_t)d0, v);
+                    pa_wait_ld();
+                    if (mine)
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(p.part + part * D + d0 + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(p.part + part * D + d0 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                 }
+                if (tid == 0) line.cut(p, k, at, count, (int)blockIdx.x);
             } else {
-                // Where the block's one tile has two results, the second goes to shared memory, where Q was, chunks of 16 bytes xor the row; its maximum and
-                // sum by way of the score's columns of the first.
+                // Where the block's one tile has two results, the second goes to shared memory, where Q was, chunks of 16 bytes xor the row.
                 float f_own = 1.f, f_other = 0.f;
-                float4* other = reinterpret_cast<float4*>(smem) + (tid & (kPaRows - 1)) * (D / 4);
-                const int xr = tid & (D / 4 - 1);
-                if (!two_rows) {
-                    __shared__ float2 s_ml[kPaRows];
+                float4* other = reinterpret_cast<float4*>(smem) + rt * (D / 4);
+                const int xr = rt & (D / 4 - 1);
+                if (joins) {
                     if (m == 1) {
-                        s_ml[r] = make_float2(m_ref, l);
+                        s_ml[rt] = make_float2(m_ref, l);
 #pragma unroll 1
-                        for (int d0 = 0; d0 < D; d0 += 16) {
-                            float v[16];
-                            tc_ld16(to + (uint32_t)d0, v);
+                        for (int d0 = 0; d0 < D; d0 += 32) {
+                            uint32_t v[32];
+                            pa_ld32(to + (uint32_t)d0, v);
+                            pa_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; i += 4) other[((d0 + i) >> 2) ^ xr] = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                            for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(other + (((d0 + i) >> 2) ^ xr)) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                         }
                     }
+                    pa_fence_async();   // what Q's next copy writes over
                     asm volatile("bar.sync 3, 256;" ::: "memory");
                     if (m == 0) {
-                        const float2 x = s_ml[r];
+                        const float2 x = s_ml[rt];
                         const float top = fmaxf(m_ref, x.x);
                         f_own = pa_exp2(m_ref - top), f_other = pa_exp2(x.x - top);
                         l = fmaf(x.y, f_other, l * f_own);
@@ -256,25 +261,28 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
                     bool broken = false;
 #pragma unroll 1
-                    for (int d0 = 0; d0 < D; d0 += 16) {
-                        float v[16];
-                        tc_ld16(to + (uint32_t)d0, v);
-                        if (!two_rows)
+                    for (int d0 = 0; d0 < D; d0 += 32) {
+                        uint32_t v[32];
+                        pa_ld32(to + (uint32_t)d0, v);
+                        pa_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; i += 4) {
-                                const float4 y = other[((d0 + i) >> 2) ^ xr];
-                                v[i] = fmaf(y.x, f_other, v[i] * f_own), v[i + 1] = fmaf(y.y, f_other, v[i + 1] * f_own);
-                                v[i + 2] = fmaf(y.z, f_other, v[i + 2] * f_own), v[i + 3] = fmaf(y.w, f_other, v[i + 3] * f_own);
-                            }
-                        if (r < k.rows) {
-                            float f[2][8];
+                        for (int i = 0; i < 32; i += 8) {
+                            float f[8];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) f[i >> 3][i & 7] = l == 0.f ? 0.f : v[i] * inv, broken |= f[i >> 3][i & 7] != f[i >> 3][i & 7];
-                            *reinterpret_cast<uint4*>(dst + d0) = pack8<T>(f[0]);
-                            *reinterpret_cast<uint4*>(dst + d0 + 8) = pack8<T>(f[1]);
+                            for (int u = 0; u < 8; ++u) f[u] = __uint_as_float(v[i + u]);
+                            if (joins)
+#pragma unroll
+                                for (int u = 0; u < 8; u += 4) {
+                                    const float4 y = other[((d0 + i + u) >> 2) ^ xr];
+                                    f[u] = fmaf(y.x, f_other, f[u] * f_own), f[u + 1] = fmaf(y.y, f_other, f[u + 1] * f_own);
+                                    f[u + 2] = fmaf(y.z, f_other, f[u + 2] * f_own), f[u + 3] = fmaf(y.w, f_other, f[u + 3] * f_own);
+                                }
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) f[u] = l == 0.f ? 0.f : f[u] * inv, broken |= f[u] != f[u];
+                            if (mine) *reinterpret_cast<uint4*>(dst + d0 + i) = pack8<T>(f);
                         }
                     }
-                    for (unsigned left = __ballot_sync(0xffffffffu, broken); left; left &= left - 1) {
+                    for (unsigned left = __ballot_sync(0xffffffffu, broken && mine); left; left &= left - 1) {
                         const int src = __ffs(left) - 1;
                         __syncwarp();
                         paged_row_exact<T, D>(p, c, k.seq, __shfl_sync(0xffffffffu, k.first + t, src), __shfl_sync(0xffffffffu, head, src),
@@ -283,11 +291,15 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 }
             }
             tc_fence_before();   // the next block's products write where this one's results were read
+            if (joins) pa_fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free);
+            if (lane == 0 && joins && m == 0) mbar_arrive(&joined);
         } else if (warp == kPtWarpS) {
-            asm volatile("bar.sync 1, 320;" ::: "memory");
             if (tc_elect_one()) {
                 constexpr uint32_t id = pa_idesc(!kHalf, kPtHalf, false);
                 const uint64_t qd = tc_desc_sw128(smem_u32(smem));
+                ok = ok && tc2_wait1(&q_full, (uint32_t)blocks & 1u, s_abort, err, 0x5000);
                 // The scores of 64 keys come under the softmax of the 64 before; they lie over the probabilities of those before these, which P V has to have read.
                 for (int j = 0; j < 2 * count && ok; ++j)
 #pragma unroll
@@ -297,7 +309,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                             ok = ok && tc2_wait1(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5100 + slot);
                             if (!box) pa_fence_async();
                         }
-                        if (j > 1) ok = ok && tc2_wait1(&o_done[m][j & 1], (uint32_t)(turn + (j >> 1) - 1) & 1u, s_abort, err, 0x5400 + m);
+                        if (turn + (j >> 1) > 0) ok = ok && tc2_wait1(&o_done[m][j & 1], (uint32_t)(turn + (j >> 1) - 1) & 1u, s_abort, err, 0x5400 + m);
                         if (!ok) break;
                         tc_fence_after();
                         const uint64_t kd = tc_desc_sw128(smem_u32(smem + C::kRingOff + slot * C::kTile + (j & 1) * (kPtHalf * 128)));
@@ -309,12 +321,13 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                         tc_commit(&s_full[m][j & 1]);
                         if ((j & 1) && (m == 1 || !two_rows)) tc_commit(&empty[slot]);
                     }
+                tc_commit(&q_free);
             }
             __syncwarp();
         } else if (warp == kPtWarpO) {
-            asm volatile("bar.sync 1, 320;" ::: "memory");
             if (tc_elect_one()) {
                 constexpr uint32_t id = pa_idesc(!kHalf, D, true);
+                if (blocks > 0) ok = ok && tc2_wait1(&o_free, (uint32_t)(blocks - 1) & 1u, s_abort, err, 0x5080);   // the block before has been written
                 for (int j = 0; j < 2 * count && ok; ++j)
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
@@ -336,11 +349,26 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                     }
             }
             __syncwarp();
-        } else if (box) {
-            if (warp == kPtWarpLoad) {
+        } else if (warp >= kPtWarpLoad) {
+            // Q, behind the first turn's keys and values: the scores of the block before have been made, and its two results do not lie there any more
+            auto load_q = [&]() {
+                if (warp != kPtWarpLoad) return;
+                if (blocks > 0) ok = ok && tc2_wait(&q_free, (uint32_t)(blocks - 1) & 1u, s_abort, err, 0x5900);
+                if (was_joined) ok = ok && tc2_wait(&joined, (uint32_t)(joins_before - 1) & 1u, s_abort, err, 0x5980);
+                if (lane == 0 && ok) {
+                    const int tokens = p.by_group(p.tile_rows), t = k.first + p.by_group(k.row0);
+                    mbar_expect_tx(&q_full, (two_rows ? 2 : 1) * C::kAtoms * p.tile_rows * 128);
+                    for (int m = 0; m < (two_rows ? 2 : 1); ++m)
+                        for (int a = 0; a < C::kAtoms; ++a)
+                            pt_load_3d(smem_u32(smem) + (uint32_t)(m * C::kQ + a * (kPaRows * 128)), &q_map, a * 64, at.hk * p.group, t + m * tokens, &q_full);
+                }
+                __syncwarp();
+            };
+            if (box && warp == kPtWarpLoad) {
                 // a lane for each box of a tile: its rows, and 64 columns
                 const int boxes = kPtKeys / box;
                 for (int i = 0; i < count * items; ++i) {
+                    if (i == items) load_q();
                     const int it = ring + i, slot = it % C::kRing, tile = t0 + (two_rows ? i >> 1 : 2 * (i >> 2) + (i & 1));
                     const bool is_v = two_rows ? i & 1 : i & 2;
                     const int row = tile * kPtKeys + (lane % boxes) * box, pg = c.by_page(row);
@@ -355,34 +383,37 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                         pt_load_4d(smem_u32(smem + C::kRingOff + slot * C::kTile) + (uint32_t)(b / boxes * (kPtKeys * 128) + b % boxes * (box * 128)),
                                    is_v ? &v_map : &k_map, b / boxes * 64, row - pg * c.page_size, at.hk, id, &full[slot]);
                 }
-            }
-        } else if (warp >= kPtWarpLoad) {
-            // two rows (four of 64 columns) a copy of a warp; a lane looks up every 32nd row
-            const int ch = lane % CH;
-            constexpr int kRowsAtOnce = 32 / CH;
-            for (int i = 0; i < count * items; ++i) {
-                const int it = ring + i, slot = it % C::kRing, tile = t0 + (two_rows ? i >> 1 : 2 * (i >> 2) + (i & 1));
-                const bool is_v = two_rows ? i & 1 : i & 2;
-                long long offs[kPtKeys / 32];
+            } else if (!box) {
+                // two rows (four of 64 columns) a copy of a warp; a lane looks up every 32nd row
+                const int ch = lane % CH;
+                constexpr int kRowsAtOnce = 32 / CH;
+                for (int i = 0; i < count * items; ++i) {
+                    if (i == items) load_q();
+                    const int it = ring + i, slot = it % C::kRing, tile = t0 + (two_rows ? i >> 1 : 2 * (i >> 2) + (i & 1));
+                    const bool is_v = two_rows ? i & 1 : i & 2;
+                    long long offs[kPtKeys / 32];
 #pragma unroll
-                for (int u = 0; u < kPtKeys / 32; ++u) {
-                    const int row = tile * kPtKeys + u * 32 + lane;
-                    offs[u] = row <= k.hi ? c.row_at(k.seq, row) : -1;
-                }
-                if (it >= C::kRing) ok = ok && tc2_wait(&empty[slot], (uint32_t)(it / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
-                if (!ok) break;
-                const T* from = static_cast<const T*>(is_v ? c.v : c.k) + (long long)at.hk * c.head_stride + ch * 8;
-                const uint32_t to = smem_u32(smem) + (uint32_t)(C::kRingOff + slot * C::kTile + (ch >> 3) * (kPtKeys * 128));
-#pragma unroll
-                for (int u = 0; u < kPtKeys / 32; ++u)
-                    for (int x = (warp - kPtWarpLoad) * kRowsAtOnce; x < 32; x += 2 * kRowsAtOnce) {
-                        const int r = x + lane / CH;
-                        const long long off = __shfl_sync(0xffffffffu, offs[u], r);
-                        pa_cp16(to + (uint32_t)((u * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4)), from + (off < 0 ? 0 : off), off >= 0);
+                    for (int u = 0; u < kPtKeys / 32; ++u) {
+                        const int row = tile * kPtKeys + u * 32 + lane;
+                        offs[u] = row <= k.hi ? c.row_at(k.seq, row) : -1;
                     }
-                pa_landed(&full[slot]);
+                    if (it >= C::kRing) ok = ok && tc2_wait(&empty[slot], (uint32_t)(it / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
+                    if (!ok) break;
+                    const T* from = static_cast<const T*>(is_v ? c.v : c.k) + (long long)at.hk * c.head_stride + ch * 8;
+                    const uint32_t to = smem_u32(smem) + (uint32_t)(C::kRingOff + slot * C::kTile + (ch >> 3) * (kPtKeys * 128));
+#pragma unroll
+                    for (int u = 0; u < kPtKeys / 32; ++u)
+                        for (int x = (warp - kPtWarpLoad) * kRowsAtOnce; x < 32; x += 2 * kRowsAtOnce) {
+                            const int r = x + lane / CH;
+                            const long long off = __shfl_sync(0xffffffffu, offs[u], r);
+                            pa_cp16(to + (uint32_t)((u * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4)), from + (off < 0 ? 0 : off), off >= 0);
+                        }
+                    pa_landed(&full[slot]);
+                }
             }
+            if (count == 1) load_q();
         }
+        was_joined = joins, joins_before += joins;
         turn += count, ring += count * items;
     }
     if (!box && warp >= kPtWarpLoad) asm volatile("cp.async.wait_all;" ::: "memory");
