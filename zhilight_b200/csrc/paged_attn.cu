@@ -86,7 +86,7 @@ static int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool p
     }
     ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D>, dim3(ctas), dim3(kPtThreads), PtCfg<D>::kBytes, stream, pdl, p, c, maps[0], maps[1], maps[2], box,
                          words + kWaitAttnPaged));
-    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, kPtRows>, dim3(ctas, kPtRows / kJoinRows), dim3(kJoinRows * 32), 0, stream, true, p, c));
+    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join_tiles<T, D>, dim3(ctas, kPtRows / 32), dim3(256), 0, stream, true, p, c));
     return ZL_OK;
 }
 

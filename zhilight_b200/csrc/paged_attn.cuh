@@ -54,7 +54,7 @@ struct PagedLine {
     int total, per;                    // length of the line and of a stretch
     int b0, before, upto, cum[4];      // first sequence in view and its place; units of a kv head up to and with this lane's, and of this lane's four
 
-    __device__ __forceinline__ int block(const PagedAttn& p, PagedBlock& k, int row0) {
+    static __device__ __forceinline__ int block(const PagedAttn& p, PagedBlock& k, int row0) {
         k.row0 = row0, k.rows = min(p.block_rows, k.n - row0);
         paged_sees(p, k);
         return KIND::units(p, k);
@@ -159,22 +159,43 @@ struct PagedLine {
         place.off = rem;
         place.start = w - rem;
     }
-    // the block behind this one, at place w
-    __device__ __forceinline__ void next(const PagedAttn& p, const PagedCache& c, int w, PagedBlock& k, PagedPlace& place) {
+};
+
+// A CTA's way along its stretch of the line
+template <typename KIND>
+struct PagedWalk {
+    PagedBlock k;
+    PagedPlace place;
+    int w, end, per;   // place in the line, end of the stretch, length of a stretch
+
+    // at w, or (w < 0) at the beginning of the CTA's stretch
+    __device__ __forceinline__ void find(const PagedAttn& p, const PagedCache& c, int at) {
+        PagedLine<KIND> line;
+        line.begin(p, c, (int)gridDim.x);
+        per = line.per;
+        const int first = min(line.total, per * (int)blockIdx.x);
+        w = at < 0 ? first : at;
+        end = min(line.total, first + per);
+        if (w < end) line.at(p, c, w, k, place);
+    }
+    // behind `count` units, at another block; the rest of the stretch begins there
+    __device__ __forceinline__ void go(const PagedAttn& p, const PagedCache& c, int count) {
+        w += count;
+        if (w >= end) return;
         int row0 = k.row0 + p.block_rows;
         if (row0 >= k.n) {
-            if (place.hk + 1 == p.kv_heads) return at(p, c, w, k, place);
+            if (place.hk + 1 == p.kv_heads) return find(p, c, w);
             row0 = 0, ++place.hk;
         }
-        place.units = block(p, k, row0);
+        place.units = PagedLine<KIND>::block(p, k, row0);
         place.off = 0;
         place.start = w;
     }
-    // whether this block, of which `count` units are done here, is the one that CTA i's stretch cuts
-    __device__ __forceinline__ void cut(const PagedAttn& p, const PagedBlock& k, const PagedPlace& place, int count, int i) {
+    // whether this block, of which `count` units are done here, is the one that the CTA's stretch cuts
+    __device__ __forceinline__ void cut(const PagedAttn& p, int count) const {
         if (place.off == 0 && count < place.units) {
-            PagedCut x = {k, place.hk, (place.start + place.units - 1) / per - i + 1};
-            p.cuts[i] = x;
+            PagedCut x = {k, place.hk, (place.start + place.units - 1) / per - (int)blockIdx.x + 1};
+            p.cuts[blockIdx.x] = x;
         }
     }
 };
@@ -229,9 +250,8 @@ __device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedCac
     }
 }
 
-// Blocks that were cut.  grid (the CTAs of the first kernel, groups of kJoinRows rows), a warp a row: the first part of a block lies in its CTA's place 1,
-// the others in the place 0 of theirs, R rows each.  Of a block with two tiles of rows the second begins at row R / 2 of its place; one with a single tile
-// has two results in a place, the second there.
+// Blocks that were cut, of the kernel for few rows.  grid (its CTAs, groups of kJoinRows rows), a warp a row: the first part of a block lies in its CTA's
+// place 1, the others in the place 0 of theirs, R rows each.
 constexpr int kJoinRows = 8;
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(kJoinRows * 32) k_paged_join(const PagedAttn p, const PagedCache c) {
@@ -241,20 +261,15 @@ __global__ void __launch_bounds__(kJoinRows * 32) k_paged_join(const PagedAttn p
     pdl_wait();
     const PagedCut x = p.cuts[blockIdx.x];
     if (x.parts == 0 || r >= x.k.rows) return;
-    const bool twice = p.tile_rows && x.k.rows <= p.tile_rows;
-    const int parts = twice ? 2 * x.parts : x.parts, row = p.tile_rows && r >= p.tile_rows ? r - p.tile_rows + R / 2 : r;
-    auto place = [&](int s) {
-        const int i = twice ? s >> 1 : s;
-        return ((size_t)(blockIdx.x + i) * 2 + (i == 0)) * R + row + (twice && (s & 1) ? R / 2 : 0);
-    };
+    auto place = [&](int s) { return ((size_t)(blockIdx.x + s) * 2 + (s == 0)) * R + r; };
     float m = -INFINITY, l = 0.f, v[E] = {};
-    for (int s = lane; s < parts; s += 32) m = fmaxf(m, p.ml[place(s)].x);
+    for (int s = lane; s < x.parts; s += 32) m = fmaxf(m, p.ml[place(s)].x);
     m = warp_max(m);
-    for (int s0 = 0; s0 < parts; s0 += 32) {
-        const float2 y = s0 + lane < parts ? p.ml[place(s0 + lane)] : make_float2(-INFINITY, 0.f);
-        const float f = s0 + lane < parts ? exp2f(y.x - m) : 0.f;
+    for (int s0 = 0; s0 < x.parts; s0 += 32) {
+        const float2 y = s0 + lane < x.parts ? p.ml[place(s0 + lane)] : make_float2(-INFINITY, 0.f);
+        const float f = s0 + lane < x.parts ? exp2f(y.x - m) : 0.f;
         l += warp_sum(y.y * f);
-        const int n = min(32, parts - s0);
+        const int n = min(32, x.parts - s0);
 #pragma unroll 8
         for (int s = 0; s < n; ++s) {
             const float w = __shfl_sync(0xffffffffu, f, s);

@@ -64,16 +64,14 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
     const uint32_t ring_at = smem_u32(ring);
     pdl_wait();
     pdl_trigger();
-    PagedLine<PfKind> line;
-    line.begin(p, c, (int)gridDim.x);
-    const int begin = min(line.total, line.per * (int)blockIdx.x), end = min(line.total, begin + line.per);
     if (tid == 0) p.cuts[blockIdx.x].parts = 0;
-    PagedBlock k;
-    PagedPlace at;
-    for (int w = begin; w < end;) {
-        if (w == begin) line.at(p, c, w, k, at);
-        else line.next(p, c, w, k, at);
-        const int count = min(end - w, at.units - at.off), key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + at.off) * kPfKeys + warp * 16;
+    PagedWalk<PfKind> walk;
+    const PagedBlock& k = walk.k;
+    const PagedPlace& at = walk.place;
+    walk.find(p, c, -1);
+    for (int count; walk.w < walk.end; walk.go(p, c, count)) {
+        count = min(walk.end - walk.w, at.units - at.off);
+        const int key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + at.off) * kPfKeys + warp * 16;
         const long long head = (long long)at.hk * c.head_stride;
         // Copies of a stage: each lane has a chunk of some rows.  Lanes 0 - 15 ask for the page numbers of the 16 rows a stage ahead; where pages hold whole
         // 16s these are one page.
@@ -245,9 +243,8 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 else *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
             }
         }
-        if (tid == 0) line.cut(p, k, at, count, (int)blockIdx.x);
+        if (tid == 0) walk.cut(p, count);
         __syncthreads();   // the rings are the next block's
-        w += count;
     }
 }
 

@@ -98,22 +98,19 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     pdl_wait();
     pdl_trigger();
     const uint32_t tmem = s_tmem;
-    PagedLine<PtKind> line;
-    line.begin(p, c, (int)gridDim.x);
-    const int begin = min(line.total, line.per * (int)blockIdx.x), end = min(line.total, begin + line.per);
     if (tid == 0) p.cuts[blockIdx.x].parts = 0;
     // Of the blocks before: how many, their turns, their tiles of the ring.  Every barrier's phases are waited for by each of its waiters without a gap, or a
     // later one cannot end before the waiter has gone on: a phase is told from its neighbours by its parity alone.
     int blocks = 0, turn = 0, ring = 0;
     bool ok = true;           // no wait has given up
-    PagedBlock k;
-    PagedPlace at;
+    PagedWalk<PtKind> walk;
+    const PagedBlock& k = walk.k;
+    const PagedPlace& at = walk.place;
+    walk.find(p, c, -1);
     bool was_joined = false;  // the block before had one tile of rows, and its two results met where Q lies
     int joins_before = 0;     // blocks so far that did
-    for (int w = begin, count; w < end; w += count, ++blocks) {
-        if (w == begin) line.at(p, c, w, k, at);
-        else line.next(p, c, w, k, at);
-        count = min(end - w, at.units - at.off);
+    for (int count; walk.w < walk.end; walk.go(p, c, count), ++blocks) {
+        count = min(walk.end - walk.w, at.units - at.off);
         const bool two_rows = k.rows > p.tile_rows, joins = !two_rows && count == at.units;   // two row tiles; else two key tiles
         const int t0 = (k.hi >= 0 ? k.lo / kPtKeys : 0) + (two_rows ? at.off : 2 * at.off), items = two_rows ? 2 : 4;   // of the ring in a turn
         if (warp < kPtWarpS) {
@@ -216,19 +213,21 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             for (int b = 0; b < 2; ++b) tc2_wait(&o_done[m][b], (uint32_t)(turn + count - 1) & 1u, s_abort, err, 0x5700 + m);
             tc_fence_after();
             if (count < at.units) {
-                // a part: {maximum, sum}, then the output as it stands
-                const size_t part = ((size_t)blockIdx.x * 2 + (at.off > 0 ? 0 : 1)) * kPtRows + tid;
-                if (mine) p.ml[part] = make_float2(m_ref, l);
+                // A part: {maximum, sum}, then the output as it stands, column by column: the lanes of a warp are neighbours there.
+                const size_t part = (size_t)blockIdx.x * 2 + (at.off > 0 ? 0 : 1);
+                if (mine) p.ml[part * kPtRows + tid] = make_float2(m_ref, l);
+                float* dst = p.part + part * kPtRows * D + tid;
+                if (__any_sync(0xffffffffu, mine))
 #pragma unroll 1
-                for (int d0 = 0; d0 < D; d0 += 32) {
-                    uint32_t v[32];
-                    pa_ld32(to + (uint32_t)d0, v);
-                    pa_wait_ld();
-                    if (mine)
+                    for (int d0 = 0; d0 < D; d0 += 32) {
+                        uint32_t v[32];
+                        pa_ld32(to + (uint32_t)d0, v);
+                        pa_wait_ld();
+                        if (mine)
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(p.part + part * D + d0 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                }
-                if (tid == 0) line.cut(p, k, at, count, (int)blockIdx.x);
+                            for (int i = 0; i < 32; ++i) dst[(d0 + i) * kPtRows] = __uint_as_float(v[i]);
+                    }
+                if (tid == 0) walk.cut(p, count);
             } else {
                 // Where the block's one tile has two results, the second goes to shared memory, where Q was, chunks of 16 bytes xor the row.
                 float f_own = 1.f, f_other = 0.f;
@@ -237,6 +236,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 if (joins) {
                     if (m == 1) {
                         s_ml[rt] = make_float2(m_ref, l);
+                        if (__any_sync(0xffffffffu, mine))
 #pragma unroll 1
                         for (int d0 = 0; d0 < D; d0 += 32) {
                             uint32_t v[32];
@@ -255,7 +255,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                         l = fmaf(x.y, f_other, l * f_own);
                     }
                 }
-                if (two_rows || m == 0) {
+                if ((two_rows || m == 0) && __any_sync(0xffffffffu, mine)) {
                     const int head = at.hk * p.group + row - t * p.group;
                     T* dst = static_cast<T*>(p.out) + ((size_t)(k.first + t) * p.heads + head) * D;
                     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -424,6 +424,66 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     if (warp == kPtWarpS) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
+    }
+}
+
+// Blocks that were cut: grid (the CTAs of k_paged_attn_tiles, groups of 32 rows), lane = row, a warp for D / 8 columns.  The first part of a block lies in its
+// CTA's place 1, the others in the place 0 of theirs.  Of a block with two tiles of rows the second begins at row 128 of its place; one with a single tile has
+// two results in a place, the second there.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_paged_join_tiles(const PagedAttn p, const PagedCache c) {
+    constexpr int W = D / 8;
+    __shared__ unsigned s_bad[8];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d0 = warp * W;
+    pdl_trigger();
+    pdl_wait();
+    const PagedCut x = p.cuts[blockIdx.x];
+    const int r0 = blockIdx.y * 32, r = r0 + lane;
+    if (x.parts == 0 || r0 >= x.k.rows) return;
+    const bool twice = x.k.rows <= p.tile_rows, mine = r < x.k.rows;
+    const int row = r >= p.tile_rows ? r - p.tile_rows + kPaRows : r;   // not more than 255
+    float m = -INFINITY, l = 0.f, v[W] = {};
+    // as the softmax goes, from part to part
+    for (int s = 0; s < (twice ? 2 * x.parts : x.parts); ++s) {
+        const int i = twice ? s >> 1 : s;
+        const size_t part = (size_t)(blockIdx.x + i) * 2 + (i == 0);
+        const int at = min(row + (twice && (s & 1) ? kPaRows : 0), kPtRows - 1);
+        const float2 y = p.ml[part * kPtRows + at];
+        float z[W];
+#pragma unroll
+        for (int u = 0; u < W; ++u) z[u] = p.part[(part * D + d0 + u) * kPtRows + at];
+        const float up = fmaxf(m, y.x), f = pa_exp2(m - up), g = pa_exp2(y.x - up);
+        m = up;
+        l = fmaf(y.y, g, l * f);
+#pragma unroll
+        for (int u = 0; u < W; ++u) v[u] = fmaf(z[u], g, v[u] * f);
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int u = 0; u < W; ++u) v[u] = l == 0.f ? 0.f : v[u] * inv, bad |= v[u] != v[u];
+    const int at = x.k.row0 + (mine ? r : 0), t = p.by_group(at), head = x.hk * p.group + at - t * p.group, place = x.k.place0 + t;
+    if (mine) {
+        T* dst = static_cast<T*>(p.out) + ((size_t)(x.k.first + t) * p.heads + head) * D + d0;
+#pragma unroll
+        for (int u = 0; u < W; u += 8) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = v[u + i];
+            *reinterpret_cast<uint4*>(dst + u) = pack8<T>(f);
+        }
+    }
+    const unsigned some = __ballot_sync(0xffffffffu, bad && mine);
+    if (lane == 0) s_bad[warp] = some;
+    __syncthreads();
+    unsigned all = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all |= s_bad[i];
+    for (; all; all &= all - 1) {
+        const int src = __ffs(all) - 1;
+        if (src % 8 == warp)
+            paged_row_exact<T, D>(p, c, x.k.seq, x.k.first + __shfl_sync(0xffffffffu, t, src), __shfl_sync(0xffffffffu, head, src),
+                                  p.window ? max(0, __shfl_sync(0xffffffffu, place, src) - p.window + 1) : 0, min(__shfl_sync(0xffffffffu, place, src), x.k.have - 1));
     }
 }
 
