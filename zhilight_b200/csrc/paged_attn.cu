@@ -74,7 +74,7 @@ static int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool p
     }
     // boxes of K and V: the rows that a tile and a page have in common wherever they meet
     int box = 1;
-    while (box < kPtKeys && c.page_size % (2 * box) == 0) box *= 2;
+    while (box < kPtHalf && c.page_size % (2 * box) == 0) box *= 2;
     if (box < 8) box = 0;
     if (box) {
         auto step = [](long long elements, bool more) { return more ? (uint64_t)elements * 2 : (uint64_t)(D * 2); };   // of one alone none is taken

@@ -6,8 +6,8 @@
 //   warps 0-3, 4-7  softmax of a tile each: thread = row = lane of tensor memory; running maximum and sum in 32 bits; probabilities go back over the scores
 //   warp 8          one thread issues S = Q K^T of both tiles, 64 keys at a time into two buffers each
 //   warp 9          one thread issues O += P V of both tiles (P from tensor memory, V as it lies: rows of keys, the B operand along n)
-//   warp 10         Q by TMA, once for a block; K and V from the pages into a ring of tiles by TMA, a box for the rows of a tile that one page has
-//                   (where that is no multiple of 8 rows, of the swizzle's period, warps 10 and 11 copy 16 bytes at a time)
+//   warps 10, 11    Q by TMA, once for a block; K and V, a warp each, from the pages into a ring of tiles of 64 keys by TMA, a box for the rows of a tile
+//                   that one page has (where that is no multiple of 8 rows, of the swizzle's period, both copy 16 bytes at a time)
 //
 // A page's rows behind the last visible key may hold anything.  Copies of 16 bytes leave them out; behind TMA the softmax's threads make those values zeros
 // before they hand the tile's probabilities on.  Rows behind a page number outside the pool are zeros either way.  Tensor memory: scores of the two tiles (128 columns each, probabilities over their first
@@ -39,8 +39,8 @@ template <int D>
 struct PtCfg {
     static constexpr int kAtoms = D / 64;
     static constexpr int kQ = kAtoms * kPaRows * 128;       // a tile of Q: [64 of d][128 rows][128 B]
-    static constexpr int kTile = kAtoms * kPtKeys * 128;    // K or V: [64 of d][128 keys][128 B]
-    static constexpr int kRing = D == 128 ? 5 : 8;
+    static constexpr int kTile = kAtoms * kPtHalf * 128;    // K or V: [64 of d][64 keys][128 B]
+    static constexpr int kRing = D == 128 ? 10 : 16;
     static constexpr int kRingOff = 2 * kQ, kBytes = kRingOff + kRing * kTile + 1024;   // + slack for the manual 1024-byte alignment
     static_assert(tmem_alone(kBytes) && kBytes + 1024 <= 227 * 1024, "all of tensor memory, an SM to itself");
     static_assert(2 * kQ >= kPaRows * D * 4, "the second result of a row, where Q was");
@@ -112,7 +112,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     for (int count; walk.w < walk.end; walk.go(p, c, count), ++blocks) {
         count = min(walk.end - walk.w, at.units - at.off);
         const bool two_rows = k.rows > p.tile_rows, joins = !two_rows && count == at.units;   // two row tiles; else two key tiles
-        const int t0 = (k.hi >= 0 ? k.lo / kPtKeys : 0) + (two_rows ? at.off : 2 * at.off), items = two_rows ? 2 : 4;   // of the ring in a turn
+        const int t0 = (k.hi >= 0 ? k.lo / kPtKeys : 0) + (two_rows ? at.off : 2 * at.off), items = two_rows ? 2 : 4;   // of the ring for 64 keys
         if (warp < kPtWarpS) {
             const int m = warp >> 2, rt = tid & (kPaRows - 1), r = two_rows ? m * p.tile_rows + rt : rt;   // tile; row of it and of the block
             const bool mine = rt < p.tile_rows && r < k.rows;
@@ -195,13 +195,13 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 // The tile with the last visible key, where that ends within a box: values behind it become zeros.  Of two row tiles the first sees to it, whose
                 // product comes first.  The tile is there or on its way: the ring's tiles before it have been used.
                 const int behind = k.hi + 1 - base;
-                if (box && b == 0 && behind > 0 && behind < kPtKeys && behind % box != 0 && (m == 0 || !two_rows)) {
-                    const int it = ring + (j >> 1) * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
+                if (box && behind > 0 && behind < kPtHalf && behind % box != 0 && (m == 0 || !two_rows)) {
+                    const int it = ring + j * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
                     if (!tc2_wait(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5800 + slot)) break;
                     const int r1 = (behind + box - 1) / box * box;   // further boxes are zeros already
                     for (int x = tid & (kPaRows - 1); x < (r1 - behind) * CH; x += kPaRows) {
                         const int rz = behind + x / CH, cz = x % CH;   // whole rows: the swizzle stays within them
-                        *reinterpret_cast<uint4*>(smem + C::kRingOff + slot * C::kTile + (cz >> 3) * (kPtKeys * 128) + rz * 128 + ((cz & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(smem + C::kRingOff + slot * C::kTile + (cz >> 3) * (kPtHalf * 128) + rz * 128 + ((cz & 7) << 4)) = make_uint4(0, 0, 0, 0);
                     }
                     pa_fence_async();
                 }
@@ -304,22 +304,22 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 for (int j = 0; j < 2 * count && ok; ++j)
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
-                        const int it = ring + (j >> 1) * items + (two_rows ? 0 : m), slot = it % C::kRing;
-                        if (!(j & 1) && (m == 0 || !two_rows)) {
+                        const int it = ring + j * items + (two_rows ? 0 : m), slot = it % C::kRing;
+                        if (m == 0 || !two_rows) {
                             ok = ok && tc2_wait1(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5100 + slot);
                             if (!box) pa_fence_async();
                         }
                         if (turn + (j >> 1) > 0) ok = ok && tc2_wait1(&o_done[m][j & 1], (uint32_t)(turn + (j >> 1) - 1) & 1u, s_abort, err, 0x5400 + m);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t kd = tc_desc_sw128(smem_u32(smem + C::kRingOff + slot * C::kTile + (j & 1) * (kPtHalf * 128)));
+                        const uint64_t kd = tc_desc_sw128(smem_u32(smem + C::kRingOff + slot * C::kTile));
                         const uint64_t qm = qd + (uint64_t)((two_rows ? m : 0) * (C::kQ / 16));
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i)
                             pa_mma_ss(tmem + (uint32_t)(m * 128 + (j & 1) * kPtHalf), qm + (uint64_t)((i >> 2) * (kPaRows * 128 / 16) + (i & 3) * 2),
-                                      kd + (uint64_t)((i >> 2) * (kPtKeys * 128 / 16) + (i & 3) * 2), id, i > 0 ? 1u : 0u);
+                                      kd + (uint64_t)((i >> 2) * (kPtHalf * 128 / 16) + (i & 3) * 2), id, i > 0 ? 1u : 0u);
                         tc_commit(&s_full[m][j & 1]);
-                        if ((j & 1) && (m == 1 || !two_rows)) tc_commit(&empty[slot]);
+                        if (m == 1 || !two_rows) tc_commit(&empty[slot]);
                     }
                 tc_commit(&q_free);
             }
@@ -331,26 +331,31 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 for (int j = 0; j < 2 * count && ok; ++j)
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
-                        const int it = ring + (j >> 1) * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
-                        if (!(j & 1) && (m == 0 || !two_rows)) {
+                        const int it = ring + j * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
+                        if (m == 0 || !two_rows) {
                             ok = ok && tc2_wait1(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5200 + slot);
                             if (!box) pa_fence_async();
                         }
                         ok = ok && tc2_wait1(&p_full[m][j & 1], (uint32_t)(turn + (j >> 1)) & 1u, s_abort, err, 0x5300 + m);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t vd = pa_desc_mn(smem_u32(smem + C::kRingOff + slot * C::kTile + (j & 1) * (kPtHalf * 128)), kPtKeys * 128);
+                        const uint64_t vd = pa_desc_mn(smem_u32(smem + C::kRingOff + slot * C::kTile), kPtHalf * 128);
 #pragma unroll
                         for (int i = 0; i < kPtHalf / 16; ++i)
                             pa_mma_ts(tmem + (uint32_t)(C::kO + m * D), tmem + (uint32_t)(m * 128 + (j & 1) * kPtHalf + i * 8), vd + (uint64_t)(i * (16 * 128 / 16)), id,
                                       (j > 0 || i > 0) ? 1u : 0u);
                         tc_commit(&o_done[m][j & 1]);
-                        if ((j & 1) && (m == 1 || !two_rows)) tc_commit(&empty[slot]);
+                        if (m == 1 || !two_rows) tc_commit(&empty[slot]);
                     }
             }
             __syncwarp();
         } else if (warp >= kPtWarpLoad) {
-            // Q, behind the first turn's keys and values: the scores of the block before have been made, and its two results do not lie there any more
+            // first key of the ring's tile i of this block
+            auto row_of = [&](int i) {
+                const int j = two_rows ? i >> 1 : i >> 2;
+                return (t0 + (two_rows ? j >> 1 : 2 * (j >> 1) + (i & 1))) * kPtKeys + (j & 1) * kPtHalf;
+            };
+            // Q, behind the first keys and values: the scores of the block before have been made, and its two results do not lie there any more
             auto load_q = [&]() {
                 if (warp != kPtWarpLoad) return;
                 if (blocks > 0) ok = ok && tc2_wait(&q_free, (uint32_t)(blocks - 1) & 1u, s_abort, err, 0x5900);
@@ -364,45 +369,51 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 }
                 __syncwarp();
             };
-            if (box && warp == kPtWarpLoad) {
-                // a lane for each box of a tile: its rows, and 64 columns
-                const int boxes = kPtKeys / box;
-                for (int i = 0; i < count * items; ++i) {
-                    if (i == items) load_q();
-                    const int it = ring + i, slot = it % C::kRing, tile = t0 + (two_rows ? i >> 1 : 2 * (i >> 2) + (i & 1));
-                    const bool is_v = two_rows ? i & 1 : i & 2;
-                    const int row = tile * kPtKeys + (lane % boxes) * box, pg = c.by_page(row);
-                    int id = -1;
-                    if (row <= k.hi && pg < c.max_pages) id = c.table[(size_t)k.seq * c.ld_table + pg];
-                    if (id < 0 || id >= c.num_pages) id = -1;   // outside of the tensor: reads as zeros
-                    if (it >= C::kRing) ok = ok && tc2_wait(&empty[slot], (uint32_t)(it / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
-                    if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(&full[slot], C::kTile);
-                    __syncwarp();
-                    for (int b = lane; b < boxes * C::kAtoms; b += 32)
-                        pt_load_4d(smem_u32(smem + C::kRingOff + slot * C::kTile) + (uint32_t)(b / boxes * (kPtKeys * 128) + b % boxes * (box * 128)),
-                                   is_v ? &v_map : &k_map, b / boxes * 64, row - pg * c.page_size, at.hk, id, &full[slot]);
+            if (box) {
+                // One warp for keys, one for values; a lane for each box of a tile, its rows and 64 columns.  The lanes hold the numbers of 32 pages in a row.
+                const bool is_v = warp != kPtWarpLoad;
+                const int boxes = kPtHalf / box, b_row = lane % boxes * box, last_page = min(c.by_page(max(k.hi, 0)), c.max_pages - 1);
+                int page0 = -32, ids = -1;
+                for (int j = 0; j < 2 * count && ok; ++j) {
+                    if (j == 1) load_q();
+                    for (int m = 0; m < (two_rows ? 1 : 2); ++m) {
+                        const int i = j * items + (two_rows ? (is_v ? 1 : 0) : (is_v ? 2 : 0) + m), it = ring + i, slot = it % C::kRing;
+                        const int row0 = row_of(i), row = row0 + b_row, pg = c.by_page(row);
+                        if (c.by_page(row0 + kPtHalf - 1) >= page0 + 32) {
+                            page0 = c.by_page(row0);
+                            ids = page0 + lane <= last_page ? c.table[(size_t)k.seq * c.ld_table + page0 + lane] : -1;
+                        }
+                        int id = __shfl_sync(0xffffffffu, ids, pg - page0);
+                        if (row > k.hi || id < 0 || id >= c.num_pages) id = -1;   // outside of the tensor: reads as zeros
+                        if (it >= C::kRing) ok = ok && tc2_wait(&empty[slot], (uint32_t)(it / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
+                        if (!ok) break;
+                        if (lane == 0) mbar_expect_tx(&full[slot], C::kTile);
+                        __syncwarp();
+                        for (int b = lane; b < boxes * C::kAtoms; b += 32)
+                            pt_load_4d(smem_u32(smem + C::kRingOff + slot * C::kTile) + (uint32_t)(b / boxes * (kPtHalf * 128) + b_row * 128), is_v ? &v_map : &k_map,
+                                       b / boxes * 64, row - pg * c.page_size, at.hk, id, &full[slot]);
+                    }
                 }
             } else if (!box) {
                 // two rows (four of 64 columns) a copy of a warp; a lane looks up every 32nd row
                 const int ch = lane % CH;
                 constexpr int kRowsAtOnce = 32 / CH;
-                for (int i = 0; i < count * items; ++i) {
+                for (int i = 0; i < 2 * count * items; ++i) {
                     if (i == items) load_q();
-                    const int it = ring + i, slot = it % C::kRing, tile = t0 + (two_rows ? i >> 1 : 2 * (i >> 2) + (i & 1));
+                    const int it = ring + i, slot = it % C::kRing;
                     const bool is_v = two_rows ? i & 1 : i & 2;
-                    long long offs[kPtKeys / 32];
+                    long long offs[kPtHalf / 32];
 #pragma unroll
-                    for (int u = 0; u < kPtKeys / 32; ++u) {
-                        const int row = tile * kPtKeys + u * 32 + lane;
+                    for (int u = 0; u < kPtHalf / 32; ++u) {
+                        const int row = row_of(i) + u * 32 + lane;
                         offs[u] = row <= k.hi ? c.row_at(k.seq, row) : -1;
                     }
                     if (it >= C::kRing) ok = ok && tc2_wait(&empty[slot], (uint32_t)(it / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
                     if (!ok) break;
                     const T* from = static_cast<const T*>(is_v ? c.v : c.k) + (long long)at.hk * c.head_stride + ch * 8;
-                    const uint32_t to = smem_u32(smem) + (uint32_t)(C::kRingOff + slot * C::kTile + (ch >> 3) * (kPtKeys * 128));
+                    const uint32_t to = smem_u32(smem) + (uint32_t)(C::kRingOff + slot * C::kTile + (ch >> 3) * (kPtHalf * 128));
 #pragma unroll
-                    for (int u = 0; u < kPtKeys / 32; ++u)
+                    for (int u = 0; u < kPtHalf / 32; ++u)
                         for (int x = (warp - kPtWarpLoad) * kRowsAtOnce; x < 32; x += 2 * kRowsAtOnce) {
                             const int r = x + lane / CH;
                             const long long off = __shfl_sync(0xffffffffu, offs[u], r);
@@ -411,10 +422,9 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                     pa_landed(&full[slot]);
                 }
             }
-            if (count == 1) load_q();
         }
         was_joined = joins, joins_before += joins;
-        turn += count, ring += count * items;
+        turn += count, ring += 2 * count * items;
     }
     if (!box && warp >= kPtWarpLoad) asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
