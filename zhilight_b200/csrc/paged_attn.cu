@@ -25,7 +25,7 @@ static PagedPlan paged_plan(int rows, int max_new, int seqs, int max_keys, int h
     s.block_rows = s.tiles ? 2 * s.tile_rows : most <= 16 ? 16 : 32;
     s.places = s.tiles ? kPtRows : s.block_rows;
     // no more CTAs than the line can be long: every sequence adds less than one block to those of the rows, each of all the keys there is room for
-    const long long units = (all / s.block_rows + seqs) * cdiv(max_keys, s.tiles ? kPtKeys : kPfKeys) * kv_heads;
+    const long long units = (all / s.block_rows + seqs) * (s.tiles ? PtKind::kSetup + cdiv(max_keys, kPtKeys) : PfKind::kSetup + cdiv(max_keys, kPfKeys)) * kv_heads;
     const int most_ctas = s.tiles ? sms : kPfPerSm * sms;
     s.ctas = (int)(units < most_ctas ? units : most_ctas);
     const size_t parts = (size_t)s.ctas * 2 * s.places;
@@ -118,7 +118,7 @@ extern "C" int zl_paged_attention(const void* q, const void* k_cache, const void
     const long long room = (long long)max_pages * page_size;
     const PagedPlan s = paged_plan(rows, max_new, seqs, (int)(room < INT_MAX - 255 ? room : INT_MAX - 255), heads, kv_heads, dim);
     // the kernels count tiles in 32 bits
-    ZL_CHECK_SUPPORTED(((long long)rows * (heads / kv_heads) / 16 + seqs) * (room / kPfKeys + 1) < INT_MAX / kv_heads);
+    ZL_CHECK_SUPPORTED(((long long)rows * (heads / kv_heads) / 16 + seqs) * (room / kPfKeys + 4) < INT_MAX / kv_heads);
     ZL_CHECK_ARG(workspace && workspace_bytes >= s.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
     const PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), num_pages, page_stride, row_stride, head_stride, page_table, ld_table, max_pages,
                           page_size, seqs, paged_divisor(page_size)};

@@ -35,7 +35,7 @@ __device__ __forceinline__ void paged_sees(const PagedAttn& p, PagedBlock& k) {
     if (k.lo > k.hi) k.hi = -1, k.lo = 0;
 }
 struct PagedPlace {
-    int hk, off, units;   // kv head; unit within the block, and how many that has
+    int hk, off, units;   // kv head; place within the block, and its length in the line: KIND::kSetup, what a block costs beside its turns, and then those
     int start;            // the block's place in the line
 };
 
@@ -46,7 +46,7 @@ struct PagedCut {
 };
 
 // A warp's view of the line that the blocks of a kernel's work stand in: sequence by sequence, in it kv head by kv head, in that block by block, each
-// KIND::units() long.  A CTA of the grid takes an equal stretch of the line.  128 sequences are in view at a time, four to a lane; the blocks of a
+// KIND::kSetup + KIND::turns() long.  A CTA of the grid takes an equal stretch of the line.  128 sequences are in view at a time, four to a lane; the blocks of a
 // sequence that has many are looked at by the whole warp.  Everything fits 32 bits, which the entry point sees to.
 template <typename KIND>
 struct PagedLine {
@@ -57,7 +57,7 @@ struct PagedLine {
     static __device__ __forceinline__ int block(const PagedAttn& p, PagedBlock& k, int row0) {
         k.row0 = row0, k.rows = min(p.block_rows, k.n - row0);
         paged_sees(p, k);
-        return KIND::units(p, k);
+        return KIND::kSetup + KIND::turns(p, k);
     }
     __device__ __forceinline__ void view(const PagedAttn& p, const PagedCache& c) {
         const int lane = threadIdx.x & 31, b = b0 + lane * 4;
@@ -178,9 +178,15 @@ struct PagedWalk {
         end = min(line.total, first + per);
         if (w < end) line.at(p, c, w, k, place);
     }
-    // behind `count` units, at another block; the rest of the stretch begins there
-    __device__ __forceinline__ void go(const PagedAttn& p, const PagedCache& c, int count) {
-        w += count;
+    // turns first .. first + count - 1 of the block are this CTA's; none where the stretch ends before the block's first turn
+    __device__ __forceinline__ void share(int& first, int& count) const {
+        first = max(place.off - KIND::kSetup, 0);
+        count = max(place.off + min(end - w, place.units - place.off) - KIND::kSetup, 0) - first;
+    }
+    __device__ __forceinline__ bool whole(int count) const { return count == place.units - KIND::kSetup; }
+    // on to the next block
+    __device__ __forceinline__ void go(const PagedAttn& p, const PagedCache& c) {
+        w += min(end - w, place.units - place.off);
         if (w >= end) return;
         int row0 = k.row0 + p.block_rows;
         if (row0 >= k.n) {
@@ -191,9 +197,9 @@ struct PagedWalk {
         place.off = 0;
         place.start = w;
     }
-    // whether this block, of which `count` units are done here, is the one that the CTA's stretch cuts
-    __device__ __forceinline__ void cut(const PagedAttn& p, int count) const {
-        if (place.off == 0 && count < place.units) {
+    // notes a block that this CTA has the first, but not all turns of: there is one at the most
+    __device__ __forceinline__ void cut(const PagedAttn& p, int first, int count) const {
+        if (first == 0 && !whole(count)) {
             PagedCut x = {k, place.hk, (place.start + place.units - 1) / per - (int)blockIdx.x + 1};
             p.cuts[blockIdx.x] = x;
         }

@@ -25,7 +25,8 @@ struct PfCfg {
 
 // tiles of 64 keys; at least one: a block that sees nothing is written too
 struct PfKind {
-    static __device__ __forceinline__ int units(const PagedAttn&, const PagedBlock& k) { return k.hi >= 0 ? k.hi / kPfKeys - k.lo / kPfKeys + 1 : 1; }
+    static constexpr int kSetup = 2;
+    static __device__ __forceinline__ int turns(const PagedAttn&, const PagedBlock& k) { return k.hi >= 0 ? k.hi / kPfKeys - k.lo / kPfKeys + 1 : 1; }
 };
 
 __device__ __forceinline__ void pf_ldsm(uint32_t (&r)[4], uint32_t addr) {
@@ -69,9 +70,11 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
     const PagedBlock& k = walk.k;
     const PagedPlace& at = walk.place;
     walk.find(p, c, -1);
-    for (int count; walk.w < walk.end; walk.go(p, c, count)) {
-        count = min(walk.end - walk.w, at.units - at.off);
-        const int key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + at.off) * kPfKeys + warp * 16;
+    for (; walk.w < walk.end; walk.go(p, c)) {
+        int first, count;
+        walk.share(first, count);
+        if (count == 0) continue;
+        const int key0 = ((k.hi >= 0 ? k.lo / kPfKeys : 0) + first) * kPfKeys + warp * 16;
         const long long head = (long long)at.hk * c.head_stride;
         // Copies of a stage: each lane has a chunk of some rows.  Lanes 0 - 15 ask for the page numbers of the 16 rows a stage ahead; where pages hold whole
         // 16s these are one page.
@@ -219,8 +222,8 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(mine + r * C::kPitch + n * 8 + t4 * 2) = make_float2(o[m][n][2 * u], o[m][n][2 * u + 1]);
             }
         __syncthreads();
-        const bool whole = count == at.units;
-        const size_t part = ((size_t)blockIdx.x * 2 + (at.off > 0 ? 0 : 1)) * R;
+        const bool whole = walk.whole(count);
+        const size_t part = ((size_t)blockIdx.x * 2 + (first > 0 ? 0 : 1)) * R;
         for (int r = warp; r < k.rows; r += kPfWarps) {
             constexpr int E = D / 32;
             float m = s_ml[0][r].x, sum = 0.f, v[E] = {};
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 else *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
             }
         }
-        if (tid == 0) walk.cut(p, count);
+        if (tid == 0) walk.cut(p, first, count);
         __syncthreads();   // the rings are the next block's
     }
 }

@@ -29,7 +29,8 @@ constexpr int kPtRows = 256, kPtKeys = 128, kPtHalf = 64, kPtThreads = 384, kPtW
 
 // turns of a block, at least one: a block that sees nothing is written too
 struct PtKind {
-    static __device__ __forceinline__ int units(const PagedAttn& p, const PagedBlock& k) {
+    static constexpr int kSetup = 2;
+    static __device__ __forceinline__ int turns(const PagedAttn& p, const PagedBlock& k) {
         const int tiles = k.hi >= 0 ? k.hi / kPtKeys - k.lo / kPtKeys + 1 : 1;
         return k.rows > p.tile_rows ? tiles : (tiles + 1) >> 1;
     }
@@ -109,10 +110,12 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     walk.find(p, c, -1);
     bool was_joined = false;  // the block before had one tile of rows, and its two results met where Q lies
     int joins_before = 0;     // blocks so far that did
-    for (int count; walk.w < walk.end; walk.go(p, c, count), ++blocks) {
-        count = min(walk.end - walk.w, at.units - at.off);
-        const bool two_rows = k.rows > p.tile_rows, joins = !two_rows && count == at.units;   // two row tiles; else two key tiles
-        const int t0 = (k.hi >= 0 ? k.lo / kPtKeys : 0) + (two_rows ? at.off : 2 * at.off), items = two_rows ? 2 : 4;   // of the ring for 64 keys
+    for (; walk.w < walk.end; walk.go(p, c)) {
+        int first, count;
+        walk.share(first, count);
+        if (count == 0) continue;
+        const bool two_rows = k.rows > p.tile_rows, joins = !two_rows && walk.whole(count);   // two row tiles; else two key tiles
+        const int t0 = (k.hi >= 0 ? k.lo / kPtKeys : 0) + (two_rows ? first : 2 * first), items = two_rows ? 2 : 4;   // of the ring for 64 keys
         if (warp < kPtWarpS) {
             const int m = warp >> 2, rt = tid & (kPaRows - 1), r = two_rows ? m * p.tile_rows + rt : rt;   // tile; row of it and of the block
             const bool mine = rt < p.tile_rows && r < k.rows;
@@ -212,9 +215,9 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             }
             for (int b = 0; b < 2; ++b) tc2_wait(&o_done[m][b], (uint32_t)(turn + count - 1) & 1u, s_abort, err, 0x5700 + m);
             tc_fence_after();
-            if (count < at.units) {
+            if (!walk.whole(count)) {
                 // A part: {maximum, sum}, then the output as it stands, column by column: the lanes of a warp are neighbours there.
-                const size_t part = (size_t)blockIdx.x * 2 + (at.off > 0 ? 0 : 1);
+                const size_t part = (size_t)blockIdx.x * 2 + (first > 0 ? 0 : 1);
                 if (mine) p.ml[part * kPtRows + tid] = make_float2(m_ref, l);
                 float* dst = p.part + part * kPtRows * D + tid;
                 if (__any_sync(0xffffffffu, mine))
@@ -227,7 +230,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
 #pragma unroll
                             for (int i = 0; i < 32; ++i) dst[(d0 + i) * kPtRows] = __uint_as_float(v[i]);
                     }
-                if (tid == 0) walk.cut(p, count);
+                if (tid == 0) walk.cut(p, first, count);
             } else {
                 // Where the block's one tile has two results, the second goes to shared memory, where Q was, chunks of 16 bytes xor the row.
                 float f_own = 1.f, f_other = 0.f;
@@ -424,7 +427,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             }
         }
         was_joined = joins, joins_before += joins;
-        turn += count, ring += 2 * count * items;
+        turn += count, ring += 2 * count * items, ++blocks;
     }
     if (!box && warp >= kPtWarpLoad) asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
