@@ -54,7 +54,7 @@ static int paged_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pdl
     static bool done[64] = {};
     ZL_CHECK_CUDA(allow_smem(k_paged_attn_few<T, D, MT>, PfCfg<D>::kBytes, done));
     ZL_CHECK_CUDA(launch(k_paged_attn_few<T, D, MT>, dim3(ctas), dim3(kPfWarps * 32), PfCfg<D>::kBytes, stream, pdl, p, c));
-    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 16 * MT>, dim3(ctas, 16 * MT / kJoinRows), dim3(kJoinRows * 32), 0, stream, true, p, c));
+    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 16 * MT>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p, c));
     return ZL_OK;
 }
 
