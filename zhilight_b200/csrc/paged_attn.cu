@@ -7,8 +7,10 @@
 
 namespace zl {
 
-// Calls whose sequences bring at most so many (token, head) rows of a kv head each go to the kernel for few rows, as do groups that no tile holds a token of
-constexpr int kFewRows = 32;
+// Calls whose sequences bring at most so many (token, head) rows of a kv head each go to the kernel for few rows, as do groups that no tile holds a token of.
+// us, it / the tiles, 32 heads on 8, 2000 keys: 16 sequences with 4 rows 41 / 52, with 16 rows 42 / 52; two with 16 rows 19 / 29; one with 16 rows on 30000
+// keys 44 / 83.  A variant for 32 rows took 58 to 60 where the tiles take 53 (16 sequences; 26 / 28 for two, 66 / 70 for one on 30000 keys) and was left out.
+constexpr int kFewRows = kPfRows;
 
 struct PagedPlan {
     bool tiles;                       // on the 5th-generation tensor cores
@@ -22,8 +24,8 @@ static PagedPlan paged_plan(int rows, int max_new, int seqs, int max_keys, int h
     const long long all = (long long)rows * group, most = (long long)max_new * group;
     s.tiles = most > kFewRows && group <= kPaRows;
     s.tile_rows = s.tiles ? kPaRows / group * group : 0;
-    s.block_rows = s.tiles ? 2 * s.tile_rows : most <= 16 ? 16 : 32;
-    s.places = s.tiles ? kPtRows : s.block_rows;
+    s.block_rows = s.tiles ? 2 * s.tile_rows : kPfRows;
+    s.places = s.tiles ? kPtRows : kPfRows;
     // no more CTAs than the line can be long: every sequence adds less than one block to those of the rows, each of all the keys there is room for
     const long long units = (all / s.block_rows + seqs) * (s.tiles ? PtKind::kSetup + cdiv(max_keys, kPtKeys) : PfKind::kSetup + cdiv(max_keys, kPfKeys)) * kv_heads;
     const int most_ctas = s.tiles ? sms : kPfPerSm * sms;
@@ -49,12 +51,12 @@ static cudaError_t allow_smem(void (*kernel)(KArgs...), int bytes, bool (&done)[
     return e;
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D>
 static int paged_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pdl, zl_stream_t stream) {
     static bool done[64] = {};
-    ZL_CHECK_CUDA(allow_smem(k_paged_attn_few<T, D, MT>, PfCfg<D>::kBytes, done));
-    ZL_CHECK_CUDA(launch(k_paged_attn_few<T, D, MT>, dim3(ctas), dim3(kPfWarps * 32), PfCfg<D>::kBytes, stream, pdl, p, c));
-    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 16 * MT>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p, c));
+    ZL_CHECK_CUDA(allow_smem(k_paged_attn_few<T, D>, PfCfg<D>::kBytes, done));
+    ZL_CHECK_CUDA(launch(k_paged_attn_few<T, D>, dim3(ctas), dim3(kPfWarps * 32), PfCfg<D>::kBytes, stream, pdl, p, c));
+    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, kPfRows>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p, c));
     return ZL_OK;
 }
 
@@ -92,8 +94,7 @@ static int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool p
 
 template <typename T, int D>
 static int paged_attention(const PagedAttn& p, const PagedCache& c, const PagedPlan& s, bool pdl, zl_stream_t stream) {
-    if (s.tiles) return paged_tiles<T, D>(p, c, s.ctas, pdl, stream);
-    return s.block_rows == 16 ? paged_few<T, D, 1>(p, c, s.ctas, pdl, stream) : paged_few<T, D, 2>(p, c, s.ctas, pdl, stream);
+    return s.tiles ? paged_tiles<T, D>(p, c, s.ctas, pdl, stream) : paged_few<T, D>(p, c, s.ctas, pdl, stream);
 }
 
 }  // namespace zl

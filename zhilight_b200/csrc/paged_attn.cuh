@@ -259,75 +259,73 @@ __device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedCac
 // Blocks that were cut, of the kernel for few rows.  grid (its CTAs): the first part of a block lies in its CTA's place 1, the others in the place 0 of theirs,
 // R rows each.  A chain of three loads bounds it, so the warps share out the rows and, where there are fewer, the parts of a row too, and ask for many at
 // once; more CTAs, a row each, cost more than they give (37 blocks that nothing cuts: 13.4 -> 22.5 us a call).
-constexpr int kJoinWarps = 16, kJoinAhead = 4;
+constexpr int kJoinWarps = 16, kJoinAhead = 4;   // not fewer warps than rows
 template <typename T, int D, int R>
 __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_join(const PagedAttn p, const PagedCache c) {
     constexpr int E = D / 32;
+    static_assert(R <= kJoinWarps, "a warp for every row");
     __shared__ float s_m[kJoinWarps], s_l[kJoinWarps], s_v[kJoinWarps][D];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_trigger();
     pdl_wait();
     const PagedCut x = p.cuts[blockIdx.x];
     if (x.parts == 0) return;
-    const int rows = min(x.k.rows, kJoinWarps), each = kJoinWarps / rows, group = warp % each;   // warps of a row
-    for (int r0 = 0; r0 < x.k.rows; r0 += rows) {
-        const int r = r0 + warp / each;
-        const bool mine = warp / each < rows && r < x.k.rows;
-        auto place = [&](int s) { return ((size_t)(blockIdx.x + s) * 2 + (s == 0)) * R + r; };
-        float m = -INFINITY, l = 0.f, v[E] = {};
-        for (int s0 = group; s0 < x.parts && mine; s0 += each * kJoinAhead) {
-            float2 ml[kJoinAhead];
-            float z[kJoinAhead][E];
+    const int each = kJoinWarps / x.k.rows, group = warp % each, r = warp / each;   // warps of a row, and this one's
+    const bool mine = r < x.k.rows;
+    auto place = [&](int s) { return ((size_t)(blockIdx.x + s) * 2 + (s == 0)) * R + r; };
+    float m = -INFINITY, l = 0.f, v[E] = {};
+    for (int s0 = group; s0 < x.parts && mine; s0 += each * kJoinAhead) {
+        float2 ml[kJoinAhead];
+        float z[kJoinAhead][E];
 #pragma unroll
-            for (int u = 0; u < kJoinAhead; ++u) {
-                const int s = s0 + u * each;
-                ml[u] = make_float2(-INFINITY, 0.f);
-                if (s < x.parts) {
-                    ml[u] = p.ml[place(s)];
-                    const float* from = p.part + place(s) * D + lane * E;
+        for (int u = 0; u < kJoinAhead; ++u) {
+            const int s = s0 + u * each;
+            ml[u] = make_float2(-INFINITY, 0.f);
+            if (s < x.parts) {
+                ml[u] = p.ml[place(s)];
+                const float* from = p.part + place(s) * D + lane * E;
 #pragma unroll
-                    for (int e = 0; e < E; e += 2) *reinterpret_cast<float2*>(&z[u][e]) = *reinterpret_cast<const float2*>(from + e);
-                }
+                for (int e = 0; e < E; e += 2) *reinterpret_cast<float2*>(&z[u][e]) = *reinterpret_cast<const float2*>(from + e);
             }
-            float up = m;
+        }
+        float up = m;
 #pragma unroll
-            for (int u = 0; u < kJoinAhead; ++u) up = fmaxf(up, ml[u].x);
+        for (int u = 0; u < kJoinAhead; ++u) up = fmaxf(up, ml[u].x);
+        const float f = exp2f(m - up);
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= f;
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; ++u) {
+            if (s0 + u * each >= x.parts) break;
+            const float g = exp2f(ml[u].x - up);
+            l = fmaf(ml[u].y, g, l);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = fmaf(z[u][e], g, v[e]);
+        }
+        m = up;
+    }
+    if (each > 1) {
+        if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_v[warp][lane * E + e] = v[e];
+        __syncthreads();
+        if (group == 0 && mine) {
+            float up = m;
+            for (int w = 1; w < each; ++w) up = fmaxf(up, s_m[warp + w]);
             const float f = exp2f(m - up);
             l *= f;
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] *= f;
+            for (int w = 1; w < each; ++w) {
+                const float g = s_m[warp + w] == -INFINITY ? 0.f : exp2f(s_m[warp + w] - up);   // a warp without a part
+                l = fmaf(s_l[warp + w], g, l);
 #pragma unroll
-            for (int u = 0; u < kJoinAhead; ++u) {
-                if (s0 + u * each >= x.parts) break;
-                const float g = exp2f(ml[u].x - up);
-                l = fmaf(ml[u].y, g, l);
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = fmaf(z[u][e], g, v[e]);
-            }
-            m = up;
-        }
-        if (each > 1) {
-            if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-#pragma unroll
-            for (int e = 0; e < E; ++e) s_v[warp][lane * E + e] = v[e];
-            __syncthreads();
-            if (group == 0 && mine) {
-                float up = m;
-                for (int w = 1; w < each; ++w) up = fmaxf(up, s_m[warp + w]);
-                const float f = exp2f(m - up);
-                l *= f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] *= f;
-                for (int w = 1; w < each; ++w) {
-                    const float g = s_m[warp + w] == -INFINITY ? 0.f : exp2f(s_m[warp + w] - up);   // a warp without a part
-                    l = fmaf(s_l[warp + w], g, l);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) v[e] = fmaf(s_v[warp + w][lane * E + e], g, v[e]);
-                }
+                for (int e = 0; e < E; ++e) v[e] = fmaf(s_v[warp + w][lane * E + e], g, v[e]);
             }
         }
-        if (group == 0 && mine) paged_row_out<T, D>(p, c, x.k, x.hk, r, l, v);
     }
+    if (group == 0 && mine) paged_row_out<T, D>(p, c, x.k, x.hk, r, l, v);
 }
 
 }  // namespace zl

@@ -1,5 +1,5 @@
 // Attention of few (token, head) rows of a kv head -- single tokens, drafts of small groups -- over pages: bound by the bytes of K and V, which the CTAs
-// of the grid share out evenly, whatever the sequences' lengths are.  All tiles of 64 keys of all blocks (16 or 32 rows of one kv head of one sequence)
+// of the grid share out evenly, whatever the sequences' lengths are.  All tiles of 64 keys of all blocks (up to 16 rows of one kv head of one sequence)
 // stand in one line; a CTA takes an equal stretch of it.  A block that lies in one stretch is written at once, the parts of one that is cut go to the
 // workspace, its first part to the CTA's place 1, others to its place 0, and k_paged_join puts them together.
 //
@@ -13,7 +13,7 @@
 
 namespace zl {
 
-constexpr int kPfWarps = 4, kPfKeys = 16 * kPfWarps, kPfStages = 3, kPfPerSm = 2;
+constexpr int kPfWarps = 4, kPfKeys = 16 * kPfWarps, kPfStages = 3, kPfPerSm = 2, kPfRows = 16;
 
 template <int D>
 struct PfCfg {
@@ -52,11 +52,11 @@ __device__ __forceinline__ uint32_t pf_pack(float a, float b) {
 }
 
 // grid: CTAs that share the line
-template <typename T, int D, int MT>
+template <typename T, int D>
 __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(const PagedAttn p, const PagedCache c) {
     using C = PfCfg<D>;
     constexpr bool kHalf = std::is_same<T, __half>::value;
-    constexpr int R = 16 * MT, CH = D / 8, KS = D / 16;
+    constexpr int R = kPfRows, CH = D / 8, KS = D / 16;
     constexpr float kTau = kHalf ? 5.f : 8.f, kUp = kHalf ? 10.f : 0.f;
     extern __shared__ __align__(128) uint8_t pf_smem[];
     __shared__ float2 s_ml[kPfWarps][R];
@@ -111,28 +111,23 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
             id = next;
         }
         // rows of q: (g, g + 8) of each 16
-        uint32_t qa[MT][KS][4];
-        int hi[MT][2], lo[MT][2];
+        uint32_t qa[KS][4];
+        int hi[2], lo[2];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int u = 0; u < 2; ++u) {
+            const int r = g + u * 8;
+            const bool in = r < k.rows;
+            const int row = k.row0 + (in ? r : 0), t = p.by_group(row), place = k.place0 + t;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + ((size_t)(k.first + t) * p.heads + at.hk * p.group + row - t * p.group) * D);
+            hi[u] = in ? min(place, k.have - 1) : -1;
+            lo[u] = p.window ? max(0, place - p.window + 1) : 0;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int r = m * 16 + g + u * 8;
-                const bool in = r < k.rows;
-                const int row = k.row0 + (in ? r : 0), t = p.by_group(row), place = k.place0 + t;
-                const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + ((size_t)(k.first + t) * p.heads + at.hk * p.group + row - t * p.group) * D);
-                hi[m][u] = in ? min(place, k.have - 1) : -1;
-                lo[m][u] = p.window ? max(0, place - p.window + 1) : 0;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) qa[m][s][u] = in ? src[s * 8 + t4] : 0u, qa[m][s][2 + u] = in ? src[s * 8 + 4 + t4] : 0u;
-            }
-        float o[MT][D / 8][4], l[MT][2], m_ref[MT][2];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
-            l[m][0] = l[m][1] = 0.f, m_ref[m][0] = m_ref[m][1] = -1.4426950e20f;
+            for (int s = 0; s < KS; ++s) qa[s][u] = in ? src[s * 8 + t4] : 0u, qa[s][2 + u] = in ? src[s * 8 + 4 + t4] : 0u;
         }
+        float o[D / 8][4], l[2], m_ref[2];
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        l[0] = l[1] = 0.f, m_ref[0] = m_ref[1] = -1.4426950e20f;
         for (int j = 0; j < count; ++j) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kPfStages - 2) : "memory");
             __syncwarp();
@@ -143,7 +138,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
             const int kb = key0 + j * kPfKeys;
             if (kb > k.hi || kb + 15 < k.lo) continue;
             const uint32_t st = ring_at + (uint32_t)(j % kPfStages) * C::kStage;
-            float s[MT][2][4] = {};
+            float s[2][4] = {};
             {
                 // matrices of 8 keys x 8 columns: (keys 0-7, first 8), (0-7, next 8), (8-15, first 8), (8-15, next 8)
                 const int r = (lane & 7) + ((lane >> 4) << 3), ch0 = (lane >> 3) & 1;
@@ -151,48 +146,44 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 for (int i = 0; i < KS; ++i) {
                     uint32_t b[4];
                     pf_ldsm(b, st + (uint32_t)(r * (D * 2) + (((2 * i + ch0) ^ (r & 7)) << 4)));
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) pf_mma<T>(s[m][0], qa[m][i], b[0], b[1]), pf_mma<T>(s[m][1], qa[m][i], b[2], b[3]);
+                    pf_mma<T>(s[0], qa[i], b[0], b[1]), pf_mma<T>(s[1], qa[i], b[2], b[3]);
                 }
             }
-            uint32_t pa[MT][4];
+            uint32_t pa[4];
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int e = 0; e < 4; ++e) {
+                    const int key = kb + n * 8 + t4 * 2 + (e & 1);
+                    s[n][e] = key <= hi[e >> 1] && key >= lo[e >> 1] ? s[n][e] * p.scale : -INFINITY;
+                }
+            bool up = false;
+            float top[2];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = kb + n * 8 + t4 * 2 + (e & 1);
-                        s[m][n][e] = key <= hi[m][e >> 1] && key >= lo[m][e >> 1] ? s[m][n][e] * p.scale : -INFINITY;
-                    }
-                bool up = false;
-                float top[2];
+            for (int u = 0; u < 2; ++u) {
+                top[u] = fmaxf(fmaxf(s[0][2 * u], s[0][2 * u + 1]), fmaxf(s[1][2 * u], s[1][2 * u + 1]));
+                up |= top[u] > m_ref[u] + kTau;
+            }
+            if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    top[u] = fmaxf(fmaxf(s[m][0][2 * u], s[m][0][2 * u + 1]), fmaxf(s[m][1][2 * u], s[m][1][2 * u + 1]));
-                    up |= top[u] > m_ref[m][u] + kTau;
+                    top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
+                    top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
+                    const float f = top[u] > m_ref[u] ? pf_exp2(m_ref[u] - top[u]) : 1.f;
+                    m_ref[u] = fmaxf(m_ref[u], top[u]);
+                    l[u] *= f;
+#pragma unroll
+                    for (int n = 0; n < D / 8; ++n) o[n][2 * u] *= f, o[n][2 * u + 1] *= f;
                 }
-                if (__any_sync(0xffffffffu, up)) {
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
-                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
-                        const float f = top[u] > m_ref[m][u] ? pf_exp2(m_ref[m][u] - top[u]) : 1.f;
-                        m_ref[m][u] = fmaxf(m_ref[m][u], top[u]);
-                        l[m][u] *= f;
-#pragma unroll
-                        for (int n = 0; n < D / 8; ++n) o[m][n][2 * u] *= f, o[m][n][2 * u + 1] *= f;
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float x = pf_exp2(s[m][n][2 * u] + (kUp - m_ref[m][u])), y = pf_exp2(s[m][n][2 * u + 1] + (kUp - m_ref[m][u]));
-                        l[m][u] += x + y;
-                        pa[m][2 * n + u] = pf_pack<T>(x, y);
-                    }
             }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float x = pf_exp2(s[n][2 * u] + (kUp - m_ref[u])), y = pf_exp2(s[n][2 * u + 1] + (kUp - m_ref[u]));
+                    l[u] += x + y;
+                    pa[2 * n + u] = pf_pack<T>(x, y);
+                }
             {
                 // transposed: (keys 0-7, first 8 columns), (keys 8-15, first 8), (0-7, next 8), (8-15, next 8)
                 const int r = (lane & 7) + (((lane >> 3) & 1) << 3), ch0 = lane >> 4;
@@ -200,8 +191,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 for (int n = 0; n < D / 8; n += 2) {
                     uint32_t b[4];
                     pf_ldsm_t(b, st + (uint32_t)(16 * D * 2 + r * (D * 2) + (((n + ch0) ^ (r & 7)) << 4)));
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) pf_mma<T>(o[m][n], pa[m], b[0], b[1]), pf_mma<T>(o[m][n + 1], pa[m], b[2], b[3]);
+                    pf_mma<T>(o[n], pa, b[0], b[1]), pf_mma<T>(o[n + 1], pa, b[2], b[3]);
                 }
             }
         }
@@ -210,17 +200,15 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
         __syncwarp();
         float* mine = reinterpret_cast<float*>(ring);
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int u = 0; u < 2; ++u) {
+            const int r = g + u * 8;
+            float sum = l[u];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (t4 == 0) s_ml[warp][r] = make_float2(m_ref[u], sum);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int r = m * 16 + g + u * 8;
-                float sum = l[m][u];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (t4 == 0) s_ml[warp][r] = make_float2(m_ref[m][u], sum);
-#pragma unroll
-                for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(mine + r * C::kPitch + n * 8 + t4 * 2) = make_float2(o[m][n][2 * u], o[m][n][2 * u + 1]);
-            }
+            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(mine + r * C::kPitch + n * 8 + t4 * 2) = make_float2(o[n][2 * u], o[n][2 * u + 1]);
+        }
         __syncthreads();
         const bool whole = walk.whole(count);
         const size_t part = ((size_t)blockIdx.x * 2 + (first > 0 ? 0 : 1)) * R;
