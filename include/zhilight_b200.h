@@ -1138,7 +1138,7 @@ int zl_qkv_axes_rope_append(const void* qkv, long long ldq, const int32_t* pos, 
  * stands at place p = seq_lens[b] - n + i and sees the keys j <= p that the sequence has, with window > 0 those with j > p - window only;
  * out = softmax(scale q k) v, zeros where a row sees nothing.  Rows of q of no sequence: out stays as it is.  seq_lens counts the new tokens, whose
  * keys and values are appended already.  What masked keys and values hold (infinities, NaN) does not matter.  max_new: a bound of the sequences' new
- * tokens, which chooses the kernels; results do not depend on it.  scale > 0; dim 64 or 128; dtype fp16 or bf16. */
+ * tokens, which chooses the kernels (results agree within their rounding).  scale > 0; dim 64 or 128; dtype fp16 or bf16. */
 size_t zl_paged_attention_workspace_bytes(int rows, int max_new, int seqs, int max_keys /* max_pages * page_size */, int heads, int kv_heads, int dim);
 int zl_paged_attention(const void* q, const void* k_cache, const void* v_cache, long long num_pages, int page_size, long long page_stride,
                        long long row_stride, long long head_stride, const int32_t* page_table, int ld_table, int max_pages,

@@ -220,6 +220,48 @@ def test_attention_rows_before_a_broken_token(cuda, bad, new, dim, window):
                 assert not torch.isfinite(got[sees][:, heads // 2:, 5]).any()
 
 
+@pytest.mark.parametrize("new,heads", [(1, 8), (20, 8), (70, 8), (9, 2)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_blocks_with_broken_tokens(cuda, new, heads, bad):
+    """Enough sequences for whole blocks in a CTA: values that are no numbers, in the last new token of every third sequence, stay with its row."""
+    g = torch.Generator().manual_seed(9)
+    kv_heads, dim, page, seqs = 2, 64, 32, 90
+    lens = [new + 40 + 7 * (i % 5) for i in range(seqs)]
+    pages = sum(-(-n // page) for n in lens)
+    table, starts = tables(g, lens, page, pages), starts_of([new] * seqs)
+    q = torch.randn(seqs * new, heads, dim, generator=g).to(BF16)
+    k, v = pool(g, pages, page, kv_heads, dim, BF16, "rows")
+    for i in range(0, seqs, 3):
+        v[int(table[i, (lens[i] - 1) // page]), (lens[i] - 1) % page, 0, 7] = bad
+    got = ops.paged_attention(q.cuda(), *on_gpu(k, v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), starts.cuda(), dim ** -0.5, max_new=new).cpu().double()
+    want, off = oracle.attention(q, k, v, table, lens, starts, dim ** -0.5, 0)
+    fine = torch.ones(want.shape, dtype=torch.bool)
+    fine[new - 1::3 * new, :heads // 2, 7] = False
+    assert ((got - want).abs() <= off)[fine].all()
+    assert not torch.isfinite(got[~fine]).any()
+
+
+@pytest.mark.parametrize("new,heads,kv_heads", [(1, 4, 2), (3, 4, 1), (20, 8, 2)])
+def test_attention_of_many_sequences(cuda, new, heads, kv_heads):
+    """More sequences than a warp looks at at a time, some without tokens or keys, also at the ends of what is in view."""
+    seqs = [(1 + (37 * i) % 150 + new, 1 + i % new) if i % 11 and i not in (127, 128, 255) else (i % 2 * 30, 0) for i in range(300)]
+    check_attention(F16, heads, kv_heads, 64, 16, "rows", 0, seqs, max_new=new)
+    check_attention(F16, heads, kv_heads, 64, 16, "heads", 33, seqs[:129], max_new=new)
+
+
+@pytest.mark.parametrize("window", [0, 700])
+def test_attention_of_a_sequence_of_many_blocks(cuda, window):
+    """Blocks that a warp looks at 32 at a time, beside sequences of a few."""
+    check_attention(BF16, 2, 1, 64, 64, "rows", window, [(50, 20), (4500, 4400), (300, 300), (1300, 1200)])
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(160, 1), (129, 1), (256, 2), (128, 1), (65, 1)])
+@pytest.mark.parametrize("new", [1, 3])
+def test_attention_of_wide_groups(cuda, heads, kv_heads, new):
+    """Groups with more heads than a tile has rows, and those of one token a tile."""
+    check_attention(BF16, heads, kv_heads, 64, 16, "rows", 0, [(100, new), (new, new), (300, new)], max_new=new)
+
+
 def test_attention_with_equal_rows_and_large_scores(cuda):
     """One score far above the others, and all of them equal: no overflow, no loss."""
     g = torch.Generator().manual_seed(6)
