@@ -241,6 +241,15 @@ def test_attention_blocks_with_broken_tokens(cuda, new, heads, bad):
     assert not torch.isfinite(got[~fine]).any()
 
 
+@pytest.mark.parametrize("page", [4, 8, 12, 20, 24, 28, 40, 48, 56, 72, 100, 136])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_over_pages_of_any_size(cuda, page, dim):
+    """Page borders anywhere in the tiles of blocks of one and of two tiles, for more pages than a warp holds the numbers of."""
+    seqs = [(2600 + 100 * i, 1 + 5 * i) for i in range(5)] + [(1500, 200), (700, 70)]
+    check_attention(BF16, 16, 2, dim, page, "rows", 0, seqs, max_new=200)
+    check_attention(F16, 16, 2, dim, page, "heads", 1000, seqs[:4], max_new=16)
+
+
 @pytest.mark.parametrize("new,heads,kv_heads", [(1, 4, 2), (3, 4, 1), (20, 8, 2)])
 def test_attention_of_many_sequences(cuda, new, heads, kv_heads):
     """More sequences than a warp looks at at a time, some without tokens or keys, also at the ends of what is in view."""

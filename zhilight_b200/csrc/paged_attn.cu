@@ -77,7 +77,7 @@ static int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool p
     // boxes of K and V: the rows that a tile and a page have in common wherever they meet
     int box = 1;
     while (box < kPtHalf && c.page_size % (2 * box) == 0) box *= 2;
-    if (box < 8) box = 0;
+    if (box < 4 || c.page_size < 8) box = 0;   // a turn's 256 keys in the 32 pages that a warp's lanes know; smaller boxes are more copies than 16 bytes at a time save
     if (box) {
         auto step = [](long long elements, bool more) { return more ? (uint64_t)elements * 2 : (uint64_t)(D * 2); };   // of one alone none is taken
         const uint64_t dims[4] = {(uint64_t)D, (uint64_t)c.page_size, (uint64_t)p.kv_heads, (uint64_t)c.num_pages};

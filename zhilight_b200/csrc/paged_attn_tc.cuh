@@ -7,7 +7,7 @@
 //   warp 8          one thread issues S = Q K^T of both tiles, 64 keys at a time into two buffers each
 //   warp 9          one thread issues O += P V of both tiles (P from tensor memory, V as it lies: rows of keys, the B operand along n)
 //   warps 10, 11    Q by TMA, once for a block; K and V, a warp each, from the pages into a ring of tiles of 64 keys by TMA, a box for the rows of a tile
-//                   that one page has (where that is no multiple of 8 rows, of the swizzle's period, both copy 16 bytes at a time)
+//                   that one page has (where these are fewer than four, or a page has fewer than 8, both copy 16 bytes at a time)
 //
 // A page's rows behind the last visible key may hold anything.  Copies of 16 bytes leave them out; behind TMA the softmax's threads make those values zeros
 // before they hand the tile's probabilities on.  Rows behind a page number outside the pool are zeros either way.  Tensor memory: scores of the two tiles (128 columns each, probabilities over their first
@@ -380,7 +380,8 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 __syncwarp();
             };
             if (box) {
-                // One warp for keys, one for values; a lane for each box of a tile, its rows and 64 columns.  The lanes hold the numbers of 32 pages in a row.
+                // One warp for keys, one for values; a lane for each box of a tile, its rows and 64 columns.  The lanes hold the numbers of 32 pages in
+                // a row, which is a turn's keys at least.
                 const bool is_v = warp != kPtWarpLoad;
                 const int boxes = kPtHalf / box, b_row = lane % boxes * box, last_page = min(c.by_page(max(k.hi, 0)), c.max_pages - 1);
                 int page0 = -32, ids = -1;
@@ -389,7 +390,8 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                     for (int m = 0; m < (two_rows ? 1 : 2); ++m) {
                         const int i = j * items + (two_rows ? (is_v ? 1 : 0) : (is_v ? 2 : 0) + m), it = ring + i, slot = it % C::kRing;
                         const int row0 = row_of(i), row = row0 + b_row, pg = c.by_page(row);
-                        if (c.by_page(row0 + kPtHalf - 1) >= page0 + 32) {
+                        // those of a whole turn, whose tiles are not in the order of their keys
+                        if (m == 0 && !(j & 1) && c.by_page(row0 + (two_rows ? kPtKeys : 2 * kPtKeys) - 1) >= page0 + 32) {
                             page0 = c.by_page(row0);
                             ids = page0 + lane <= last_page ? c.table[(size_t)k.seq * c.ld_table + page0 + lane] : -1;
                         }
@@ -463,20 +465,29 @@ __global__ void __launch_bounds__(256) k_paged_join_tiles(const PagedAttn p, con
     const bool twice = x.k.rows <= p.tile_rows, mine = r < x.k.rows;
     const int row = r >= p.tile_rows ? r - p.tile_rows + kPaRows : r;   // not more than 255
     float m = -INFINITY, l = 0.f, v[W] = {};
-    // as the softmax goes, from part to part
-    for (int s = 0; s < (twice ? 2 * x.parts : x.parts); ++s) {
-        const int i = twice ? s >> 1 : s;
-        const size_t part = (size_t)(blockIdx.x + i) * 2 + (i == 0);
-        const int at = min(row + (twice && (s & 1) ? kPaRows : 0), kPtRows - 1);
-        const float2 y = p.ml[part * kPtRows + at];
-        float z[W];
+    // as the softmax goes, from part to part, the loads of two at once
+    const int parts = twice ? 2 * x.parts : x.parts;
+    for (int s0 = 0; s0 < parts; s0 += 2) {
+        float2 y[2];
+        float z[2][W];
 #pragma unroll
-        for (int u = 0; u < W; ++u) z[u] = p.part[(part * D + d0 + u) * kPtRows + at];
-        const float up = fmaxf(m, y.x), f = pa_exp2(m - up), g = pa_exp2(y.x - up);
-        m = up;
-        l = fmaf(y.y, g, l * f);
+        for (int h = 0; h < 2; ++h) {
+            const int s = min(s0 + h, parts - 1), i = twice ? s >> 1 : s;
+            const size_t part = (size_t)(blockIdx.x + i) * 2 + (i == 0);
+            const int at = min(row + (twice && (s & 1) ? kPaRows : 0), kPtRows - 1);
+            y[h] = p.ml[part * kPtRows + at];
 #pragma unroll
-        for (int u = 0; u < W; ++u) v[u] = fmaf(z[u], g, v[u] * f);
+            for (int u = 0; u < W; ++u) z[h][u] = p.part[(part * D + d0 + u) * kPtRows + at];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (s0 + h >= parts) break;
+            const float up = fmaxf(m, y[h].x), f = pa_exp2(m - up), g = pa_exp2(y[h].x - up);
+            m = up;
+            l = fmaf(y[h].y, g, l * f);
+#pragma unroll
+            for (int u = 0; u < W; ++u) v[u] = fmaf(z[h][u], g, v[u] * f);
+        }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     bool bad = false;
