@@ -407,31 +407,53 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                     }
                 }
             } else if (!box) {
-                // two rows (four of 64 columns) a copy of a warp; a lane looks up every 32nd row
-                const int ch = lane % CH;
+                // Two rows (four of 64 columns) a copy of a warp.  A lane looks up every 32nd row of the 64 keys, once for K and V, and asks for the next ones'
+                // page numbers before it copies these.
+                const int ch = lane % CH, tiles = two_rows ? 1 : 2;
                 constexpr int kRowsAtOnce = 32 / CH;
-                for (int i = 0; i < 2 * count * items; ++i) {
-                    if (i == items) load_q();
-                    const int it = ring + i, slot = it % C::kRing;
-                    const bool is_v = two_rows ? i & 1 : i & 2;
-                    long long offs[kPtHalf / 32];
+                int ids[2][kPtHalf / 32];
+                auto ask = [&](int j) {
 #pragma unroll
-                    for (int u = 0; u < kPtHalf / 32; ++u) {
-                        const int row = row_of(i) + u * 32 + lane;
-                        offs[u] = row <= k.hi ? c.row_at(k.seq, row) : -1;
-                    }
-                    if (it >= C::kRing) ok = ok && tc2_wait(&empty[slot], (uint32_t)(it / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
-                    if (!ok) break;
-                    const T* from = static_cast<const T*>(is_v ? c.v : c.k) + (long long)at.hk * c.head_stride + ch * 8;
-                    const uint32_t to = smem_u32(smem) + (uint32_t)(C::kRingOff + slot * C::kTile + (ch >> 3) * (kPtHalf * 128));
+                    for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int u = 0; u < kPtHalf / 32; ++u)
-                        for (int x = (warp - kPtWarpLoad) * kRowsAtOnce; x < 32; x += 2 * kRowsAtOnce) {
-                            const int r = x + lane / CH;
-                            const long long off = __shfl_sync(0xffffffffu, offs[u], r);
-                            pa_cp16(to + (uint32_t)((u * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4)), from + (off < 0 ? 0 : off), off >= 0);
+                        for (int u = 0; u < kPtHalf / 32; ++u) {
+                            const int row = row_of(j * items + m) + u * 32 + lane, pg = c.by_page(row);
+                            ids[m][u] = m < tiles && j < 2 * count && row <= k.hi && pg < c.max_pages ? c.table[(size_t)k.seq * c.ld_table + pg] : -1;
                         }
-                    pa_landed(&full[slot]);
+                };
+                ask(0);
+                for (int j = 0; j < 2 * count && ok; ++j) {
+                    if (j == 1) load_q();
+                    long long offs[2][kPtHalf / 32];
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int u = 0; u < kPtHalf / 32; ++u) {
+                            const int row = row_of(j * items + m) + u * 32 + lane, id = ids[m][u];
+                            offs[m][u] = id >= 0 && id < c.num_pages ? (long long)id * c.page_stride + (long long)(row - c.by_page(row) * c.page_size) * c.row_stride : -1;
+                        }
+                    ask(j + 1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i >= items) break;
+                        const int it = ring + j * items + i, slot = it % C::kRing;
+                        const bool is_v = two_rows ? i & 1 : i & 2;
+                        if (it >= C::kRing) ok = ok && tc2_wait(&empty[slot], (uint32_t)(it / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
+                        if (!ok) break;
+                        const T* from = static_cast<const T*>(is_v ? c.v : c.k) + (long long)at.hk * c.head_stride + ch * 8;
+                        const uint32_t to = smem_u32(smem) + (uint32_t)(C::kRingOff + slot * C::kTile + (ch >> 3) * (kPtHalf * 128));
+#pragma unroll
+                        for (int u = 0; u < kPtHalf / 32; ++u) {
+                            const long long mine = two_rows || !(i & 1) ? offs[0][u] : offs[1][u];
+#pragma unroll 4
+                            for (int x = (warp - kPtWarpLoad) * kRowsAtOnce; x < 32; x += 2 * kRowsAtOnce) {
+                                const int r = x + lane / CH;
+                                const long long off = __shfl_sync(0xffffffffu, mine, r);
+                                pa_cp16(to + (uint32_t)((u * 32 + r) * 128 + (((ch & 7) ^ (r & 7)) << 4)), from + (off < 0 ? 0 : off), off >= 0);
+                            }
+                        }
+                        pa_landed(&full[slot]);
+                    }
                 }
             }
         }
