@@ -24,6 +24,7 @@ def append_args(**kw):
     (dict(qkv=None), -1), (dict(T=0), -1), (dict(half=65), -1), (dict(axes=0), -1), (dict(ld_pos=3), -1), (dict(layout=2), -1), (dict(ldq=767), -1),
     (dict(ldq=772), -2), (dict(page_stride=2044), -2), (dict(page_size=0), -1), (dict(num_pages=0), -1), (dict(ld_table=3), -1), (dict(seqs=0), -1),
     (dict(k_cache=ctypes.c_void_p(8)), -2), (dict(dtype=ops.F32), -2), (dict(dim=132, half=4, ldq=2000), -2), (dict(axis=None), -1), (dict(row_stride=-8), -1),
+    (dict(heads=900, ldq=902 * 128), -2),
 ])
 def test_append_refuses(lib, kw, code):
     assert lib.zl_qkv_axes_rope_append(*append_args(**kw)) == code, lib.zl_last_error()

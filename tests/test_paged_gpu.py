@@ -62,7 +62,8 @@ def hide(cache, table, lens, value):
 @pytest.mark.parametrize("heads,kv_heads,dim,half,adjacent,page,order,t", [
     (32, 8, 128, 64, False, 16, "rows", 1), (32, 8, 128, 64, False, 16, "heads", 37), (4, 4, 64, 16, True, 1, "rows", 9), (6, 2, 64, 20, False, 5, "both", 33),
     (7, 1, 72, 13, True, 20, "rows", 12), (3, 3, 8, 4, False, 3, "heads", 5), (2, 1, 64, 0, False, 16, "rows", 4), (64, 8, 128, 48, False, 64, "rows", 70),
-    (1, 1, 1024, 512, True, 2, "rows", 3), (1, 1, 256, 128, False, 7, "heads", 300)])
+    (1, 1, 1024, 512, True, 2, "rows", 3), (1, 1, 256, 128, False, 7, "heads", 300),
+    (128, 128, 128, 64, False, 16, "heads", 5), (256, 128, 128, 32, True, 8, "rows", 400), (64, 8, 128, 64, False, 16, "both", 2000)])
 def test_append(cuda, dtype, heads, kv_heads, dim, half, adjacent, page, order, t):
     g = torch.Generator().manual_seed(heads * 1000 + t)
     lens = [t, t + 11, 2 * t]
@@ -454,6 +455,35 @@ def test_step_captured_and_replayed(cuda):
         torch.cuda.synchronize()
         for s, out in zip(steps, outs):
             s.check(out)
+
+
+@pytest.mark.parametrize("rows,max_new", [(12, 4), (260, None)])
+def test_attention_replayed_with_other_lengths(cuda, rows, max_new):
+    """A graph takes lengths, starts and pages as they are when it is replayed."""
+    g = torch.Generator().manual_seed(12)
+    heads, kv_heads, dim, page = 4, 2, 64, 16
+    k, v = pool(g, 120, page, kv_heads, dim, BF16, "rows")
+    kd, vd = on_gpu(k, v)
+    q = torch.randn(rows, heads, dim, generator=g).to(BF16)
+    steps = []
+    for shares in ((rows // 4,) * 4, (1, rows - 3, 0, 2), (0, 0, 3, 1)) if max_new is None else ((3, 3, 3, 3), (1, 4, 0, 2), (4, 4, 4, 0)):
+        lens = [n + 100 * (i + 1) for i, n in enumerate(shares)]
+        steps.append((tables(g, lens, page, 120, extra=0), lens, starts_of(shares)))
+    table, lens, starts = torch.full((4, 50), -1, dtype=torch.int32).cuda(), torch.zeros(4, dtype=torch.int32).cuda(), torch.zeros(5, dtype=torch.int32).cuda()
+    out, dq, graph = torch.zeros_like(q).cuda(), q.cuda(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_attention(dq, kd, vd, table, lens, starts, dim ** -0.5, max_new=max_new, out=out)
+    for t, n, s in steps:
+        table[:, :t.shape[1]].copy_(t)
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        starts.copy_(s)
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        used = int(s[-1])
+        want, off = oracle.attention(q, k, v, t, n, s, dim ** -0.5, 0)
+        got = out.cpu().double()
+        assert ((got - want).abs() <= off)[:used].all() and (got[used:] == 7.0).all()
 
 
 def test_steps_on_two_streams(cuda):
