@@ -18,7 +18,7 @@
 // A masked probability is exactly zero, but zero times an infinity or NaN that a row must not see (a later token's value) is NaN in its sum.  A row that
 // comes out as NaN is therefore done once more from the definition, key by key (paged_row_exact); numbers never take that path.
 //
-// 4096 tokens behind 4096, 32 heads on 8, bf16: 390 to 450 us by the box, 0.92 to 1.06 PFLOP/s.  A turn takes 3000 cycles, of which the MMAs need 2050 at least and
+// 4096 tokens behind 4096, 32 heads on 8, bf16: 390 to 450 us by the GPU it ran on, 0.92 to 1.06 PFLOP/s.  A turn takes 3000 cycles, of which the MMAs need 2050 at least and
 // the exponentials of both groups 2050; under this load the SM runs at 1.2 GHz.  Before, the same in us: copies of 16 bytes by two warps 693 (they bound it),
 // TMA 544, scores of 64 keys ahead of the softmax in two buffers 503 (128 keys at a time leave no room for a second one, and S -> softmax -> P V is
 // then one chain of 4400 cycles), a thread each for S and P V 434, Q and the first scores under the results of the block before 420, parts column by column 395.

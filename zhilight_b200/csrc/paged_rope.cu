@@ -7,7 +7,7 @@
 // place, and bulk copies take them on to q and to the pages (values go by untouched).  One thread for each frequency works out the next token's cosine and
 // sine meanwhile.  Angle and reduction are in 64 bits (at position 4e6 a 32-bit angle is off by 0.25 rad): the angle in turns, less the nearest whole
 // number, is exact to 1e-9 of a turn, and what is left of it goes through CUDA's 32-bit functions (within 2e-7).  Products and sums are in 32 bits,
-// rounded once.  Bound by bytes, a row is read once and written once: 4525 rows of 32 + 2 * 8 heads of 128 (111 MB) 21.5 to 23 us by the box, 4.8 to 5.2 TB/s,
+// rounded once.  Bound by bytes, a row is read once and written once: 4525 rows of 32 + 2 * 8 heads of 128 (111 MB) 21.5 to 23 us by the GPU it ran on, 4.8 to 5.2 TB/s,
 // where an elementwise product of as many bytes takes 19.5; through registers, a row ahead, 25 to 31.  A third row ahead gives nothing (22.5).
 #include "attn_ptx.cuh"
 #include "paged.cuh"

@@ -3,7 +3,7 @@
 // from the weights max(p - q, 0) of that row, behind the last draft from p itself: the first index whose running sum passes u * (sum of all).
 //
 // Only that one row of p and q is read whole.  The CTAs of a cluster share the vocabulary, a warp has a run of neighbouring words: a pass for the sums
-// of the warps, which every CTA gets from the others' shared memory, then the one warp whose run holds the word goes over its run once more.
+// of the warps, which every CTA gets from the others' shared memory, then the CTA that has the word's run goes over that run once more.
 // Differences, products and sums are in 64 bits: products of two 32-bit numbers are exact there, sums of probabilities above 2^-29 too, and
 // a tie falls as the formula says.  Bound by bytes, the latency of a chain of three loads and a cluster's barrier where there are few sequences:
 // 64 sequences of 128256 words 15.4 us (65.7 MB: 4.3 TB/s), one of 32000 7.1 us.  Eight warps of 16 loads ahead; 16 warps of 8, of which an SM holds three
