@@ -5,9 +5,10 @@
 //
 // A warp has 16 keys of a tile to itself, in a ring of its own (16-byte cp.async; no barrier between the warps until a block's end):
 // S = Q K^T and O += P V by mma.sync with Q as the 16-row operand, whose accumulators are the next product's operand as they stand.  The probabilities are
-// rounded to the type of the rows, their sum is not; the reference maximum of a row follows lazily as in paged_attn_tc.cuh.
+// carried as a 16-bit value and the rest of it as another, their sum in 32 bits; the reference maximum of a row follows lazily as in paged_attn_tc.cuh.
 //
-// One token over 131072 keys, 32 heads on 8: 87 us (6.2 TB/s of the 6.45 that a copy reaches), 101 with the join.  32 sequences up to 4096 keys: 43 and 49 us for
+// One token over 131072 keys, 32 heads on 8: 89 us (6.0 TB/s of the 6.45 that a copy reaches), 103 with the join; 101 with probabilities of 16 bits alone, whose
+// results are 1.4 times as far from 64 bits.  32 sequences up to 4096 keys: 43 and 49 us for
 // 174 MB, behind the first loads of every block: its setup stands in the line as two tiles (64 us where it did not).  Two CTAs share an SM, one's
 // first loads and joins come under the other's stream.  Q by way of shared memory, for fewer registers, is slower (101 -> 108, 49 -> 57), and so is one warp that finds the
 // way for all (49 -> 53).
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                     pf_mma<T>(s[0], qa[i], b[0], b[1]), pf_mma<T>(s[1], qa[i], b[2], b[3]);
                 }
             }
-            uint32_t pa[4];
+            uint32_t pa[4], pb[4];   // probabilities, and what their rounding left of them
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -188,6 +189,8 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                     const float x = pf_exp2(s[n][2 * u] + (kUp - m_ref[u])), y = pf_exp2(s[n][2 * u + 1] + (kUp - m_ref[u]));
                     l[u] += x + y;
                     pa[2 * n + u] = pf_pack<T>(x, y);
+                    const T* two = reinterpret_cast<const T*>(&pa[2 * n + u]);
+                    pb[2 * n + u] = pf_pack<T>(x - to_f32<T>(two[0]), y - to_f32<T>(two[1]));
                 }
             {
                 // transposed: (keys 0-7, first 8 columns), (keys 8-15, first 8), (0-7, next 8), (8-15, next 8)
@@ -197,6 +200,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                     uint32_t b[4];
                     pf_ldsm_t(b, st + (uint32_t)(16 * D * 2 + r * (D * 2) + (((n + ch0) ^ (r & 7)) << 4)));
                     pf_mma<T>(o[n], pa, b[0], b[1]), pf_mma<T>(o[n + 1], pa, b[2], b[3]);
+                    pf_mma<T>(o[n], pb, b[0], b[1]), pf_mma<T>(o[n + 1], pb, b[2], b[3]);
                 }
             }
         }
