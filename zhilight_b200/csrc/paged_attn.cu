@@ -8,8 +8,8 @@
 namespace zl {
 
 // Calls whose sequences bring at most so many (token, head) rows of a kv head each go to the kernel for few rows, as do groups that no tile holds a token of.
-// us, it / the tiles, 32 heads on 8, 2000 keys: 16 sequences with 4 rows 41 / 52, with 16 rows 42 / 52; two with 16 rows 19 / 29; one with 16 rows on 30000
-// keys 44 / 83 (its probabilities of 16 bits alone; their rest adds some 2 %).  A variant for 32 rows took 58 to 60 where the tiles take 53 (16 sequences; 26 / 28 for two, 66 / 70 for one on 30000 keys) and was left out.
+// us, it / the tiles, 32 heads on 8, 2000 keys: 16 sequences with 4 rows 41 / 52, with 16 rows 43 / 52; two with 16 rows 19 / 28; one with 16 rows on 30000
+// keys 45 / 83.  A variant for 32 rows took 58 to 60 where the tiles take 53 (16 sequences; 26 / 28 for two, 66 / 70 for one on 30000 keys) and was left out.
 constexpr int kFewRows = kPfRows;
 
 struct PagedPlan {
