@@ -18,6 +18,8 @@ struct PagedAttn {
     struct PagedCut* cuts;            // for every CTA
 };
 
+constexpr float kPagedNone = -1.4426950e20f;   // reference maximum of a row that has not seen a key yet
+
 // One block of up to `size` (token, head) rows of a kv head of one sequence.
 struct PagedBlock {
     int seq, first, n;   // its sequence, whose new tokens begin at row `first` of q and make up n (token, head) rows

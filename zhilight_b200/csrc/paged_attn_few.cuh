@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
         float o[D / 8][4], l[2], m_ref[2];
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-        l[0] = l[1] = 0.f, m_ref[0] = m_ref[1] = -1.4426950e20f;
+        l[0] = l[1] = 0.f, m_ref[0] = m_ref[1] = kPagedNone;
         for (int j = 0; j < count; ++j) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kPfStages - 2) : "memory");
             __syncwarp();
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 top[u] = fmaxf(fmaxf(s[0][2 * u], s[0][2 * u + 1]), fmaxf(s[1][2 * u], s[1][2 * u + 1]));
-                up |= top[u] > m_ref[u] + kTau;
+                up |= top[u] - m_ref[u] > kTau;
             }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -185,8 +185,8 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float x = pf_exp2(s[n][2 * u] + (kUp - m_ref[u])), y = pf_exp2(s[n][2 * u + 1] + (kUp - m_ref[u]));
+                for (int u = 0; u < 2; ++u) {   // the difference first: it is as exact as the scores, whatever their size is
+                    const float x = pf_exp2((s[n][2 * u] - m_ref[u]) + kUp), y = pf_exp2((s[n][2 * u + 1] - m_ref[u]) + kUp);
                     l[u] += x + y;
                     pa[2 * n + u] = pf_pack<T>(x, y);
                     const T* two = reinterpret_cast<const T*>(&pa[2 * n + u]);

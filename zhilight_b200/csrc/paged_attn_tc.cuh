@@ -34,6 +34,11 @@ namespace zl {
 
 constexpr int kPtRows = 256, kPtKeys = 128, kPtHalf = 64, kPtThreads = 384, kPtWarpS = 8, kPtWarpO = 9, kPtWarpLoad = 10, kPtLoaders = 64;
 
+// The exponent of a probability is a score times the scale less the reference, in one fused step that does not round the product, where the reference is
+// one that was rounded: all exponents of a row are off by what that left, half a step of 32-bit numbers of its size.  That cancels in the quotient, but from here on
+// (2^22, half a step of 1/4) it could leave the range of the probabilities, so the product is rounded as the reference was before the difference is taken.
+constexpr float kPtFar = 4194304.f;
+
 // turns of a block, at least one: a block that sees nothing is written too
 struct PtKind {
     static constexpr int kSetup = 2;
@@ -132,7 +137,9 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             const int row = k.row0 + (mine ? r : 0), t = p.by_group(row), place = k.place0 + t;
             const int hi = mine ? min(place, k.have - 1) : -1, lo = mine && p.window ? max(0, place - p.window + 1) : 0;
             const int key0 = (t0 + (two_rows ? 0 : m)) * kPtKeys, step = two_rows ? kPtKeys : 2 * kPtKeys;
-            float l = 0.f, m_ref = -1.4426950e20f;
+            float l = 0.f, m_ref = kPagedNone;
+            float times = cs, less = m_ref;                            // an exponent is a score times the one less the other
+            bool far = false;                                          // a reference of this warp is beyond kPtFar
             for (int j = 0; j < 2 * count; ++j) {                      // 64 keys
                 const int b = j & 1, base = key0 + (j >> 1) * step + b * kPtHalf, h = hi - base, from_ = lo - base;   // this row sees from_ .. h of them
                 const uint32_t tb = ts + (uint32_t)(b * kPtHalf);
@@ -158,12 +165,12 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 mx[0] = pa_max3(mx[0], __uint_as_float(raw[kPtHalf - 4]), __uint_as_float(raw[kPtHalf - 3]));
                 mx[1] = pa_max3(mx[1], __uint_as_float(raw[kPtHalf - 2]), __uint_as_float(raw[kPtHalf - 1]));
                 const float m_tile = pa_max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * cs;
-                const bool up = m_tile > m_ref + kTau;
-                if (__any_sync(0xffffffffu, up)) {
+                const bool up = m_tile - m_ref > kTau;
+                if (__any_sync(0xffffffffu, up | far)) {
                     const float f = up ? pa_exp2(m_ref - m_tile) : 1.f;
                     if (up) m_ref = m_tile;
                     l *= f;
-                    if (j > 0) {
+                    if (j > 0 && __any_sync(0xffffffffu, up)) {
                         if (!tc2_wait(&o_done[m][b ^ 1], (uint32_t)(turn + ((j - 1) >> 1)) & 1u, s_abort, err, 0x5680 + m)) break;   // P V of the keys before
                         tc_fence_after();
 #pragma unroll 1
@@ -176,8 +183,15 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                             tc_st16(to + (uint32_t)d0, x);
                         }
                     }
+                    far = __any_sync(0xffffffffu, fabsf(m_ref) >= kPtFar && m_ref != kPagedNone);
+                    times = cs, less = m_ref;
+                    if (far) {
+#pragma unroll
+                        for (int i = 0; i < kPtHalf; ++i) raw[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(raw[i]), cs), m_ref));
+                        times = 1.f, less = 0.f;
+                    }
                 }
-                const uint64_t c2 = pa_two(cs, cs), m2 = pa_two(kUp - m_ref, kUp - m_ref);
+                const uint64_t c2 = pa_two(times, times), m2 = pa_two(kUp - less, kUp - less);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int part = 0; part < kPtHalf; part += 32) {
