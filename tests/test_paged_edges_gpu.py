@@ -67,3 +67,12 @@ def check_steep(dtype, q_size, k_size, dim, seqs, window=0):
 def test_attention_of_large_scores(cuda, dtype, q_size, k_size, dim, seqs):
     """Scores of 2^23 to 2^62: their distances decide, and steps between 32-bit numbers of their size are larger than any exponent."""
     check_steep(dtype, q_size, k_size, dim, STEEP_SEQS[seqs])
+
+
+@pytest.mark.parametrize("q_size,k_size", [(2.0 ** 34, 2.0 ** 34), (2.0 ** 50, 2.0 ** 58), (2.0 ** 60, 2.0 ** 59)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("seqs", list(STEEP_SEQS))
+@pytest.mark.parametrize("window", [0, 40])
+def test_attention_of_scores_near_the_largest_numbers(cuda, q_size, k_size, dim, seqs, window):
+    """Scores of 2^74 to 2^126 on both sides of zero: rows whose scores all lie far below it are softmaxes like others."""
+    check_steep(BF16, q_size, k_size, dim, STEEP_SEQS[seqs], window)

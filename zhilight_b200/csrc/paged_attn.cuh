@@ -2,6 +2,8 @@
 #pragma once
 #include "paged.cuh"
 
+#include <cfloat>
+
 namespace zl {
 
 struct PagedAttn {
@@ -18,7 +20,7 @@ struct PagedAttn {
     struct PagedCut* cuts;            // for every CTA
 };
 
-constexpr float kPagedNone = -1.4426950e20f;   // reference maximum of a row that has not seen a key yet
+constexpr float kPagedNone = -FLT_MAX;   // reference maximum of a row that has not seen a key yet: below every score, and finite (a masked score less it is -inf)
 
 // One block of up to `size` (token, head) rows of a kv head of one sequence.
 struct PagedBlock {
