@@ -76,3 +76,26 @@ def test_attention_of_large_scores(cuda, dtype, q_size, k_size, dim, seqs):
 def test_attention_of_scores_near_the_largest_numbers(cuda, q_size, k_size, dim, seqs, window):
     """Scores of 2^74 to 2^126 on both sides of zero: rows whose scores all lie far below it are softmaxes like others."""
     check_steep(BF16, q_size, k_size, dim, STEEP_SEQS[seqs], window)
+
+
+# ---- values of any size ---------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("size", [2.0 ** 127, 2.0 ** 100, 2.0 ** -70])
+@pytest.mark.parametrize("new", [1, 4, 150])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_large_and_small_values(cuda, size, new, dim):
+    """bf16 values up to the largest number: a mean of them is one that fits, whatever the sum is.  Small ones keep their bits."""
+    g = torch.Generator().manual_seed(22)
+    heads, kv_heads, page, seqs = 8, 2, 16, [(3000, new), (200, new), (new, new)]
+    lens = [n for n, _ in seqs]
+    pages = sum(-(-n // page) for n in lens) + 2
+    table, starts = tables(g, lens, page, pages), starts_of([new] * 3)
+    k, v = pool(g, pages, page, kv_heads, dim, BF16, "rows")
+    k.mul_(3.0)                                                      # maxima that grow from tile to tile
+    v.copy_(((torch.rand(v.shape, generator=g) + 0.99).double() * size).clamp(max=torch.finfo(BF16).max))
+    hide(k, table, lens, math.nan)
+    hide(v, table, lens, math.nan)
+    q = torch.randn(3 * new, heads, dim, generator=g).to(BF16)
+    got = attend(q, k, v, table, lens, starts, dim ** -0.5, max_new=new)
+    want, off = oracle.attention(q, k, v, table, lens, starts, dim ** -0.5, 0)
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= off).all(), float(((got - want).abs() - off).max() / size)

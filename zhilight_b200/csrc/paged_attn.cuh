@@ -20,6 +20,13 @@ struct PagedAttn {
     struct PagedCut* cuts;            // for every CTA
 };
 
+// Exponentials carry 2^up, and a row's reference follows its maximum once that is more than `tau` above it.  fp16 probabilities are at most 2^15, and with 2^10 the
+// small ones keep their bits.  bf16 ones have the exponents of 32-bit numbers: 2^(tau - 40) times the largest value, for as many keys as 31 bits count, stays
+// below the largest 32-bit number; what is lost behind the lowest exponent is less than 2^-86, of the largest probability or of a product with a value.
+template <bool HALF>
+struct PagedExp {
+    static constexpr float kTau = HALF ? 5.f : 8.f, kUp = HALF ? 10.f : -40.f;
+};
 constexpr float kPagedNone = -FLT_MAX;   // reference maximum of a row that has not seen a key yet: below every score, and finite (a masked score less it is -inf)
 
 // One block of up to `size` (token, head) rows of a kv head of one sequence.

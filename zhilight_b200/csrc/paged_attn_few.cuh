@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
     using C = PfCfg<D>;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int R = kPfRows, CH = D / 8, KS = D / 16;
-    constexpr float kTau = kHalf ? 5.f : 8.f, kUp = kHalf ? 10.f : 0.f;
+    constexpr float kTau = PagedExp<kHalf>::kTau, kUp = PagedExp<kHalf>::kUp;
     extern __shared__ __align__(128) uint8_t pf_smem[];
     __shared__ float2 s_ml[kPfWarps][R];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;

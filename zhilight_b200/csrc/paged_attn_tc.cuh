@@ -12,8 +12,8 @@
 // A page's rows behind the last visible key may hold anything.  Copies of 16 bytes leave them out; behind TMA the softmax's threads make those values zeros
 // before they hand the tile's probabilities on.  Rows behind a page number outside the pool are zeros either way.  Tensor memory: scores of the two tiles (128 columns each, probabilities over their first
 // half), then their outputs.  Probabilities are rounded to the rows' type once (half a step each, of random sign: beside the output's own rounding), the
-// sums that divide them are not.  A row's reference maximum follows the true one only once that has grown by 2^5 (fp16, whose probabilities carry 2^10) or
-// 2^8: any reference gives the same quotient.
+// sums that divide them are not.  A row's reference maximum follows the true one only once that has grown by 2^5 (fp16) or 2^8:
+// any reference gives the same quotient (PagedExp).
 //
 // A masked probability is exactly zero, but zero times an infinity or NaN that a row must not see (a later token's value) is NaN in its sum.  A row that
 // comes out as NaN is therefore done once more from the definition, key by key (paged_row_exact); numbers never take that path.
@@ -132,7 +132,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             const int m = warp >> 2, rt = tid & (kPaRows - 1), r = two_rows ? m * p.tile_rows + rt : rt;   // tile; row of it and of the block
             const bool mine = rt < p.tile_rows && r < k.rows;
             const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = taddr + (uint32_t)(m * 128), to = taddr + (uint32_t)(C::kO + m * D);
-            constexpr float kTau = kHalf ? 5.f : 8.f, kUp = kHalf ? 10.f : 0.f;
+            constexpr float kTau = PagedExp<kHalf>::kTau, kUp = PagedExp<kHalf>::kUp;
             const float cs = p.scale;
             const int row = k.row0 + (mine ? r : 0), t = p.by_group(row), place = k.place0 + t;
             const int hi = mine ? min(place, k.have - 1) : -1, lo = mine && p.window ? max(0, place - p.window + 1) : 0;
