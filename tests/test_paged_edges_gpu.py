@@ -99,3 +99,88 @@ def test_attention_of_large_and_small_values(cuda, size, new, dim):
     want, off = oracle.attention(q, k, v, table, lens, starts, dim ** -0.5, 0)
     assert torch.isfinite(got).all()
     assert ((got - want).abs() <= off).all(), float(((got - want).abs() - off).max() / size)
+
+
+# ---- keys and values that are no numbers ----------------------------------------------------------------------------------------
+def softmax_of(q, k, v, table, lens, starts, scale, window):
+    """oracle.attention where keys and values may be no numbers: a row's column is what 0 < p times the values it sees adds up to (NaN, or an infinity)."""
+    out, off = oracle.attention(q, k, v, table, lens, starts, scale, window)
+    for b, n in enumerate(lens):
+        lo, hi = int(starts[b]), int(starts[b + 1])
+        kk, vv = oracle.rows_of(k, table, b, n), oracle.rows_of(v, table, b, n)
+        at, j = torch.arange(n - (hi - lo), n), torch.arange(n)
+        seen = (j[None] <= at[:, None]) & ((j[None] > at[:, None] - window) if window else True)
+        for x in range(kk.shape[1]):
+            heads = slice(x * (q.shape[1] // kk.shape[1]), (x + 1) * (q.shape[1] // kk.shape[1]))
+            for row in torch.nonzero(~torch.isfinite(vv[:, x]).all(1))[:, 0].tolist():
+                add = torch.where(torch.isfinite(vv[row, x]), 0.0, vv[row, x])
+                out[lo:hi, heads] += torch.where(seen[:, row, None], add, 0.0)[:, None]
+            bad = ~torch.isfinite(kk[:, x]).all(1)
+            out[lo:hi, heads] += torch.where((seen & bad).any(1), math.nan, 0.0)[:, None, None]
+    return out, off
+
+
+def same(got, want, off):
+    """Numbers within `off`, infinities and NaN where they are wanted."""
+    number = torch.isfinite(want)
+    return bool(((got - want).abs() <= off)[number].all()) and torch.equal(got[~number].nan_to_num(0, 1, -1), want[~number].nan_to_num(0, 1, -1)) and \
+        torch.equal(torch.isnan(got), torch.isnan(want))
+
+
+@pytest.mark.parametrize("new,heads,kv_heads,page,window", [
+    (1, 8, 2, 16, 0), (1, 8, 2, 16, 30), (4, 8, 2, 20, 0), (9, 2, 2, 16, 25), (6, 8, 1, 64, 0), (6, 8, 1, 5, 20), (40, 8, 2, 32, 0), (64, 8, 2, 16, 0), (64, 8, 2, 3, 0),
+    (150, 8, 2, 64, 0), (150, 4, 2, 20, 50), (300, 2, 2, 128, 0), (300, 8, 1, 16, 33), (33, 40, 1, 256, 0)])
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F16, 128)])
+@pytest.mark.parametrize("before", [0, 200])
+def test_attention_of_values_that_are_no_numbers(cuda, new, heads, kv_heads, page, window, dtype, dim, before):
+    """In whole rows and in single columns, of new and of old tokens: rows that see them have them in their columns, other rows are as exact as ever."""
+    g = torch.Generator().manual_seed(new + page)
+    lens = [before + new, before + 37 + new, new]
+    pages = sum(-(-n // page) for n in lens) + 2
+    table, starts = tables(g, lens, page, pages), starts_of([new] * 3)
+    q = torch.randn(3 * new, heads, dim, generator=g).to(dtype)
+    for bad in (math.nan, math.inf, -math.inf):
+        k, v = pool(g, pages, page, kv_heads, dim, dtype, "rows")
+        for b, where in ((0, lens[0] - 1), (0, lens[0] - 1 - new // 3), (1, max(0, before - 10)), (2, new // 2)):
+            row = (int(table[b, where // page]), where % page, b % kv_heads)
+            if b == 1:
+                v[row] = bad
+            else:
+                v[row][[3, dim - 1]] = torch.tensor([bad, -bad], dtype=dtype)
+        hide(k, table, lens, math.nan)
+        hide(v, table, lens, math.nan)
+        got = attend(q, k, v, table, lens, starts, dim ** -0.5, window=window, max_new=new)
+        assert same(got, *softmax_of(q, k, v, table, lens, starts, dim ** -0.5, window)), bad
+
+
+@pytest.mark.parametrize("new,heads", [(1, 4), (3, 4), (64, 4), (300, 2)])
+@pytest.mark.parametrize("what", ["last value", "old value", "old key", "window"])
+def test_attention_of_long_sequences_with_a_broken_token(cuda, new, heads, what):
+    """One token that is no number behind 130000: right for its own sequence and for others, no wait gave up, and it takes about as long as it does without."""
+    g = torch.Generator().manual_seed(23)
+    page, dim, window = 64, 64, 100000 if what == "window" else 0
+    lens = [130000 + new, 500 + new, 70 + new]
+    pages = sum(-(-n // page) for n in lens)
+    table, starts = tables(g, lens, page, pages), starts_of([new] * 3)
+    k, v = pool(g, pages, page, 1, dim, BF16, "rows")
+    q = torch.randn(3 * new, heads, dim, generator=g).to(BF16)
+    dev = [x.cuda() for x in (q, k, v, table, torch.tensor(lens, dtype=torch.int32), starts)]
+    where = {"last value": lens[0] - 1, "old value": 7, "old key": 1000, "window": lens[0] - new - window + 1 + new // 2}[what]
+    times = []
+    for broken in (False, True):
+        if broken:
+            x, y = (k, dev[1]) if what == "old key" else (v, dev[2])
+            for z in (x, y):
+                z[int(table[0, where // page]), where % page, 0, 5] = math.nan if what == "old key" else math.inf
+        each = []
+        for _ in range(6):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            got = ops.paged_attention(*dev, dim ** -0.5, window=window, max_new=new)
+            b.record()
+            torch.cuda.synchronize()
+            each.append(a.elapsed_time(b))
+        times.append(min(each))
+    ops.check_waits()
+    assert same(got.cpu().double(), *softmax_of(q, k, v, table, lens, starts, dim ** -0.5, window))
+    assert times[1] < 3 * times[0], times

@@ -56,7 +56,7 @@ static int paged_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pdl
     static bool done[64] = {};
     ZL_CHECK_CUDA(allow_smem(k_paged_attn_few<T, D>, PfCfg<D>::kBytes, done));
     ZL_CHECK_CUDA(launch(k_paged_attn_few<T, D>, dim3(ctas), dim3(kPfWarps * 32), PfCfg<D>::kBytes, stream, pdl, p, c));
-    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, kPfRows>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p, c));
+    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, kPfRows>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p));
     return ZL_OK;
 }
 
@@ -88,7 +88,7 @@ static int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool p
     }
     ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D>, dim3(ctas), dim3(kPtThreads), PtCfg<D>::kBytes, stream, pdl, p, c, maps[0], maps[1], maps[2], box,
                          words + kWaitAttnPaged));
-    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join_tiles<T, D>, dim3(ctas, kPtRows / 32), dim3(256), 0, stream, true, p, c));
+    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join_tiles<T, D>, dim3(ctas, kPtRows / 32), dim3(256), 0, stream, true, p));
     return ZL_OK;
 }
 

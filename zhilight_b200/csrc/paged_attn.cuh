@@ -1,4 +1,4 @@
-// What the kernels of attention over pages share: their arguments, the blocks of rows that the sequences are cut into, and a row from its definition.
+// What the kernels of attention over pages share: their arguments, the blocks of rows that the sequences are cut into, the join of few rows.
 #pragma once
 #include "paged.cuh"
 
@@ -217,54 +217,18 @@ struct PagedWalk {
     }
 };
 
-// Row t of q, one head, from the definition, by one warp: keys lo .. hi, one at a time.
+// Row r of a block, D columns, E neighbouring ones of this lane: rounded and stored
 template <typename T, int D>
-__device__ __noinline__ void paged_row_exact(const PagedAttn& p, const PagedCache& c, int seq, int t, int h, int lo, int hi) {
+__device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedBlock& k, int hk, int r, float l, const float (&o)[D / 32]) {
     constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long head = (long long)p.by_group(h) * c.head_stride + lane;
-    const size_t row = ((size_t)t * p.heads + h) * D + lane;
-    float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) q[e] = to_f32<T>(static_cast<const T*>(p.q)[row + e * 32]);
-    for (int j = lo; j <= hi; ++j) {
-        const long long r = c.row_at(seq, j);
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (r >= 0) s = fmaf(q[e], to_f32<T>(static_cast<const T*>(c.k)[r + head + e * 32]), s);
-        s = warp_sum(s) * p.scale;
-        const float up = s != s ? s : fmaxf(m, s), f = up == -INFINITY ? 1.f : exp2f(m - up), w = up == -INFINITY ? 0.f : exp2f(s - up);
-        m = up;
-        l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * f + (r >= 0 ? w * to_f32<T>(static_cast<const T*>(c.v)[r + head + e * 32]) : 0.f);
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) static_cast<T*>(p.out)[row + e * 32] = from_f32<T>(l > 0.f || l != l ? o[e] / l : 0.f);
-}
-
-// Row r of a block, D columns from `o`(e) of this lane, E neighbouring ones each: rounded and stored, or done again where it is no number
-template <typename T, int D>
-__device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedCache& c, const PagedBlock& k, int hk, int r, float l, const float (&o)[D / 32]) {
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31, row = k.row0 + r, t = p.by_group(row), head = hk * p.group + row - t * p.group, place = k.place0 + t;
+    const int lane = threadIdx.x & 31, row = k.row0 + r, t = p.by_group(row), head = hk * p.group + row - t * p.group;
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     T v[E];
-    bool broken = false;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float x = l == 0.f ? 0.f : o[e] * inv;
-        broken |= x != x;
-        v[e] = from_f32<T>(x);
-    }
+    for (int e = 0; e < E; ++e) v[e] = from_f32<T>(l == 0.f ? 0.f : o[e] * inv);
     T* dst = static_cast<T*>(p.out) + ((size_t)(k.first + t) * p.heads + head) * D + lane * E;
     if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
     else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(v);
-    if (__any_sync(0xffffffffu, broken)) {
-        __syncwarp();
-        paged_row_exact<T, D>(p, c, k.seq, k.first + t, head, p.window ? max(0, place - p.window + 1) : 0, min(place, k.have - 1));
-    }
 }
 
 // Blocks that were cut, of the kernel for few rows.  grid (its CTAs): the first part of a block lies in its CTA's place 1, the others in the place 0 of theirs,
@@ -272,7 +236,7 @@ __device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedCac
 // once; more CTAs, a row each, cost more than they give (37 blocks that nothing cuts: 13.4 -> 22.5 us a call).
 constexpr int kJoinWarps = 16, kJoinAhead = 4;   // not fewer warps than rows
 template <typename T, int D, int R>
-__global__ void __launch_bounds__(kJoinWarps * 32) k_paged_join(const PagedAttn p, const PagedCache c) {
+__global__ void __launch_bounds__(kJoinWarps * 32) k_paged_join(const PagedAttn p) {
     constexpr int E = D / 32;
     static_assert(R <= kJoinWarps, "a warp for every row");
     __shared__ float s_m[kJoinWarps], s_l[kJoinWarps], s_v[kJoinWarps][D];
@@ -336,7 +300,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_join(const PagedAttn 
             }
         }
     }
-    if (group == 0 && mine) paged_row_out<T, D>(p, c, x.k, x.hk, r, l, v);
+    if (group == 0 && mine) paged_row_out<T, D>(p, x.k, x.hk, r, l, v);
 }
 
 }  // namespace zl

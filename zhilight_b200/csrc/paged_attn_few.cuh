@@ -108,14 +108,6 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 16 * D * 2), "l"(static_cast<const T*>(c.v) + from), "r"(bytes) : "memory");
             }
         };
-        int id = find(0);
-#pragma unroll 1
-        for (int j = 0; j < kPfStages - 1; ++j) {
-            const int next = find(j + 1);
-            if (j < count) copy(j, id);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            id = next;
-        }
         // rows of q: (g, g + 8) of each 16
         uint32_t qa[KS][4];
         int hi[2], lo[2];
@@ -131,78 +123,135 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
             for (int s = 0; s < KS; ++s) qa[s][u] = in ? src[s * 8 + t4] : 0u, qa[s][2 + u] = in ? src[s * 8 + 4 + t4] : 0u;
         }
         float o[D / 8][4], l[2], m_ref[2];
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-        l[0] = l[1] = 0.f, m_ref[0] = m_ref[1] = kPagedNone;
-        for (int j = 0; j < count; ++j) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kPfStages - 2) : "memory");
-            __syncwarp();
-            const int next = find(j + kPfStages);
-            if (j + kPfStages - 1 < count) copy(j + kPfStages - 1, id);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            id = next;
-            const int kb = key0 + j * kPfKeys;
-            if (kb > k.hi || kb + 15 < k.lo) continue;
-            const uint32_t st = ring_at + (uint32_t)(j % kPfStages) * C::kStage;
-            float s[2][4] = {};
-            {
-                // matrices of 8 keys x 8 columns: (keys 0-7, first 8), (0-7, next 8), (8-15, first 8), (8-15, next 8)
-                const int r = (lane & 7) + ((lane >> 4) << 3), ch0 = (lane >> 3) & 1;
-#pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                    uint32_t b[4];
-                    pf_ldsm(b, st + (uint32_t)(r * (D * 2) + (((2 * i + ch0) ^ (r & 7)) << 4)));
-                    pf_mma<T>(s[0], qa[i], b[0], b[1]), pf_mma<T>(s[1], qa[i], b[2], b[3]);
-                }
+        // Once, mostly.  A masked probability is exactly zero, but zero times an infinity or NaN that a row must not see is NaN in its sum (and the rest of a
+        // probability times an infinity may be one too).  Where the warp's sums hold a NaN that no score explains, it goes over its keys once more and looks at the
+        // values: of 16 keys that are not all numbers it takes the product key by key, of those that a row sees.
+        for (bool again = false;; again = true) {
+            int id = find(0);
+#pragma unroll 1
+            for (int j = 0; j < kPfStages - 1; ++j) {
+                const int next = find(j + 1);
+                if (j < count) copy(j, id);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                id = next;
             }
-            uint32_t pa[4], pb[4];   // probabilities, and what their rounding left of them
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+            l[0] = l[1] = 0.f, m_ref[0] = m_ref[1] = kPagedNone;
+            for (int j = 0; j < count; ++j) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kPfStages - 2) : "memory");
+                __syncwarp();
+                const int next = find(j + kPfStages);
+                if (j + kPfStages - 1 < count) copy(j + kPfStages - 1, id);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                id = next;
+                const int kb = key0 + j * kPfKeys;
+                if (kb > k.hi || kb + 15 < k.lo) continue;
+                const uint32_t st = ring_at + (uint32_t)(j % kPfStages) * C::kStage;
+                float s[2][4] = {};
+                {
+                    // matrices of 8 keys x 8 columns: (keys 0-7, first 8), (0-7, next 8), (8-15, first 8), (8-15, next 8)
+                    const int r = (lane & 7) + ((lane >> 4) << 3), ch0 = (lane >> 3) & 1;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = kb + n * 8 + t4 * 2 + (e & 1);
-                    s[n][e] = key <= hi[e >> 1] && key >= lo[e >> 1] ? s[n][e] * p.scale : -INFINITY;
+                    for (int i = 0; i < KS; ++i) {
+                        uint32_t b[4];
+                        pf_ldsm(b, st + (uint32_t)(r * (D * 2) + (((2 * i + ch0) ^ (r & 7)) << 4)));
+                        pf_mma<T>(s[0], qa[i], b[0], b[1]), pf_mma<T>(s[1], qa[i], b[2], b[3]);
+                    }
                 }
-            bool up = false;
-            float top[2];
+                uint32_t pa[4], pb[4];   // probabilities, and what their rounding left of them
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                top[u] = fmaxf(fmaxf(s[0][2 * u], s[0][2 * u + 1]), fmaxf(s[1][2 * u], s[1][2 * u + 1]));
-                up |= top[u] - m_ref[u] > kTau;
-            }
-            if (__any_sync(0xffffffffu, up)) {
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = kb + n * 8 + t4 * 2 + (e & 1);
+                        s[n][e] = key <= hi[e >> 1] && key >= lo[e >> 1] ? s[n][e] * p.scale : -INFINITY;
+                    }
+                bool up = false;
+                float top[2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
-                    top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
-                    const float f = top[u] > m_ref[u] ? pf_exp2(m_ref[u] - top[u]) : 1.f;
-                    m_ref[u] = fmaxf(m_ref[u], top[u]);
-                    l[u] *= f;
+                    top[u] = fmaxf(fmaxf(s[0][2 * u], s[0][2 * u + 1]), fmaxf(s[1][2 * u], s[1][2 * u + 1]));
+                    up |= top[u] - m_ref[u] > kTau;
+                }
+                if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
-                    for (int n = 0; n < D / 8; ++n) o[n][2 * u] *= f, o[n][2 * u + 1] *= f;
+                    for (int u = 0; u < 2; ++u) {
+                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
+                        top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
+                        const float f = top[u] > m_ref[u] ? pf_exp2(m_ref[u] - top[u]) : 1.f;
+                        m_ref[u] = fmaxf(m_ref[u], top[u]);
+                        l[u] *= f;
+#pragma unroll
+                        for (int n = 0; n < D / 8; ++n) o[n][2 * u] *= f, o[n][2 * u + 1] *= f;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {   // the difference first: it is as exact as the scores, whatever their size is
+                        const float x = pf_exp2((s[n][2 * u] - m_ref[u]) + kUp), y = pf_exp2((s[n][2 * u + 1] - m_ref[u]) + kUp);
+                        l[u] += x + y;
+                        s[n][2 * u] = x, s[n][2 * u + 1] = y;
+                        pa[2 * n + u] = pf_pack<T>(x, y);
+                        const T* two = reinterpret_cast<const T*>(&pa[2 * n + u]);
+                        pb[2 * n + u] = pf_pack<T>(x - to_f32<T>(two[0]), y - to_f32<T>(two[1]));
+                    }
+                bool apart = false;   // the product key by key
+                if (again) {
+                    const uint4* v = reinterpret_cast<const uint4*>(ring + (j % kPfStages) * C::kStage + 16 * D * 2);
+                    uint32_t top = 0;
+                    for (int x = lane; x < 16 * CH; x += 32) {
+                        const uint4 w = v[x];
+                        top = __vmaxu2(__vmaxu2(top, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+                    }
+                    constexpr uint32_t kInf = kHalf ? 0x7c00 : 0x7f80;
+                    apart = __any_sync(0xffffffffu, (top & 0xffffu) >= kInf || top >> 16 >= kInf);
+                }
+                if (apart) {
+#pragma unroll 1
+                    for (int key = 0; key < 16; ++key) {
+                        const T* v = reinterpret_cast<const T*>(ring + (j % kPfStages) * C::kStage + 16 * D * 2 + key * (D * 2));
+                        float w[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            w[u] = __shfl_sync(0xffffffffu, key & 1 ? (key & 8 ? s[1][2 * u + 1] : s[0][2 * u + 1]) : (key & 8 ? s[1][2 * u] : s[0][2 * u]),
+                                               (lane & ~3) | (key >> 1 & 3));
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            if (kb + key <= hi[u] && kb + key >= lo[u])
+#pragma unroll
+                                for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) o[n][2 * u + e] = fmaf(w[u], to_f32<T>(v[((n ^ (key & 7)) << 3) + t4 * 2 + e]), o[n][2 * u + e]);
+                    }
+                } else {
+                    // transposed: (keys 0-7, first 8 columns), (keys 8-15, first 8), (0-7, next 8), (8-15, next 8)
+                    const int r = (lane & 7) + (((lane >> 3) & 1) << 3), ch0 = lane >> 4;
+#pragma unroll
+                    for (int n = 0; n < D / 8; n += 2) {
+                        uint32_t b[4];
+                        pf_ldsm_t(b, st + (uint32_t)(16 * D * 2 + r * (D * 2) + (((n + ch0) ^ (r & 7)) << 4)));
+                        pf_mma<T>(o[n], pa, b[0], b[1]), pf_mma<T>(o[n + 1], pa, b[2], b[3]);
+                        pf_mma<T>(o[n], pb, b[0], b[1]), pf_mma<T>(o[n + 1], pb, b[2], b[3]);
+                    }
                 }
             }
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {   // the difference first: it is as exact as the scores, whatever their size is
-                    const float x = pf_exp2((s[n][2 * u] - m_ref[u]) + kUp), y = pf_exp2((s[n][2 * u + 1] - m_ref[u]) + kUp);
-                    l[u] += x + y;
-                    pa[2 * n + u] = pf_pack<T>(x, y);
-                    const T* two = reinterpret_cast<const T*>(&pa[2 * n + u]);
-                    pb[2 * n + u] = pf_pack<T>(x - to_f32<T>(two[0]), y - to_f32<T>(two[1]));
-                }
-            {
-                // transposed: (keys 0-7, first 8 columns), (keys 8-15, first 8), (0-7, next 8), (8-15, next 8)
-                const int r = (lane & 7) + (((lane >> 3) & 1) << 3), ch0 = lane >> 4;
-#pragma unroll
-                for (int n = 0; n < D / 8; n += 2) {
-                    uint32_t b[4];
-                    pf_ldsm_t(b, st + (uint32_t)(16 * D * 2 + r * (D * 2) + (((n + ch0) ^ (r & 7)) << 4)));
-                    pf_mma<T>(o[n], pa, b[0], b[1]), pf_mma<T>(o[n + 1], pa, b[2], b[3]);
-                    pf_mma<T>(o[n], pb, b[0], b[1]), pf_mma<T>(o[n + 1], pb, b[2], b[3]);
-                }
+            for (int u = 0; u < 2; ++u) {
+                l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+                l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
             }
+            if (again) break;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                bool none = false;
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) none |= o[n][2 * u] != o[n][2 * u] || o[n][2 * u + 1] != o[n][2 * u + 1];
+                again |= none && l[u] == l[u] && g + u * 8 < k.rows;
+            }
+            if (!__any_sync(0xffffffffu, again)) break;
+            __syncwarp();
         }
         // the warps' parts, in their rings
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -211,10 +260,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int r = g + u * 8;
-            float sum = l[u];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (t4 == 0) s_ml[warp][r] = make_float2(m_ref[u], sum);
+            if (t4 == 0) s_ml[warp][r] = make_float2(m_ref[u], l[u]);
 #pragma unroll
             for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(mine + r * C::kPitch + n * 8 + t4 * 2) = make_float2(o[n][2 * u], o[n][2 * u + 1]);
         }
@@ -235,7 +281,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 for (int e = 0; e < E; ++e) v[e] = fmaf(from[e], f, v[e]);
             }
             if (whole) {
-                paged_row_out<T, D>(p, c, k, at.hk, r, sum, v);
+                paged_row_out<T, D>(p, k, at.hk, r, sum, v);
             } else {
                 if (lane == 0) p.ml[part + r] = make_float2(m, sum);
                 float* dst = p.part + (part + r) * D + lane * E;

@@ -15,8 +15,9 @@
 // sums that divide them are not.  A row's reference maximum follows the true one only once that has grown by 2^5 (fp16) or 2^8:
 // any reference gives the same quotient (PagedExp).
 //
-// A masked probability is exactly zero, but zero times an infinity or NaN that a row must not see (a later token's value) is NaN in its sum.  A row that
-// comes out as NaN is therefore done once more from the definition, key by key (paged_row_exact); numbers never take that path.
+// A masked probability is exactly zero, but zero times an infinity or NaN that a row must not see (a later token's value, one before its window) is NaN in its
+// sum.  Of the keys that not all rows of a block see (its last ones, and the first ones of a window) the softmax's threads therefore look the values over before they
+// hand the tile's probabilities on, and put zeros where they are no numbers (pt_clean); at the block's end they add those to the rows that do see them (pt_add_broken).
 //
 // 4096 tokens behind 4096, 32 heads on 8, bf16: 390 to 450 us by the GPU it ran on, 0.92 to 1.06 PFLOP/s.  A turn takes 3000 cycles, of which the MMAs need 2050 at least and
 // the exponentials of both groups 2050; under this load the SM runs at 1.2 GHz.  Before, the same in us: copies of 16 bytes by two warps 693 (they bound it),
@@ -78,6 +79,62 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || tc2_wait(bar, parity, s_abort, err, code);
 }
 
+template <typename T>
+constexpr uint32_t kPtInf = std::is_same<T, __half>::value ? 0x7c00 : 0x7f80;   // magnitudes from here on are no numbers
+// the larger magnitudes of pairs of elements
+__device__ __forceinline__ uint32_t pt_magnitude(const uint4& w) {
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    return __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs), __vmaxu2(w.z & kAbs, w.w & kAbs));
+}
+// 8 values: those that are no numbers become zeros.  Whether there are any
+template <typename T>
+__device__ __forceinline__ bool pt_clean(uint4* at) {
+    const uint32_t top = pt_magnitude(*at);
+    if ((top & 0xffffu) < kPtInf<T> && top >> 16 < kPtInf<T>) return false;
+    uint16_t* w = reinterpret_cast<uint16_t*>(at);
+    for (int i = 0; i < 8; ++i)
+        if ((w[i] & 0x7fffu) >= kPtInf<T>) w[i] = 0;
+    return true;
+}
+// Adds the values that pt_clean takes out, of keys lo .. hi that a row sees, to the outputs of a warp's rows (tensor memory, D columns from `ob`): of the keys
+// first .. last without those in from .. to, in tiles of 128 the first of every `step`.  A lane looks at a key at a time.
+template <typename T, int D>
+__device__ __noinline__ void pt_add_broken(const PagedCache& c, int seq, long long head, uint32_t ob, int lo, int hi, int first, int last, int from, int to, int step) {
+    const int lane = threadIdx.x & 31;
+    for (int key0 = first; key0 <= last; key0 += 32) {
+        if (key0 >= from && key0 + 31 <= to) {
+            key0 = to - 31;
+            continue;
+        }
+        const int mine = key0 + lane;
+        const long long at = mine <= last && (mine < from || mine > to) && (mine - first) / kPtKeys % step == 0 ? c.row_at(seq, mine) : -1;
+        uint32_t top = 0;
+        if (at >= 0)
+#pragma unroll
+            for (int d0 = 0; d0 < D; d0 += 8) top = __vmaxu2(top, pt_magnitude(*reinterpret_cast<const uint4*>(static_cast<const T*>(c.v) + at + head + d0)));
+        for (unsigned left = __ballot_sync(0xffffffffu, (top & 0xffffu) >= kPtInf<T> || top >> 16 >= kPtInf<T>); left; left &= left - 1) {
+            const int key = key0 + __ffs(left) - 1;
+            const long long row = __shfl_sync(0xffffffffu, at, key - key0);
+#pragma unroll 1
+            for (int d0 = 0; d0 < D; d0 += 16) {
+                float o[16];
+                tc_ld16(ob + (uint32_t)d0, o);
+                const uint4* v = reinterpret_cast<const uint4*>(static_cast<const T*>(c.v) + row + head + d0);
+                const uint4 two[2] = {v[0], v[1]};
+                const T* x = reinterpret_cast<const T*>(two);
+                uint32_t r[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float y = to_f32<T>(x[i]);
+                    r[i] = __float_as_uint(key >= lo && key <= hi && !(fabsf(y) < INFINITY) ? o[i] + y : o[i]);
+                }
+                tc_st16(ob + (uint32_t)d0, r);
+                tc_wait_st();
+            }
+        }
+    }
+}
+
 // grid: CTAs that share the line.  box: rows of a TMA box of K and V, 0: no TMA
 template <typename T, int D>
 __global__ void __launch_bounds__(kPtThreads, 1)
@@ -91,14 +148,15 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2][2], p_full[2][2], o_done[2][2], q_full, q_free, o_free, joined;
     __shared__ float2 s_ml[kPaRows];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_gave_up;
-    volatile int* s_abort = &s_gave_up;
+    __shared__ int s_gave_up, s_blocks[2];
+    // s_broken[i % 2] is i + 1 where block i had values that are no numbers and that not all rows see; no warp of the softmax is two blocks ahead of another
+    volatile int *s_abort = &s_gave_up, *s_broken = s_blocks;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], box ? 1 : kPtLoaders), mbar_init(&empty[i], 1);
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i >> 1][i & 1], 1), mbar_init(&p_full[i >> 1][i & 1], 4), mbar_init(&o_done[i >> 1][i & 1], 1);
         mbar_init(&q_full, 1), mbar_init(&q_free, 1), mbar_init(&o_free, 8), mbar_init(&joined, 4);
-        s_gave_up = 0;
+        s_gave_up = s_blocks[0] = s_blocks[1] = 0;
         mbar_fence_init();
     }
     if (warp == kPtWarpS) {
@@ -128,6 +186,9 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
         if (count == 0) continue;
         const bool two_rows = k.rows > p.tile_rows, joins = !two_rows && walk.whole(count);   // two row tiles; else two key tiles
         const int t0 = (k.hi >= 0 ? k.lo / kPtKeys : 0) + (two_rows ? first : 2 * first), items = two_rows ? 2 : 4;   // of the ring for 64 keys
+        // keys that all rows of the block see
+        const int all_hi = min(k.place0 + p.by_group(k.row0), k.have - 1);
+        const int all_lo = p.window ? max(0, k.place0 + p.by_group(k.row0 + k.rows - 1) - p.window + 1) : 0;
         if (warp < kPtWarpS) {
             const int m = warp >> 2, rt = tid & (kPaRows - 1), r = two_rows ? m * p.tile_rows + rt : rt;   // tile; row of it and of the block
             const bool mine = rt < p.tile_rows && r < k.rows;
@@ -216,18 +277,27 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 float s0, s1;
                 pa_split(pa_add2(sum[0], sum[1]), s0, s1);
                 l += s0 + s1;
-                // The tile with the last visible key, where that ends within a box: values behind it become zeros.  Of two row tiles the first sees to it, whose
-                // product comes first.  The tile is there or on its way: the ring's tiles before it have been used.
-                const int behind = k.hi + 1 - base;
-                if (box && behind > 0 && behind < kPtHalf && behind % box != 0 && (m == 0 || !two_rows)) {
-                    const int it = ring + j * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
-                    if (!tc2_wait(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5800 + slot)) break;
-                    const int r1 = (behind + box - 1) / box * box;   // further boxes are zeros already
-                    for (int x = tid & (kPaRows - 1); x < (r1 - behind) * CH; x += kPaRows) {
-                        const int rz = behind + x / CH, cz = x % CH;   // whole rows: the swizzle stays within them
-                        *reinterpret_cast<uint4*>(smem + C::kRingOff + slot * C::kTile + (cz >> 3) * (kPtHalf * 128) + rz * 128 + ((cz & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                // Values of keys that not all rows see are looked over, and where the last visible key ends within a TMA box, those behind it become zeros (further boxes
+                // are zeros already).  Of two row tiles the first sees to it, whose product comes first.  The tile is there or on its way: the ring's tiles before it
+                // have been used.
+                if (m == 0 || !two_rows) {
+                    const int behind = min(k.hi + 1 - base, kPtHalf);   // rows that hold keys
+                    const bool look = behind > 0 && (base + behind - 1 > all_hi || base < all_lo), cut = box && behind > 0 && behind % box != 0;
+                    if (look || cut) {
+                        const int it = ring + j * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
+                        if (!tc2_wait(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5800 + slot)) break;
+                        const int r1 = cut ? (behind + box - 1) / box * box : behind;
+                        bool broken = false;
+#pragma unroll 1
+                        for (int x = tid & (kPaRows - 1); x < r1 * CH; x += kPaRows) {   // whole rows: the swizzle stays within them
+                            const int row = x / CH, ch = x % CH;
+                            uint4* w = reinterpret_cast<uint4*>(smem + C::kRingOff + slot * C::kTile + (ch >> 3) * (kPtHalf * 128) + row * 128 + ((ch & 7) << 4));
+                            if (row >= behind) *w = make_uint4(0, 0, 0, 0);
+                            else if (base + row < all_lo || base + row > all_hi) broken |= pt_clean<T>(w);
+                        }
+                        if (broken) s_broken[blocks & 1] = blocks + 1;
+                        pa_fence_async();
                     }
-                    pa_fence_async();
                 }
                 tc_wait_st();
                 tc_fence_before();
@@ -236,6 +306,9 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             }
             for (int b = 0; b < 2; ++b) tc2_wait(&o_done[m][b], (uint32_t)(turn + count - 1) & 1u, s_abort, err, 0x5700 + m);
             tc_fence_after();
+            // noted before the tile's probabilities were handed on, whose product has ended
+            if (__any_sync(0xffffffffu, s_broken[blocks & 1] == blocks + 1))
+                pt_add_broken<T, D>(c, k.seq, (long long)at.hk * c.head_stride, to, lo, hi, key0, min(t0 * kPtKeys + count * step - 1, k.hi), all_lo, all_hi, step / kPtKeys);
             if (!walk.whole(count)) {
                 // A part: {maximum, sum}, then the output as it stands, column by column: the lanes of a warp are neighbours there.
                 const size_t part = (size_t)blockIdx.x * 2 + (first > 0 ? 0 : 1);
@@ -283,7 +356,6 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                     const int head = at.hk * p.group + row - t * p.group;
                     T* dst = static_cast<T*>(p.out) + ((size_t)(k.first + t) * p.heads + head) * D;
                     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-                    bool broken = false;
 #pragma unroll 1
                     for (int d0 = 0; d0 < D; d0 += 32) {
                         uint32_t v[32];
@@ -302,15 +374,9 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                                     f[u + 2] = fmaf(y.z, f_other, f[u + 2] * f_own), f[u + 3] = fmaf(y.w, f_other, f[u + 3] * f_own);
                                 }
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) f[u] = l == 0.f ? 0.f : f[u] * inv, broken |= f[u] != f[u];
+                            for (int u = 0; u < 8; ++u) f[u] = l == 0.f ? 0.f : f[u] * inv;
                             if (mine) *reinterpret_cast<uint4*>(dst + d0 + i) = pack8<T>(f);
                         }
-                    }
-                    for (unsigned left = __ballot_sync(0xffffffffu, broken && mine); left; left &= left - 1) {
-                        const int src = __ffs(left) - 1;
-                        __syncwarp();
-                        paged_row_exact<T, D>(p, c, k.seq, __shfl_sync(0xffffffffu, k.first + t, src), __shfl_sync(0xffffffffu, head, src),
-                                              __shfl_sync(0xffffffffu, lo, src), __shfl_sync(0xffffffffu, hi, src));
                     }
                 }
             }
@@ -489,9 +555,8 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
 // CTA's place 1, the others in the place 0 of theirs.  Of a block with two tiles of rows the second begins at row 128 of its place; one with a single tile has
 // two results in a place, the second there.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) k_paged_join_tiles(const PagedAttn p, const PagedCache c) {
+__global__ void __launch_bounds__(256) k_paged_join_tiles(const PagedAttn p) {
     constexpr int W = D / 8;
-    __shared__ unsigned s_bad[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d0 = warp * W;
     pdl_trigger();
     pdl_wait();
@@ -526,10 +591,9 @@ __global__ void __launch_bounds__(256) k_paged_join_tiles(const PagedAttn p, con
         }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    bool bad = false;
 #pragma unroll
-    for (int u = 0; u < W; ++u) v[u] = l == 0.f ? 0.f : v[u] * inv, bad |= v[u] != v[u];
-    const int at = x.k.row0 + (mine ? r : 0), t = p.by_group(at), head = x.hk * p.group + at - t * p.group, place = x.k.place0 + t;
+    for (int u = 0; u < W; ++u) v[u] = l == 0.f ? 0.f : v[u] * inv;
+    const int at = x.k.row0 + (mine ? r : 0), t = p.by_group(at), head = x.hk * p.group + at - t * p.group;
     if (mine) {
         T* dst = static_cast<T*>(p.out) + ((size_t)(x.k.first + t) * p.heads + head) * D + d0;
 #pragma unroll
@@ -539,18 +603,6 @@ __global__ void __launch_bounds__(256) k_paged_join_tiles(const PagedAttn p, con
             for (int i = 0; i < 8; ++i) f[i] = v[u + i];
             *reinterpret_cast<uint4*>(dst + u) = pack8<T>(f);
         }
-    }
-    const unsigned some = __ballot_sync(0xffffffffu, bad && mine);
-    if (lane == 0) s_bad[warp] = some;
-    __syncthreads();
-    unsigned all = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) all |= s_bad[i];
-    for (; all; all &= all - 1) {
-        const int src = __ffs(all) - 1;
-        if (src % 8 == warp)
-            paged_row_exact<T, D>(p, c, x.k.seq, x.k.first + __shfl_sync(0xffffffffu, t, src), __shfl_sync(0xffffffffu, head, src),
-                                  p.window ? max(0, __shfl_sync(0xffffffffu, place, src) - p.window + 1) : 0, min(__shfl_sync(0xffffffffu, place, src), x.k.have - 1));
     }
 }
 
