@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import paged_oracle as oracle
-from tests.test_paged_gpu import hide, on_gpu, pool, starts_of, tables
+from tests.test_paged_gpu import check_attention, hide, on_gpu, pool, starts_of, tables
 from zhilight_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -184,3 +184,13 @@ def test_attention_of_long_sequences_with_a_broken_token(cuda, new, heads, what)
     ops.check_waits()
     assert same(got.cpu().double(), *softmax_of(q, k, v, table, lens, starts, dim ** -0.5, window))
     assert times[1] < 3 * times[0], times
+
+
+# ---- windows of any size --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 40, 2 ** 30])
+@pytest.mark.parametrize("new", [1, 5, 100, 200])
+def test_attention_of_the_widest_windows(cuda, window, new):
+    """A window that is wider than every sequence hides nothing, also where rows stand before the first key."""
+    for dim in (64, 128):
+        check_attention(BF16, 8, 2, dim, 16, "rows", window, [(new // 2, new), (0, new), (new, new), (new + 300, new)])
+        check_attention(F16, 8, 2, dim, 16, "rows", window, [(new // 2, new), (new - new // 4, new)], max_new=new)

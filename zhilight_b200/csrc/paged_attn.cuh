@@ -38,11 +38,14 @@ struct PagedBlock {
     int lo, hi;          // keys that any row of the block sees; hi < 0: none
 };
 
+// The first key that a row at `place` sees.  Rows before the sequence's beginning have negative places and see none; windows go up to the largest int.
+__device__ __forceinline__ int paged_from(const PagedAttn& p, int place) { return p.window ? max(max(place + 1, 0) - p.window, 0) : 0; }
+
 // What the block's rows see
 __device__ __forceinline__ void paged_sees(const PagedAttn& p, PagedBlock& k) {
     const int t0 = p.by_group(k.row0), t1 = p.by_group(k.row0 + k.rows - 1);
     k.hi = min(k.place0 + t1, k.have - 1);
-    k.lo = p.window ? max(0, k.place0 + t0 - p.window + 1) : 0;
+    k.lo = paged_from(p, k.place0 + t0);
     if (k.lo > k.hi) k.hi = -1, k.lo = 0;
 }
 struct PagedPlace {

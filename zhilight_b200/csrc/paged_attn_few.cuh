@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
             const int row = k.row0 + (in ? r : 0), t = p.by_group(row), place = k.place0 + t;
             const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + ((size_t)(k.first + t) * p.heads + at.hk * p.group + row - t * p.group) * D);
             hi[u] = in ? min(place, k.have - 1) : -1;
-            lo[u] = p.window ? max(0, place - p.window + 1) : 0;
+            lo[u] = paged_from(p, place);
 #pragma unroll
             for (int s = 0; s < KS; ++s) qa[s][u] = in ? src[s * 8 + t4] : 0u, qa[s][2 + u] = in ? src[s * 8 + 4 + t4] : 0u;
         }

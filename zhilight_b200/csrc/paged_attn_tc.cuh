@@ -188,7 +188,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
         const int t0 = (k.hi >= 0 ? k.lo / kPtKeys : 0) + (two_rows ? first : 2 * first), items = two_rows ? 2 : 4;   // of the ring for 64 keys
         // keys that all rows of the block see
         const int all_hi = min(k.place0 + p.by_group(k.row0), k.have - 1);
-        const int all_lo = p.window ? max(0, k.place0 + p.by_group(k.row0 + k.rows - 1) - p.window + 1) : 0;
+        const int all_lo = paged_from(p, k.place0 + p.by_group(k.row0 + k.rows - 1));
         if (warp < kPtWarpS) {
             const int m = warp >> 2, rt = tid & (kPaRows - 1), r = two_rows ? m * p.tile_rows + rt : rt;   // tile; row of it and of the block
             const bool mine = rt < p.tile_rows && r < k.rows;
@@ -196,7 +196,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             constexpr float kTau = PagedExp<kHalf>::kTau, kUp = PagedExp<kHalf>::kUp;
             const float cs = p.scale;
             const int row = k.row0 + (mine ? r : 0), t = p.by_group(row), place = k.place0 + t;
-            const int hi = mine ? min(place, k.have - 1) : -1, lo = mine && p.window ? max(0, place - p.window + 1) : 0;
+            const int hi = mine ? min(place, k.have - 1) : -1, lo = mine ? paged_from(p, place) : 0;
             const int key0 = (t0 + (two_rows ? 0 : m)) * kPtKeys, step = two_rows ? kPtKeys : 2 * kPtKeys;
             float l = 0.f, m_ref = kPagedNone;
             float times = cs, less = m_ref;                            // an exponent is a score times the one less the other
