@@ -194,3 +194,23 @@ def test_attention_of_the_widest_windows(cuda, window, new):
     for dim in (64, 128):
         check_attention(BF16, 8, 2, dim, 16, "rows", window, [(new // 2, new), (0, new), (new, new), (new + 300, new)])
         check_attention(F16, 8, 2, dim, 16, "rows", window, [(new // 2, new), (new - new // 4, new)], max_new=new)
+
+
+def test_numbers_beyond_32_bits(cuda):
+    """Python's integers do not come around: a wider window is as wide as any, a layout or a window below zero is refused."""
+    from zhilight_b200 import _lib
+    g = torch.Generator().manual_seed(24)
+    k, v = (x.cuda() for x in pool(g, 8, 16, 2, 64, BF16, "rows"))
+    table, lens, starts = torch.arange(8, dtype=torch.int32)[None].cuda(), torch.tensor([100], dtype=torch.int32).cuda(), starts_of([20]).cuda()
+    q = torch.randn(20, 8 * 64, generator=g).to(BF16).cuda()
+    want = ops.paged_attention(q, k, v, table, lens, starts, 0.1)
+    for window in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 63 + 5):
+        assert torch.equal(ops.paged_attention(q, k, v, table, lens, starts, 0.1, window=window), want)
+    for window in (-1, -2 ** 32 + 5):
+        with pytest.raises(_lib.ZLError):
+            ops.paged_attention(q, k, v, table, lens, starts, 0.1, window=window)
+    assert torch.equal(ops.paged_attention(q, k, v, table, lens, starts, 0.1, max_new=2 ** 32 + 1), want)
+    t = torch.zeros(20, dtype=torch.int32).cuda()
+    with pytest.raises(_lib.ZLError):
+        ops.qkv_axes_rope_append(torch.zeros(20, 12 * 64, dtype=BF16).cuda(), t[None], torch.ones(32, dtype=torch.float64).cuda(), torch.zeros(32, dtype=torch.int32).cuda(),
+                                 t, t - 1, table, k, v, 8, layout=2 ** 32)

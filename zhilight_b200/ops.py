@@ -1173,6 +1173,7 @@ def qkv_axes_rope_append(qkv, pos, inv_freq, axis, token_seq, placement, page_ta
     _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and 2 * half <= dim,
           "inv_freq must be contiguous float64, two columns of a head for each")
     _ints("axis", axis, (half,))
+    _need(layout in (ROT_HALVES, ROT_ADJACENT), "layout must be ROT_HALVES or ROT_ADJACENT")
     _need(pos.dim() == 2 and pos.shape[0] > 0, "pos must be (axes, T)")
     _ints("pos", pos, (pos.shape[0], t))
     _ints("token_seq", token_seq, (t,))
@@ -1208,6 +1209,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
     _ints("q_starts", q_starts, (seqs + 1,))
     _need(out is None or (out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous()), "out must be contiguous, of q's shape and type")
     _need(max_new is None or max_new > 0, "max_new must be positive")
+    window = int(window)
+    _need(window >= 0, "window must not be negative")
     _here(q, k_cache, v_cache, page_table, seq_lens, q_starts, out)
     if out is None:
         out = torch.empty_like(q)
@@ -1218,7 +1221,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _lib.call("zl_paged_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, *steps, page_table.data_ptr(),
               page_table.stride(0) if seqs > 1 else page_table.shape[1], page_table.shape[1], seq_lens.data_ptr(), q_starts.data_ptr(), seqs, float(scale),
-              int(window), out.data_ptr(), t, most, heads, kv_heads, dim, _dp(ws), nbytes, _dt(q), int(pdl), _stream())
+              min(window, 2 ** 31 - 1), out.data_ptr(), t, most, heads, kv_heads, dim, _dp(ws), nbytes, _dt(q), int(pdl), _stream())
     return out
 
 
