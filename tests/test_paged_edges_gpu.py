@@ -214,3 +214,48 @@ def test_numbers_beyond_32_bits(cuda):
     with pytest.raises(_lib.ZLError):
         ops.qkv_axes_rope_append(torch.zeros(20, 12 * 64, dtype=BF16).cuda(), t[None], torch.ones(32, dtype=torch.float64).cuda(), torch.zeros(32, dtype=torch.int32).cuda(),
                                  t, t - 1, table, k, v, 8, layout=2 ** 32)
+
+
+# ---- what tells which rows are whose ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("starts", [(0, 5, 3, 8), (8, 0, 8, 0), (0, 40, 30, 60), (3, 2, 60, 60), (5, -1, 10, 20)])
+@pytest.mark.parametrize("max_new", [1, None])
+def test_attention_of_starts_that_do_not_ascend(cuda, starts, max_new):
+    """No row is written."""
+    g = torch.Generator().manual_seed(25)
+    k, v = (x.cuda() for x in pool(g, 8, 16, 2, 64, BF16, "rows"))
+    table, lens = torch.arange(8, dtype=torch.int32).expand(3, 8).contiguous().cuda(), torch.tensor([100, 60, 70], dtype=torch.int32).cuda()
+    q, out = torch.randn(60, 4, 64, generator=g).to(BF16).cuda(), torch.full((60, 4, 64), 7.0, dtype=BF16, device="cuda")
+    ops.paged_attention(q, k, v, table, lens, torch.tensor(starts, dtype=torch.int32).cuda(), 0.1, max_new=max_new, out=out)
+    assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("starts,lens", [((-5, 3, 20, 90), (50, 60, 70)), ((0, 0, 60, 60), (-3, 60, 2 ** 31 - 1)), ((2, 10, 11, 2 ** 31 - 1), (0, 5, -2 ** 31)),
+                                         ((0, 20, 40, 60), (2 ** 31 - 1, 128, 129))])
+@pytest.mark.parametrize("max_new", [1, None])
+def test_attention_of_starts_and_lengths_out_of_range(cuda, starts, lens, max_new):
+    """Rows before the first and behind the last one are none, lengths go as far as the table has room."""
+    g = torch.Generator().manual_seed(26)
+    k, v = pool(g, 8, 16, 2, 64, BF16, "rows")
+    table, rows = torch.arange(8, dtype=torch.int32).expand(3, 8).contiguous(), 60
+    q, out = torch.randn(rows, 4, 64, generator=g).to(BF16), torch.full((rows, 4, 64), 7.0, dtype=BF16, device="cuda")
+    got = ops.paged_attention(q.cuda(), *on_gpu(k, v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor(starts, dtype=torch.int32).cuda(), 0.1,
+                              max_new=max_new, out=out).cpu().double()
+    mine = torch.zeros(rows, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        first, last = max(starts[b], 0), min(starts[b + 1], rows)
+        if first >= last:
+            continue
+        mine[first:last] = True
+        # the rows that there are, at the places that the sequence's own end gives them
+        place = n - starts[b + 1] + first
+        have = max(0, min(n, 128))
+        kk, vv = (oracle.rows_of(x, table, b, have) for x in (k, v))
+        for i in range(first, last):
+            sees = max(0, min(place + i - first + 1, have))
+            for h in range(4):
+                p = torch.softmax(kk[:sees, h // 2] @ q[i, h].double() * 0.1, 0)
+                o, spread = p @ vv[:sees, h // 2], p @ vv[:sees, h // 2].abs()
+                # scores below 20 in magnitude: 2 (64 + 8) 2^-24 times that; a rounded probability, a rounded result
+                err = spread * (2.0 ** -8 + 40 * 72 * 2.0 ** -24 + 2.0 ** -14)
+                assert ((got[i, h] - o).abs() <= err + oracle.half_step(o.abs() + err, BF16)).all(), (b, i, h)
+    assert (got[~mine] == 7.0).all()

@@ -119,7 +119,7 @@ extern "C" int zl_paged_attention(const void* q, const void* k_cache, const void
     const long long room = (long long)max_pages * page_size;
     const PagedPlan s = paged_plan(rows, max_new, seqs, (int)(room < INT_MAX - 255 ? room : INT_MAX - 255), heads, kv_heads, dim);
     // the kernels count tiles in 32 bits
-    ZL_CHECK_SUPPORTED(((long long)rows * (heads / kv_heads) / 16 + seqs) * (room / kPfKeys + 4) < INT_MAX / kv_heads);
+    ZL_CHECK_SUPPORTED(((long long)rows * (heads / kv_heads) / 16 + seqs) * (room / kPfKeys + 4) < (INT_MAX - (1 << 16)) / kv_heads);   // with room for a stretch more
     ZL_CHECK_ARG(workspace && workspace_bytes >= s.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
     const PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), num_pages, page_stride, row_stride, head_stride, page_table, ld_table, max_pages,
                           page_size, seqs, paged_divisor(page_size)};

@@ -61,12 +61,14 @@ struct PagedCut {
 
 // A warp's view of the line that the blocks of a kernel's work stand in: sequence by sequence, in it kv head by kv head, in that block by block, each
 // KIND::kSetup + KIND::turns() long.  A CTA of the grid takes an equal stretch of the line.  128 sequences are in view at a time, four to a lane; the blocks of a
-// sequence that has many are looked at by the whole warp.  Everything fits 32 bits, which the entry point sees to.
+// sequence that has many are looked at by the whole warp.  Everything fits 32 bits, which the entry point sees to, for sequences whose rows do not overlap: where
+// the starts do not ascend the line is empty.  No loop here goes by the lengths alone: one that changes under the kernel cannot keep it running.
 template <typename KIND>
 struct PagedLine {
     static constexpr int kAlone = 4;   // blocks of a sequence that a lane looks at by itself
     int total, per;                    // length of the line and of a stretch
     int b0, before, upto, cum[4];      // first sequence in view and its place; units of a kv head up to and with this lane's, and of this lane's four
+    bool ascends;                      // the starts of this lane's four
 
     static __device__ __forceinline__ int block(const PagedAttn& p, PagedBlock& k, int row0) {
         k.row0 = row0, k.rows = min(p.block_rows, k.n - row0);
@@ -81,8 +83,10 @@ struct PagedLine {
 #pragma unroll
         for (int u = 0; u < 4; ++u) len[u] = b + u < c.seqs ? p.lens[b + u] : 0;
         int all = 0;
+        ascends = true;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
+            ascends = ascends && (b + u >= c.seqs || at[u] <= at[u + 1]);
             PagedBlock k;
             k.first = max(at[u], 0);
             k.n = b + u < c.seqs ? max(min(at[u + 1], p.rows) - k.first, 0) * p.group : 0;
@@ -114,20 +118,24 @@ struct PagedLine {
     // length of the line, which `ctas` share; the view is at its beginning then
     __device__ __forceinline__ void begin(const PagedAttn& p, const PagedCache& c, int ctas) {
         total = before = 0;
+        bool all = true;
         for (b0 = (c.seqs - 1) & ~127;; b0 -= 128) {
             view(p, c);
+            all = __all_sync(0xffffffffu, all && ascends);
             total += __shfl_sync(0xffffffffu, upto, 31) * p.kv_heads;
             if (b0 == 0) break;
         }
+        if (!all) total = 0;
         per = (total + ctas - 1) / ctas;
     }
-    // the block at place w, which is in view or behind it
-    __device__ __forceinline__ void at(const PagedAttn& p, const PagedCache& c, int w, PagedBlock& k, PagedPlace& place) {
+    // the block at place w, which is in view or behind it; false: there is none
+    __device__ __forceinline__ bool at(const PagedAttn& p, const PagedCache& c, int w, PagedBlock& k, PagedPlace& place) {
         const int lane = threadIdx.x & 31;
         unsigned hit;
         while (!(hit = __ballot_sync(0xffffffffu, before + upto * p.kv_heads > w))) {
             before += __shfl_sync(0xffffffffu, upto, 31) * p.kv_heads;
             b0 += 128;
+            if (b0 >= c.seqs) return false;
             view(p, c);
         }
         const int src = __ffs(hit) - 1;
@@ -151,7 +159,7 @@ struct PagedLine {
         k.have = min(max(len, 0), c.room());
         // 32 blocks at a time
         int row0 = 0;
-        for (int r0 = 0; k.n > p.block_rows; r0 += 32 * p.block_rows) {
+        for (int r0 = 0; k.n > p.block_rows && r0 < k.n; r0 += 32 * p.block_rows) {
             PagedBlock o = k;
             const int r = r0 + lane * p.block_rows, mine = r < k.n ? block(p, o, r) : 0;
             int up = mine;
@@ -170,8 +178,9 @@ struct PagedLine {
             rem -= __shfl_sync(0xffffffffu, up, 31);
         }
         place.units = block(p, k, row0);
-        place.off = rem;
-        place.start = w - rem;
+        place.off = min(rem, place.units - 1);
+        place.start = w - place.off;
+        return true;
     }
 };
 
@@ -190,7 +199,7 @@ struct PagedWalk {
         const int first = min(line.total, per * (int)blockIdx.x);
         w = at < 0 ? first : at;
         end = min(line.total, first + per);
-        if (w < end) line.at(p, c, w, k, place);
+        if (w < end && !line.at(p, c, w, k, place)) w = end;
     }
     // turns first .. first + count - 1 of the block are this CTA's; none where the stretch ends before the block's first turn
     __device__ __forceinline__ void share(int& first, int& count) const {
