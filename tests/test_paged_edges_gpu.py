@@ -259,3 +259,36 @@ def test_attention_of_starts_and_lengths_out_of_range(cuda, starts, lens, max_ne
                 err = spread * (2.0 ** -8 + 40 * 72 * 2.0 ** -24 + 2.0 ** -14)
                 assert ((got[i, h] - o).abs() <= err + oracle.half_step(o.abs() + err, BF16)).all(), (b, i, h)
     assert (got[~mine] == 7.0).all()
+
+
+# ---- what the kernel for few rows does not round ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,part,keys", [(BF16, 0.9 * 2.0 ** -9, 300), (BF16, 0.9 * 2.0 ** -9, 1500), (F16, 0.9 * 2.0 ** -12, 200)])
+@pytest.mark.parametrize("seqs,new,heads,kv_heads", [(1, 1, 8, 2), (3, 4, 8, 2), (300, 2, 4, 2), (2, 1, 258, 2)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_probabilities_of_few_rows_are_not_rounded_to_the_type(cuda, dtype, part, keys, seqs, new, heads, kv_heads, dim):
+    """Half of the keys have probabilities of 1 and values of 1, the others just so much less that one rounding to 16 bits would make them 1 too, and values of -1: the
+    result is that difference.  Carried as 16 bits and the rest in 16 bits, a probability is off by eps^2 / 4; its exponent, below 64 in size, by 2^-19, its exponential by
+    2^-22 more; scores by (dim + 8) steps of 2^-24 of themselves; sums by a unit for each key; the result is rounded once."""
+    g = torch.Generator().manual_seed(27)
+    page = 16
+    lens = [keys - 7 * (b % 3) for b in range(seqs)]
+    pages = sum(-(-n // page) for n in lens)
+    table, starts = tables(g, lens, page, pages), starts_of([new] * seqs)
+    k, v = (x.zero_() for x in pool(g, pages, page, kv_heads, dim, dtype, "rows"))
+    k[:, 1::2, :, 0] = math.log1p(-part)
+    v[:, 0::2], v[:, 1::2] = 1.0, -1.0
+    q = torch.zeros(seqs * new, heads, dim).to(dtype)
+    q[..., 0] = 1.0
+    got = attend(q, k, v, table, lens, starts, 1.0, max_new=new)
+    eps = oracle.EPS[dtype]
+    low = math.exp(float(k[0, 1, 0, 0]))                             # of odd keys (a page has an even number of rows)
+    for b, n in enumerate(lens):
+        for i in range(new):
+            sees = n - new + i + 1
+            even, odd = (sees + 1) // 2, sees // 2
+            want = (even - odd * low) / (even + odd * low)
+            off = eps * eps / 4 + 2 * (2.0 ** -19 + 2.0 ** -22 + part * (dim + 8) * 2.0 ** -24) + 2 * (sees + 64) * 2.0 ** -24
+            off += (abs(want) + off) * eps / 2 + 2.0 ** -25
+            assert abs((even - odd) / (even + odd) - want) > off     # one rounding would not pass
+            row = got[int(starts[b]) + i]
+            assert ((row - want).abs() <= off).all(), (b, i, float((row - want).abs().max()), off)
