@@ -40,6 +40,35 @@ constexpr int kPtRows = 256, kPtKeys = 128, kPtHalf = 64, kPtThreads = 384, kPtW
 // (2^22, half a step of 1/4) it could leave the range of the probabilities, so the product is rounded as the reference was before the difference is taken.
 constexpr float kPtFar = 4194304.f;
 
+// The probabilities of 64 keys, of which a row sees from .. to, written over their scores at tb, where the reference is that far off: -> their sum
+template <typename T>
+__device__ __noinline__ float pt_far(uint32_t tb, float scale, float m_ref, float up, int from, int to) {
+    float sum = 0.f;
+#pragma unroll 1
+    for (int part = 0; part < kPtHalf; part += 32) {
+        uint32_t x[16];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float v[16];
+            tc_ld16(tb + (uint32_t)(part + half * 16), v);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                T two[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = part + half * 16 + i + e;
+                    const float y = key >= from && key <= to ? pa_exp2(__fadd_rn(__fsub_rn(__fmul_rn(v[i + e], scale), m_ref), up)) : 0.f;
+                    sum += y;
+                    two[e] = from_f32<T>(y);
+                }
+                x[half * 8 + i / 2] = *reinterpret_cast<const uint32_t*>(two);
+            }
+        }
+        tc_st16(tb + (uint32_t)(part / 2), x);
+    }
+    return sum;
+}
+
 // turns of a block, at least one: a block that sees nothing is written too
 struct PtKind {
     static constexpr int kSetup = 2;
@@ -199,7 +228,6 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             const int hi = mine ? min(place, k.have - 1) : -1, lo = mine ? paged_from(p, place) : 0;
             const int key0 = (t0 + (two_rows ? 0 : m)) * kPtKeys, step = two_rows ? kPtKeys : 2 * kPtKeys;
             float l = 0.f, m_ref = kPagedNone;
-            float times = cs, less = m_ref;                            // an exponent is a score times the one less the other
             bool far = false;                                          // a reference of this warp is beyond kPtFar
             for (int j = 0; j < 2 * count; ++j) {                      // 64 keys
                 const int b = j & 1, base = key0 + (j >> 1) * step + b * kPtHalf, h = hi - base, from_ = lo - base;   // this row sees from_ .. h of them
@@ -245,15 +273,11 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                         }
                     }
                     far = __any_sync(0xffffffffu, fabsf(m_ref) >= kPtFar && m_ref != kPagedNone);
-                    times = cs, less = m_ref;
-                    if (far) {
-#pragma unroll
-                        for (int i = 0; i < kPtHalf; ++i) raw[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(raw[i]), cs), m_ref));
-                        times = 1.f, less = 0.f;
-                    }
                 }
-                const uint64_t c2 = pa_two(times, times), m2 = pa_two(kUp - less, kUp - less);
+                const uint64_t c2 = pa_two(cs, cs), m2 = pa_two(kUp - m_ref, kUp - m_ref);
                 uint64_t sum[2] = {0, 0};
+                if (far) l += pt_far<T>(tb, cs, m_ref, kUp, from_, h);
+                else
 #pragma unroll
                 for (int part = 0; part < kPtHalf; part += 32) {
                     uint32_t x[16];
