@@ -292,3 +292,19 @@ def test_probabilities_of_few_rows_are_not_rounded_to_the_type(cuda, dtype, part
             assert abs((even - odd) / (even + odd) - want) > off     # one rounding would not pass
             row = got[int(starts[b]) + i]
             assert ((row - want).abs() <= off).all(), (b, i, float((row - want).abs().max()), off)
+
+
+@pytest.mark.parametrize("seqs", list(STEEP_SEQS))
+@pytest.mark.parametrize("heads,kv_heads", [(8, 2), (12, 4), (160, 1)])
+def test_attention_in_place(cuda, seqs, heads, kv_heads):
+    """out may be q itself."""
+    g = torch.Generator().manual_seed(28)
+    lens, new = [n for n, _ in STEEP_SEQS[seqs]], [m for _, m in STEEP_SEQS[seqs]]
+    pages = sum(-(-n // 16) for n in lens)
+    table, starts = tables(g, lens, 16, pages).cuda(), starts_of(new).cuda()
+    k, v = (x.cuda() for x in pool(g, pages, 16, kv_heads, 64, BF16, "rows"))
+    q = torch.randn(sum(new), heads, 64, generator=g).to(BF16).cuda()
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    want = ops.paged_attention(q, k, v, table, n, starts, 0.125, max_new=max(new))
+    got = ops.paged_attention(q, k, v, table, n, starts, 0.125, max_new=max(new), out=q)
+    assert got is q and torch.equal(q, want)
