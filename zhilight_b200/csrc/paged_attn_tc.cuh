@@ -579,7 +579,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
 // CTA's place 1, the others in the place 0 of theirs.  Of a block with two tiles of rows the second begins at row 128 of its place; one with a single tile has
 // two results in a place, the second there.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) k_paged_join_tiles(const PagedAttn p) {
+__global__ void __launch_bounds__(256, 1) k_paged_join_tiles(const PagedAttn p) {
     constexpr int W = D / 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d0 = warp * W;
     pdl_trigger();
@@ -590,14 +590,16 @@ __global__ void __launch_bounds__(256) k_paged_join_tiles(const PagedAttn p) {
     const bool twice = x.k.rows <= p.tile_rows, mine = r < x.k.rows;
     const int row = r >= p.tile_rows ? r - p.tile_rows + kPaRows : r;   // not more than 255
     float m = -INFINITY, l = 0.f, v[W] = {};
-    // as the softmax goes, from part to part, the loads of two at once
+    // As the softmax goes, from part to part, the loads of two at once: for which the compiler takes the registers (79) only where the bounds name a single CTA (one token
+    // of 64 heads on one over 30000 keys, a block in 148 parts: 76 us a call, 201 with 48 registers).
     const int parts = twice ? 2 * x.parts : x.parts;
-    for (int s0 = 0; s0 < parts; s0 += 2) {
-        float2 y[2];
-        float z[2][W];
+    auto take = [&](auto count, int s0) {
+        constexpr int N = decltype(count)::value;
+        float2 y[N];
+        float z[N][W];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int s = min(s0 + h, parts - 1), i = twice ? s >> 1 : s;
+        for (int h = 0; h < N; ++h) {
+            const int s = s0 + h, i = twice ? s >> 1 : s;
             const size_t part = (size_t)(blockIdx.x + i) * 2 + (i == 0);
             const int at = min(row + (twice && (s & 1) ? kPaRows : 0), kPtRows - 1);
             y[h] = p.ml[part * kPtRows + at];
@@ -605,15 +607,17 @@ __global__ void __launch_bounds__(256) k_paged_join_tiles(const PagedAttn p) {
             for (int u = 0; u < W; ++u) z[h][u] = p.part[(part * D + d0 + u) * kPtRows + at];
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (s0 + h >= parts) break;
+        for (int h = 0; h < N; ++h) {
             const float up = fmaxf(m, y[h].x), f = pa_exp2(m - up), g = pa_exp2(y[h].x - up);
             m = up;
             l = fmaf(y[h].y, g, l * f);
 #pragma unroll
             for (int u = 0; u < W; ++u) v[u] = fmaf(z[h][u], g, v[u] * f);
         }
-    }
+    };
+    int s0 = 0;
+    for (; s0 + 2 <= parts; s0 += 2) take(std::integral_constant<int, 2>{}, s0);
+    if (s0 < parts) take(std::integral_constant<int, 1>{}, s0);
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
     for (int u = 0; u < W; ++u) v[u] = l == 0.f ? 0.f : v[u] * inv;
