@@ -13,6 +13,7 @@
 // first loads and joins come under the other's stream.  Q by way of shared memory, for fewer registers, is slower (101 -> 108, 49 -> 57), and so is one warp that finds the
 // way for all (49 -> 53).
 #pragma once
+#include "attn_ptx.cuh"
 #include "paged_attn.cuh"
 
 #include <type_traits>
@@ -45,11 +46,6 @@ template <typename T>
 __device__ __forceinline__ void pf_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same<T, __half>::value) mma_16816_f16(d, a, b0, b1, d);
     else mma_16816_bf16(d, a, b0, b1, d);
-}
-__device__ __forceinline__ float pf_exp2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pf_pack(float a, float b) {
@@ -179,7 +175,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                     for (int u = 0; u < 2; ++u) {
                         top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 1));
                         top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], 2));
-                        const float f = top[u] > m_ref[u] ? pf_exp2(m_ref[u] - top[u]) : 1.f;
+                        const float f = top[u] > m_ref[u] ? pa_exp2(m_ref[u] - top[u]) : 1.f;
                         m_ref[u] = fmaxf(m_ref[u], top[u]);
                         l[u] *= f;
 #pragma unroll
@@ -190,7 +186,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {   // the difference first: it is as exact as the scores, whatever their size is
-                        const float x = pf_exp2((s[n][2 * u] - m_ref[u]) + kUp), y = pf_exp2((s[n][2 * u + 1] - m_ref[u]) + kUp);
+                        const float x = pa_exp2((s[n][2 * u] - m_ref[u]) + kUp), y = pa_exp2((s[n][2 * u + 1] - m_ref[u]) + kUp);
                         l[u] += x + y;
                         s[n][2 * u] = x, s[n][2 * u + 1] = y;
                         pa[2 * n + u] = pf_pack<T>(x, y);
@@ -274,7 +270,7 @@ __global__ void __launch_bounds__(kPfWarps * 32, kPfPerSm) k_paged_attn_few(cons
             for (int x = 1; x < kPfWarps; ++x) m = fmaxf(m, s_ml[x][r].x);
 #pragma unroll
             for (int x = 0; x < kPfWarps; ++x) {
-                const float f = pf_exp2(s_ml[x][r].x - m);
+                const float f = pa_exp2(s_ml[x][r].x - m);
                 sum = fmaf(s_ml[x][r].y, f, sum);
                 const float* from = reinterpret_cast<const float*>(pf_smem + x * C::kWarp) + r * C::kPitch + lane * E;
 #pragma unroll

@@ -510,7 +510,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                                        b / boxes * 64, row - pg * c.page_size, at.hk, id, &full[slot]);
                     }
                 }
-            } else if (!box) {
+            } else {
                 // Two rows (four of 64 columns) a copy of a warp.  A lane looks up every 32nd row of the 64 keys, once for K and V, and asks for the next ones'
                 // page numbers before it copies these.
                 const int ch = lane % CH, tiles = two_rows ? 1 : 2;
