@@ -8,8 +8,10 @@
 namespace zl {
 
 // Calls whose sequences bring at most so many (token, head) rows of a kv head each go to the kernel for few rows, as do groups that no tile holds a token of.
-// us, it / the tiles, 32 heads on 8, 2000 keys: 16 sequences with 4 rows 41 / 52, with 16 rows 43 / 52; two with 16 rows 19 / 28; one with 16 rows on 30000
-// keys 45 / 83.  A variant for 32 rows took 58 to 60 where the tiles take 53 (16 sequences; 26 / 28 for two, 66 / 70 for one on 30000 keys) and was left out.
+// us in a graph, it / the tiles, 32 heads on 8, 2000 keys: 16 sequences with 4 rows 35 / 48, with 16 rows 37 / 49; two with 16 rows 16 / 24; one with 16 rows on 30000
+// keys 41 / 54.  A variant for 32 rows took 58 to 60 where the tiles took 53 (16 sequences; 26 / 28 for two, 66 / 70 for one on 30000 keys) and was left out.
+// The line is drawn for groups of 4 and 8.  Single tokens of wider ones, in blocks of 16 rows here: 16 sequences of 2000 keys with 20 or 32 heads on one 19 / 25,
+// 64 heads 25 / 25, 128 heads 39 / 24; one sequence of 30000 keys 34 to 38 for all of these, 76 to 84 on the tiles, to which these calls go.
 constexpr int kFewRows = kPfRows;
 
 struct PagedPlan {

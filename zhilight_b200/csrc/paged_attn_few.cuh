@@ -7,11 +7,11 @@
 // S = Q K^T and O += P V by mma.sync with Q as the 16-row operand, whose accumulators are the next product's operand as they stand.  The probabilities are
 // carried as a 16-bit value and the rest of it as another, their sum in 32 bits; the reference maximum of a row follows lazily as in paged_attn_tc.cuh.
 //
-// One token over 131072 keys, 32 heads on 8, with the join: 104 us in a graph, errors of 1.7e-3 against 64 bits; with probabilities of 16 bits alone 101 us (87 of them, 6.2 TB/s of
-// the 6.45 that a copy reaches, in this kernel) and 2.3e-3.  The other times here were taken with 16 bits alone.  32 sequences up to 4096 keys: 43 and 49 us for
-// 174 MB, behind the first loads of every block: its setup stands in the line as two tiles (64 us where it did not).  Two CTAs share an SM, one's
-// first loads and joins come under the other's stream.  Q by way of shared memory, for fewer registers, is slower (101 -> 108, 49 -> 57), and so is one warp that finds the
-// way for all (49 -> 53).
+// One token over 131072 keys, 32 heads on 8: 99 us a call in a graph, 103 to 105 in a row of eager ones (537 MB: 5.1 TB/s or more of the 6.45 that a copy reaches), 96 of
+// them in this kernel under ncu; errors of 1.7e-3 against 64 bits, 2.3e-3 with probabilities of 16 bits alone, which takes 2 to 3 us off.  28 of 32 sequences with up to 4096 keys:
+// 41 us for 174 MB, bound by the first loads of every block, whose setup stands in the line as two tiles.  Two CTAs share an SM (167 or 238 registers), one's
+// first loads and joins come under the other's stream.  Taken when these calls took 101 and 49 us: 64 where the setup did not count; Q by way of shared memory, for fewer
+// registers, 108 and 57; one warp that finds the way for all 53.
 #pragma once
 #include "attn_ptx.cuh"
 #include "paged_attn.cuh"

@@ -10,8 +10,8 @@
 //                   that one page has (where these are fewer than four, or a page has fewer than 8, both copy 16 bytes at a time)
 //
 // A page's rows behind the last visible key may hold anything.  Copies of 16 bytes leave them out; behind TMA the softmax's threads make those values zeros
-// before they hand the tile's probabilities on.  Rows behind a page number outside the pool are zeros either way.  Tensor memory: scores of the two tiles (128 columns each, probabilities over their first
-// half), then their outputs.  Probabilities are rounded to the rows' type once (half a step each, of random sign: beside the output's own rounding), the
+// before they hand the tile's probabilities on.  Rows behind a page number outside the pool are zeros either way.  Tensor memory: scores of the two tiles
+// (128 columns each, probabilities over their first half), then their outputs.  Probabilities are rounded to the rows' type once (half a step each, of random sign: beside the output's own rounding), the
 // sums that divide them are not.  A row's reference maximum follows the true one only once that has grown by 2^5 (fp16) or 2^8:
 // any reference gives the same quotient (PagedExp).
 //
@@ -19,12 +19,16 @@
 // sum.  Of the keys that not all rows of a block see (its last ones, and the first ones of a window) the softmax's threads therefore look the values over before they
 // hand the tile's probabilities on, and put zeros where they are no numbers (pt_clean); at the block's end they add those to the rows that do see them (pt_add_broken).
 //
-// 4096 tokens behind 4096, 32 heads on 8, bf16: 390 to 450 us by the GPU it ran on, 0.92 to 1.06 PFLOP/s.  A turn takes 3000 cycles, of which the MMAs need 2050 at least and
-// the exponentials of both groups 2050; under this load the SM runs at 1.2 GHz.  Before, the same in us: copies of 16 bytes by two warps 693 (they bound it),
+// 4096 tokens behind 4096, 32 heads on 8, bf16: 395 us in a graph, 455 in a row of calls, 0.91 to 1.04 PFLOP/s; the look at the values takes 5 us of it.  A turn takes 3000 cycles, of
+// which the MMAs need 2050 at least and the exponentials of both groups 2050; under this load the SM runs at 1.2 GHz.  On the way, the same in us: copies of 16 bytes by two warps 693 (they bound it),
 // TMA 544, scores of 64 keys ahead of the softmax in two buffers 503 (128 keys at a time leave no room for a second one, and S -> softmax -> P V is
 // then one chain of 4400 cycles), a thread each for S and P V 434, Q and the first scores under the results of the block before 420, parts column by column 395.
 // Scores of 64 keys read Q twice as often; they are 450 cycles each instead of 300.  Blocks of up to 128 rows stream K and V like the kernel for few rows, five turns
-// of 64 keys in flight: drafts of 16 users, 64 heads on 8, 57 us for 186 MB, 68 with the join (a block's setup as two turns: 103 where it did not count).
+// of 64 keys in flight: drafts of 16 users, 64 heads on 8, 57 us for 186 MB under ncu, 65 a call with the join (when it took 68: 103 where a block's setup did not count
+// as two turns).
+//
+// Where the look at the values stands was measured, drafts / mixed portions with a window / this prompt in us without it 68 / 68 / 388: here 70 / 69 / 393; with a barrier
+// and the product of such tiles by the softmax's threads 69 / 78 / 394; by warp 9 before its products 73 / 80 / 404; by the loaders, once a tile has landed, 77 / 81 / 406.
 #pragma once
 #include "attn_ptx.cuh"
 #include "paged_attn.cuh"

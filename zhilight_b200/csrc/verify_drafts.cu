@@ -5,9 +5,10 @@
 // Only that one row of p and q is read whole.  The CTAs of a cluster share the vocabulary, a warp has a run of neighbouring words: a pass for the sums
 // of the warps, which every CTA gets from the others' shared memory, then the CTA that has the word's run goes over that run once more.
 // Differences, products and sums are in 64 bits: products of two 32-bit numbers are exact there, sums of probabilities above 2^-29 too, and
-// a tie falls as the formula says.  Bound by bytes, the latency of a chain of three loads and a cluster's barrier where there are few sequences:
-// 64 sequences of 128256 words 15.4 us (65.7 MB: 4.3 TB/s), one of 32000 7.1 us.  Eight warps of 16 loads ahead; 16 warps of 8, of which an SM holds three
-// CTAs, take 21.5 us, of 16 23.1; four CTAs of 32 registers 19.5.
+// a tie falls as the formula says.  A sequence whose drafts were all taken reads no row of q: of 64 sequences with up to 5 drafts 21 to 24 refuse one, 44 to 45 MB for
+// 128256 words.  15.4 us in a graph with the rows in L2 (2.9 TB/s), 17 a call, 18 under ncu with cold caches (2.5 TB/s; DRAM 31 %, SMs 28 % busy): bound by neither, but by a chain of
+// three dependent loads, a pass behind them, the cluster's barrier and the run once more (6.9 us for one sequence of 32000 words), all CTAs in one wave.
+// Eight warps of 16 loads ahead; 16 warps of 8, of which an SM holds three CTAs, took 21.5 us where these took 15.4, of 16 23.1; four CTAs of 32 registers 19.5.
 #include "paged.cuh"
 #include "tc2_common.cuh"
 
