@@ -1134,12 +1134,14 @@ int zl_qkv_axes_rope_append(const void* qkv, long long ldq, const int32_t* pos, 
                             const int32_t* page_table, int ld_table, int max_pages, int seqs, void* k_cache, void* v_cache, long long num_pages,
                             int page_size, long long page_stride, long long row_stride, long long head_stride, void* q_out, int T, int heads,
                             int kv_heads, int dim, int dtype, int pdl, zl_stream_t stream);
-/* Attention of the rows q_starts[b] .. q_starts[b + 1] - 1 (q_starts (seqs + 1) ascending, or no row is written) of q (rows, heads * dim) over sequence b: row i of its n rows
+/* Attention of the rows q_starts[b] .. q_starts[b + 1] - 1 (q_starts (seqs + 1) ascending) of q (rows, heads * dim) over sequence b: row i of its n rows
  * stands at place p = seq_lens[b] - n + i and sees the keys j <= p that the sequence has, with window > 0 those with j > p - window only;
  * out = softmax(scale q k) v, zeros where a row sees nothing or -inf alone.  Scores are 32-bit numbers: sums of q k and 1.4427 times a score have to stay
- * below 3.4e38.  Rows of q of no sequence: out stays as it is.  out may be q.  seq_lens counts the new tokens, whose keys and values are appended already.
+ * below 3.4e38.  Rows of q of no sequence: out stays as it is; a sequence whose start is not before its end has none, and where all together have more rows
+ * than q no row is written.  out may be q.  seq_lens counts the new tokens, whose keys and values are appended already.
  * What masked keys and values hold (infinities, NaN) does not matter; a value that a row sees and that is an infinity or NaN makes its column one, such a
- * key the row.  max_new: a bound of the sequences' new tokens, which chooses the kernels (results agree within their rounding).  scale > 0; dim 64 or 128; dtype fp16 or bf16. */
+ * key the row.  max_new: a bound of the sequences' new tokens, which chooses the kernels (results agree within their rounding).  scale > 0; dim 64 or 128;
+ * dtype fp16 or bf16. */
 size_t zl_paged_attention_workspace_bytes(int rows, int max_new, int seqs, int max_keys /* max_pages * page_size */, int heads, int kv_heads, int dim);
 int zl_paged_attention(const void* q, const void* k_cache, const void* v_cache, long long num_pages, int page_size, long long page_stride,
                        long long row_stride, long long head_stride, const int32_t* page_table, int ld_table, int max_pages,

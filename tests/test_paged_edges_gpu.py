@@ -217,10 +217,10 @@ def test_numbers_beyond_32_bits(cuda):
 
 
 # ---- what tells which rows are whose ---------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("starts", [(0, 5, 3, 8), (8, 0, 8, 0), (0, 40, 30, 60), (3, 2, 60, 60), (5, -1, 10, 20)])
+@pytest.mark.parametrize("starts", [(0, 40, 30, 60), (0, 60, 0, 60), (0, 60, 59, 60), (-7, 70, 5, 6)])
 @pytest.mark.parametrize("max_new", [1, None])
-def test_attention_of_starts_that_do_not_ascend(cuda, starts, max_new):
-    """No row is written."""
+def test_attention_of_more_rows_than_there_are(cuda, starts, max_new):
+    """Sequences that have more rows together than q: no row is written."""
     g = torch.Generator().manual_seed(25)
     k, v = (x.cuda() for x in pool(g, 8, 16, 2, 64, BF16, "rows"))
     table, lens = torch.arange(8, dtype=torch.int32).expand(3, 8).contiguous().cuda(), torch.tensor([100, 60, 70], dtype=torch.int32).cuda()
@@ -230,10 +230,11 @@ def test_attention_of_starts_that_do_not_ascend(cuda, starts, max_new):
 
 
 @pytest.mark.parametrize("starts,lens", [((-5, 3, 20, 90), (50, 60, 70)), ((0, 0, 60, 60), (-3, 60, 2 ** 31 - 1)), ((2, 10, 11, 2 ** 31 - 1), (0, 5, -2 ** 31)),
-                                         ((0, 20, 40, 60), (2 ** 31 - 1, 128, 129))])
+                                         ((0, 20, 40, 60), (2 ** 31 - 1, 128, 129)), ((0, 20, 50, 0), (30, 60, 70)), ((8, 0, 8, 0), (30, 60, 70)), ((5, -1, 10, 20), (9, 60, 70)),
+                                         ((60, 60, 0, 60), (9, 60, 70))])
 @pytest.mark.parametrize("max_new", [1, None])
 def test_attention_of_starts_and_lengths_out_of_range(cuda, starts, lens, max_new):
-    """Rows before the first and behind the last one are none, lengths go as far as the table has room."""
+    """Rows before the first and behind the last one are none, lengths go as far as the table has room, a sequence that ends before it begins has no rows."""
     g = torch.Generator().manual_seed(26)
     k, v = pool(g, 8, 16, 2, 64, BF16, "rows")
     table, rows = torch.arange(8, dtype=torch.int32).expand(3, 8).contiguous(), 60

@@ -61,14 +61,14 @@ struct PagedCut {
 
 // A warp's view of the line that the blocks of a kernel's work stand in: sequence by sequence, in it kv head by kv head, in that block by block, each
 // KIND::kSetup + KIND::turns() long.  A CTA of the grid takes an equal stretch of the line.  128 sequences are in view at a time, four to a lane; the blocks of a
-// sequence that has many are looked at by the whole warp.  Everything fits 32 bits, which the entry point sees to, for sequences whose rows do not overlap: where
-// the starts do not ascend the line is empty.  No loop here goes by the lengths alone: one that changes under the kernel cannot keep it running.
+// sequence that has many are looked at by the whole warp.  Everything fits 32 bits, which the entry point sees to, for sequences that have no more rows together
+// than q: where they have, their rows overlap, and the line is empty.  No loop here goes by the lengths alone: one that changes under the kernel cannot keep it running.
 template <typename KIND>
 struct PagedLine {
     static constexpr int kAlone = 4;   // blocks of a sequence that a lane looks at by itself
     int total, per;                    // length of the line and of a stretch
     int b0, before, upto, cum[4];      // first sequence in view and its place; units of a kv head up to and with this lane's, and of this lane's four
-    bool ascends;                      // the starts of this lane's four
+    unsigned low, high;                // new tokens of this lane's four, 16 bits each and the rest
 
     static __device__ __forceinline__ int block(const PagedAttn& p, PagedBlock& k, int row0) {
         k.row0 = row0, k.rows = min(p.block_rows, k.n - row0);
@@ -83,13 +83,14 @@ struct PagedLine {
 #pragma unroll
         for (int u = 0; u < 4; ++u) len[u] = b + u < c.seqs ? p.lens[b + u] : 0;
         int all = 0;
-        ascends = true;
+        low = high = 0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            ascends = ascends && (b + u >= c.seqs || at[u] <= at[u + 1]);
             PagedBlock k;
             k.first = max(at[u], 0);
-            k.n = b + u < c.seqs ? max(min(at[u + 1], p.rows) - k.first, 0) * p.group : 0;
+            k.n = b + u < c.seqs ? max(min(at[u + 1], p.rows) - k.first, 0) : 0;
+            low += k.n & 0xffff, high += k.n >> 16;
+            k.n *= p.group;
             k.place0 = len[u] - at[u + 1] + k.first;
             k.have = min(max(len[u], 0), c.room());
             const bool many = k.n > kAlone * p.block_rows;
@@ -118,14 +119,14 @@ struct PagedLine {
     // length of the line, which `ctas` share; the view is at its beginning then
     __device__ __forceinline__ void begin(const PagedAttn& p, const PagedCache& c, int ctas) {
         total = before = 0;
-        bool all = true;
+        long long rows = 0;
         for (b0 = (c.seqs - 1) & ~127;; b0 -= 128) {
             view(p, c);
-            all = __all_sync(0xffffffffu, all && ascends);
+            rows += ((long long)__reduce_add_sync(0xffffffffu, high) << 16) + __reduce_add_sync(0xffffffffu, low);
             total += __shfl_sync(0xffffffffu, upto, 31) * p.kv_heads;
             if (b0 == 0) break;
         }
-        if (!all) total = 0;
+        if (rows > p.rows) total = 0;
         per = (total + ctas - 1) / ctas;
     }
     // the block at place w, which is in view or behind it; false: there is none

@@ -1196,7 +1196,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
     behind page_table (sequences, pages) int32.  Each sees the keys up to its own, with a window only the last `window` of them; a row that sees none
     gives zeros.  seq_lens (sequences) and q_starts (sequences + 1), ascending, int32.  max_new: a bound of the new tokens of one sequence (None: all
     rows), which chooses kernels and nothing else: without it a batch of single tokens takes those for many rows (32 users of up to 4096 keys 62 us
-    instead of 43).  Rows of no sequence, and all rows where q_starts descends: out, if given, keeps what it holds there; it may be q.  -> out, like q."""
+    instead of 43).  A sequence whose start is not before its end has no rows.  Rows of
+    no sequence, and all rows where the sequences have more together than q: out, if given, keeps what it holds there; it may be q.  -> out, like q."""
     if _lib.host is not None:
         y = _lib.host.paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl)
         if y is not None:
