@@ -129,10 +129,12 @@ def _lens(case):
 
 def _pack(x):
     """Rows (..., dim) in 16 bits -> (..., dim / 2 + dim / 8) bytes: 4-bit codes, then step and lowest value of every 32 columns in the rows' type.
-    The step is a 15th of the range, rounded; a code is the nearest whole number of steps above the lowest, at most 15."""
+    The step is a 15th of the range, rounded down: no code stands for more than the highest; a code is the nearest whole number of steps, at most 15."""
     v = x.float().unflatten(-1, (-1, GROUP))
     low, high = v.amin(-1, keepdim=True), v.amax(-1, keepdim=True)
-    step = ((high * 0.5 - low * 0.5) / 7.5).to(x.dtype)               # halves: a range may be beyond the largest number
+    part = (high * 0.5 - low * 0.5) / 7.5                             # halves: a range may be beyond the largest number
+    step = part.to(x.dtype)
+    step = (step.view(torch.int16) - (step.float() > part).to(torch.int16)).view(x.dtype)
     s = step.float()
     code = torch.where(s >= 2.0 ** -126, ((v * 0.5 - low * 0.5) / torch.where(s > 0, s, 1.0) * 2.0).round().clamp(0, 15), 0.0).to(torch.uint8).flatten(-2)
     code = code.unflatten(-1, (-1, 8))[..., NIBBLE].flatten(-2)
@@ -390,12 +392,13 @@ def _values64(rows, dtype):
 
 def _stored64(x, dtype):
     """What rows (T, heads, dim) stand for once they have been written: columns of a group between its ends in 15 equal steps."""
-    out = torch.empty(x.shape, dtype=torch.float64, device=x.device)
+    out, bits = torch.empty(x.shape, dtype=torch.float64, device=x.device), 8 if dtype == torch.bfloat16 else 11
     x = x.to(dtype).double()
     for i in range(0, x.shape[-1], GROUP):
         part = x[..., i:i + GROUP]
         low = part.min(-1, keepdim=True).values
-        step = ((part.max(-1, keepdim=True).values - low) / 15).to(dtype).double()
+        mantissa, power = torch.frexp((part.max(-1, keepdim=True).values - low) / 15)
+        step = torch.floor(mantissa * 2.0 ** bits) * torch.exp2((power - bits).double())
         out[..., i:i + GROUP] = low + step * torch.where(step > 0, torch.round((part - low) / step), 0.0).clamp(max=15)
     return out.to(dtype).double()
 
