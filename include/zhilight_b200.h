@@ -1156,6 +1156,41 @@ int zl_paged_attention(const void* q, const void* k_cache, const void* v_cache, 
 int zl_verify_drafts(const float* target, long long target_seq, long long target_row, const float* draft, long long draft_seq, long long draft_row,
                      const int32_t* drafted, const float* accept, const float* sample, const int32_t* count, int32_t* accepted, int32_t* tokens,
                      int seqs, int drafts, int vocab, int pdl, zl_stream_t stream);
+/* The same cache in 4 bits.  A head's row is dim / 2 bytes of codes and, for every 32 columns, a pair (step, lowest value) in the rows' type: 5 dim / 8 bytes (80 for
+ * heads of 128, 40 for 64; no other dim).  A code c stands for lowest + step * c, rounded to that type; the step is a 15th of the range of the 32 values, rounded down, a
+ * value becomes the nearest whole number of steps, at most 15.  32 values with an infinity or NaN among them read as NaN.  Columns 8i .. 8i + 7 lie in bits
+ * 0 16 4 20 8 24 12 28 of word i.  Strides are bytes here, multiples of dim / 8, as both bases are.
+ * zl_qkv_axes_rope_append_int4 is zl_qkv_axes_rope_append into such a cache: two rows of qkv have to fit shared memory (56000 elements). */
+int zl_qkv_axes_rope_append_int4(const void* qkv, long long ldq, const int32_t* pos, long long ld_pos, int axes, const double* inv_freq,
+                                 const int32_t* axis, int half, int layout, float mscale, const int32_t* token_seq, const int32_t* placement,
+                                 const int32_t* page_table, int ld_table, int max_pages, int seqs, void* k_cache, void* v_cache, long long num_pages,
+                                 int page_size, long long page_stride, long long row_stride, long long head_stride, void* q_out, int T, int heads,
+                                 int kv_heads, int dim, int dtype, int pdl, zl_stream_t stream);
+/* What n pages stand for: k_out and v_out (n, page_size, kv_heads, dim) in `dtype`, the type that their rows were written from.  pages (n) int32 page numbers, one outside
+ * the pool reads as zeros; NULL: the first n.  v_cache NULL: k_cache alone. */
+int zl_int4_cache_values(const void* k_cache, const void* v_cache, long long num_pages, int page_size, long long page_stride, long long row_stride,
+                         long long head_stride, const int32_t* pages, long long n, void* k_out, void* v_out, int kv_heads, int dim, int dtype, int pdl,
+                         zl_stream_t stream);
+/* zl_paged_attention over such a cache.  A broken group (NaN) of a key or value reaches the rows that see it and no others. */
+size_t zl_paged_attention_int4_workspace_bytes(int rows, int max_new, int seqs, int max_keys /* max_pages * page_size */, int heads, int kv_heads, int dim);
+int zl_paged_attention_int4(const void* q, const void* k_cache, const void* v_cache, long long num_pages, int page_size, long long page_stride,
+                            long long row_stride, long long head_stride, const int32_t* page_table, int ld_table, int max_pages,
+                            const int32_t* seq_lens, const int32_t* q_starts, int seqs, float scale, int window, void* out, int rows, int max_new,
+                            int heads, int kv_heads, int dim, void* workspace, size_t workspace_bytes, int dtype, int pdl, zl_stream_t stream);
+/* Penalties, biases, temperature and grammar masks on logits (rows, ld_logits >= vocab) in `dtype` -> out (rows, ld_out) in the same type or fp32; out may be logits.
+ * History of row r: the first token_lens[r] (clamped to 0 .. longest) words of row token_seq[r] (NULL: r; outside [0, seqs): no history) of tokens (seqs, ld_tokens), the
+ * first prompt_lens[r] (NULL: 0) of them a prompt; words outside the vocabulary are passed over.  In this order, each in 32 bits:
+ *   a word of the history:         z = z > 0 ? z / repetition[r] : z * repetition[r]
+ *   n > 0 times behind the prompt: z = z - frequency[r] * n - presence[r]
+ *   biases bias_starts[r] .. bias_starts[r + 1] - 1 (clamped to 0 .. n_bias): z = z + bias[i] for the word bias_words[i], in the list's order
+ *   temperature[r] >= 2^-126:      z = z * (1 / temperature[r]); else z stays
+ *   mask row mask_row[r] (NULL: r; outside [0, masks): none), bit w % 32 of word w / 32 is clear: z = -inf.  A mask may leave nothing.
+ * Arrays that are NULL take no part.  Whole numbers are counted: the same result in every run. */
+int zl_adjust_logits(const void* logits, long long ld_logits, int dtype, void* out, long long ld_out, int out_dtype, int rows, int vocab,
+                     const int32_t* tokens, long long ld_tokens, int seqs, int longest, const int32_t* token_seq, const int32_t* token_lens,
+                     const int32_t* prompt_lens, const float* repetition, const float* frequency, const float* presence, const int32_t* bias_starts,
+                     const int32_t* bias_words, const float* bias, int n_bias, const float* temperature, const int32_t* mask, long long ld_mask,
+                     int masks, const int32_t* mask_row, int pdl, zl_stream_t stream);
 #ifdef __cplusplus
 }
 #endif

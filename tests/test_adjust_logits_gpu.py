@@ -1,0 +1,215 @@
+"""Penalties, biases, temperature and grammar masks on logits on a GPU, against the formula in 64 bits (int4_oracle.adjust)."""
+import math
+
+import pytest
+import torch
+
+from tests import int4_oracle as oracle
+from tests.test_paged_gpu import Own, both_ways
+from zhilight_b200 import ops
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def settings(g, rows, vocab, seqs, longest, biases, masks, repeated=0.3):
+    """Everything at once, on the host: words that come again, words outside the vocabulary, lengths and lists beyond their ends, neutral settings among the others."""
+    words = torch.randint(-2, vocab + 2, (seqs, longest), generator=g, dtype=torch.int32)
+    again = torch.rand(seqs, longest, generator=g) < repeated
+    words[again] = torch.randint(0, min(vocab, 7), (int(again.sum()),), generator=g, dtype=torch.int32)
+    counts = torch.randint(0, 2 * biases + 1, (rows,), generator=g)
+    counts[::3] = 0
+    starts = torch.zeros(rows + 1, dtype=torch.int32)
+    starts[1:] = counts.cumsum(0)
+    n = int(starts[-1])
+    bias = torch.randn(n, generator=g) * 5
+    bias[::5] = -100.0
+    at = torch.randint(-1, vocab + 1, (n,), generator=g, dtype=torch.int32)
+    at[::4] = torch.randint(0, min(vocab, 5), (len(at[::4]),), generator=g, dtype=torch.int32)   # words that are listed more than once
+    mix = lambda lo, hi, plain: torch.where(torch.rand(rows, generator=g) < 0.3, plain, lo + (hi - lo) * torch.rand(rows, generator=g))  # noqa: E731
+    return dict(tokens=words, token_seq=torch.randint(-1, seqs + 1, (rows,), generator=g, dtype=torch.int32),
+                token_lens=torch.randint(-1, longest + 3, (rows,), generator=g, dtype=torch.int32),
+                prompt_lens=torch.randint(-1, longest + 3, (rows,), generator=g, dtype=torch.int32), repetition=mix(0.7, 1.5, 1.0), frequency=mix(-0.3, 0.8, 0.0),
+                presence=mix(-0.3, 0.8, 0.0), bias_starts=starts, bias_words=at, bias=bias, temperature=mix(0.1, 2.0, 0.0),
+                mask=torch.randint(-2 ** 31, 2 ** 31 - 1, (masks, (vocab - 1) // 32 + 2), generator=g, dtype=torch.int32),
+                mask_row=torch.randint(-1, masks + 1, (rows,), generator=g, dtype=torch.int32))
+
+
+def on_gpu(kw):
+    return {n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in kw.items()}
+
+
+def check(z, kw, out_dtype=None, got=None):
+    kind = out_dtype or z.dtype
+    got = (ops.adjust_logits(z.cuda(), out_dtype=out_dtype, **on_gpu(kw)) if got is None else got).cpu()
+    assert got.dtype == kind and got.shape == z.shape
+    want, off = oracle.adjust(z, kind, **kw)
+    want, off, got = torch.from_numpy(want), torch.from_numpy(off), got.double()
+    assert torch.equal(torch.isnan(want), torch.isnan(got)) and torch.equal(want == -math.inf, got == -math.inf) and torch.equal(want == math.inf, got == math.inf)
+    fine = torch.isfinite(want)
+    assert ((want - got).abs() <= off)[fine].all(), float(((want - got).abs() - off)[fine].max())
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(BF16, None), (BF16, F32), (F16, None), (F16, F32), (F32, None)])
+@pytest.mark.parametrize("rows,vocab,seqs,longest", [(1, 1, 1, 1), (3, 7, 2, 5), (5, 100, 3, 70), (9, 1000, 4, 33), (4, 4099, 4, 700), (2, 32000, 2, 3000), (7, 50257, 3, 257),
+                                                     (3, 128256, 2, 5000), (2, 152064, 1, 100)])
+def test_adjust(cuda, dtype, out_dtype, rows, vocab, seqs, longest):
+    g = torch.Generator().manual_seed(rows * 100 + vocab)
+    z = (torch.randn(rows, vocab, generator=g) * 4).to(dtype)
+    check(z, settings(g, rows, vocab, seqs, longest, 9, 3), out_dtype)
+
+
+def test_adjust_of_the_widest_vocabularies(cuda):
+    """More words than a cluster has room for at once."""
+    g = torch.Generator().manual_seed(1)
+    for vocab in (393216, 393248, 900001):
+        z = torch.randn(2, vocab, generator=g).to(BF16)
+        kw = settings(g, 2, vocab, 2, 3000, 30, 2)
+        kw["token_seq"][:], kw["token_lens"][:] = torch.tensor([1, 0]), torch.tensor([3000, 2900])
+        check(z, kw, F32)
+
+
+@pytest.mark.parametrize("only", [(), ("tokens", "token_lens"), ("tokens", "token_lens", "repetition"), ("tokens", "token_lens", "token_seq", "frequency"),
+                                  ("tokens", "token_lens", "prompt_lens", "presence"), ("bias_starts", "bias_words", "bias"), ("temperature",), ("mask",),
+                                  ("mask", "mask_row", "temperature"), ("bias_starts", "bias_words", "bias", "mask")])
+@pytest.mark.parametrize("vocab", [1000, 33000, 33001])
+def test_adjust_by_parts(cuda, only, vocab):
+    """Each argument alone: the others take no part."""
+    g = torch.Generator().manual_seed(vocab)
+    z = (torch.randn(6, vocab, generator=g) * 3).to(BF16)
+    kw = settings(g, 6, vocab, 8, 400, 12, 7)
+    check(z, {n: kw[n] for n in only})
+
+
+@pytest.mark.parametrize("vocab", [64, 1003, 40000])
+def test_adjust_strided_and_in_place(cuda, vocab):
+    g = torch.Generator().manual_seed(4)
+    for dtype in (BF16, F32):
+        wide = (torch.randn(5, vocab + 24, generator=g) * 3).to(dtype)
+        kw = settings(g, 5, vocab, 3, 90, 5, 2)
+        kw["tokens"] = torch.cat([kw["tokens"]] * 2, 1)[:, :90]
+        kw["mask"] = torch.cat([kw["mask"]] * 2, 1)[:, :kw["mask"].shape[1]]
+        dev = on_gpu(kw)
+        for first in (0, 8, 3):
+            z = wide[:, first:first + vocab]
+            dz = wide.cuda()[:, first:first + vocab]
+            check(z, kw, F32, got=ops.adjust_logits(dz, out_dtype=F32, **dev))
+            room = torch.full((5, vocab + 16), 9.0, dtype=dtype, device="cuda")
+            got = ops.adjust_logits(dz, out=room[:, 5:vocab + 5], **dev)
+            check(z, kw, got=got)
+            assert (room[:, :5] == 9.0).all() and (room[:, vocab + 5:] == 9.0).all()
+            got = ops.adjust_logits(dz, out=dz, **dev)
+            assert got is dz
+            check(z, kw, got=got)
+            assert torch.equal(dz._base[:, :first].cpu(), wide[:, :first]) and torch.equal(dz._base[:, first + vocab:].cpu(), wide[:, first + vocab:])
+
+
+def test_adjust_of_special_numbers(cuda):
+    """Infinities and NaN in logits, biases and settings; masks that leave nothing or hide them; empty histories and lists."""
+    vocab = 300
+    z = torch.zeros(8, vocab)
+    z[:, 0], z[:, 1], z[:, 2], z[:, 3], z[:, 4] = math.nan, math.inf, -math.inf, 3.0e38, -1e-42
+    z[:, 5:] = torch.randn(8, vocab - 5, generator=torch.Generator().manual_seed(3))
+    kw = dict(tokens=torch.arange(20, dtype=torch.int32).expand(1, 20).contiguous(), token_seq=torch.zeros(8, dtype=torch.int32),
+              token_lens=torch.tensor([20, 0, 20, 20, 5, 20, 20, 20], dtype=torch.int32), prompt_lens=torch.tensor([20, 0, 0, 10, 0, 0, 0, 0], dtype=torch.int32),
+              repetition=torch.tensor([1.3, 1.3, 0.5, 1.0, 2.0, 1e30, 1e-30, 1.0]), frequency=torch.tensor([0.0, 1.0, 0.5, 0.5, 0.0, 0.0, 0.0, math.inf]),
+              presence=torch.zeros(8), bias_starts=torch.tensor([0, 0, 3, 3, 3, 3, 3, 3, 4], dtype=torch.int32), bias_words=torch.tensor([1, 9, 9, 40], dtype=torch.int32),
+              bias=torch.tensor([-math.inf, math.inf, -1.0, math.nan]), temperature=torch.tensor([0.0, 1.0, -1.0, 1e-30, 1e-40, math.inf, 0.5, math.nan]),
+              mask=torch.zeros(3, 10, dtype=torch.int32), mask_row=torch.tensor([0, 1, 2, -1, 3, 1, 2, -5], dtype=torch.int32))
+    kw["mask"][1], kw["mask"][2, 0] = -1, ~0b11111
+    check(z, kw)
+    got = ops.adjust_logits(z.cuda(), **on_gpu(kw)).cpu()
+    assert (got[0] == -math.inf).all()                               # a mask that leaves nothing
+    assert (got[2, :5] == -math.inf).all() and (got[6, 32:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("words", ["one", "few", "all"])
+@pytest.mark.parametrize("prompt", [0, 30000, 70000])
+def test_adjust_of_long_histories(cuda, words, prompt):
+    """Counts are whole numbers, however often a word comes."""
+    g = torch.Generator().manual_seed(5)
+    vocab, n = 32000, 70000
+    most = {"one": 1, "few": 40, "all": vocab}[words]
+    kw = dict(tokens=torch.randint(0, most, (2, n), generator=g, dtype=torch.int32), token_lens=torch.tensor([n, n - 5], dtype=torch.int32),
+              prompt_lens=torch.tensor([prompt, 7], dtype=torch.int32), repetition=torch.tensor([1.1, 1.2]), frequency=torch.tensor([2.0 ** -10, 0.01]),
+              presence=torch.tensor([0.5, 0.25]))
+    check(torch.randn(2, vocab, generator=g), kw)
+
+
+def test_adjust_of_long_bias_lists(cuda):
+    """More biases than a CTA lists, all in one piece of the vocabulary, words among them twice: one after the other."""
+    g = torch.Generator().manual_seed(6)
+    vocab, n = 20000, 1500
+    for spread in (40, 700, vocab):
+        kw = dict(bias_starts=torch.tensor([0, n, n, 2 * n], dtype=torch.int32), bias_words=torch.randint(0, spread, (2 * n,), generator=g, dtype=torch.int32),
+                  bias=torch.randn(2 * n, generator=g))
+        check(torch.randn(3, vocab, generator=g), kw)
+    kw["bias_starts"] = torch.tensor([-4, n, 2 * n + 9, 5], dtype=torch.int32)   # beyond the list's ends, and backwards
+    check(torch.randn(3, vocab, generator=g), kw)
+
+
+def test_adjust_without_rows_or_histories(cuda):
+    z = torch.randn(3, 40, device="cuda")
+    none = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
+    lens, one = torch.full((3,), 5, dtype=torch.int32).cuda(), torch.full((3,), 2.0).cuda()
+    assert torch.equal(ops.adjust_logits(z, tokens=none, token_lens=lens, repetition=one), z)
+    assert torch.equal(ops.adjust_logits(z, bias_starts=torch.zeros(4, dtype=torch.int32).cuda(), bias_words=none[0], bias=none[0].float()), z)
+    assert ops.adjust_logits(z[:0]).shape == (0, 40)
+
+
+def test_adjust_captured_and_on_streams(cuda):
+    """A graph takes lengths and settings as they are when it is replayed; calls on several streams at once."""
+    g = torch.Generator().manual_seed(7)
+    vocab, rows = 9000, 6
+    cases = [((torch.randn(rows, vocab, generator=g) * 3).to(BF16), settings(g, rows, vocab, 4, 300, 60, 3)) for _ in range(3)]
+    for _, kw in cases:                                              # lists of one length
+        kw["bias_words"], kw["bias"] = kw["bias_words"][:20].clone(), kw["bias"][:20].clone()
+        kw["bias_starts"].clamp_(max=20)
+    z, kw = cases[0][0].cuda(), on_gpu(cases[0][1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.adjust_logits(z, out_dtype=F32, **kw)
+    for hz, hkw in cases:
+        z.copy_(hz)
+        for n in kw:
+            kw[n].copy_(hkw[n])
+        graph.replay()
+        torch.cuda.synchronize()
+        check(hz, hkw, F32, got=out)
+    streams, dev = [torch.cuda.Stream() for _ in cases], [(hz.cuda(), on_gpu(hkw)) for hz, hkw in cases]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        outs = []
+        for st, (dz, dkw) in zip(streams, dev):
+            with torch.cuda.stream(st):
+                outs.append(ops.adjust_logits(dz, pdl=True, **dkw))
+    torch.cuda.synchronize()
+    for (hz, hkw), got in zip(cases, outs):
+        check(hz, hkw, got=got)
+
+
+def test_adjust_same_call_same_bits(cuda):
+    g = torch.Generator().manual_seed(8)
+    z, kw = torch.randn(20, 30000, generator=g).cuda(), on_gpu(settings(g, 20, 30000, 5, 4000, 50, 4, repeated=0.8))
+    first = ops.adjust_logits(z, **kw)
+    for _ in range(5):
+        assert torch.equal(first, ops.adjust_logits(z, **kw))
+
+
+def test_both_ways_from_tensors_to_launches(cuda, monkeypatch):
+    g = torch.Generator().manual_seed(9)
+    z, kw = torch.randn(4, 600, generator=g).to(BF16).cuda(), on_gpu(settings(g, 4, 600, 5, 50, 5, 4))
+
+    def call(**more):
+        return lambda: ops.adjust_logits(**dict(dict(kw, logits=z), **more))
+
+    for more in (dict(), dict(out_dtype=F32), dict(out_dtype=BF16, pdl=True), dict(out=torch.zeros(4, 600, device="cuda")), dict(out=torch.zeros_like(z)), dict(mask_row=None),
+                 dict(mask=None, mask_row=None), dict(token_seq=None), dict(bias_starts=None, bias=None, bias_words=None), dict(prompt_lens=None, frequency=None),
+                 dict(bias_words=kw["bias_words"][:0], bias=kw["bias"][:0]), dict(tokens=kw["tokens"][:, ::2][:, :1]), dict(logits=torch.cat([z, z], 1)[:, 7:607])):
+        both_ways(monkeypatch, call(**more))
+    for more in (dict(logits=z.as_subclass(Own)), dict(tokens=kw["tokens"][:, :0])):
+        both_ways(monkeypatch, call(**more), served=False)
+    for more in (dict(logits=z[0]), dict(out_dtype=F16), dict(out=torch.zeros(4, 601, device="cuda")), dict(tokens=None), dict(token_lens=None), dict(mask=None), dict(bias=None),
+                 dict(bias_starts=kw["bias_starts"][1:]), dict(repetition=kw["repetition"].double()), dict(mask=kw["mask"][:, :18]), dict(temperature=kw["temperature"].cpu()),
+                 dict(tokens=kw["tokens"][:1].expand(5, 50)), dict(mask=kw["mask"][:2], mask_row=None), dict(bias_starts=None), dict(out=torch.zeros(4, 600, device="cuda"), out_dtype=BF16)):
+        both_ways(monkeypatch, call(**more), served=False, refused=True)

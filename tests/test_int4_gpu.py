@@ -1,0 +1,549 @@
+"""Operators over a paged cache of 4 bits on a GPU, against their formulas in 64 bits (paged_oracle, int4_oracle)."""
+import math
+
+import pytest
+import torch
+
+from tests import int4_oracle as codes
+from tests import paged_oracle as oracle
+from tests.test_paged_gpu import Own, Step as WideStep, both_ways, probabilities, starts_of, tables
+from zhilight_b200 import ops
+
+pytestmark = pytest.mark.gpu
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def rows_in(x, order, dtype):
+    """Rows (pages, page, kv_heads, dim) -> bytes of the same order: (`rows`) as it is, (`heads`) heads outside the rows, (`wide`) within wider rows."""
+    b = codes.encode(x, dtype)
+    if order == "heads":
+        return b.transpose(1, 2).contiguous().transpose(1, 2)
+    if order == "wide":
+        big = torch.full((*b.shape[:2], b.shape[2] + 1, b.shape[3] * 2), 0xa5, dtype=torch.uint8)
+        big[:, :, :-1, :b.shape[3]] = b
+        return big[:, :, :-1, :b.shape[3]]
+    return b
+
+
+def to_gpu(x):
+    """The same strides on the device."""
+    y = torch.empty(max(1, sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1), dtype=x.dtype, device="cuda").as_strided(x.shape, x.stride())
+    return y.copy_(x)
+
+
+def pool(g, pages, page, kv_heads, dim, dtype, order, spread=1.0):
+    """Caches of random rows whose columns differ in their middle: keys, values."""
+    middle = torch.randn(kv_heads, dim, generator=g) * spread
+    k = (torch.randn(pages, page, kv_heads, dim, generator=g) + middle).to(dtype)
+    return rows_in(k, order, dtype), rows_in(torch.randn(pages, page, kv_heads, dim, generator=g).to(dtype), order, dtype)
+
+
+def hide(cache, table, lens, byte=0xff):
+    """Bytes of 0xff (codes of 15, steps of NaN) in every row of the pool that no sequence has."""
+    pages, page = cache.shape[:2]
+    used = torch.zeros(pages, page, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for i in range(n):
+            if 0 <= int(table[b, i // page]) < pages:
+                used[int(table[b, i // page]), i % page] = True
+    cache[~used] = byte
+
+
+# ---- append --------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim,half,adjacent,page,order,t", [
+    (32, 8, 128, 64, False, 16, "rows", 1), (32, 8, 128, 64, False, 16, "heads", 37), (4, 4, 64, 16, True, 1, "rows", 9), (6, 2, 64, 20, False, 5, "wide", 33),
+    (7, 1, 64, 13, True, 20, "rows", 12), (3, 3, 128, 4, False, 3, "heads", 5), (2, 1, 64, 0, False, 16, "rows", 4), (64, 8, 128, 48, False, 64, "rows", 70),
+    (1, 1, 64, 32, True, 2, "rows", 3), (3, 1, 64, 31, False, 7, "heads", 300), (200, 100, 128, 64, False, 16, "heads", 5), (128, 128, 64, 32, True, 8, "rows", 400),
+    (64, 8, 128, 64, False, 16, "wide", 2000)])
+def test_append(cuda, dtype, heads, kv_heads, dim, half, adjacent, page, order, t):
+    """Keys are given as the first heads of q: q, turned and rounded, says what the keys' codes have to be, bit by bit."""
+    g = torch.Generator().manual_seed(heads * 1000 + t)
+    lens = [t, t + 11, 2 * t]
+    pages = sum(-(-n // page) for n in lens) + 2
+    table = tables(g, lens, page, pages)
+    k, v = pool(g, pages, page, kv_heads, dim, dtype, order)
+    width = (heads + 2 * kv_heads) * dim
+    wide = torch.randn(t, width + 16, generator=g).to(dtype)
+    wide[:, heads * dim:(heads + kv_heads) * dim] = wide[:, :kv_heads * dim]
+    pos = torch.randint(0, 5_000_000, (3, t), generator=g, dtype=torch.int32)
+    axis = torch.randint(0, 3, (half,), generator=g, dtype=torch.int32)
+    if half > 4:
+        axis[3], axis[4] = -1, 3                                     # axes that do not exist do not turn
+    freq = 10000.0 ** (-torch.arange(half, dtype=torch.float64) / max(half, 1))
+    seq = torch.randint(0, 3, (t,), generator=g, dtype=torch.int32)
+    place = torch.tensor([lens[int(s)] - t + i for i, s in enumerate(seq)], dtype=torch.int32)
+    if t > 4:
+        place[2], seq[3], place[4] = -1, 3, page * table.shape[1]    # nowhere, no such sequence, behind the table
+    want_q, _, _, off_q, _ = oracle.axes_rope(wide[:, :width].contiguous(), pos, freq, axis, heads, kv_heads, dim, adjacent, 1.25)
+    kd, vd = to_gpu(k), to_gpu(v)
+    q = ops.qkv_axes_rope_append_int4(wide.cuda()[:, :width], pos.cuda(), freq.cuda(), axis.cuda(), seq.cuda(), place.cuda(), table.cuda(), kd, vd, heads,
+                                      layout=ops.ROT_ADJACENT if adjacent else ops.ROT_HALVES, mscale=1.25).cpu().view(t, heads, dim)
+    assert ((q.double() - want_q).abs() <= off_q).all()
+    new_k, new_v = codes.encode(q[:, :kv_heads], dtype), codes.encode(wide[:, (heads + kv_heads) * dim:width].reshape(t, kv_heads, dim), dtype)
+    for i in range(t):
+        s, p = int(seq[i]), int(place[i])
+        if 0 <= s < 3 and 0 <= p < page * table.shape[1] and 0 <= int(table[s, p // page]) < pages:
+            k[int(table[s, p // page]), p % page], v[int(table[s, p // page]), p % page] = new_k[i], new_v[i]
+    assert torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), v)     # places of no row are as they were
+    for pages_of in (None, torch.randperm(pages, generator=g)[:3].to(torch.int32)):
+        got = ops.int4_cache_values(kd, vd, dtype, pages_of if pages_of is None else pages_of.cuda())
+        for x, y in zip(got, (k, v)):
+            assert x.is_contiguous() and torch.equal(x.cpu(), codes.decode(y if pages_of is None else y[pages_of.long()], dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_append_at_the_ends_of_the_type(cuda, dtype, dim):
+    """Constants, the largest and smallest numbers, halves between two codes, infinities and NaN: the values that come back are the formula's."""
+    g = torch.Generator().manual_seed(2)
+    top, least = codes.TOP[dtype], 2.0 ** (codes.BITS[dtype][1] - codes.BITS[dtype][0] + 1)
+    x = torch.randn(24, 1, dim, generator=g).to(dtype)
+    x[0], x[1], x[2] = 0.0, 3.25, -top
+    x[3, 0, ::2], x[3, 0, 1::2] = top, -top
+    x[4] = torch.randint(0, 16, (dim,), generator=g).to(dtype) * least      # the smallest numbers
+    x[5] = torch.randint(-3, 4, (dim,), generator=g).to(dtype) * least * 64
+    x[6] = torch.arange(dim).remainder(31).to(dtype) * 0.5                  # steps of one: every second number between two codes
+    x[7] = torch.arange(dim).remainder(16).to(dtype)
+    x[8], x[8, 0, 7] = 1.0, 1.0 + 2.0 ** (1 - codes.BITS[dtype][0])
+    x[9, 0, 3], x[10, 0, 35], x[11, 0, dim - 1] = math.nan, math.inf, -math.inf
+    x[12, 0, :32] = math.inf
+    x[13, 0, 0], x[13, 0, 1] = math.inf, -math.inf
+    x[14] = (x[14].float() * 2.0 ** 13).to(dtype)
+    x[15, 0, 4] = top
+    x[16] *= least
+    qkv = torch.cat([x[:, 0], x[:, 0], x[:, 0]], 1)                         # position 0 turns nothing
+    for page, order in ((8, "rows"), (24, "heads")):
+        k = rows_in(torch.zeros(24 // page, page, 1, dim, dtype=dtype), order, dtype)
+        kd, vd = to_gpu(k), to_gpu(k)
+        table = torch.arange(24 // page, dtype=torch.int32)[None].cuda()
+        one = torch.zeros(24, dtype=torch.int32).cuda()
+        q = ops.qkv_axes_rope_append_int4(qkv.cuda(), one[None], torch.ones(1, dtype=torch.float64).cuda(), one[:1] - 1, one, torch.arange(24, dtype=torch.int32).cuda(),
+                                          table, kd, vd, 1)
+        assert torch.equal(q.cpu().view(torch.int16)[:9], qkv[:9, :dim].view(torch.int16))
+        want = codes.decode(codes.encode(x, dtype), dtype).view(24 // page, page, 1, dim)
+        broken = torch.isnan(want)
+        assert int(broken.sum()) == 32 * 5
+        for y in ops.int4_cache_values(kd, vd, dtype):
+            y = y.cpu()
+            assert torch.equal(torch.isnan(y), broken) and torch.equal(y[~broken], want[~broken])
+
+
+def test_append_takes_pages_of_the_table_only(cuda):
+    """Page numbers outside the pool take no writes and read as zeros."""
+    g = torch.Generator().manual_seed(3)
+    k, v = pool(g, 4, 8, 2, 64, BF16, "rows")
+    kd, vd = to_gpu(k), to_gpu(v)
+    table = torch.tensor([[1, -1], [4, 2 ** 31 - 1]], dtype=torch.int32)
+    qkv = torch.randn(4, 8 * 64, generator=g).to(BF16)
+    seq, place = torch.tensor([0, 0, 1, 1], dtype=torch.int32), torch.tensor([3, 9, 0, 12], dtype=torch.int32)
+    q = ops.qkv_axes_rope_append_int4(qkv.cuda(), torch.zeros(1, 4, dtype=torch.int32).cuda(), torch.ones(32, dtype=torch.float64).cuda(),
+                                      torch.zeros(32, dtype=torch.int32).cuda(), seq.cuda(), place.cuda(), table.cuda(), kd, vd, 4)
+    assert torch.equal(q.cpu(), qkv[:, :4 * 64])                     # position 0 turns nothing
+    k[1, 3], v[1, 3] = codes.encode(qkv[0, 4 * 64:6 * 64].view(2, 64), BF16), codes.encode(qkv[0, 6 * 64:].view(2, 64), BF16)
+    assert torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), v)
+    ids = torch.tensor([3, -1, 4, 1, 1, 2 ** 31 - 1], dtype=torch.int32)
+    got = ops.int4_cache_values(kd, None, BF16, ids.cuda()).cpu()
+    want = torch.zeros(6, 8, 2, 64, dtype=BF16)
+    for i in (0, 3, 4):
+        want[i] = codes.decode(k[int(ids[i])], BF16)
+    assert torch.equal(got, want)
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------------------
+def check_attention(dtype, heads, kv_heads, dim, page, order, window, seqs, seed=0, max_new=None, break_pages=False, behind=3, scale=None):
+    """seqs: [(keys, new tokens)]."""
+    g = torch.Generator().manual_seed(seed)
+    lens, new = [n for n, _ in seqs], [m for _, m in seqs]
+    pages = sum(-(-n // page) for n in lens) + 2
+    table = tables(g, lens, page, pages)
+    k, v = pool(g, pages, page, kv_heads, dim, dtype, order)
+    if break_pages:
+        table[0, 0], table[-1, 1] = pages, -1
+    hide(k, table, lens)
+    hide(v, table, lens)
+    t = sum(new)
+    q = torch.randn(t + behind, heads, dim, generator=g).to(dtype)
+    starts, n = starts_of(new), torch.tensor(lens, dtype=torch.int32)
+    scale = scale or dim ** -0.5
+    want, off = oracle.attention(q, codes.decode(k, dtype), codes.decode(v, dtype), table, lens, starts, scale, window)
+    out = torch.full_like(q, 7.0).cuda()
+    got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), n.cuda(), starts.cuda(), scale, window=window, max_new=max_new, out=out)
+    assert got is out
+    got = got.cpu().double()
+    assert (got[t:] == 7.0).all()                                    # rows behind the last sequence
+    far = (got[:t] - want[:t]).abs() - off[:t]
+    assert (far <= 0).all(), (float(far.nan_to_num(1e9).max()), torch.nonzero(~(far <= 0))[:5].tolist())
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(BF16, 32, 8, 128), (F16, 32, 8, 128), (BF16, 16, 16, 64), (F16, 8, 1, 64), (BF16, 28, 4, 128),
+                                                      (F16, 20, 1, 128), (BF16, 3, 1, 64), (F16, 40, 1, 128), (F16, 12, 1, 64)])
+@pytest.mark.parametrize("page,order", [(16, "rows"), (64, "heads"), (20, "wide"), (1, "rows"), (256, "rows")])
+def test_attention_single_tokens(cuda, dtype, heads, kv_heads, dim, page, order):
+    check_attention(dtype, heads, kv_heads, dim, page, order, 0, [(1, 1), (17, 1), (300, 1), (64, 1), (0, 0), (129, 1), (5, 0), (1025, 1)], max_new=1)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(BF16, 32, 8, 128), (F16, 64, 8, 128), (BF16, 8, 8, 64), (F16, 12, 4, 64)])
+@pytest.mark.parametrize("window", [0, 1, 50, 1000])
+def test_attention_drafts(cuda, dtype, heads, kv_heads, dim, window):
+    check_attention(dtype, heads, kv_heads, dim, 16, "rows", window, [(6, 6), (200, 5), (77, 2), (500, 9), (33, 1), (1500, 4), (0, 0), (70, 7)], max_new=9)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,order", [(BF16, 8, 2, 128, 16, "rows"), (F16, 8, 2, 64, 64, "heads"), (BF16, 4, 4, 128, 20, "wide"),
+                                                                 (F16, 7, 1, 128, 128, "rows"), (BF16, 16, 1, 64, 8, "rows"), (F16, 5, 5, 64, 1, "rows")])
+@pytest.mark.parametrize("window", [0, 100, 300])
+@pytest.mark.parametrize("seqs", [[(300, 300)], [(700, 130), (1, 1), (129, 129), (513, 257), (40, 0)], [(1000, 64), (65, 65), (128, 128)]])
+def test_attention_portions(cuda, dtype, heads, kv_heads, dim, page, order, window, seqs):
+    check_attention(dtype, heads, kv_heads, dim, page, order, window, seqs)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,window,seqs", [
+    (BF16, 16, 2, 64, 16, 0, [(2000, 900)]), (F16, 8, 2, 128, 48, 0, [(2111, 700), (1900, 333), (1800, 1)]), (BF16, 8, 2, 128, 20, 900, [(2500, 900), (1111, 40)]),
+    (F16, 64, 8, 128, 64, 0, [(1000 + 131 * i, 1 + i % 16) for i in range(10)]), (BF16, 48, 8, 64, 32, 1000, [(2000 + 77 * i, 9 + i) for i in range(6)]),
+    (F16, 24, 8, 64, 256, 0, [(3001, 43), (2048, 30), (130, 130), (2500, 12)]), (BF16, 32, 8, 128, 128, 0, [(20000, 1)]), (F16, 16, 8, 64, 20, 0, [(20000, 3), (9, 1)])])
+def test_attention_of_long_stretches(cuda, dtype, heads, kv_heads, dim, page, window, seqs):
+    """Enough keys for every CTA to go round its buffers several times, blocks whole and cut."""
+    check_attention(dtype, heads, kv_heads, dim, page, "rows", window, seqs, max_new=max(n for _, n in seqs))
+
+
+@pytest.mark.parametrize("max_new", [1, 3, 20, 200, None])
+def test_attention_does_not_depend_on_the_bound_of_new_tokens(cuda, max_new):
+    check_attention(BF16, 8, 2, 128, 16, "rows", 0, [(300, 200), (40, 1), (90, 3), (600, 18)], max_new=max_new)
+
+
+@pytest.mark.parametrize("new", [1, 4, 150])
+def test_attention_over_bad_pages(cuda, new):
+    """A page number outside the pool reads as rows of zeros."""
+    check_attention(F16, 8, 2, 128, 16, "rows", 0, [(200, new), (220, new)], break_pages=True)
+    check_attention(BF16, 8, 2, 64, 20, "heads", 0, [(200, new), (220, new)], break_pages=True)
+
+
+@pytest.mark.parametrize("new", [1, 5, 100, 200])
+def test_attention_rows_before_the_first_key(cuda, new):
+    """More new tokens than keys: the rows before the first key see nothing and give zeros."""
+    check_attention(BF16, 8, 2, 64, 16, "rows", 0, [(new // 2, new), (0, new), (new, new)])
+    check_attention(BF16, 8, 2, 64, 16, "rows", 3, [(new // 2, new), (0, new), (new, new)])
+
+
+@pytest.mark.parametrize("page", [4, 8, 12, 24, 40, 56, 100, 136])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_over_pages_of_any_size(cuda, page, dim):
+    seqs = [(1600 + 100 * i, 1 + 5 * i) for i in range(5)] + [(900, 200), (700, 70)]
+    check_attention(BF16, 16, 2, dim, page, "rows", 0, seqs, max_new=200)
+    check_attention(F16, 16, 2, dim, page, "heads", 1000, seqs[:4], max_new=16)
+
+
+@pytest.mark.parametrize("new,heads,kv_heads", [(1, 4, 2), (3, 4, 1), (20, 8, 2)])
+def test_attention_of_many_sequences(cuda, new, heads, kv_heads):
+    """More sequences than a warp looks at at a time, some without tokens or keys, also at the ends of what is in view."""
+    seqs = [(1 + (37 * i) % 150 + new, 1 + i % new) if i % 11 and i not in (127, 128, 255) else (i % 2 * 30, 0) for i in range(300)]
+    check_attention(F16, heads, kv_heads, 64, 16, "rows", 0, seqs, max_new=new)
+    check_attention(F16, heads, kv_heads, 64, 16, "heads", 33, seqs[:129], max_new=new)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(160, 1), (129, 1), (256, 2), (65, 1)])
+@pytest.mark.parametrize("new", [1, 3])
+def test_attention_of_wide_groups(cuda, heads, kv_heads, new):
+    check_attention(BF16, heads, kv_heads, 64, 16, "rows", 0, [(100, new), (new, new), (300, new)], max_new=new)
+
+
+@pytest.mark.parametrize("window", [0, 2 ** 31 - 1, 2 ** 31 - 40])
+@pytest.mark.parametrize("new", [1, 5, 100])
+def test_attention_of_the_widest_windows(cuda, window, new):
+    check_attention(BF16, 8, 2, 64, 16, "rows", window, [(new // 2, new), (300, new), (new, new)])
+
+
+@pytest.mark.parametrize("new,dim", [(1, 128), (3, 64), (6, 128), (140, 128), (300, 64)])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("order", ["rows", "heads"])
+def test_attention_rows_before_a_broken_token(cuda, new, dim, window, order):
+    """Groups of keys and values that are NaN reach the rows that see them and no others."""
+    g = torch.Generator().manual_seed(5)
+    heads, kv_heads, page, n = 8, 2, 16, 400
+    table = tables(g, [n], page, 40)
+    q = torch.randn(new, heads, dim, generator=g).to(BF16)
+    starts, lens = starts_of([new]), torch.tensor([n], dtype=torch.int32)
+    for where in (n - new // 2 - 1, n - 1, n - new - 30):
+        for which in range(2):
+            k, v = pool(g, 40, page, kv_heads, dim, BF16, order)
+            (k, v)[which][int(table[0, where // page]), where % page, 1, dim // 2 + 4:dim // 2 + 8] = 0xff   # columns 32 to 63
+            got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), lens.cuda(), starts.cuda(), dim ** -0.5, window=window).cpu().double()
+            want, off = oracle.attention(q, codes.decode(k, BF16), codes.decode(v, BF16), table, [n], starts, dim ** -0.5, window)
+            at = torch.arange(n - new, n)
+            sees = (at >= where) & ((at < where + window) if window else torch.ones_like(at, dtype=torch.bool))
+            fine = torch.ones(new, heads, dim, dtype=torch.bool)
+            fine[sees, heads // 2:, 32:64 if which else None] = False
+            if not which:
+                fine[sees, heads // 2:] = False
+            assert ((got - want).abs() <= off)[fine].all(), (where, which)
+            assert torch.isnan(got[~fine]).all()
+
+
+@pytest.mark.parametrize("new,heads", [(1, 8), (20, 8), (70, 8), (9, 2)])
+def test_attention_blocks_with_broken_tokens(cuda, new, heads):
+    """Enough sequences for whole blocks in a CTA: broken values in the last new token of every third sequence stay with its row."""
+    g = torch.Generator().manual_seed(9)
+    kv_heads, dim, page, seqs = 2, 64, 32, 90
+    lens = [new + 40 + 7 * (i % 5) for i in range(seqs)]
+    pages = sum(-(-n // page) for n in lens)
+    table, starts = tables(g, lens, page, pages), starts_of([new] * seqs)
+    q = torch.randn(seqs * new, heads, dim, generator=g).to(BF16)
+    k, v = pool(g, pages, page, kv_heads, dim, BF16, "rows")
+    for i in range(0, seqs, 3):
+        v[int(table[i, (lens[i] - 1) // page]), (lens[i] - 1) % page, 0, 32:36] = 0xff   # columns 0 to 31
+    got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), starts.cuda(), dim ** -0.5,
+                                   max_new=new).cpu().double()
+    want, off = oracle.attention(q, codes.decode(k, BF16), codes.decode(v, BF16), table, lens, starts, dim ** -0.5, 0)
+    fine = torch.ones(want.shape, dtype=torch.bool)
+    fine[new - 1::3 * new, :heads // 2, :32] = False
+    assert ((got - want).abs() <= off)[fine].all()
+    assert torch.isnan(got[~fine]).all()
+
+
+@pytest.mark.parametrize("dtype,size", [(BF16, 2.0 ** 124), (BF16, 2.0 ** -100), (BF16, 2.0 ** -70), (F16, 2.0 ** 13), (F16, 2.0 ** -14)])
+@pytest.mark.parametrize("new,heads", [(1, 4), (4, 8), (150, 8)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_large_and_small_values(cuda, dtype, size, new, heads, dim):
+    """Means of values near the ends of the type stay in it and keep their bits.  Probabilities of bf16 rows carry 2^-40, the largest of a row's is that at least: a product
+    or sum that 32 bits lose behind their lowest exponent is below 2^-126, so each key takes at most 2^-86 off a quotient, whatever its size is."""
+    g = torch.Generator().manual_seed(31)
+    lens, page = [300, new + 7], 16
+    table, starts = tables(g, lens, page, 50), starts_of([new, new])
+    k, _ = pool(g, 50, page, 2, dim, dtype, "rows")
+    v = rows_in((torch.randn(50, page, 2, dim, generator=g).clamp(-3.9, 3.9) * size).to(dtype), "rows", dtype)
+    q = torch.randn(2 * new, heads, dim, generator=g).to(dtype)
+    got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), starts.cuda(), dim ** -0.5,
+                                   max_new=new).cpu().double()
+    want, off = oracle.attention(q, codes.decode(k, dtype), codes.decode(v, dtype), table, lens, starts, dim ** -0.5, 0)
+    lost = 2.0 ** -86 * max(lens) if dtype == BF16 else 0.0
+    assert ((got - want).abs() <= off + lost).all()
+
+
+@pytest.mark.parametrize("new", [1, 5, 150])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attention_with_equal_rows_and_large_scores(cuda, dtype, new):
+    """One score far above the others, and all of them equal: no overflow, no loss."""
+    g = torch.Generator().manual_seed(6)
+    k = torch.randn(20, 16, 1, 128, generator=g).to(dtype)
+    v = rows_in(torch.randn(20, 16, 1, 128, generator=g).to(dtype), "rows", dtype)
+    table = tables(g, [300], 16, 20)
+    k[int(table[0, 3]), 5] = 30.0
+    k = rows_in(k, "rows", dtype)
+    q = torch.full((new, 2, 128), 2.0).to(dtype)
+    q[new // 2:] = 0.0
+    starts, lens = starts_of([new]), torch.tensor([300], dtype=torch.int32)
+    want, off = oracle.attention(q, codes.decode(k, dtype), codes.decode(v, dtype), table, [300], starts, 1.0, 0)
+    got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), lens.cuda(), starts.cuda(), 1.0).cpu().double()
+    assert ((got - want).abs() <= off).all()
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """A pool of more than 2^32 bytes a cache, rows at its far end."""
+    page, kv_heads, dim, heads, n = 64, 8, 128, 32, 150
+    pages = (1 << 32) // (page * kv_heads * 80) + 200
+    g = torch.Generator().manual_seed(8)
+    k, v = (torch.empty(pages, page, kv_heads, 80, dtype=torch.uint8, device="cuda") for _ in range(2))
+    ids = torch.tensor([pages - 1, pages - 90, pages - 3], dtype=torch.int32)
+    hk, hv = pool(g, 3, page, kv_heads, dim, BF16, "rows")
+    for i, p in enumerate(ids.tolist()):
+        k[p], v[p] = hk[i].cuda(), hv[i].cuda()
+    small = torch.arange(3, dtype=torch.int32)[None]
+    for new in (1, 5, 140):
+        qkv = torch.randn(new, (heads + 2 * kv_heads) * dim, generator=g).to(BF16)
+        place = torch.arange(n - new, n, dtype=torch.int32)
+        q = ops.qkv_axes_rope_append_int4(qkv.cuda(), torch.zeros(1, new, dtype=torch.int32).cuda(), torch.ones(64, dtype=torch.float64).cuda(),
+                                          torch.zeros(64, dtype=torch.int32).cuda(), torch.zeros(new, dtype=torch.int32).cuda(), place.cuda(), ids[None].cuda(), k, v, heads)
+        hk.view(-1, kv_heads, 80)[n - new:n] = codes.encode(qkv[:, heads * dim:(heads + kv_heads) * dim].view(new, kv_heads, dim), BF16)
+        hv.view(-1, kv_heads, 80)[n - new:n] = codes.encode(qkv[:, (heads + kv_heads) * dim:].view(new, kv_heads, dim), BF16)
+        got = ops.paged_attention_int4(q, k, v, ids[None].cuda(), torch.tensor([n], dtype=torch.int32).cuda(), starts_of([new]).cuda(), dim ** -0.5)
+        kk, vv = codes.decode(hk, BF16), codes.decode(hv, BF16)
+        want, off = oracle.attention(qkv[:, :heads * dim].reshape(new, heads, dim), kk, vv, small, [n], starts_of([new]), dim ** -0.5, 0)
+        assert ((got.cpu().double().view(new, heads, dim) - want).abs() <= off).all()
+        for x, y in zip(ops.int4_cache_values(k, v, BF16, ids.cuda()), (kk, vv)):
+            assert torch.equal(x.cpu(), y)
+
+
+@pytest.mark.parametrize("starts,lens", [((-5, 3, 20, 90), (50, 60, 70)), ((0, 0, 60, 60), (-3, 60, 2 ** 31 - 1)), ((2, 10, 11, 2 ** 31 - 1), (0, 5, -2 ** 31))])
+@pytest.mark.parametrize("max_new", [1, None])
+def test_attention_of_starts_and_lengths_out_of_range(cuda, starts, lens, max_new):
+    """Whatever the lengths and starts are, no row outside of q is touched and those of sequences in range are right."""
+    g = torch.Generator().manual_seed(14)
+    rows, page, dim = 60, 16, 64
+    table = torch.randperm(30, generator=g)[:15].view(3, 5).to(torch.int32)
+    k, v = pool(g, 30, page, 1, dim, F16, "rows")
+    q = torch.randn(rows, 2, dim, generator=g).to(F16)
+    out = torch.full((rows + 20, 2, dim), 7.0, dtype=F16, device="cuda")
+    ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor(starts, dtype=torch.int32).cuda(),
+                             0.125, max_new=max_new, out=out[:rows])
+    out = out.cpu().double()
+    assert (out[rows:] == 7.0).all()
+    kk, vv = codes.decode(k, F16), codes.decode(v, F16)
+    for b in range(3):
+        lo, hi = max(starts[b], 0), min(starts[b + 1], rows)
+        if lo >= hi or not 0 <= lens[b] <= 80 or starts[b + 1] > rows or starts[b] < 0:
+            continue
+        want, off = oracle.attention(q[lo:hi], kk, vv, table[b:b + 1], [lens[b]], [0, hi - lo], 0.125, 0)
+        assert ((out[lo:hi] - want).abs() <= off).all()
+
+
+def test_no_rows_and_odd_forms(cuda):
+    k = torch.zeros(2, 16, 1, 40, dtype=torch.uint8, device="cuda")
+    table, lens = torch.zeros(1, 1, dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+    q = torch.zeros(0, 64, dtype=BF16, device="cuda")
+    assert ops.paged_attention_int4(q, k, k, table, lens, torch.zeros(2, dtype=torch.int32).cuda(), 1.0).shape == (0, 64)
+    assert ops.qkv_axes_rope_append_int4(torch.zeros(0, 192, dtype=BF16).cuda(), torch.zeros(1, 0, dtype=torch.int32).cuda(), torch.ones(1, dtype=torch.float64).cuda(),
+                                         torch.zeros(1, dtype=torch.int32).cuda(), lens[:0], lens[:0], table, k, k, 1).shape == (0, 64)
+    assert ops.int4_cache_values(k, None, BF16, lens[:0]).shape == (0, 16, 1, 64)
+
+
+@pytest.mark.parametrize("heads,kv_heads,new", [(8, 2, 1), (12, 4, 4), (16, 2, 40), (160, 1, 2)])
+def test_attention_in_place(cuda, heads, kv_heads, new):
+    g = torch.Generator().manual_seed(17)
+    k, v = pool(g, 40, 16, kv_heads, 64, BF16, "rows")
+    table, lens, starts = tables(g, [200, 300], 16, 40).cuda(), torch.tensor([200, 300], dtype=torch.int32).cuda(), starts_of([new, new]).cuda()
+    q = torch.randn(2 * new, heads, 64, generator=g).to(BF16).cuda()
+    want = ops.paged_attention_int4(q, k.cuda(), v.cuda(), table, lens, starts, 0.125, max_new=new)
+    got = ops.paged_attention_int4(q, k.cuda(), v.cuda(), table, lens, starts, 0.125, max_new=new, out=q)
+    assert got is q and torch.equal(got, want)
+
+
+# ---- as a program uses them ----------------------------------------------------------------------------------------------------
+class Step(WideStep):
+    """Rows of three users through the operators of a step: append, attend, from the last rows logits that are adjusted and become the target's probabilities, verify."""
+
+    def __init__(self, seed, new=(3, 3, 130), before=(100, 40, 0)):
+        super().__init__(seed, new=new, before=before)
+        g = torch.Generator().manual_seed(seed + 100)
+        self.k, self.v = pool(g, 60, 16, 2, 128, BF16, "heads")
+        self.head = (torch.randn(1024, 9000, generator=g) * 0.2).to(BF16)
+        self.last = (self.starts[1:, None] - 3 + torch.arange(3)).reshape(-1).long()
+        self.words_of = torch.randint(0, 9000, (3, 200), generator=g, dtype=torch.int32)
+        self.token_seq = torch.arange(3, dtype=torch.int32).repeat_interleave(3)
+        self.token_lens = torch.tensor([50, 51, 52, 0, 1, 2, 198, 199, 200], dtype=torch.int32)
+        self.prompt = torch.tensor([20] * 3 + [0] * 3 + [150] * 3, dtype=torch.int32)
+        self.settings = torch.tensor([[1.2] * 3 + [1.0] * 3 + [0.9] * 3, [0.5] * 9, [0.1] * 9, [0.7] * 3 + [0.0] * 3 + [1.3] * 3])
+        self.mask = torch.randint(-2 ** 31, 2 ** 31 - 1, (2, 282), generator=g, dtype=torch.int32)
+        self.mask_row = torch.tensor([0, 0, 0, 1, 1, 1, -1, -1, -1], dtype=torch.int32)
+        self.dev = {n: x.cuda() for n, x in vars(self).items() if isinstance(x, torch.Tensor)}
+        self.dev["k"], self.dev["v"] = to_gpu(self.k), to_gpu(self.v)
+
+    def run(self):
+        d = self.dev
+        q = ops.qkv_axes_rope_append_int4(d["qkv"], d["pos"], d["freq"], d["axis"], d["seq"], d["place"], d["table"], d["k"], d["v"], self.heads, pdl=True)
+        o = ops.paged_attention_int4(q, d["k"], d["v"], d["table"], d["lens"], d["starts"], self.dim ** -0.5)
+        logits = torch.mm(o[d["last"]], d["head"])
+        s = d["settings"]
+        z = ops.adjust_logits(logits, tokens=d["words_of"], token_seq=d["token_seq"], token_lens=d["token_lens"], prompt_lens=d["prompt"], repetition=s[0], frequency=s[1],
+                              presence=s[2], temperature=s[3], mask=d["mask"], mask_row=d["mask_row"], out_dtype=torch.float32)
+        target = torch.softmax(z, -1).view(3, 3, 9000)
+        return (q, o, logits, z, target) + ops.verify_drafts(target, d["draft"], d["words"], d["accept"], d["sample"])
+
+    def check(self, got):
+        want_q, want_k, want_v, off_q, off_k = oracle.axes_rope(self.qkv, self.pos, self.freq, self.axis, 8, 2, 128, False, 1.0)
+        q, kb, vb = got[0].cpu().view(want_q.shape), self.dev["k"].cpu(), self.dev["v"].cpu()
+        assert ((q.double() - want_q).abs() <= off_q).all()
+        kc, vc = codes.decode(kb, BF16), codes.decode(vb, BF16)
+        far_k = codes.off_by(kb, BF16)
+        for i, (s, p) in enumerate(zip(self.seq.tolist(), self.place.tolist())):
+            at = (int(self.table[s, p // 16]), p % 16)
+            assert ((kc[at].double() - want_k[i]).abs() <= off_k[i] + far_k[at]).all()
+            assert torch.equal(vb[at], codes.encode(want_v[i].to(BF16), BF16))
+        want, off = oracle.attention(q, kc, vc, self.table, self.lens.tolist(), self.starts, self.dim ** -0.5, 0)
+        assert ((got[1].cpu().double().view(want.shape) - want).abs() <= off).all()
+        z, far = codes.adjust(got[2].cpu(), torch.float32, tokens=self.words_of, token_seq=self.token_seq, token_lens=self.token_lens, prompt_lens=self.prompt,
+                              repetition=self.settings[0], frequency=self.settings[1], presence=self.settings[2], temperature=self.settings[3], mask=self.mask,
+                              mask_row=self.mask_row)
+        z, y = torch.from_numpy(z), got[3].cpu().double()
+        assert torch.equal(z == -math.inf, y == -math.inf)
+        assert ((z - y).abs() <= torch.from_numpy(far))[z > -math.inf].all()
+        a, t = oracle.verify(got[4].cpu(), self.draft, self.words, self.accept, self.sample, None)
+        assert got[5].tolist() == a.tolist() and got[6].tolist() == t.tolist()
+
+
+def test_step(cuda):
+    s = Step(0)
+    s.check(s.run())
+
+
+def test_step_captured_and_replayed(cuda):
+    """The first step of these sizes inside a capture; replays with other inputs, and two graphs in turn."""
+    steps = [Step(1, new=(3, 4, 97), before=(61, 77, 5)), Step(2, new=(3, 3, 3), before=(200, 3, 0))]
+    torch.mm(steps[0].dev["head"][:9, :64].t(), steps[0].dev["head"][:9, :64])   # the library's handle is made outside of the capture
+    graphs, outs = [], []
+    for s in steps:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(s.run())
+        graphs.append(graph)
+    for turn in range(3):
+        for s in steps:
+            s.qkv = torch.randn(s.qkv.shape, generator=torch.Generator().manual_seed(turn)).to(BF16)
+            s.dev["qkv"].copy_(s.qkv)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for s, out in zip(steps, outs):
+            s.check(out)
+
+
+def test_steps_on_streams(cuda):
+    steps = [Step(i, new=(4, 200, 150), before=(300, 0, 70)) for i in range(3, 6)]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        outs = []
+        for s, st in zip(steps, streams):
+            with torch.cuda.stream(st):
+                outs.append(s.run())
+    torch.cuda.synchronize()
+    for s, out in zip(steps, outs):
+        s.check(out)
+
+
+def test_same_call_same_bits(cuda):
+    s = Step(9, new=(5, 90, 64), before=(150, 0, 20))
+    first = [x.clone() for x in s.run()]
+    for _ in range(5):
+        for a, b in zip(first, s.run()):
+            assert torch.equal(a, b)
+
+
+def test_both_ways_from_tensors_to_launches(cuda, monkeypatch):
+    s = Step(11)
+    d = dict(s.dev)
+    d["q"] = torch.randn(s.qkv.shape[0], 8 * 128, device="cuda").to(BF16)
+    d["pages"] = torch.tensor([4, 0, 59, 60], dtype=torch.int32).cuda()
+
+    def append(**kw):
+        e = dict(d, **kw)
+        return lambda: ops.qkv_axes_rope_append_int4(e["qkv"], e["pos"], e["freq"], e["axis"], e["seq"], e["place"], e["table"], e["k"], e["v"], e.get("heads", 8),
+                                                     layout=e.get("layout", 0), mscale=e.get("mscale", 1), pdl=e.get("pdl", False))
+
+    def attend(**kw):
+        e = dict(d, **kw)
+        return lambda: ops.paged_attention_int4(e["q"], e["k"], e["v"], e["table"], e["lens"], e["starts"], e.get("scale", 0.1), window=e.get("window", 0),
+                                                max_new=e.get("max_new"), out=e.get("out"), pdl=e.get("pdl", False))
+
+    def values(**kw):
+        e = dict(d, **kw)
+        return lambda: ops.int4_cache_values(e["k"], e["v"], e.get("dtype", BF16), e["pages"], pdl=e.get("pdl", False))
+
+    wide = torch.cat([d["qkv"], d["qkv"]], 1)[:, :12 * 128]
+    for kw in (dict(), dict(mscale=1.5), dict(layout=1, pdl=True), dict(qkv=wide)):
+        both_ways(monkeypatch, append(**kw))
+    both_ways(monkeypatch, append(qkv=d["qkv"].as_subclass(Own)), served=False)
+    for kw in (dict(layout=2), dict(qkv=wide[:, :-1]), dict(axis=d["axis"][1:]), dict(k=d["k"].view(torch.int8)), dict(freq=d["freq"].float()), dict(heads=7),
+               dict(k=d["k"][..., :40], v=d["v"][..., :40]), dict(table=d["table"][:, ::2])):
+        both_ways(monkeypatch, append(**kw), served="layout" in kw, refused=True)
+    out = torch.zeros_like(d["q"])
+    for kw in (dict(), dict(q=d["q"].view(-1, 8, 128)), dict(window=7, max_new=130, pdl=True), dict(out=out), dict(scale=1)):
+        both_ways(monkeypatch, attend(**kw))
+    both_ways(monkeypatch, attend(table=d["table"].as_subclass(Own)), served=False)
+    for kw in (dict(scale=-1.0), dict(window=-1), dict(q=d["q"][:, :100]), dict(lens=d["lens"][1:]), dict(max_new=0), dict(out=out.float()), dict(q=d["q"].float()),
+               dict(k=d["k"][:, :, :1].expand(d["k"].shape)), dict(v=d["v"].cpu())):
+        both_ways(monkeypatch, attend(**kw), served=kw.get("scale", 0) < 0 or "window" in kw, refused=True)
+    for kw in (dict(), dict(v=None), dict(pages=None), dict(dtype=F16, pdl=True)):
+        both_ways(monkeypatch, values(**kw))
+    both_ways(monkeypatch, values(pages=d["pages"][:0]), served=False)
+    for kw in (dict(dtype=torch.float32), dict(pages=d["pages"].long()), dict(v=d["v"][1:]), dict(k=d["k"].cpu())):
+        both_ways(monkeypatch, values(**kw), served=False, refused=True)

@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -36,6 +37,11 @@ struct {
     decltype(&zl_paged_attention_workspace_bytes) paged_bytes;
     decltype(&zl_paged_attention) paged;
     decltype(&zl_verify_drafts) verify;
+    decltype(&zl_qkv_axes_rope_append_int4) axes_rope4;
+    decltype(&zl_int4_cache_values) values4;
+    decltype(&zl_paged_attention_int4_workspace_bytes) paged4_bytes;
+    decltype(&zl_paged_attention_int4) paged4;
+    decltype(&zl_adjust_logits) adjust;
 } zl;
 
 struct NotPlain {};   // the general path's
@@ -93,6 +99,13 @@ int unlocked(F&& f) {
 // pdl of a call: early reads, or a dependent that waits for everything earlier first
 int launched(PyObject* pdl) { return truth(pdl) ? 1 : 2; }
 PyObject* result(int rc, const at::Tensor& out) { return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out); }
+
+PyObject* pair_of(const at::Tensor& x, const at::Tensor& y) {
+    PyObject *first = THPVariable_Wrap(x), *second = THPVariable_Wrap(y), *pair = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return pair;
+}
 
 template <typename F>
 PyObject* guarded(F&& f) {
@@ -261,28 +274,39 @@ struct Paged {
     long long pages, step[3];
     int page_size, kv_heads, dim, ld_table, max_pages, seqs;
 };
-Paged paged_cache(PyObject* k_cache, PyObject* v_cache, PyObject* page_table, at::ScalarType type) {
-    const at::Tensor &k = here(k_cache, false), &v = here(v_cache, false), &t = here(page_table, false);
-    must(k.dim() == 4 && v.sizes() == k.sizes() && k.scalar_type() == type && v.scalar_type() == type && (type == at::kHalf || type == at::kBFloat16));
-    must(k.numel() > 0 && k.size(3) > 1 && k.stride(3) == 1 && v.stride(3) == 1 && t.dim() == 2 && t.scalar_type() == at::kInt && t.numel() > 0 && t.stride(1) == 1);
-    Paged p = {k.data_ptr(), v.data_ptr(), static_cast<const int32_t*>(t.data_ptr()), k.size(0)};
+// int4: bytes, 5 dim / 8 a row, whose rows were written from `type`
+void caches(Paged& p, const at::Tensor& k, const at::Tensor& v, at::ScalarType type, bool int4) {
+    const at::ScalarType held = int4 ? at::kByte : type;
+    must(k.dim() == 4 && v.sizes() == k.sizes() && k.scalar_type() == held && v.scalar_type() == held && (type == at::kHalf || type == at::kBFloat16));
+    must(k.numel() > 0 && k.size(3) > 1 && k.stride(3) == 1 && v.stride(3) == 1 && (!int4 || k.size(3) == 40 || k.size(3) == 80));
+    p.k = k.data_ptr(), p.v = v.data_ptr(), p.pages = k.size(0);
     for (int i = 0; i < 3; ++i) {
         p.step[i] = k.size(i) == 1 ? 0 : k.stride(i);
         must(p.step[i] == (k.size(i) == 1 ? 0 : v.stride(i)) && (p.step[i] > 0 || k.size(i) == 1));
     }
-    must(k.size(1) < 1 << 30 && t.size(0) < 1 << 30 && t.size(1) < 1 << 30 && t.stride(0) < 1ll << 31 && k.size(2) < 1 << 16 && k.size(3) < 1 << 16);
-    p.page_size = (int)k.size(1), p.kv_heads = (int)k.size(2), p.dim = (int)k.size(3);
+    must(k.size(1) < 1 << 30 && k.size(2) < 1 << 16 && k.size(3) < 1 << 16);
+    p.page_size = (int)k.size(1), p.kv_heads = (int)k.size(2), p.dim = (int)(int4 ? k.size(3) / 5 * 8 : k.size(3));
+}
+Paged paged_cache(PyObject* k_cache, PyObject* v_cache, PyObject* page_table, at::ScalarType type, bool int4) {
+    const at::Tensor &k = here(k_cache, false), &v = here(v_cache, false), &t = here(page_table, false);
+    must(t.dim() == 2 && t.scalar_type() == at::kInt && t.numel() > 0 && t.stride(1) == 1);
+    Paged p = {};
+    caches(p, k, v, type, int4);
+    must(t.size(0) < 1 << 30 && t.size(1) < 1 << 30 && t.stride(0) < 1ll << 31);
+    p.table = static_cast<const int32_t*>(t.data_ptr());
     p.seqs = (int)t.size(0), p.max_pages = (int)t.size(1), p.ld_table = p.seqs > 1 ? (int)t.stride(0) : p.max_pages;
     return p;
 }
 
 // qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout, mscale, pdl
-PyObject* qkv_axes_rope_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
+template <bool INT4>
+PyObject* axes_rope_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
     return guarded([&]() -> PyObject* {
         args(na, 13);
-        must(zl.axes_rope);
+        const auto entry = INT4 ? zl.axes_rope4 : zl.axes_rope;
+        must(entry);
         const at::Tensor& x = here(a[0], false);
-        const Paged c = paged_cache(a[7], a[8], a[6], x.scalar_type());
+        const Paged c = paged_cache(a[7], a[8], a[6], x.scalar_type(), INT4);
         const int heads = to_int(a[9]), layout = to_int(a[10]), pdl = truth(a[12]);
         const double mscale = to_double(a[11]);
         must(x.dim() == 2 && heads > 0 && heads < 1 << 16 && x.size(1) == (int64_t)(heads + 2 * c.kv_heads) * c.dim && x.stride(1) == 1);
@@ -297,22 +321,25 @@ PyObject* qkv_axes_rope_append(PyObject*, PyObject* const* a, Py_ssize_t na) {
         const int dt = dtype_of(x);
         const zl_stream_t s = stream();
         return result(unlocked([&] {
-                          return zl.axes_rope(x.data_ptr(), ld, static_cast<const int32_t*>(pos.data_ptr()), t, (int)pos.size(0),
-                                              static_cast<const double*>(freq.data_ptr()), axis, (int)freq.size(0), layout, (float)mscale, seq, place, c.table,
-                                              c.ld_table, c.max_pages, c.seqs, c.k, c.v, c.pages, c.page_size, c.step[0], c.step[1], c.step[2], q.data_ptr(), (int)t,
-                                              heads, c.kv_heads, c.dim, dt, pdl, s);
+                          return entry(x.data_ptr(), ld, static_cast<const int32_t*>(pos.data_ptr()), t, (int)pos.size(0),
+                                         static_cast<const double*>(freq.data_ptr()), axis, (int)freq.size(0), layout, (float)mscale, seq, place, c.table,
+                                         c.ld_table, c.max_pages, c.seqs, c.k, c.v, c.pages, c.page_size, c.step[0], c.step[1], c.step[2], q.data_ptr(), (int)t,
+                                         heads, c.kv_heads, c.dim, dt, pdl, s);
                       }),
                       q);
     });
 }
 
 // q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl
-PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
+template <bool INT4>
+PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t na) {
     return guarded([&]() -> PyObject* {
         args(na, 11);
-        must(zl.paged && zl.paged_bytes);
+        const auto entry = INT4 ? zl.paged4 : zl.paged;
+        const auto room_of = INT4 ? zl.paged4_bytes : zl.paged_bytes;
+        must(entry && room_of);
         const at::Tensor& q = here(a[0], true);
-        const Paged c = paged_cache(a[1], a[2], a[3], q.scalar_type());
+        const Paged c = paged_cache(a[1], a[2], a[3], q.scalar_type(), INT4);
         must((q.dim() == 2 || q.dim() == 3) && (q.dim() == 2 || q.size(2) == c.dim));
         const int64_t t = q.size(0), width = q.size(1) * (q.dim() == 3 ? c.dim : 1);
         must(t > 0 && t < 1ll << 31 && width > 0 && width < 1 << 24 && width % ((int64_t)c.kv_heads * c.dim) == 0);
@@ -326,15 +353,15 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
         }
         const at::Tensor out = a[9] == Py_None ? empty(q, q.sizes(), q.scalar_type()) : THPVariable_Unpack(a[9]);
         const int heads = (int)(width / c.dim), new_ = (int)std::min<int64_t>(most, t);
-        const size_t bytes = zl.paged_bytes((int)t, new_, c.seqs, (int)std::min<long long>((long long)c.max_pages * c.page_size, (1ll << 31) - 256), heads, c.kv_heads, c.dim);
+        const size_t bytes = room_of((int)t, new_, c.seqs, (int)std::min<long long>((long long)c.max_pages * c.page_size, (1ll << 31) - 256), heads, c.kv_heads, c.dim);
         at::Tensor room;
         if (bytes) room = empty(q, {(int64_t)bytes}, at::kByte);
         void* const ws = bytes ? room.data_ptr() : nullptr;
         const int dt = dtype_of(q);
         const zl_stream_t s = stream();
         return result(unlocked([&] {
-                          return zl.paged(q.data_ptr(), c.k, c.v, c.pages, c.page_size, c.step[0], c.step[1], c.step[2], c.table, c.ld_table, c.max_pages, lens, starts,
-                                          c.seqs, (float)scale, window, out.data_ptr(), (int)t, new_, heads, c.kv_heads, c.dim, ws, bytes, dt, pdl, s);
+                          return entry(q.data_ptr(), c.k, c.v, c.pages, c.page_size, c.step[0], c.step[1], c.step[2], c.table, c.ld_table, c.max_pages, lens, starts,
+                                       c.seqs, (float)scale, window, out.data_ptr(), (int)t, new_, heads, c.kv_heads, c.dim, ws, bytes, dt, pdl, s);
                       }),
                       out);
     });
@@ -368,11 +395,124 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t na) {
                              static_cast<const float*>(accept.data_ptr()), static_cast<const float*>(sample.data_ptr()), count, static_cast<int32_t*>(accepted.data_ptr()),
                              static_cast<int32_t*>(tokens.data_ptr()), (int)b, (int)k, (int)vocab, pdl, s);
         });
-        if (rc) return PyLong_FromLong(rc);
-        PyObject *first = THPVariable_Wrap(accepted), *second = THPVariable_Wrap(tokens), *pair = first && second ? PyTuple_Pack(2, first, second) : nullptr;
-        Py_XDECREF(first);
-        Py_XDECREF(second);
-        return pair;
+        return rc ? PyLong_FromLong(rc) : pair_of(accepted, tokens);
+    });
+}
+
+// k_cache, v_cache, dtype, pages, pdl: a pair of tensors, or one where v_cache is None
+PyObject* int4_cache_values(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    return guarded([&]() -> PyObject* {
+        args(na, 5);
+        must(zl.values4 && THPDtype_Check(a[2]));
+        const at::ScalarType type = reinterpret_cast<THPDtype*>(a[2])->scalar_type;
+        const at::Tensor &k = here(a[0], false), &v = a[1] == Py_None ? k : here(a[1], false);
+        Paged c = {};
+        caches(c, k, v, type, true);
+        const int32_t* pages = nullptr;
+        int64_t n = c.pages;
+        if (a[3] != Py_None) {
+            const at::Tensor& t = here(a[3], true);
+            must(t.scalar_type() == at::kInt && t.dim() == 1);
+            pages = static_cast<const int32_t*>(t.data_ptr()), n = t.size(0);
+        }
+        must(n > 0);
+        const int pdl = truth(a[4]);
+        const at::Tensor k_out = empty(k, {n, c.page_size, c.kv_heads, c.dim}, type);
+        at::Tensor v_out;
+        if (a[1] != Py_None) v_out = empty(k, k_out.sizes(), type);
+        void* const second = a[1] != Py_None ? v_out.data_ptr() : nullptr;
+        const int dt = dtype_of(k_out);
+        const zl_stream_t s = stream();
+        const int rc = unlocked([&] {
+            return zl.values4(c.k, second ? c.v : nullptr, c.pages, c.page_size, c.step[0], c.step[1], c.step[2], pages, n, k_out.data_ptr(), second, c.kv_heads, c.dim, dt,
+                              pdl, s);
+        });
+        if (rc || !second) return result(rc, k_out);
+        return pair_of(k_out, v_out);
+    });
+}
+
+// logits, tokens, token_seq, token_lens, prompt_lens, repetition, frequency, presence, bias_starts, bias_words, bias, temperature, mask, mask_row, out_dtype, out, pdl
+PyObject* adjust_logits(PyObject*, PyObject* const* a, Py_ssize_t na) {
+    return guarded([&]() -> PyObject* {
+        args(na, 17);
+        must(zl.adjust);
+        const at::Tensor& x = here(a[0], false);
+        must(x.dim() == 2 && x.size(0) > 0 && x.size(0) < 1 << 30 && x.size(1) > 0 && x.size(1) <= 1 << 24 && x.stride(1) == 1);
+        const int64_t r = x.size(0), vocab = x.size(1);
+        const int dt = dtype_of(x);
+        at::ScalarType type = x.scalar_type();
+        if (a[14] != Py_None) {
+            must(THPDtype_Check(a[14]));
+            type = reinterpret_cast<THPDtype*>(a[14])->scalar_type;
+        } else if (a[15] != Py_None) {
+            type = here(a[15], false).scalar_type();
+        }
+        must(type == x.scalar_type() || type == at::kFloat);
+        const long long ld = r > 1 ? x.stride(0) : vocab;
+        must(ld >= vocab);
+        auto rows = [&](PyObject* o) { return o == Py_None ? nullptr : ints(o, r); };
+        auto floats = [&](PyObject* o, int64_t n) -> const float* {
+            if (o == Py_None) return nullptr;
+            const at::Tensor& t = here(o, true);
+            must(t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n);
+            return static_cast<const float*>(t.data_ptr());
+        };
+        struct Table {
+            const int32_t* at;
+            long long ld;
+            int rows, cols;
+        };
+        auto table = [&](PyObject* o) -> Table {   // (rows, columns) int32
+            const at::Tensor& t = here(o, false);
+            must(t.scalar_type() == at::kInt && t.dim() == 2 && t.numel() > 0 && t.size(0) < 1 << 30 && t.size(1) <= 1 << 29 && (t.stride(1) == 1 || t.size(1) == 1));
+            const long long step = t.size(0) > 1 ? t.stride(0) : t.size(1);
+            must(step >= t.size(1));
+            return {static_cast<const int32_t*>(t.data_ptr()), step, (int)t.size(0), (int)t.size(1)};
+        };
+        Table words = {}, mask = {};
+        if (a[1] != Py_None) {
+            words = table(a[1]);
+            must(a[3] != Py_None && (a[2] != Py_None || words.rows >= r));
+        } else {
+            for (int i = 2; i < 8; ++i) must(a[i] == Py_None);
+        }
+        const int32_t *seq = rows(a[2]), *lens = rows(a[3]), *prompt = rows(a[4]);
+        const float *rep = floats(a[5], r), *freq = floats(a[6], r), *pres = floats(a[7], r), *heat = floats(a[11], r);
+        const int32_t *starts = nullptr, *bias_words = nullptr;
+        const float* bias = nullptr;
+        int64_t n = 0;
+        if (a[8] != Py_None) {
+            starts = ints(a[8], r + 1);
+            const at::Tensor& w = here(a[9], true);
+            must(w.dim() == 1 && w.size(0) < 1ll << 31 && a[10] != Py_None);
+            n = w.size(0);
+            bias_words = ints(a[9], n), bias = floats(a[10], n);
+            if (n == 0) starts = nullptr;
+        } else {
+            must(a[9] == Py_None && a[10] == Py_None);
+        }
+        const int32_t* mask_row = nullptr;
+        if (a[12] != Py_None) {
+            mask = table(a[12]), mask_row = rows(a[13]);
+            must(mask.cols * 32ll >= vocab && (mask_row || mask.rows >= r));
+        } else {
+            must(a[13] == Py_None);
+        }
+        if (a[15] != Py_None) {
+            const at::Tensor& o = here(a[15], false);
+            must(o.sizes() == x.sizes() && o.scalar_type() == type && o.stride(1) == 1);
+        }
+        const at::Tensor out = a[15] == Py_None ? empty(x, {r, vocab}, type) : THPVariable_Unpack(a[15]);
+        const long long ld_out = r > 1 ? out.stride(0) : vocab;
+        must(ld_out >= vocab);
+        const int out_dt = dtype_of(out), pdl = truth(a[16]);
+        const zl_stream_t s = stream();
+        return result(unlocked([&] {
+                          return zl.adjust(x.data_ptr(), ld, dt, out.data_ptr(), ld_out, out_dt, (int)r, (int)vocab, words.at, words.ld, words.rows, words.cols, seq, lens,
+                                           prompt, rep, freq, pres, starts, bias_words, bias, (int)n, heat, mask.at, mask.ld, mask.rows, mask_row, pdl, s);
+                      }),
+                      out);
     });
 }
 
@@ -397,13 +537,21 @@ PyObject* bind(PyObject*, PyObject* d) {
     set(zl.paged_bytes, "zl_paged_attention_workspace_bytes");
     set(zl.paged, "zl_paged_attention");
     set(zl.verify, "zl_verify_drafts");
+    set(zl.axes_rope4, "zl_qkv_axes_rope_append_int4");
+    set(zl.values4, "zl_int4_cache_values");
+    set(zl.paged4_bytes, "zl_paged_attention_int4_workspace_bytes");
+    set(zl.paged4, "zl_paged_attention_int4");
+    set(zl.adjust, "zl_adjust_logits");
     if (PyErr_Occurred()) return nullptr;
     Py_RETURN_NONE;
 }
 
-#define ZL_FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
+#define ZL_FAST_AS(name, ...) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(__VA_ARGS__)), METH_FASTCALL, nullptr}
+#define ZL_FAST(name) ZL_FAST_AS(#name, name)
 PyMethodDef methods[] = {ZL_FAST(w4a16_gemm_fused), ZL_FAST(dense_gemm_skinny), ZL_FAST(w8_linear), ZL_FAST(decode_attention),
-                         ZL_FAST(qkv_axes_rope_append), ZL_FAST(paged_attention), ZL_FAST(verify_drafts),
+                         ZL_FAST_AS("qkv_axes_rope_append", axes_rope_append<false>), ZL_FAST_AS("paged_attention", attend<false>), ZL_FAST(verify_drafts),
+                         ZL_FAST_AS("qkv_axes_rope_append_int4", axes_rope_append<true>), ZL_FAST_AS("paged_attention_int4", attend<true>),
+                         ZL_FAST(int4_cache_values), ZL_FAST(adjust_logits),
                          {"bind", bind, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

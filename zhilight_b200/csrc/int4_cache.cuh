@@ -1,0 +1,111 @@
+// Rows of a key / value cache that is held in 4 bits.  A head's row: dim / 2 bytes of codes, then for every 32 columns a pair (step, lowest value) in the type
+// T of the rows that it was written from, 5 dim / 8 bytes in all.  A code c stands for T(lowest + step * c), rounded once.
+//
+// Of a group with lowest and highest value lo and hi, the step is (hi - lo) / 15 rounded down to T, so that no code stands for more than hi, and x becomes
+// the nearest whole number of steps above lo, at most 15 (ties to even): off by half a step, and by at most 15 * eps(T) / 2 of one more at the upper end, which the step's rounding leaves.  lo
+// is one of the values, so T holds it as it is.  Differences are taken of halves: a range may be beyond the largest 32-bit number.  A step below the normal
+// 32-bit numbers counts as none.  A group with an infinity or NaN reads as NaN.
+//
+// 32 bits hold 8 columns, columns 0 2 4 6 in the lower half and 1 3 5 7 in the upper one: one `and` and one `or` with the bits of 2^10 (fp16, whose step is 1 there)
+// or 2^7 (bf16) make two neighbouring columns' codes numbers of T, off by that power, which a subtraction takes away exactly.
+#pragma once
+#include "common.cuh"
+
+#include <type_traits>
+
+namespace zl {
+
+constexpr int kInt4Group = 32;
+constexpr int int4_row_bytes(int dim) { return dim / 8 * 5; }
+
+template <typename T>
+struct Int4Pair {
+    using type = __half2;
+};
+template <>
+struct Int4Pair<__nv_bfloat16> {
+    using type = __nv_bfloat162;
+};
+
+// (step, step) and (lowest, lowest) of a group
+template <typename T>
+__device__ __forceinline__ void int4_meta(uint32_t meta, uint32_t& step, uint32_t& low) {
+    step = __byte_perm(meta, 0, 0x1010);
+    low = __byte_perm(meta, 0, 0x3232);
+}
+// Two values from the codes at bits 4 J .. of both halves of x, whose steps and lowest values stand in the halves of step and low
+template <typename T, int J>
+__device__ __forceinline__ uint32_t int4_two(uint32_t x, uint32_t step, uint32_t low) {
+    using P = typename Int4Pair<T>::type;
+    P c;
+    if constexpr (std::is_same<T, __half>::value) {
+        if constexpr (J & 1) {   // 16 c + 2^10, without a shift
+            const uint32_t w = lop3_and_or<0x00f000f0u, 0x64006400u>(J & 2 ? x >> 8 : x);
+            c = __hfma2(*reinterpret_cast<const P*>(&w), __half2half2(__ushort_as_half(0x2c00)), __half2half2(__ushort_as_half(0xd400)));   // 1 / 16, -64
+        } else {
+            const uint32_t w = lop3_and_or<0x000f000fu, 0x64006400u>(J & 2 ? x >> 8 : x);
+            c = __hsub2(*reinterpret_cast<const P*>(&w), __half2half2(__ushort_as_half(0x6400)));
+        }
+    } else {
+        const uint32_t w = lop3_and_or<0x000f000fu, 0x43004300u>(x >> (4 * J));
+        c = __hsub2(*reinterpret_cast<const P*>(&w), __bfloat162bfloat162(__ushort_as_bfloat16(0x4300)));
+    }
+    const P y = __hfma2(c, *reinterpret_cast<const P*>(&step), *reinterpret_cast<const P*>(&low));
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
+// 8 neighbouring columns
+template <typename T>
+__device__ __forceinline__ uint4 int4_eight(uint32_t x, uint32_t step, uint32_t low) {
+    return make_uint4(int4_two<T, 0>(x, step, low), int4_two<T, 1>(x, step, low), int4_two<T, 2>(x, step, low), int4_two<T, 3>(x, step, low));
+}
+// one column
+template <typename T>
+__device__ __forceinline__ float int4_value(const uint8_t* row, int dim, int col) {
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(row + (col >> 3) * 4), meta = *reinterpret_cast<const uint32_t*>(row + dim / 2 + (col / kInt4Group) * 4);
+    const T* two = reinterpret_cast<const T*>(&meta);
+    const float c = (float)(word >> ((col & 1) * 16 + (col & 6) * 2) & 15u);
+    return round_to<T>(fmaf(c, to_f32<T>(two[0]), to_f32<T>(two[1])));
+}
+// whether a group's pair is one of numbers
+template <typename T>
+__device__ __forceinline__ bool int4_finite(uint32_t meta) {
+    constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00 : 0x7f80;
+    return (meta & 0x7fffu) < kInf && (meta >> 16 & 0x7fffu) < kInf;
+}
+
+template <typename T>
+__device__ __forceinline__ T int4_round_down(float x);
+template <>
+__device__ __forceinline__ __half int4_round_down<__half>(float x) { return __float2half_rz(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 int4_round_down<__nv_bfloat16>(float x) { return __float2bfloat16_rz(x); }
+
+// 8 columns of a group whose other columns are in the neighbouring lanes of this group of four; all lanes of the warp call it.  -> the codes; the group's pair
+template <typename T>
+__device__ __forceinline__ uint32_t int4_encode(const uint4& x, uint32_t& meta) {
+    constexpr unsigned kAll = 0xffffffffu;
+    float f[8];
+    unpack8<T>(x, f);
+    float lo = f[0], hi = f[0];
+    bool number = fabsf(f[0]) < INFINITY;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) lo = fminf(lo, f[i]), hi = fmaxf(hi, f[i]), number = number && fabsf(f[i]) < INFINITY;
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) lo = fminf(lo, __shfl_xor_sync(kAll, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(kAll, hi, o));
+    const unsigned numbers = __ballot_sync(kAll, number) >> (threadIdx.x & 28) & 15u;
+    const float half = __fmul_rn(lo, 0.5f);
+    T two[2] = {int4_round_down<T>(__fdiv_rn(__fsub_rn(__fmul_rn(hi, 0.5f), half), 7.5f)), from_f32<T>(lo)};
+    meta = numbers == 15u ? *reinterpret_cast<const uint32_t*>(two) : 0x7fff7fffu;
+    const float step = to_f32<T>(two[0]);
+    uint32_t codes = 0;
+    if (numbers == 15u && step >= 1.17549435e-38f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float n = rintf(2.f * __fdiv_rn(__fsub_rn(__fmul_rn(f[i], 0.5f), half), step));
+            codes |= (uint32_t)(int)fminf(n, 15.f) << ((i & 1) * 16 + (i & 6) * 2);
+        }
+    }
+    return codes;
+}
+
+}  // namespace zl

@@ -45,3 +45,9 @@ struct PagedCache {
     ZL_CHECK_ARG((page_stride) >= 0 && (row_stride) >= 0 && (head_stride) >= 0);                                                                   \
     ZL_CHECK_SUPPORTED(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0);                                             \
     ZL_CHECK_SUPPORTED((page_stride) % 8 == 0 && (row_stride) % 8 == 0 && (head_stride) % 8 == 0)
+// of a cache of 4 bits, strides in bytes: a chunk of a row is dim / 8 bytes, which the kernels copy at once
+#define ZL_CHECK_PAGED_INT4(k, v, num_pages, page_size, page_stride, row_stride, head_stride, dim)                                                \
+    ZL_CHECK_ARG((k) && (v) && (num_pages) > 0 && (page_size) > 0 && (page_stride) >= 0 && (row_stride) >= 0 && (head_stride) >= 0);               \
+    ZL_CHECK_SUPPORTED((dim) == 64 || (dim) == 128);                                                                                               \
+    ZL_CHECK_SUPPORTED(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & ((dim) / 8 - 1)) == 0);                                \
+    ZL_CHECK_SUPPORTED((page_stride) % ((dim) / 8) == 0 && (row_stride) % ((dim) / 8) == 0 && (head_stride) % ((dim) / 8) == 0)

@@ -42,17 +42,6 @@ static PagedPlan paged_plan(int rows, int max_new, int seqs, int max_keys, int h
     return s;
 }
 
-// once for every device: `done` remembers
-template <typename... KArgs>
-static cudaError_t allow_smem(void (*kernel)(KArgs...), int bytes, bool (&done)[64]) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
-    return e;
-}
-
 template <typename T, int D>
 static int paged_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pdl, zl_stream_t stream) {
     static bool done[64] = {};

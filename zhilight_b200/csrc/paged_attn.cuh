@@ -6,6 +6,17 @@
 
 namespace zl {
 
+// once for every device: `done` remembers
+template <typename... KArgs>
+static cudaError_t allow_smem(void (*kernel)(KArgs...), int bytes, bool (&done)[64]) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && done[dev]) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    return e;
+}
+
 struct PagedAttn {
     const void* q;
     void* out;

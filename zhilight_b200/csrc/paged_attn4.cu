@@ -1,0 +1,82 @@
+// Attention of the new tokens of every sequence over pages of 4 bits (int4_cache.cuh): what paged_attn.cu does over pages of 16.
+#include "paged_attn4_few.cuh"
+
+#include <climits>
+
+namespace zl {
+
+struct Paged4Plan {
+    int ctas, block_rows;
+    size_t ml, part, cuts, bytes;   // what lies where in the workspace
+};
+
+template <int D>
+static int paged4_most_ctas(bool eight) { return device_sm_count() * (eight ? P4Cfg<D, 1>::kPerSm : P4Cfg<D, 2>::kPerSm); }
+
+static Paged4Plan paged4_plan(int rows, int max_new, int seqs, int max_keys, int heads, int kv_heads, int dim) {
+    Paged4Plan s = {};
+    const int group = heads / kv_heads;
+    const long long all = (long long)rows * group, most = (long long)max_new * group;
+    s.block_rows = most <= 8 ? 8 : 16;
+    // no more CTAs than the line can be long: every sequence adds less than one block to those of the rows, each of all the keys there is room for
+    const long long units = (all / s.block_rows + seqs) * (P4Kind::kSetup + cdiv(max_keys, kP4Keys)) * kv_heads;
+    const int most_ctas = dim == 64 ? paged4_most_ctas<64>(s.block_rows == 8) : paged4_most_ctas<128>(s.block_rows == 8);
+    s.ctas = (int)(units < most_ctas ? units : most_ctas);
+    const size_t parts = (size_t)s.ctas * 2 * s.block_rows;
+    auto take = [&](size_t bytes) {
+        const size_t at = s.bytes;
+        s.bytes += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    s.ml = take(parts * sizeof(float2)), s.part = take(parts * dim * sizeof(float)), s.cuts = take((size_t)s.ctas * sizeof(PagedCut));
+    return s;
+}
+
+template <typename T, int D, int NT>
+static int paged4_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pdl, zl_stream_t stream) {
+    using C = P4Cfg<D, NT>;
+    static bool done[64] = {};
+    ZL_CHECK_CUDA(allow_smem(k_paged_attn4_few<T, D, NT>, C::kBytes, done));
+    ZL_CHECK_CUDA(launch(k_paged_attn4_few<T, D, NT>, dim3(ctas), dim3(kP4Warps * 32), C::kBytes, stream, pdl, p, c));
+    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 8 * NT>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p));
+    return ZL_OK;
+}
+
+template <typename T, int D>
+static int paged4(const PagedAttn& p, const PagedCache& c, const Paged4Plan& s, bool pdl, zl_stream_t stream) {
+    return s.block_rows == 8 ? paged4_few<T, D, 1>(p, c, s.ctas, pdl, stream) : paged4_few<T, D, 2>(p, c, s.ctas, pdl, stream);
+}
+
+}  // namespace zl
+
+using namespace zl;
+
+extern "C" size_t zl_paged_attention_int4_workspace_bytes(int rows, int max_new, int seqs, int max_keys, int heads, int kv_heads, int dim) {
+    if (rows <= 0 || max_new <= 0 || seqs <= 0 || max_keys <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || dim <= 0) return 0;
+    return paged4_plan(rows, max_new, seqs, max_keys, heads, kv_heads, dim).bytes;
+}
+
+extern "C" int zl_paged_attention_int4(const void* q, const void* k_cache, const void* v_cache, long long num_pages, int page_size, long long page_stride,
+                                       long long row_stride, long long head_stride, const int32_t* page_table, int ld_table, int max_pages,
+                                       const int32_t* seq_lens, const int32_t* q_starts, int seqs, float scale, int window, void* out, int rows, int max_new,
+                                       int heads, int kv_heads, int dim, void* workspace, size_t workspace_bytes, int dtype, int pdl, zl_stream_t stream) {
+    ZL_CHECK_ARG(q && seq_lens && q_starts && out && rows > 0 && max_new > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0);
+    ZL_CHECK_ARG(scale > 0.f && scale < INFINITY && window >= 0);
+    ZL_CHECK_PAGED_INT4(k_cache, v_cache, num_pages, page_size, page_stride, row_stride, head_stride, dim);
+    ZL_CHECK_ARG(page_table && max_pages > 0 && ld_table >= max_pages && seqs > 0);
+    ZL_CHECK_SUPPORTED(dtype == ZL_F16 || dtype == ZL_BF16);
+    ZL_CHECK_SUPPORTED(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0);
+    ZL_CHECK_SUPPORTED(heads <= 65535 && (long long)rows * heads < INT_MAX);
+    const long long room = (long long)max_pages * page_size;
+    const Paged4Plan s = paged4_plan(rows, max_new, seqs, (int)(room < INT_MAX - 255 ? room : INT_MAX - 255), heads, kv_heads, dim);
+    // the kernels count tiles in 32 bits
+    ZL_CHECK_SUPPORTED(((long long)rows * (heads / kv_heads) / s.block_rows + seqs) * (room / kP4Keys + 2 + P4Kind::kSetup) < (INT_MAX - (1 << 16)) / kv_heads);
+    ZL_CHECK_ARG(workspace && workspace_bytes >= s.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
+    const PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), num_pages, page_stride, row_stride, head_stride, page_table, ld_table, max_pages,
+                          page_size, seqs, paged_divisor(page_size)};
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const PagedAttn p = {q, out, seq_lens, q_starts, rows, heads, heads / kv_heads, window, paged_divisor(heads / kv_heads), scale * 1.4426950408889634f, kv_heads,
+                         s.block_rows, 0, reinterpret_cast<float2*>(ws + s.ml), reinterpret_cast<float*>(ws + s.part), reinterpret_cast<PagedCut*>(ws + s.cuts)};
+    if (dtype == ZL_F16) return dim == 64 ? paged4<__half, 64>(p, c, s, pdl != 0, stream) : paged4<__half, 128>(p, c, s, pdl != 0, stream);
+    return dim == 64 ? paged4<__nv_bfloat16, 64>(p, c, s, pdl != 0, stream) : paged4<__nv_bfloat16, 128>(p, c, s, pdl != 0, stream);
+}

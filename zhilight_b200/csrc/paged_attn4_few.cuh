@@ -1,0 +1,349 @@
+// Attention of few (token, head) rows of a kv head over pages of 4 bits (int4_cache.cuh).  Work is shared out as in paged_attn_few.cuh: tiles of 64 keys of all
+// blocks stand in one line, a CTA takes an equal stretch, a warp has 16 keys of a tile and a ring of its own.
+//
+// What 4 bits take off the memory they put on the instructions: a key and its value are 160 bytes instead of 512, and every code costs two to three of them.
+// So the products are turned around, S^T = K Q^T and O^T += V^T P^T by mma.sync with the keys' and values' 16 rows as the first operand and 8 rows of queries as the
+// second: blocks of 8 rows (one token of a group of 8, two of 4) take half the products, exponentials and registers that 16 rows would.
+//   K: columns may be summed in any order as long as Q's are in the same one, so lane (g, t) takes a quarter of the columns of keys g and g + 8 in one piece,
+//      one 16-byte load and one pair (step, lowest) each.
+//   V: the operand wants two keys in a register; codes of two keys come together by one byte permutation per four columns, before they become numbers, so
+//      that this costs an eighth of an instruction a value.  Output columns may lie anywhere: lane g takes D / 8 neighbouring ones.
+//   P: the scores' accumulators, rounded to 16 bits, are the second operand once 8 x 8 of them are transposed (movmatrix).
+// Probabilities are rounded to the rows' type once (half a step each, of random sign: beside the output's own rounding), sums are in 32 bits.
+#pragma once
+#include "int4_cache.cuh"
+#include "paged_attn_few.cuh"
+
+namespace zl {
+
+constexpr int kP4Warps = 4, kP4Keys = 16 * kP4Warps, kP4Stages = 4;
+
+template <int D, int NT>
+struct P4Cfg {
+    static constexpr int kChunk = D / 8;                             // bytes copied at once; a row is four of codes and one of pairs
+    static constexpr int kVc = 8 * D, kKm = 16 * D, kVm = 18 * D;    // of a stage: codes of K, of V, pairs of K, of V
+    static constexpr int kStage = 20 * D;
+    static constexpr int kWarp = kP4Stages * kStage;
+    static constexpr int kBytes = kP4Warps * kWarp;
+    static constexpr int kPitch = D + 8;                             // floats; of a row of a warp's output in its ring
+    static_assert(8 * NT * kPitch * 4 <= kWarp, "a warp's output, where its ring was");
+    static constexpr int kPerSm = NT == 1 ? 4 : 3;
+};
+
+// tiles of 64 keys; at least one: a block that sees nothing is written too
+struct P4Kind {
+    static constexpr int kSetup = 2;
+    static __device__ __forceinline__ int turns(const PagedAttn&, const PagedBlock& k) { return k.hi >= 0 ? k.hi / kP4Keys - k.lo / kP4Keys + 1 : 1; }
+};
+
+template <int BYTES>
+__device__ __forceinline__ void p4_copy(uint32_t dst, const void* src, int bytes) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t p4_transpose(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+// N words in one load
+template <int N>
+__device__ __forceinline__ void p4_words(uint32_t (&w)[N], const uint8_t* at) {
+    if constexpr (N == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else if constexpr (N == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(at);
+        w[0] = x.x, w[1] = x.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(at);
+    }
+}
+
+// grid: CTAs that share the line; blocks of up to 8 NT rows
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged_attn4_few(const PagedAttn p, const PagedCache c) {
+    using C = P4Cfg<D, NT>;
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr int R = 8 * NT, KS = D / 16, MT = D / 16, KW = D / 32, VW = D / 64;
+    constexpr float kTau = PagedExp<kHalf>::kTau, kUp = PagedExp<kHalf>::kUp;
+    extern __shared__ __align__(128) uint8_t p4_smem[];
+    __shared__ float2 s_ml[kP4Warps][R];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    uint8_t* ring = p4_smem + warp * C::kWarp;
+    const uint32_t ring_at = smem_u32(ring);
+    // This lane's five chunks of a stage's 160: the chunk of which row, where in the stage.  V's rows stand as the lanes read them, 2t + {0, 1, 8, 9} four behind one
+    // another, and (D = 128) every second pair of them with the halves of its codes changed: reads of four rows touch all banks once.
+    int place[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        const int x = lane + 32 * i, is_v = x >= 80, r = (x - 80 * is_v) / 5, ch = (x - 80 * is_v) % 5;
+        const int slot = is_v ? (r & 8) + (r & 1) * 4 + ((r & 7) >> 1) : r;
+        place[i] = r | is_v << 4 | ch << 5 | (ch == 4 ? (is_v ? C::kVm : C::kKm) + slot * C::kChunk
+                                                      : (is_v ? C::kVc : 0) + slot * (D / 2) + (ch ^ (is_v && D == 128 ? slot & 2 : 0)) * C::kChunk) << 8;
+    }
+    pdl_wait();
+    pdl_trigger();
+    if (tid == 0) p.cuts[blockIdx.x].parts = 0;
+    PagedWalk<P4Kind> walk;
+    const PagedBlock& k = walk.k;
+    const PagedPlace& at = walk.place;
+    walk.find(p, c, -1);
+    for (; walk.w < walk.end; walk.go(p, c)) {
+        int first, count;
+        walk.share(first, count);
+        if (count == 0) continue;
+        const int key0 = ((k.hi >= 0 ? k.lo / kP4Keys : 0) + first) * kP4Keys + warp * 16;
+        const long long head = (long long)at.hk * c.head_stride;
+        // Lanes 0 - 15 ask for the page numbers of the 16 rows a stage ahead; where pages hold whole 16s these are one page
+        const bool one_page = c.page_size % 16 == 0;
+        auto find = [&](int j) {
+            const int row = key0 + j * kP4Keys + (lane & 15), pg = c.by_page(row);
+            return j < count && row <= k.hi && pg < c.max_pages ? c.table[(size_t)k.seq * c.ld_table + pg] : -1;
+        };
+        auto copy = [&](int j, int id) {
+            const uint32_t to = ring_at + (uint32_t)(j % kP4Stages) * C::kStage;
+            const int row0 = key0 + j * kP4Keys, mine = row0 + (one_page ? 0 : lane & 15);
+            long long off = id >= 0 && id < c.num_pages ? (long long)id * c.page_stride + (long long)(mine - c.by_page(mine) * c.page_size) * c.row_stride + head : -1;
+            if (one_page) off = __shfl_sync(0xffffffffu, off, 0);
+#pragma unroll
+            for (int i = 0; i < 5; ++i) {
+                const int r = place[i] & 15;
+                long long o = one_page ? off : __shfl_sync(0xffffffffu, off, r);
+                const bool in = o >= 0 && row0 + r <= k.hi;
+                if (one_page) o += r * c.row_stride;
+                o += (place[i] >> 5 & 7) * C::kChunk;
+                p4_copy<C::kChunk>(to + (uint32_t)(place[i] >> 8), static_cast<const uint8_t*>(place[i] & 16 ? c.v : c.k) + (in ? o : 0), in ? C::kChunk : 0);
+            }
+        };
+        // rows of q: row g of each 8, as the columns of the second operand; what rows 2t and 2t + 1 see
+        uint32_t qb[NT][KS][2];
+        int hi[NT][2], lo[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 8 + g;
+            const bool in = r < k.rows;
+            const int row = k.row0 + (in ? r : 0), t = p.by_group(row);
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + ((size_t)(k.first + t) * p.heads + at.hk * p.group + row - t * p.group) * D) + t4 * (D / 8);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                uint2 x = make_uint2(0u, 0u);
+                if (in) x = *reinterpret_cast<const uint2*>(src + 2 * s);
+                qb[n][s][0] = x.x, qb[n][s][1] = x.y;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row_e = n * 8 + t4 * 2 + e;
+                const bool is = row_e < k.rows;
+                const int at_place = k.place0 + p.by_group(k.row0 + (is ? row_e : 0));
+                hi[n][e] = is ? min(at_place, k.have - 1) : -1;
+                lo[n][e] = paged_from(p, at_place);
+            }
+        }
+        float o[MT][NT][4], l[NT][2], m_ref[NT][2];
+        // Once, mostly.  A masked probability is exactly zero, but zero times NaN, which a broken group of a row's values reads as, is NaN in its sum.  Where the warp's sums hold
+        // a NaN that no score explains, it goes over its keys once more: of 16 keys with a broken group it takes the product key by key, of those that a row sees.
+        for (bool again = false;; again = true) {
+            int id = find(0);
+#pragma unroll 1
+            for (int j = 0; j < kP4Stages - 1; ++j) {
+                const int next = find(j + 1);
+                if (j < count) copy(j, id);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                id = next;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
+                l[n][0] = l[n][1] = 0.f, m_ref[n][0] = m_ref[n][1] = kPagedNone;
+            }
+            for (int j = 0; j < count; ++j) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kP4Stages - 2) : "memory");
+                __syncwarp();
+                const int next = find(j + kP4Stages);
+                if (j + kP4Stages - 1 < count) copy(j + kP4Stages - 1, id);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                id = next;
+                const int kb = key0 + j * kP4Keys;
+                if (kb > k.hi || kb + 15 < k.lo) continue;
+                const uint8_t* st = ring + (j % kP4Stages) * C::kStage;
+                float s[NT][4] = {};
+                {
+                    uint32_t x[2][KW], step[2], low[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int r = g + u * 8;
+                        p4_words<KW>(x[u], st + r * (D / 2) + t4 * C::kChunk);
+                        int4_meta<T>(*reinterpret_cast<const uint32_t*>(st + C::kKm + r * C::kChunk + t4 * (D / 4) / kInt4Group * 4), step[u], low[u]);
+                    }
+#pragma unroll
+                    for (int w = 0; w < KW; ++w) {
+                        const uint32_t a[4] = {int4_two<T, 0>(x[0][w], step[0], low[0]), int4_two<T, 0>(x[1][w], step[1], low[1]),
+                                               int4_two<T, 1>(x[0][w], step[0], low[0]), int4_two<T, 1>(x[1][w], step[1], low[1])};
+                        const uint32_t b[4] = {int4_two<T, 2>(x[0][w], step[0], low[0]), int4_two<T, 2>(x[1][w], step[1], low[1]),
+                                               int4_two<T, 3>(x[0][w], step[0], low[0]), int4_two<T, 3>(x[1][w], step[1], low[1])};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            pf_mma<T>(s[n], a, qb[n][2 * w][0], qb[n][2 * w][1]);
+                            pf_mma<T>(s[n], b, qb[n][2 * w + 1][0], qb[n][2 * w + 1][1]);
+                        }
+                    }
+                }
+                bool up = false;
+                float top[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int key = kb + g + u * 8;
+                            float& x = s[n][2 * u + e];
+                            x = key <= hi[n][e] && key >= lo[n][e] ? x * p.scale : -INFINITY;
+                        }
+                        top[n][e] = fmaxf(s[n][e], s[n][2 + e]);
+                        up |= top[n][e] - m_ref[n][e] > kTau;
+                    }
+                if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                            for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], x));
+                            const float f = top[n][e] > m_ref[n][e] ? pa_exp2(m_ref[n][e] - top[n][e]) : 1.f;
+                            m_ref[n][e] = fmaxf(m_ref[n][e], top[n][e]);
+                            l[n][e] *= f;
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) o[m][n][e] *= f, o[m][n][2 + e] *= f;
+                        }
+                }
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {   // the difference first: it is as exact as the scores, whatever their size is
+                        float &x = s[n][2 * u], &y = s[n][2 * u + 1];
+                        x = pa_exp2((x - m_ref[n][0]) + kUp), y = pa_exp2((y - m_ref[n][1]) + kUp);
+                        l[n][0] += x, l[n][1] += y;
+                        pb[n][u] = p4_transpose(pf_pack<T>(x, y));
+                    }
+                bool apart = false;   // the product key by key
+                if (again) {
+                    bool whole = true;
+                    for (int x = lane; x < D / 2; x += 32) whole = whole && int4_finite<T>(*reinterpret_cast<const uint32_t*>(st + C::kVm + x * 4));
+                    apart = __any_sync(0xffffffffu, !whole);
+                }
+                if (apart) {
+#pragma unroll 1
+                    for (int key = 0; key < 16; ++key) {
+                        const int slot = (key & 8) + (key & 1) * 4 + ((key & 7) >> 1);
+                        const uint32_t meta = *reinterpret_cast<const uint32_t*>(st + C::kVm + slot * C::kChunk + g * (D / 8) / kInt4Group * 4);
+                        uint32_t x[VW];
+                        p4_words<VW>(x, st + C::kVc + slot * (D / 2) + (D == 128 ? ((g >> 1) ^ (slot & 2)) * 16 + (g & 1) * 8 : g * 4));
+                        const T* two = reinterpret_cast<const T*>(&meta);
+                        float v[D / 8];
+#pragma unroll
+                        for (int i = 0; i < D / 8; ++i)
+                            v[i] = round_to<T>(fmaf((float)(x[i >> 3] >> ((i & 1) * 16 + (i & 6) * 2) & 15u), to_f32<T>(two[0]), to_f32<T>(two[1])));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float w = __shfl_sync(0xffffffffu, key & 8 ? s[n][2 + e] : s[n][e], (key & 7) << 2 | t4);
+                                if (kb + key <= hi[n][e] && kb + key >= lo[n][e])
+#pragma unroll
+                                    for (int i = 0; i < D / 8; ++i) o[i >> 1][n][(i & 1) * 2 + e] = fmaf(w, v[i], o[i >> 1][n][(i & 1) * 2 + e]);
+                            }
+                    }
+                } else {
+                    uint32_t x[4][VW], meta[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int slot = 4 * u + t4;
+                        p4_words<VW>(x[u], st + C::kVc + slot * (D / 2) + (D == 128 ? ((g >> 1) ^ (t4 & 2)) * 16 + (g & 1) * 8 : g * 4));
+                        meta[u] = *reinterpret_cast<const uint32_t*>(st + C::kVm + slot * C::kChunk + g * (D / 8) / kInt4Group * 4);
+                    }
+                    const uint32_t step[2] = {__byte_perm(meta[0], meta[1], 0x5410), __byte_perm(meta[2], meta[3], 0x5410)};
+                    const uint32_t low[2] = {__byte_perm(meta[0], meta[1], 0x7632), __byte_perm(meta[2], meta[3], 0x7632)};
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        uint32_t even[2], odd[2];   // columns 0 2 4 6 and 1 3 5 7 of two keys
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) even[u] = __byte_perm(x[2 * u][w], x[2 * u + 1][w], 0x5410), odd[u] = __byte_perm(x[2 * u][w], x[2 * u + 1][w], 0x7632);
+                        auto product = [&](auto index) {
+                            constexpr int J = decltype(index)::value;
+                            const uint32_t a[4] = {int4_two<T, J>(even[0], step[0], low[0]), int4_two<T, J>(odd[0], step[0], low[0]),
+                                                   int4_two<T, J>(even[1], step[1], low[1]), int4_two<T, J>(odd[1], step[1], low[1])};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) pf_mma<T>(o[w * 4 + J][n], a, pb[n][0], pb[n][1]);
+                        };
+                        product(std::integral_constant<int, 0>{}), product(std::integral_constant<int, 1>{});
+                        product(std::integral_constant<int, 2>{}), product(std::integral_constant<int, 3>{});
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
+            if (again) break;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    bool none = false;
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) none |= o[m][n][e] != o[m][n][e] || o[m][n][2 + e] != o[m][n][2 + e];
+                    again |= none && l[n][e] == l[n][e] && n * 8 + t4 * 2 + e < k.rows;
+                }
+            if (!__any_sync(0xffffffffu, again)) break;
+            __syncwarp();
+        }
+        // the warps' parts, in their rings
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+        float* mine = reinterpret_cast<float*>(ring);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = n * 8 + t4 * 2 + e;
+                if (g == 0) s_ml[warp][r] = make_float2(m_ref[n][e], l[n][e]);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) *reinterpret_cast<float2*>(mine + r * C::kPitch + g * (D / 8) + 2 * m) = make_float2(o[m][n][e], o[m][n][2 + e]);
+            }
+        __syncthreads();
+        const bool whole = walk.whole(count);
+        const size_t part = ((size_t)blockIdx.x * 2 + (first > 0 ? 0 : 1)) * R;
+        for (int r = warp; r < k.rows; r += kP4Warps) {
+            constexpr int E = D / 32;
+            float m = s_ml[0][r].x, sum = 0.f, v[E] = {};
+#pragma unroll
+            for (int x = 1; x < kP4Warps; ++x) m = fmaxf(m, s_ml[x][r].x);
+#pragma unroll
+            for (int x = 0; x < kP4Warps; ++x) {
+                const float f = pa_exp2(s_ml[x][r].x - m);
+                sum = fmaf(s_ml[x][r].y, f, sum);
+                const float* from = reinterpret_cast<const float*>(p4_smem + x * C::kWarp) + r * C::kPitch + lane * E;
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = fmaf(from[e], f, v[e]);
+            }
+            if (whole) {
+                paged_row_out<T, D>(p, k, at.hk, r, sum, v);
+            } else {
+                if (lane == 0) p.ml[part + r] = make_float2(m, sum);
+                float* dst = p.part + (part + r) * D + lane * E;
+                if constexpr (E == 4) *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+                else *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
+            }
+        }
+        if (tid == 0) walk.cut(p, first, count);
+        __syncthreads();   // the rings are the next block's
+    }
+}
+
+}  // namespace zl

@@ -1142,10 +1142,23 @@ def _paged_cache(k_cache, v_cache, page_table, dtype):
     """(pages, page_size, kv_heads, dim) caches, views into larger pools or with the heads outside the rows too: -> strides of their pages, rows, heads."""
     _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "k_cache and v_cache must be (pages, page_size, kv_heads, dim)")
     _need(k_cache.dtype == dtype and v_cache.dtype == dtype and dtype in (torch.float16, torch.bfloat16), "caches must be fp16 or bf16, like the rows", -2)
+    return _paged_steps(k_cache, v_cache, page_table)
+
+
+def _paged_cache_int4(k_cache, v_cache, page_table, dtype):
+    """(pages, page_size, kv_heads, int4_row_bytes(dim)) caches of bytes: -> strides of their pages, rows, heads, and dim."""
+    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "k_cache and v_cache must be (pages, page_size, kv_heads, int4_row_bytes(dim))")
+    _need(k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8, "caches of 4 bits must be uint8", -2)
+    _need(dtype in (torch.float16, torch.bfloat16), "rows must be fp16 or bf16", -2)
+    _need(k_cache.shape[3] in (int4_row_bytes(64), int4_row_bytes(128)), "heads of a cache of 4 bits must be 64 or 128 wide: rows of 40 or 80 bytes", -2)
+    return _paged_steps(k_cache, v_cache, page_table), k_cache.shape[3] // 5 * 8
+
+
+def _paged_steps(k_cache, v_cache, page_table):
     steps, more = ([0 if n == 1 else s for n, s in zip(c.shape, c.stride())] for c in (k_cache, v_cache))   # of one page, row or head none is taken
     _need(steps == more and k_cache.stride(3) == 1, "k_cache and v_cache must have the same strides, heads in one piece")
     _need(all(s > 0 or n == 1 for n, s in zip(k_cache.shape, steps)), "pages, rows and heads of a cache must not share memory")
-    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.stride(1) == 1 and page_table.numel() > 0,
+    _need(page_table is None or (page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.stride(1) == 1 and page_table.numel() > 0),
           "page_table must be (sequences, pages) int32, its rows in one piece")
     _need(k_cache.numel() > 0 and k_cache.shape[3] > 1, "the cache is empty")
     return steps[:3]
@@ -1166,7 +1179,53 @@ def qkv_axes_rope_append(qkv, pos, inv_freq, axis, token_seq, placement, page_ta
         if y is not None:
             return _done(y)
     steps = _paged_cache(k_cache, v_cache, page_table, qkv.dtype)
-    pages, page_size, kv_heads, dim = k_cache.shape
+    return _append("zl_qkv_axes_rope_append", steps, k_cache.shape[3], qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout,
+                   mscale, pdl)
+
+
+def qkv_axes_rope_append_int4(qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout=ROT_HALVES, mscale=1.0, pdl=False):
+    """qkv_axes_rope_append into caches of 4 bits: (pages, page_size, kv_heads, int4_row_bytes(dim)) uint8, dim 64 or 128, read by paged_attention_int4 and
+    int4_cache_values.  Keys, once turned and rounded to qkv's type, and values are held as 16 equal steps between the lowest and the highest of every 32
+    columns: off by up to half a step, a 30th of that range; 32 columns with an infinity or NaN read as NaN.  Decoding is fastest where a page has the rows of
+    a head one behind another: caches made as (pages, kv_heads, page_size, bytes) and passed with .transpose(1, 2).  -> q (T, heads * dim)."""
+    if _lib.host is not None:
+        y = _lib.host.qkv_axes_rope_append_int4(qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout, mscale, pdl)
+        if y is not None:
+            return _done(y)
+    steps, dim = _paged_cache_int4(k_cache, v_cache, page_table, qkv.dtype)
+    return _append("zl_qkv_axes_rope_append_int4", steps, dim, qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout, mscale, pdl)
+
+
+def int4_row_bytes(dim):
+    """Bytes of a head's row in a cache of 4 bits: codes, and a step and a lowest value for every 32 columns."""
+    _need(dim in (64, 128), "heads of a cache of 4 bits must be 64 or 128 wide", -2)
+    return dim // 8 * 5
+
+
+def int4_cache_values(k_cache, v_cache, dtype, pages=None, pdl=False):
+    """What pages of caches of 4 bits (pages, page_size, kv_heads, int4_row_bytes(dim)) stand for, in the type that their rows were written from.
+    pages (n) int32: page numbers, zeros for one outside the pool; None: all of them in their order.  v_cache None: k_cache alone.
+    -> keys and values (n, page_size, kv_heads, dim), contiguous (or keys alone)."""
+    if _lib.host is not None:
+        y = _lib.host.int4_cache_values(k_cache, v_cache, dtype, pages, pdl)
+        if y is not None:
+            return _done(y)
+    steps, dim = _paged_cache_int4(k_cache, k_cache if v_cache is None else v_cache, None, dtype)
+    num, page_size, kv_heads = k_cache.shape[:3]
+    _need(pages is None or pages.dim() == 1, "pages must be (n)")
+    n = num if pages is None else pages.numel()
+    if pages is not None:
+        _ints("pages", pages, (n,))
+    _here(k_cache, v_cache, pages)
+    out = [torch.empty((n, page_size, kv_heads, dim), dtype=dtype, device=k_cache.device) for _ in range(1 if v_cache is None else 2)]
+    if n:
+        _lib.call("zl_int4_cache_values", k_cache.data_ptr(), _dp(v_cache), num, page_size, *steps, _dp(pages), n, out[0].data_ptr(),
+                  out[1].data_ptr() if v_cache is not None else None, kv_heads, dim, _dt(out[0]), int(pdl), _stream())
+    return out[0] if v_cache is None else tuple(out)
+
+
+def _append(entry, steps, dim, qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout, mscale, pdl):
+    pages, page_size, kv_heads = k_cache.shape[:3]
     _need(qkv.dim() == 2 and heads > 0 and qkv.shape[1] == (heads + 2 * kv_heads) * dim and qkv.stride(1) == 1,
           "qkv must be (T, (heads + 2 kv_heads) * dim), its rows in one piece")
     t, half = qkv.shape[0], inv_freq.numel()
@@ -1182,7 +1241,7 @@ def qkv_axes_rope_append(qkv, pos, inv_freq, axis, token_seq, placement, page_ta
     q = torch.empty((t, heads * dim), dtype=qkv.dtype, device=qkv.device)
     if t == 0:
         return q
-    _lib.call("zl_qkv_axes_rope_append", qkv.data_ptr(), qkv.stride(0) if t > 1 else qkv.shape[1], pos.data_ptr(), t, pos.shape[0],
+    _lib.call(entry, qkv.data_ptr(), qkv.stride(0) if t > 1 else qkv.shape[1], pos.data_ptr(), t, pos.shape[0],
               ctypes.cast(inv_freq.data_ptr(), ctypes.POINTER(ctypes.c_double)), axis.data_ptr(), half, layout, float(mscale), token_seq.data_ptr(),
               placement.data_ptr(), page_table.data_ptr(), page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1], page_table.shape[1],
               page_table.shape[0], k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, *steps, q.data_ptr(), t, heads, kv_heads, dim,
@@ -1203,7 +1262,22 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
         if y is not None:
             return _done(y)
     steps = _paged_cache(k_cache, v_cache, page_table, q.dtype)
-    pages, page_size, kv_heads, dim = k_cache.shape
+    return _attend("zl_paged_attention", steps, k_cache.shape[3], q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl)
+
+
+def paged_attention_int4(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window=0, max_new=None, out=None, pdl=False):
+    """paged_attention over caches of 4 bits (pages, page_size, kv_heads, int4_row_bytes(dim)) uint8 whose rows were written from q's type
+    (qkv_axes_rope_append_int4): the attention over what they stand for, int4_cache_values.  -> out, like q."""
+    if _lib.host is not None:
+        y = _lib.host.paged_attention_int4(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl)
+        if y is not None:
+            return _done(y)
+    steps, dim = _paged_cache_int4(k_cache, v_cache, page_table, q.dtype)
+    return _attend("zl_paged_attention_int4", steps, dim, q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl)
+
+
+def _attend(entry, steps, dim, q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl):
+    pages, page_size, kv_heads = k_cache.shape[:3]
     _need(q.dim() in (2, 3) and q.is_contiguous() and (q.dim() == 2 or q.shape[2] == dim), "q must be contiguous (T, heads * dim) or (T, heads, dim)")
     t, width, seqs = q.shape[0], q.shape[1] * (dim if q.dim() == 3 else 1), page_table.shape[0]
     _need(width > 0 and width % (kv_heads * dim) == 0, "the heads of q must be a multiple of the cache's")
@@ -1219,9 +1293,9 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
     if t == 0:
         return out
     heads, most = width // dim, t if max_new is None else min(max_new, t)
-    nbytes = _lib.load().zl_paged_attention_workspace_bytes(t, most, seqs, min(page_table.shape[1] * page_size, 2 ** 31 - 256), heads, kv_heads, dim)
+    nbytes = getattr(_lib.load(), entry + "_workspace_bytes")(t, most, seqs, min(page_table.shape[1] * page_size, 2 ** 31 - 256), heads, kv_heads, dim)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.call("zl_paged_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, *steps, page_table.data_ptr(),
+    _lib.call(entry, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, *steps, page_table.data_ptr(),
               page_table.stride(0) if seqs > 1 else page_table.shape[1], page_table.shape[1], seq_lens.data_ptr(), q_starts.data_ptr(), seqs, float(scale),
               min(window, 2 ** 31 - 1), out.data_ptr(), t, most, heads, kv_heads, dim, _dp(ws), nbytes, _dt(q), int(pdl), _stream())
     return out
@@ -1256,3 +1330,76 @@ def verify_drafts(target, draft, drafted, accept, sample, count=None, pdl=False)
               draft.stride(1) if draft is not None else 0, drafted.data_ptr(), accept.data_ptr(), sample.data_ptr(), _dp(count), accepted.data_ptr(),
               tokens.data_ptr(), b, k, vocab, int(pdl), _stream())
     return accepted, tokens
+
+
+def adjust_logits(logits, tokens=None, token_seq=None, token_lens=None, prompt_lens=None, repetition=None, frequency=None, presence=None, bias_starts=None,
+                  bias_words=None, bias=None, temperature=None, mask=None, mask_row=None, out_dtype=None, out=None, pdl=False):
+    """Penalties for repeated words, biases, temperature and grammar masks on logits (R, vocab) in fp16, bf16 or fp32, rows of any pitch, in this order:
+
+    tokens (S, L) int32, rows of any pitch, token_seq (R) int32 (None: row r has history r), token_lens (R) int32, prompt_lens (R) int32 (None: 0): the
+    history of row r is tokens[token_seq[r], :token_lens[r]], the first prompt_lens[r] words of it the prompt.  Rows behind drafted words share a
+    row of tokens, with lengths of their own.  repetition (R) fp32: a word of the history has z / repetition where z > 0, else z * repetition; frequency and
+    presence (R) fp32: a word that is there n > 0 times behind the prompt loses frequency * n + presence.
+    bias_starts (R + 1) int32 ascending, bias_words (N) int32, bias (N) fp32: row r's words bias_words[i] get bias[i], bias_starts[r] <= i < bias_starts[r + 1],
+    a word that is listed twice both.
+    temperature (R) fp32: z / temperature; 0 (and anything below 2^-126): as it is, for greedy rows.
+    mask (M, W >= vocab / 32) int32, rows of any pitch, mask_row (R) int32 (None: row r has mask r; outside [0, M): no mask): words w whose bit w % 32 of
+    mask[., w // 32] is clear get -inf.  A row whose mask leaves nothing is -inf throughout.
+
+    Arithmetic in 32 bits.  -> out (R, vocab) in out_dtype (logits' own or fp32; None: logits' own), which may be logits itself."""
+    if _lib.host is not None:
+        y = _lib.host.adjust_logits(logits, tokens, token_seq, token_lens, prompt_lens, repetition, frequency, presence, bias_starts, bias_words, bias, temperature,
+                                    mask, mask_row, out_dtype, out, pdl)
+        if y is not None:
+            return _done(y)
+    _need(logits.dim() == 2 and logits.shape[1] > 0 and logits.stride(1) == 1, "logits must be (R, vocab), its rows in one piece")
+    kind = _dt(logits)
+    r, vocab = logits.shape
+    _need(out_dtype in (None, logits.dtype, torch.float32), "out_dtype must be the logits' type or fp32", -2)
+    want = out.dtype if out is not None and out_dtype is None else out_dtype or logits.dtype
+    _need(out is None or (out.shape == logits.shape and out.dtype == want and want in (logits.dtype, torch.float32) and out.stride(1) == 1),
+          "out must be (R, vocab) of out_dtype, its rows in one piece")
+    pitch = [vocab if x is None or r == 1 else x.stride(0) for x in (logits, out)]
+    _need(pitch[0] >= vocab and pitch[1] >= vocab, "rows of logits and out must not share memory")
+    if tokens is None:
+        _need(all(x is None for x in (token_seq, token_lens, prompt_lens, repetition, frequency, presence)), "penalties and lengths need tokens")
+    else:
+        _need(tokens.dim() == 2 and tokens.dtype == torch.int32 and (tokens.stride(1) == 1 or tokens.shape[1] < 2), "tokens must be (S, L) int32, its rows in one piece")
+        _need(token_lens is not None and (token_seq is not None or tokens.shape[0] >= r), "tokens need token_lens, and token_seq or a row for each of the logits'")
+        _need(tokens.shape[0] < 2 or tokens.stride(0) >= tokens.shape[1], "rows of tokens must not share memory")
+    for name, x in (("token_seq", token_seq), ("token_lens", token_lens), ("prompt_lens", prompt_lens), ("mask_row", mask_row)):
+        if x is not None:
+            _ints(name, x, (r,))
+    for name, x in (("repetition", repetition), ("frequency", frequency), ("presence", presence), ("temperature", temperature)):
+        _need(x is None or (x.dtype == torch.float32 and tuple(x.shape) == (r,) and x.is_contiguous()), "%s must be contiguous fp32 (%d,)" % (name, r))
+    n = 0
+    if bias_starts is None:
+        _need(bias_words is None and bias is None, "biases need bias_starts")
+    else:
+        _ints("bias_starts", bias_starts, (r + 1,))
+        _need(bias_words is not None and bias is not None and bias_words.dim() == 1, "bias_starts need bias_words and bias")
+        n = bias_words.numel()
+        _ints("bias_words", bias_words, (n,))
+        _need(bias.dtype == torch.float32 and tuple(bias.shape) == (n,) and bias.is_contiguous(), "bias must be contiguous fp32 (%d,)" % n)
+    if mask is None:
+        _need(mask_row is None, "mask_row needs a mask")
+    else:
+        _need(mask.dim() == 2 and mask.dtype == torch.int32 and (mask.stride(1) == 1 or mask.shape[1] < 2) and mask.shape[0] > 0 and mask.shape[1] * 32 >= vocab,
+              "mask must be (M, vocab / 32 or more) int32, its rows in one piece")
+        _need(mask_row is not None or mask.shape[0] >= r, "a mask of fewer rows than the logits' needs mask_row")
+        _need(mask.shape[0] < 2 or mask.stride(0) >= mask.shape[1], "rows of mask must not share memory")
+    _here(logits, tokens, token_seq, token_lens, prompt_lens, repetition, frequency, presence, bias_starts, bias_words, bias, temperature, mask, mask_row, out)
+    if out is None:
+        out = torch.empty((r, vocab), dtype=want, device=logits.device)
+    if r == 0:
+        return out
+    if tokens is not None and tokens.numel() == 0:
+        tokens = None                                                # no history at all
+    if n == 0:
+        bias_starts = bias_words = bias = None
+    _lib.call("zl_adjust_logits", logits.data_ptr(), pitch[0], kind, out.data_ptr(), pitch[1], _dt(out), r, vocab, _dp(tokens),
+              0 if tokens is None else tokens.stride(0) if tokens.shape[0] > 1 else tokens.shape[1], 0 if tokens is None else tokens.shape[0],
+              0 if tokens is None else tokens.shape[1], _dp(token_seq), _dp(token_lens), _dp(prompt_lens), _dp(repetition), _dp(frequency), _dp(presence),
+              _dp(bias_starts), _dp(bias_words), _dp(bias), n, _dp(temperature), _dp(mask), 0 if mask is None else mask.stride(0) if mask.shape[0] > 1 else mask.shape[1],
+              0 if mask is None else mask.shape[0], _dp(mask_row), int(pdl), _stream())
+    return out
