@@ -57,7 +57,7 @@ def hide(cache, table, lens, byte=0xff):
     (1, 1, 64, 32, True, 2, "rows", 3), (3, 1, 64, 31, False, 7, "heads", 300), (200, 100, 128, 64, False, 16, "heads", 5), (128, 128, 64, 32, True, 8, "rows", 400),
     (64, 8, 128, 64, False, 16, "wide", 2000)])
 def test_append(cuda, dtype, heads, kv_heads, dim, half, adjacent, page, order, t):
-    """Keys are given as the first heads of q: q, turned and rounded, says what the keys' codes have to be, bit by bit."""
+    """Keys are turned in 64 bits and rounded to 32 and to the type: their codes, like the values', are the formula's, bit by bit."""
     g = torch.Generator().manual_seed(heads * 1000 + t)
     lens = [t, t + 11, 2 * t]
     pages = sum(-(-n // page) for n in lens) + 2
@@ -65,7 +65,6 @@ def test_append(cuda, dtype, heads, kv_heads, dim, half, adjacent, page, order, 
     k, v = pool(g, pages, page, kv_heads, dim, dtype, order)
     width = (heads + 2 * kv_heads) * dim
     wide = torch.randn(t, width + 16, generator=g).to(dtype)
-    wide[:, heads * dim:(heads + kv_heads) * dim] = wide[:, :kv_heads * dim]
     pos = torch.randint(0, 5_000_000, (3, t), generator=g, dtype=torch.int32)
     axis = torch.randint(0, 3, (half,), generator=g, dtype=torch.int32)
     if half > 4:
@@ -75,12 +74,12 @@ def test_append(cuda, dtype, heads, kv_heads, dim, half, adjacent, page, order, 
     place = torch.tensor([lens[int(s)] - t + i for i, s in enumerate(seq)], dtype=torch.int32)
     if t > 4:
         place[2], seq[3], place[4] = -1, 3, page * table.shape[1]    # nowhere, no such sequence, behind the table
-    want_q, _, _, off_q, _ = oracle.axes_rope(wide[:, :width].contiguous(), pos, freq, axis, heads, kv_heads, dim, adjacent, 1.25)
+    want_q, want_k, want_v, off_q, _ = oracle.axes_rope(wide[:, :width].contiguous(), pos, freq, axis, heads, kv_heads, dim, adjacent, 1.25)
     kd, vd = to_gpu(k), to_gpu(v)
     q = ops.qkv_axes_rope_append_int4(wide.cuda()[:, :width], pos.cuda(), freq.cuda(), axis.cuda(), seq.cuda(), place.cuda(), table.cuda(), kd, vd, heads,
                                       layout=ops.ROT_ADJACENT if adjacent else ops.ROT_HALVES, mscale=1.25).cpu().view(t, heads, dim)
     assert ((q.double() - want_q).abs() <= off_q).all()
-    new_k, new_v = codes.encode(q[:, :kv_heads], dtype), codes.encode(wide[:, (heads + kv_heads) * dim:width].reshape(t, kv_heads, dim), dtype)
+    new_k, new_v = (codes.encode(x.float().to(dtype), dtype) for x in (want_k, want_v))
     for i in range(t):
         s, p = int(seq[i]), int(place[i])
         if 0 <= s < 3 and 0 <= p < page * table.shape[1] and 0 <= int(table[s, p // page]) < pages:

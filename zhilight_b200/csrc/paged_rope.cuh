@@ -20,6 +20,7 @@ namespace zl {
 
 enum { kRopePairs, kRopeAdjacent, kRopeAny };   // halves of whole 16 bytes, a piece of the first with its partner of the second; adjacent; other halves
 constexpr int kRopeMaxStages = 4;
+constexpr int kRopeThreads = 1024, kRopeThreads4 = 768;   // of an SM: 64 registers each, 80 where keys are turned in 64 bits
 
 // two neighbouring elements as two 32-bit numbers, and back
 template <typename T>
@@ -67,10 +68,12 @@ __device__ __forceinline__ void rope_s2g(void* dst, const void* src, uint32_t by
 }
 
 // grid: CTAs that share the tokens; dynamic shared memory: `stages` rows, then cosines and sines of two tokens.  INT4: the caches hold 4 bits (int4_cache.cuh), strides are bytes,
+// keys are turned in 64 bits, whose codes are whole numbers: what is stored is what the formula says, but for sums within 1e-15 of a border between two of T's numbers
+// (in 32 bits one key in 10^4 would be the number beside it),
 // and the threads write keys and values, 8 columns each, from the row that they have turned: its place in the ring takes the next row a barrier later, so there
 // are two rows at least.
 template <typename T, int FORM, bool INT4>
-__global__ void __launch_bounds__(256, 4) k_axes_rope_append(const AxesRope p, const PagedCache c, unsigned* err) {
+__global__ void __launch_bounds__(256, INT4 ? kRopeThreads4 / 256 : kRopeThreads / 256) k_axes_rope_append(const AxesRope p, const PagedCache c, unsigned* err) {
     extern __shared__ __align__(128) uint8_t rope_smem[];
     __shared__ uint64_t full[kRopeMaxStages];
     __shared__ int s_gave_up;
@@ -81,6 +84,7 @@ __global__ void __launch_bounds__(256, 4) k_axes_rope_append(const AxesRope p, c
     constexpr int per = FORM == kRopePairs ? 8 : FORM == kRopeAdjacent ? 4 : 2;
     const int pieces = (p.half + per - 1) / per, room = 2 * pieces * per;
     float* turns = reinterpret_cast<float*>(rope_smem + p.stages * p.row_bytes);
+    double2* exact = reinterpret_cast<double2*>(rope_smem + (p.stages * p.row_bytes + 2 * room * 4 + 15) / 16 * 16);   // INT4: cosines and sines of two tokens
     auto slot = [&](int i) { return (i % per / 2 * pieces + i / per) * 4 + (i & 1); };
     if (tid == 0) {
         for (int i = 0; i < p.stages; ++i) mbar_init(&full[i], 1);
@@ -100,21 +104,33 @@ __global__ void __launch_bounds__(256, 4) k_axes_rope_append(const AxesRope p, c
         for (int i = 0; i < p.stages; ++i) fetch(i);
     // this thread's first frequency; further ones are looked up again
     const int ax = tid < p.half ? p.axis[tid] : -1, my_slot = slot(tid);
-    const double freq = tid < p.half ? p.inv_freq[tid] * 0.15915494309189533577 : 0.0;
+    constexpr double kTurn = INT4 ? 1.0 : 0.15915494309189533577;
+    const double freq = tid < p.half ? p.inv_freq[tid] * kTurn : 0.0;
     auto pos_of = [&](int axis, int t) { return (unsigned)axis < (unsigned)p.axes && t < p.rows ? p.pos[(size_t)axis * p.ld_pos + t] : 0; };
-    auto angle = [&](float* to, int pos, double f) {
+    auto angle = [&](int b, int i, int at, int pos, double f) {
+        float* to = turns + b * room + at;
         const double x = (double)pos * f;
-        float sn, cs;
-        sincospif(2.0f * (float)(x - rint(x)), &sn, &cs);
-        to[0] = cs * p.mscale, to[2] = sn * p.mscale;
+        if constexpr (INT4) {
+            // x less whole turns, 2 pi in two parts (Cody and Waite 1980): the products are not rounded, what is left is within 2^-53 of its size
+            const double n = rint(x * 0.15915494309189533577);
+            double sn, cs;
+            sincos(fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586477, x)), &sn, &cs);
+            sn *= (double)p.mscale, cs *= (double)p.mscale;
+            exact[b * p.half + i] = make_double2(cs, sn);
+            to[0] = (float)cs, to[2] = (float)sn;
+        } else {
+            float sn, cs;
+            sincospif(2.0f * (float)(x - rint(x)), &sn, &cs);
+            to[0] = cs * p.mscale, to[2] = sn * p.mscale;
+        }
     };
-    auto angles = [&](float* turn, int t, int pos) {
-        if (tid < p.half) angle(turn + my_slot, pos, freq);
+    auto angles = [&](int b, int t, int pos) {
+        if (tid < p.half) angle(b, tid, my_slot, pos, freq);
         if (t < p.rows)
-            for (int i = tid + threads; i < p.half; i += threads) angle(turn + slot(i), pos_of(p.axis[i], t), p.inv_freq[i] * 0.15915494309189533577);
+            for (int i = tid + threads; i < p.half; i += threads) angle(b, i, slot(i), pos_of(p.axis[i], t), p.inv_freq[i] * kTurn);
     };
     int t = blockIdx.x, pos = pos_of(ax, t + step), seq = p.token_seq[t], pl = p.placement[t];
-    angles(turns, t, pos_of(ax, t));
+    angles(0, t, pos_of(ax, t));
     __syncthreads();
     bool ok = true;
     for (int i = 0; t < p.rows; ++i, t += step) {
@@ -130,9 +146,22 @@ __global__ void __launch_bounds__(256, 4) k_axes_rope_append(const AxesRope p, c
         }
         ok = ok && tc2_wait1(&full[s], (uint32_t)(i / p.stages) & 1u, s_abort, err, 0x6100 + s);
         if (ok) {
+            const int turned = INT4 ? p.heads : p.heads + p.kv_heads;
+            if constexpr (INT4) {   // a pair of a key a thread
+                const double2* w = exact + (i & 1) * p.half;
+                const int second = FORM == kRopeAdjacent ? 1 : p.half, each = FORM == kRopeAdjacent ? 2 : 1;
+                for (int it = tid; it < p.kv_heads * p.half; it += threads) {
+                    const int head = it / p.half, k = it - head * p.half;
+                    T* x = reinterpret_cast<T*>(row) + (p.heads + head) * p.dim + k * each;
+                    const double2 cs = w[k];
+                    const double f = (double)to_f32<T>(x[0]), g = (double)to_f32<T>(x[second]);
+                    x[0] = from_f32<T>((float)(f * cs.x - g * cs.y));
+                    x[second] = from_f32<T>((float)(g * cs.x + f * cs.y));
+                }
+            }
             if constexpr (FORM == kRopePairs) {
                 const int h8 = p.half >> 3, d8 = p.dim >> 3;
-                for (int it = tid; it < (p.heads + p.kv_heads) * h8; it += threads) {
+                for (int it = tid; it < turned * h8; it += threads) {
                     const int head = it / h8, at = it - head * h8;
                     uint4* x = reinterpret_cast<uint4*>(row) + head * d8 + at;
                     const uint4 a = x[0], b = x[h8];
@@ -149,7 +178,7 @@ __global__ void __launch_bounds__(256, 4) k_axes_rope_append(const AxesRope p, c
                 }
             } else if constexpr (FORM == kRopeAdjacent) {
                 const int d8 = p.dim >> 3;
-                for (int it = tid; it < (p.heads + p.kv_heads) * pieces; it += threads) {
+                for (int it = tid; it < turned * pieces; it += threads) {
                     const int head = it / pieces, at = it - head * pieces;
                     uint4* x = reinterpret_cast<uint4*>(row) + head * d8 + at;
                     const uint4 a = x[0];
@@ -173,7 +202,7 @@ __global__ void __launch_bounds__(256, 4) k_axes_rope_append(const AxesRope p, c
                 }
             } else {
                 const float* w = reinterpret_cast<const float*>(w4);
-                for (int it = tid; it < (p.heads + p.kv_heads) * p.half; it += threads) {
+                for (int it = tid; it < turned * p.half; it += threads) {
                     const int head = it / p.half, k = it - head * p.half;
                     T* x = reinterpret_cast<T*>(row) + head * p.dim + k;
                     const float cs = w[k / 2 * 4 + (k & 1)], sn = w[k / 2 * 4 + 2 + (k & 1)], f = to_f32<T>(x[0]), g = to_f32<T>(x[p.half]);
@@ -182,7 +211,7 @@ __global__ void __launch_bounds__(256, 4) k_axes_rope_append(const AxesRope p, c
                 }
             }
         }
-        angles(turns + ((i + 1) & 1) * room, t + step, pos);   // the readers of that half are a barrier behind
+        angles((i + 1) & 1, t + step, pos);   // the readers of that half are a barrier behind
         pos = pos_of(ax, t + 2 * step);
         pa_fence_async();
         __syncthreads();
@@ -256,15 +285,15 @@ static int axes_rope_append(const void* qkv, long long ldq, const int32_t* pos, 
                             int layout, float mscale, const int32_t* token_seq, const int32_t* placement, const PagedCache& c, void* q_out, int T, int heads,
                             int kv_heads, int dim, int dtype, bool pdl, zl_stream_t stream) {
     const int form = layout == ZL_ROT_ADJACENT ? kRopeAdjacent : half % 8 == 0 ? kRopePairs : kRopeAny;
-    // a thread for every two pieces to turn; as many CTAs as the SMs hold threads of 64 registers, and rows in shared memory
-    const int row_bytes = (heads + 2 * kv_heads) * dim * 2, turns = 2 * 8 * (half + 7);
+    // a thread for every two pieces to turn; as many CTAs as the SMs hold threads and rows in shared memory
+    const int row_bytes = (heads + 2 * kv_heads) * dim * 2, turns = 2 * 8 * (half + 7) + (INT4 ? 16 + 2 * 16 * half : 0);
     const int items = (heads + kv_heads) * (form == kRopePairs ? half / 8 : form == kRopeAdjacent ? (half + 3) / 4 : half), two = cdiv(items, 2 * 32) * 32;
     const int threads = two < 64 ? 64 : two < 256 ? two : 256;
     int stages = kRopeMaxStages;
     while (stages > (INT4 ? 2 : 1) && stages * row_bytes + turns > kRopeSmem) --stages;
     const int smem = stages * row_bytes + turns;
     ZL_CHECK_SUPPORTED(smem <= kRopeSmem);
-    const int by_smem = kSmSmem / (smem + kCtaSmem + 256), by_threads = 1024 / threads, most = device_sm_count() * (by_smem < by_threads ? by_smem : by_threads);
+    const int by_smem = kSmSmem / (smem + kCtaSmem + 256), by_threads = (INT4 ? kRopeThreads4 : kRopeThreads) / threads, most = device_sm_count() * (by_smem < by_threads ? by_smem : by_threads);
     const AxesRope p = {qkv, q_out, pos, axis, token_seq, placement, inv_freq, ldq, ld_pos, axes, half, heads, kv_heads, dim, mscale, T, stages, row_bytes};
     if (dtype == ZL_F16) return form == kRopePairs ? axes_rope<__half, kRopePairs, INT4>(p, c, T < most ? T : most, threads, smem, pdl, stream)
                                 : form == kRopeAdjacent ? axes_rope<__half, kRopeAdjacent, INT4>(p, c, T < most ? T : most, threads, smem, pdl, stream)

@@ -1185,7 +1185,7 @@ def qkv_axes_rope_append(qkv, pos, inv_freq, axis, token_seq, placement, page_ta
 
 def qkv_axes_rope_append_int4(qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout=ROT_HALVES, mscale=1.0, pdl=False):
     """qkv_axes_rope_append into caches of 4 bits: (pages, page_size, kv_heads, int4_row_bytes(dim)) uint8, dim 64 or 128, read by paged_attention_int4 and
-    int4_cache_values.  Keys, once turned and rounded to qkv's type, and values are held as 16 equal steps between the lowest and the highest of every 32
+    int4_cache_values.  Keys, turned in 64 bits and rounded to 32 and then to qkv's type, and values are held as 16 equal steps between the lowest and the highest of every 32
     columns: off by up to half a step, a 30th of that range; 32 columns with an infinity or NaN read as NaN.  Decoding is fastest where a page has the rows of
     a head one behind another: caches made as (pages, kv_heads, page_size, bytes) and passed with .transpose(1, 2).  -> q (T, heads * dim)."""
     if _lib.host is not None:
