@@ -60,11 +60,7 @@ static int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool p
     ZL_CHECK_CUDA(allow_smem(k_paged_attn_tiles<T, D>, PtCfg<D>::kBytes, done));
     const CUtensorMapDataType dt = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     CUtensorMap maps[3] = {};
-    {   // Q: 64 columns of the heads of a group, whole tokens of a tile
-        const uint64_t dims[3] = {(uint64_t)D, (uint64_t)p.heads, (uint64_t)p.rows}, strides[2] = {D * 2, (uint64_t)p.heads * D * 2};
-        const uint32_t rows[3] = {64, (uint32_t)p.group, (uint32_t)(p.tile_rows / p.group)};
-        ZL_CHECK_CUDA(tc_make_map_nd(&maps[0], p.q, dt, 3, dims, strides, rows, CU_TENSOR_MAP_SWIZZLE_128B) ? cudaSuccess : cudaErrorInvalidValue);
-    }
+    ZL_CHECK_CUDA(pt_q_map<D>(&maps[0], p, dt) ? cudaSuccess : cudaErrorInvalidValue);
     // boxes of K and V: the rows that a tile and a page have in common wherever they meet
     int box = 1;
     while (box < kPtHalf && c.page_size % (2 * box) == 0) box *= 2;
@@ -77,7 +73,7 @@ static int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool p
         for (int i = 0; i < 2; ++i)
             if (!tc_make_map_nd(&maps[1 + i], i ? c.v : c.k, dt, 4, dims, strides, rows, CU_TENSOR_MAP_SWIZZLE_128B)) box = 0;
     }
-    ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D>, dim3(ctas), dim3(kPtThreads), PtCfg<D>::kBytes, stream, pdl, p, c, maps[0], maps[1], maps[2], box,
+    ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D>, dim3(ctas), dim3(kPtThreads<false>), PtCfg<D>::kBytes, stream, pdl, p, c, maps[0], maps[1], maps[2], box,
                          words + kWaitAttnPaged));
     if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join_tiles<T, D>, dim3(ctas, kPtRows / 32), dim3(256), 0, stream, true, p));
     return ZL_OK;

@@ -1,28 +1,35 @@
 // Attention of the new tokens of every sequence over pages of 4 bits (int4_cache.cuh): what paged_attn.cu does over pages of 16.
 #include "paged_attn4_few.cuh"
+#include "paged_attn_tc.cuh"
 
 #include <climits>
 
 namespace zl {
 
+// Calls whose sequences bring at most so many (token, head) rows of a kv head each go to the kernel for few rows, as do groups that no tile holds a token of.
+constexpr int kFewRows4 = 16;
+
 struct Paged4Plan {
-    int ctas, block_rows;
+    bool tiles;                     // on the 5th-generation tensor cores
+    int ctas, block_rows, tile_rows;
     size_t ml, part, cuts, bytes;   // what lies where in the workspace
 };
 
 template <int D>
-static int paged4_most_ctas(bool eight) { return device_sm_count() * (eight ? P4Cfg<D, 1>::kPerSm : P4Cfg<D, 2>::kPerSm); }
+static int paged4_few_ctas(bool eight) { return device_sm_count() * (eight ? P4Cfg<D, 1>::kPerSm : P4Cfg<D, 2>::kPerSm); }
 
 static Paged4Plan paged4_plan(int rows, int max_new, int seqs, int max_keys, int heads, int kv_heads, int dim) {
     Paged4Plan s = {};
     const int group = heads / kv_heads;
     const long long all = (long long)rows * group, most = (long long)max_new * group;
-    s.block_rows = most <= 8 ? 8 : 16;
+    s.tiles = most > kFewRows4 && group <= kPaRows;
+    s.tile_rows = s.tiles ? kPaRows / group * group : 0;
+    s.block_rows = s.tiles ? 2 * s.tile_rows : most <= 8 ? 8 : 16;
     // no more CTAs than the line can be long: every sequence adds less than one block to those of the rows, each of all the keys there is room for
-    const long long units = (all / s.block_rows + seqs) * (P4Kind::kSetup + cdiv(max_keys, kP4Keys)) * kv_heads;
-    const int most_ctas = dim == 64 ? paged4_most_ctas<64>(s.block_rows == 8) : paged4_most_ctas<128>(s.block_rows == 8);
+    const long long units = (all / s.block_rows + seqs) * (s.tiles ? PtKind::kSetup + cdiv(max_keys, kPtKeys) : P4Kind::kSetup + cdiv(max_keys, kP4Keys)) * kv_heads;
+    const int most_ctas = s.tiles ? device_sm_count() : dim == 64 ? paged4_few_ctas<64>(s.block_rows == 8) : paged4_few_ctas<128>(s.block_rows == 8);
     s.ctas = (int)(units < most_ctas ? units : most_ctas);
-    const size_t parts = (size_t)s.ctas * 2 * s.block_rows;
+    const size_t parts = (size_t)s.ctas * 2 * (s.tiles ? kPtRows : s.block_rows);
     auto take = [&](size_t bytes) {
         const size_t at = s.bytes;
         s.bytes += (bytes + 255) / 256 * 256;
@@ -43,7 +50,24 @@ static int paged4_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pd
 }
 
 template <typename T, int D>
+static int paged4_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool pdl, zl_stream_t stream) {
+    using C = PtCfg<D, true>;
+    static bool done[64] = {};
+    ZL_CHECK_WAITS();
+    unsigned* words = wait_words();
+    ZL_CHECK_CUDA(words ? cudaSuccess : cudaErrorMemoryAllocation);
+    ZL_CHECK_CUDA(allow_smem(k_paged_attn_tiles<T, D, true>, C::kBytes, done));
+    CUtensorMap q_map = {};
+    const CUtensorMapDataType dt = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    ZL_CHECK_CUDA(pt_q_map<D>(&q_map, p, dt) ? cudaSuccess : cudaErrorInvalidValue);
+    ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D, true>, dim3(ctas), dim3(kPtThreads<true>), C::kBytes, stream, pdl, p, c, q_map, q_map, q_map, 0, words + kWaitAttnPaged));
+    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join_tiles<T, D>, dim3(ctas, kPtRows / 32), dim3(256), 0, stream, true, p));
+    return ZL_OK;
+}
+
+template <typename T, int D>
 static int paged4(const PagedAttn& p, const PagedCache& c, const Paged4Plan& s, bool pdl, zl_stream_t stream) {
+    if (s.tiles) return paged4_tiles<T, D>(p, c, s.ctas, pdl, stream);
     return s.block_rows == 8 ? paged4_few<T, D, 1>(p, c, s.ctas, pdl, stream) : paged4_few<T, D, 2>(p, c, s.ctas, pdl, stream);
 }
 
@@ -70,13 +94,13 @@ extern "C" int zl_paged_attention_int4(const void* q, const void* k_cache, const
     const long long room = (long long)max_pages * page_size;
     const Paged4Plan s = paged4_plan(rows, max_new, seqs, (int)(room < INT_MAX - 255 ? room : INT_MAX - 255), heads, kv_heads, dim);
     // the kernels count tiles in 32 bits
-    ZL_CHECK_SUPPORTED(((long long)rows * (heads / kv_heads) / s.block_rows + seqs) * (room / kP4Keys + 2 + P4Kind::kSetup) < (INT_MAX - (1 << 16)) / kv_heads);
+    ZL_CHECK_SUPPORTED(((long long)rows * (heads / kv_heads) / (s.tiles ? kPaRows / 2 : s.block_rows) + seqs) * (room / kP4Keys + 2 + P4Kind::kSetup) < (INT_MAX - (1 << 16)) / kv_heads);
     ZL_CHECK_ARG(workspace && workspace_bytes >= s.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
     const PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), num_pages, page_stride, row_stride, head_stride, page_table, ld_table, max_pages,
                           page_size, seqs, paged_divisor(page_size)};
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     const PagedAttn p = {q, out, seq_lens, q_starts, rows, heads, heads / kv_heads, window, paged_divisor(heads / kv_heads), scale * 1.4426950408889634f, kv_heads,
-                         s.block_rows, 0, reinterpret_cast<float2*>(ws + s.ml), reinterpret_cast<float*>(ws + s.part), reinterpret_cast<PagedCut*>(ws + s.cuts)};
+                         s.block_rows, s.tile_rows, reinterpret_cast<float2*>(ws + s.ml), reinterpret_cast<float*>(ws + s.part), reinterpret_cast<PagedCut*>(ws + s.cuts)};
     if (dtype == ZL_F16) return dim == 64 ? paged4<__half, 64>(p, c, s, pdl != 0, stream) : paged4<__half, 128>(p, c, s, pdl != 0, stream);
     return dim == 64 ? paged4<__nv_bfloat16, 64>(p, c, s, pdl != 0, stream) : paged4<__nv_bfloat16, 128>(p, c, s, pdl != 0, stream);
 }

@@ -31,13 +31,19 @@
 // and the product of such tiles by the softmax's threads 69 / 78 / 394; by warp 9 before its products 73 / 80 / 404; by the loaders, once a tile has landed, 77 / 81 / 406.
 #pragma once
 #include "attn_ptx.cuh"
+#include "int4_cache.cuh"
 #include "paged_attn.cuh"
 
 #include <type_traits>
 
 namespace zl {
 
-constexpr int kPtRows = 256, kPtKeys = 128, kPtHalf = 64, kPtThreads = 384, kPtWarpS = 8, kPtWarpO = 9, kPtWarpLoad = 10, kPtLoaders = 64;
+constexpr int kPtRows = 256, kPtKeys = 128, kPtHalf = 64, kPtWarpS = 8, kPtWarpO = 9, kPtWarpLoad = 10, kPtLoaders = 64;
+// Of a cache of 4 bits: four warps make its codes numbers of T on the way into the ring, 16 rows of every tile each, with a ring of their own for the codes (all four in every
+// tile: a warp that passed over some could take one phase of their barriers for another).  Warp 10 has Q alone, 11 nothing: registers are given out for 16 warps.
+constexpr int kPtWarpLoad4 = 12;
+template <bool INT4>
+constexpr int kPtThreads = INT4 ? 512 : 384;
 
 // The exponent of a probability is a score times the scale less the reference, in one fused step that does not round the product, where the reference is
 // one that was rounded: all exponents of a row are off by what that left, half a step of 32-bit numbers of its size.  That cancels in the quotient, but from here on
@@ -82,13 +88,16 @@ struct PtKind {
     }
 };
 
-template <int D>
+template <int D, bool INT4 = false>
 struct PtCfg {
     static constexpr int kAtoms = D / 64;
     static constexpr int kQ = kAtoms * kPaRows * 128;       // a tile of Q: [64 of d][128 rows][128 B]
     static constexpr int kTile = kAtoms * kPtHalf * 128;    // K or V: [64 of d][64 keys][128 B]
-    static constexpr int kRing = D == 128 ? 10 : 16;
-    static constexpr int kRingOff = 2 * kQ, kBytes = kRingOff + kRing * kTile + 1024;   // + slack for the manual 1024-byte alignment
+    static constexpr int kRing = D == 64 ? 16 : INT4 ? 8 : 10;
+    static constexpr int kRaw = D == 64 ? 8 : 6;            // units of codes that a warp of four has room for
+    static constexpr int kUnit = 16 * (D / 8 * 5);          // 16 rows of codes and pairs
+    static constexpr int kRingOff = 2 * kQ, kRawOff = kRingOff + kRing * kTile;
+    static constexpr int kBytes = kRawOff + (INT4 ? 4 * kRaw * kUnit : 0) + 1024;   // + slack for the manual 1024-byte alignment
     static_assert(tmem_alone(kBytes) && kBytes + 1024 <= 227 * 1024, "all of tensor memory, an SM to itself");
     static_assert(2 * kQ >= kPaRows * D * 4, "the second result of a row, where Q was");
     static constexpr int kO = 256;                          // TMEM columns: scores 0, 128; outputs from here
@@ -168,12 +177,46 @@ __device__ __noinline__ void pt_add_broken(const PagedCache& c, int seq, long lo
     }
 }
 
-// grid: CTAs that share the line.  box: rows of a TMA box of K and V, 0: no TMA
+// The same for a cache of 4 bits, whose values are none where their group's pair is none: a lane looks at the pairs of a key at a time.
 template <typename T, int D>
-__global__ void __launch_bounds__(kPtThreads, 1)
+__device__ __noinline__ void pt_add_broken4(const PagedCache& c, int seq, long long head, uint32_t ob, int lo, int hi, int first, int last, int from, int to, int step) {
+    const int lane = threadIdx.x & 31;
+    for (int key0 = first; key0 <= last; key0 += 32) {
+        if (key0 >= from && key0 + 31 <= to) {
+            key0 = to - 31;
+            continue;
+        }
+        const int mine = key0 + lane;
+        const long long at = mine <= last && (mine < from || mine > to) && (mine - first) / kPtKeys % step == 0 ? c.row_at(seq, mine) : -1;
+        const uint8_t* pairs = static_cast<const uint8_t*>(c.v) + head + D / 2;
+        bool whole = true;
+        if (at >= 0)
+#pragma unroll
+            for (int g = 0; g < D / kInt4Group; ++g) whole = whole && int4_finite<T>(*reinterpret_cast<const uint32_t*>(pairs + at + g * 4));
+        for (unsigned left = __ballot_sync(0xffffffffu, !whole); left; left &= left - 1) {
+            const int key = key0 + __ffs(left) - 1;
+            const long long row = __shfl_sync(0xffffffffu, at, key - key0);
+#pragma unroll 1
+            for (int d0 = 0; d0 < D; d0 += 16) {
+                if (int4_finite<T>(*reinterpret_cast<const uint32_t*>(pairs + row + d0 / kInt4Group * 4))) continue;
+                float o[16];
+                tc_ld16(ob + (uint32_t)d0, o);
+                uint32_t r[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(key >= lo && key <= hi ? __int_as_float(0x7fffffff) : o[i]);
+                tc_st16(ob + (uint32_t)d0, r);
+                tc_wait_st();
+            }
+        }
+    }
+}
+
+// grid: CTAs that share the line.  box: rows of a TMA box of K and V, 0: no TMA.  INT4: k_map and v_map are not looked at
+template <typename T, int D, bool INT4 = false>
+__global__ void __launch_bounds__(kPtThreads<INT4>, 1)
 k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                    const __grid_constant__ CUtensorMap v_map, int box, unsigned* err) {
-    using C = PtCfg<D>;
+    using C = PtCfg<D, INT4>;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     constexpr int CH = D / 8;
     extern __shared__ uint8_t pt_smem[];
@@ -186,7 +229,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     volatile int *s_abort = &s_gave_up, *s_broken = s_blocks;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], box ? 1 : kPtLoaders), mbar_init(&empty[i], 1);
+        for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], INT4 ? kPtHalf / 16 : box ? 1 : kPtLoaders), mbar_init(&empty[i], 1);
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i >> 1][i & 1], 1), mbar_init(&p_full[i >> 1][i & 1], 4), mbar_init(&o_done[i >> 1][i & 1], 1);
         mbar_init(&q_full, 1), mbar_init(&q_free, 1), mbar_init(&o_free, 8), mbar_init(&joined, 4);
         s_gave_up = s_blocks[0] = s_blocks[1] = 0;
@@ -336,7 +379,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             tc_fence_after();
             // noted before the tile's probabilities were handed on, whose product has ended
             if (__any_sync(0xffffffffu, s_broken[blocks & 1] == blocks + 1))
-                pt_add_broken<T, D>(c, k.seq, (long long)at.hk * c.head_stride, to, lo, hi, key0, min(t0 * kPtKeys + count * step - 1, k.hi), all_lo, all_hi, step / kPtKeys);
+                (INT4 ? pt_add_broken4<T, D> : pt_add_broken<T, D>)(c, k.seq, (long long)at.hk * c.head_stride, to, lo, hi, key0, min(t0 * kPtKeys + count * step - 1, k.hi), all_lo, all_hi, step / kPtKeys);
             if (!walk.whole(count)) {
                 // A part: {maximum, sum}, then the output as it stands, column by column: the lanes of a warp are neighbours there.
                 const size_t part = (size_t)blockIdx.x * 2 + (first > 0 ? 0 : 1);
@@ -425,7 +468,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                         const int it = ring + j * items + (two_rows ? 0 : m), slot = it % C::kRing;
                         if (m == 0 || !two_rows) {
                             ok = ok && tc2_wait1(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5100 + slot);
-                            if (!box) pa_fence_async();
+                            if (!INT4 && !box) pa_fence_async();
                         }
                         if (turn + (j >> 1) > 0) ok = ok && tc2_wait1(&o_done[m][j & 1], (uint32_t)(turn + (j >> 1) - 1) & 1u, s_abort, err, 0x5400 + m);
                         if (!ok) break;
@@ -452,7 +495,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                         const int it = ring + j * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
                         if (m == 0 || !two_rows) {
                             ok = ok && tc2_wait1(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5200 + slot);
-                            if (!box) pa_fence_async();
+                            if (!INT4 && !box) pa_fence_async();
                         }
                         ok = ok && tc2_wait1(&p_full[m][j & 1], (uint32_t)(turn + (j >> 1)) & 1u, s_abort, err, 0x5300 + m);
                         if (!ok) break;
@@ -487,7 +530,83 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 }
                 __syncwarp();
             };
-            if (box) {
+            if constexpr (INT4) {
+                // Codes and pairs of a warp's 16 rows come by 80 copies of D / 8 bytes, kRaw - 1 tiles ahead.  Then lane = row, half of the warp a group of 32 columns each:
+                // reads of eight rows touch all banks once, and so do writes of 16 bytes of eight rows to the tile.
+                constexpr int kChunk = D / 8;
+                if (warp == kPtWarpLoad) load_q();
+                if (warp >= kPtWarpLoad4) {
+                    const int rg = warp - kPtWarpLoad4, tiles = 2 * count * items;
+                    const bool one_page = c.page_size % 16 == 0;
+                    const long long head = (long long)at.hk * c.head_stride;
+                    uint8_t* raw = smem + C::kRawOff + rg * (C::kRaw * C::kUnit);
+                    const uint32_t raw_at = smem_u32(raw);
+                    auto first_row = [&](int i) { return row_of(i) + rg * 16; };
+                    auto find = [&](int i) {
+                        const int row = first_row(i) + (lane & 15), pg = c.by_page(row);
+                        return i < tiles && row <= k.hi && pg < c.max_pages ? c.table[(size_t)k.seq * c.ld_table + pg] : -1;
+                    };
+                    auto copy = [&](int i, int id) {
+                        const int row0 = first_row(i), r_mine = row0 + (one_page ? 0 : lane & 15);
+                        long long off = id >= 0 && id < c.num_pages ? (long long)id * c.page_stride + (long long)(r_mine - c.by_page(r_mine) * c.page_size) * c.row_stride : -1;
+                        if (one_page) off = __shfl_sync(0xffffffffu, off, 0);
+                        const uint8_t* base = static_cast<const uint8_t*>((two_rows ? i & 1 : i & 2) ? c.v : c.k) + head;
+                        const uint32_t to = raw_at + (uint32_t)(i % C::kRaw) * C::kUnit;
+#pragma unroll
+                        for (int u = 0; u < 3; ++u) {
+                            const int x = lane + 32 * u, r = min(x / 5, 15), ch = x % 5;
+                            long long o = one_page ? off : __shfl_sync(0xffffffffu, off, r);
+                            const bool in = o >= 0 && row0 + r <= k.hi;
+                            if (one_page) o += r * c.row_stride;
+                            const uint8_t* src = in ? base + o + ch * kChunk : static_cast<const uint8_t*>(c.k);
+                            if (x < 80) {
+                                if constexpr (D == 128) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + x * kChunk), "l"(src), "r"(in ? 16 : 0) : "memory");
+                                else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to + x * kChunk), "l"(src), "r"(in ? 8 : 0) : "memory");
+                            }
+                        }
+                    };
+                    int id = find(0);
+#pragma unroll 1
+                    for (int i = 0; i < C::kRaw - 1; ++i) {
+                        const int next = find(i + 1);
+                        if (i < tiles) copy(i, id);
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        id = next;
+                    }
+                    for (int i = 0; i < tiles; ++i) {
+                        const int it = ring + i, slot = it % C::kRing;
+                        asm volatile("cp.async.wait_group %0;" ::"n"(C::kRaw - 2) : "memory");
+                        __syncwarp();
+                        const int next = find(i + C::kRaw);
+                        if (i + C::kRaw - 1 < tiles) copy(i + C::kRaw - 1, id);
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        id = next;
+                        if (it >= C::kRing) ok = ok && tc2_wait(&empty[slot], (uint32_t)(it / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
+                        if (!ok) break;
+                        const uint8_t* from = raw + (i % C::kRaw) * C::kUnit + (lane & 15) * (5 * kChunk);
+                        const int row = rg * 16 + (lane & 15);
+#pragma unroll
+                        for (int g0 = 0; g0 < D / kInt4Group; g0 += 2) {
+                            const int g = g0 + (lane >> 4);
+                            uint32_t w[4], step, low;
+                            if constexpr (D == 128) {
+                                const uint4 x = *reinterpret_cast<const uint4*>(from + g * 16);
+                                w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+                            } else {
+                                const uint2 x = *reinterpret_cast<const uint2*>(from + g * 16), y = *reinterpret_cast<const uint2*>(from + g * 16 + 8);
+                                w[0] = x.x, w[1] = x.y, w[2] = y.x, w[3] = y.y;
+                            }
+                            int4_meta<T>(*reinterpret_cast<const uint32_t*>(from + D / 2 + g * 4), step, low);
+                            uint8_t* to = smem + C::kRingOff + slot * C::kTile + (g >> 1) * (kPtHalf * 128) + row * 128;
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) *reinterpret_cast<uint4*>(to + ((((g & 1) * 4 + x) ^ (row & 7)) << 4)) = int4_eight<T>(w[x], step, low);
+                        }
+                        pa_fence_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&full[slot]);
+                    }
+                }
+            } else if (box) {
                 // One warp for keys, one for values; a lane for each box of a tile, its rows and 64 columns.  The lanes hold the numbers of 32 pages in
                 // a row, which is a turn's keys at least.
                 const bool is_v = warp != kPtWarpLoad;
@@ -577,6 +696,14 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
     }
+}
+
+// Q: 64 columns of the heads of a group, whole tokens of a tile
+template <int D>
+inline bool pt_q_map(CUtensorMap* map, const PagedAttn& p, CUtensorMapDataType dt) {
+    const uint64_t dims[3] = {(uint64_t)D, (uint64_t)p.heads, (uint64_t)p.rows}, strides[2] = {D * 2, (uint64_t)p.heads * D * 2};
+    const uint32_t rows[3] = {64, (uint32_t)p.group, (uint32_t)(p.tile_rows / p.group)};
+    return tc_make_map_nd(map, p.q, dt, 3, dims, strides, rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Blocks that were cut: grid (the CTAs of k_paged_attn_tiles, groups of 32 rows), lane = row, a warp for D / 8 columns.  The first part of a block lies in its
