@@ -39,8 +39,8 @@
 namespace zl {
 
 constexpr int kPtRows = 256, kPtKeys = 128, kPtHalf = 64, kPtWarpS = 8, kPtWarpO = 9, kPtWarpLoad = 10, kPtLoaders = 64;
-// Of a cache of 4 bits: four warps make its codes numbers of T on the way into the ring, 16 rows of every tile each, with a ring of their own for the codes (all four in every
-// tile: a warp that passed over some could take one phase of their barriers for another).  Warp 10 has Q alone, 11 nothing: registers are given out for 16 warps.
+// Of a cache of 4 bits: warps 10 and 11 bring codes of keys and of values, a ring of tiles each, as they are; warps 12 to 15 make them numbers of T on the way into the ring
+// of tiles, 16 rows of every tile each (all four in every tile: a warp that passed over some could take one phase of their barriers for another).
 constexpr int kPtWarpLoad4 = 12;
 template <bool INT4>
 constexpr int kPtThreads = INT4 ? 512 : 384;
@@ -94,10 +94,10 @@ struct PtCfg {
     static constexpr int kQ = kAtoms * kPaRows * 128;       // a tile of Q: [64 of d][128 rows][128 B]
     static constexpr int kTile = kAtoms * kPtHalf * 128;    // K or V: [64 of d][64 keys][128 B]
     static constexpr int kRing = D == 64 ? 16 : INT4 ? 8 : 10;
-    static constexpr int kRaw = D == 64 ? 8 : 6;            // units of codes that a warp of four has room for
-    static constexpr int kUnit = 16 * (D / 8 * 5);          // 16 rows of codes and pairs
+    static constexpr int kRaw = D == 64 ? 6 : 3;            // tiles of codes, of keys and as many of values
+    static constexpr int kCodes = kPtHalf * (D / 8 * 5);    // a tile's codes and pairs
     static constexpr int kRingOff = 2 * kQ, kRawOff = kRingOff + kRing * kTile;
-    static constexpr int kBytes = kRawOff + (INT4 ? 4 * kRaw * kUnit : 0) + 1024;   // + slack for the manual 1024-byte alignment
+    static constexpr int kBytes = kRawOff + (INT4 ? 2 * kRaw * kCodes : 0) + 1024;   // + slack for the manual 1024-byte alignment
     static_assert(tmem_alone(kBytes) && kBytes + 1024 <= 227 * 1024, "all of tensor memory, an SM to itself");
     static_assert(2 * kQ >= kPaRows * D * 4, "the second result of a row, where Q was");
     static constexpr int kO = 256;                          // TMEM columns: scores 0, 128; outputs from here
@@ -222,6 +222,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     extern __shared__ uint8_t pt_smem[];
     uint8_t* smem = pt_smem + ((1024u - (smem_u32(pt_smem) & 1023u)) & 1023u);
     __shared__ uint64_t full[C::kRing], empty[C::kRing], s_full[2][2], p_full[2][2], o_done[2][2], q_full, q_free, o_free, joined;
+    __shared__ uint64_t raw_full[2][INT4 ? C::kRaw : 1], raw_empty[2][INT4 ? C::kRaw : 1];
     __shared__ float2 s_ml[kPaRows];
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up, s_blocks[2];
@@ -231,6 +232,8 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     if (tid == 0) {
         for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], INT4 ? kPtHalf / 16 : box ? 1 : kPtLoaders), mbar_init(&empty[i], 1);
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i >> 1][i & 1], 1), mbar_init(&p_full[i >> 1][i & 1], 4), mbar_init(&o_done[i >> 1][i & 1], 1);
+        if constexpr (INT4)
+            for (int i = 0; i < 2 * C::kRaw; ++i) mbar_init(&raw_full[i & 1][i >> 1], 32), mbar_init(&raw_empty[i & 1][i >> 1], 4);
         mbar_init(&q_full, 1), mbar_init(&q_free, 1), mbar_init(&o_free, 8), mbar_init(&joined, 4);
         s_gave_up = s_blocks[0] = s_blocks[1] = 0;
         mbar_fence_init();
@@ -248,7 +251,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     if (tid == 0) p.cuts[blockIdx.x].parts = 0;
     // Of the blocks before: how many, their turns, their tiles of the ring.  Every barrier's phases are waited for by each of its waiters without a gap, or a
     // later one cannot end before the waiter has gone on: a phase is told from its neighbours by its parity alone.
-    int blocks = 0, turn = 0, ring = 0;
+    int blocks = 0, turn = 0, ring = 0;   // ring / 2: of keys, and of values
     bool ok = true;           // no wait has given up
     PagedWalk<PtKind> walk;
     const PagedBlock& k = walk.k;
@@ -531,79 +534,85 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 __syncwarp();
             };
             if constexpr (INT4) {
-                // Codes and pairs of a warp's 16 rows come by 80 copies of D / 8 bytes, kRaw - 1 tiles ahead.  Then lane = row, half of the warp a group of 32 columns each:
-                // reads of eight rows touch all banks once, and so do writes of 16 bytes of eight rows to the tile.
-                constexpr int kChunk = D / 8;
-                if (warp == kPtWarpLoad) load_q();
-                if (warp >= kPtWarpLoad4) {
-                    const int rg = warp - kPtWarpLoad4, tiles = 2 * count * items;
-                    const bool one_page = c.page_size % 16 == 0;
-                    const long long head = (long long)at.hk * c.head_stride;
-                    uint8_t* raw = smem + C::kRawOff + rg * (C::kRaw * C::kUnit);
-                    const uint32_t raw_at = smem_u32(raw);
-                    auto first_row = [&](int i) { return row_of(i) + rg * 16; };
-                    auto find = [&](int i) {
-                        const int row = first_row(i) + (lane & 15), pg = c.by_page(row);
-                        return i < tiles && row <= k.hi && pg < c.max_pages ? c.table[(size_t)k.seq * c.ld_table + pg] : -1;
-                    };
-                    auto copy = [&](int i, int id) {
-                        const int row0 = first_row(i), r_mine = row0 + (one_page ? 0 : lane & 15);
-                        long long off = id >= 0 && id < c.num_pages ? (long long)id * c.page_stride + (long long)(r_mine - c.by_page(r_mine) * c.page_size) * c.row_stride : -1;
-                        if (one_page) off = __shfl_sync(0xffffffffu, off, 0);
-                        const uint8_t* base = static_cast<const uint8_t*>((two_rows ? i & 1 : i & 2) ? c.v : c.k) + head;
-                        const uint32_t to = raw_at + (uint32_t)(i % C::kRaw) * C::kUnit;
+                constexpr int kChunk = D / 8, kEach = 5 * kPtHalf / 32;
+                const int tiles = count * items;   // of keys, and as many of values
+                if (warp < kPtWarpLoad4) {
+                    // A lane looks up rows lane and lane + 32 of the tile, a tile ahead, and copies ten of its 320 chunks
+                    const int is_v = warp - kPtWarpLoad;
+                    const uint8_t* from = static_cast<const uint8_t*>(is_v ? c.v : c.k) + (long long)at.hk * c.head_stride;
+                    auto first_row = [&](int n) { return row_of(two_rows ? 2 * n + is_v : (n >> 1) * 4 + 2 * is_v + (n & 1)); };
+                    int ids[2];
+                    auto ask = [&](int n) {
 #pragma unroll
-                        for (int u = 0; u < 3; ++u) {
-                            const int x = lane + 32 * u, r = min(x / 5, 15), ch = x % 5;
-                            long long o = one_page ? off : __shfl_sync(0xffffffffu, off, r);
-                            const bool in = o >= 0 && row0 + r <= k.hi;
-                            if (one_page) o += r * c.row_stride;
-                            const uint8_t* src = in ? base + o + ch * kChunk : static_cast<const uint8_t*>(c.k);
-                            if (x < 80) {
-                                if constexpr (D == 128) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + x * kChunk), "l"(src), "r"(in ? 16 : 0) : "memory");
-                                else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to + x * kChunk), "l"(src), "r"(in ? 8 : 0) : "memory");
-                            }
+                        for (int u = 0; u < 2; ++u) {
+                            const int row = first_row(n) + u * 32 + lane, pg = c.by_page(row);
+                            ids[u] = n < tiles && row <= k.hi && pg < c.max_pages ? c.table[(size_t)k.seq * c.ld_table + pg] : -1;
                         }
                     };
-                    int id = find(0);
-#pragma unroll 1
-                    for (int i = 0; i < C::kRaw - 1; ++i) {
-                        const int next = find(i + 1);
-                        if (i < tiles) copy(i, id);
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        id = next;
-                    }
-                    for (int i = 0; i < tiles; ++i) {
-                        const int it = ring + i, slot = it % C::kRing;
-                        asm volatile("cp.async.wait_group %0;" ::"n"(C::kRaw - 2) : "memory");
-                        __syncwarp();
-                        const int next = find(i + C::kRaw);
-                        if (i + C::kRaw - 1 < tiles) copy(i + C::kRaw - 1, id);
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        id = next;
-                        if (it >= C::kRing) ok = ok && tc2_wait(&empty[slot], (uint32_t)(it / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
+                    ask(0);
+                    for (int n = 0; n < tiles && ok; ++n) {
+                        if (n == 1) load_q();
+                        const int it = ring / 2 + n, slot = it % C::kRaw;
+                        long long offs[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int row = first_row(n) + u * 32 + lane;
+                            offs[u] = ids[u] >= 0 && ids[u] < c.num_pages ? (long long)ids[u] * c.page_stride + (long long)(row - c.by_page(row) * c.page_size) * c.row_stride : -1;
+                        }
+                        ask(n + 1);
+                        if (it >= C::kRaw) ok = ok && pt_wait(&raw_empty[is_v][slot], (uint32_t)(it / C::kRaw - 1) & 1u, s_abort, err, 0x5a00 + is_v);
                         if (!ok) break;
-                        const uint8_t* from = raw + (i % C::kRaw) * C::kUnit + (lane & 15) * (5 * kChunk);
-                        const int row = rg * 16 + (lane & 15);
-#pragma unroll
-                        for (int g0 = 0; g0 < D / kInt4Group; g0 += 2) {
-                            const int g = g0 + (lane >> 4);
-                            uint32_t w[4], step, low;
-                            if constexpr (D == 128) {
-                                const uint4 x = *reinterpret_cast<const uint4*>(from + g * 16);
-                                w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-                            } else {
-                                const uint2 x = *reinterpret_cast<const uint2*>(from + g * 16), y = *reinterpret_cast<const uint2*>(from + g * 16 + 8);
-                                w[0] = x.x, w[1] = x.y, w[2] = y.x, w[3] = y.y;
-                            }
-                            int4_meta<T>(*reinterpret_cast<const uint32_t*>(from + D / 2 + g * 4), step, low);
-                            uint8_t* to = smem + C::kRingOff + slot * C::kTile + (g >> 1) * (kPtHalf * 128) + row * 128;
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) *reinterpret_cast<uint4*>(to + ((((g & 1) * 4 + x) ^ (row & 7)) << 4)) = int4_eight<T>(w[x], step, low);
+                        const uint32_t to = smem_u32(smem) + (uint32_t)(C::kRawOff + (is_v * C::kRaw + slot) * C::kCodes);
+#pragma unroll 1
+                        for (int u = 0; u < kEach; ++u) {
+                            const int x = lane + 32 * u, r = x / 5, ch = x - r * 5;
+                            const long long low = __shfl_sync(0xffffffffu, offs[0], r & 31), high = __shfl_sync(0xffffffffu, offs[1], r & 31), off = r < 32 ? low : high;
+                            const uint8_t* src = from + (off < 0 ? 0 : off + ch * kChunk);
+                            if constexpr (D == 128) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + x * kChunk), "l"(src), "r"(off < 0 ? 0 : 16) : "memory");
+                            else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to + x * kChunk), "l"(src), "r"(off < 0 ? 0 : 8) : "memory");
                         }
+                        pa_landed(&raw_full[is_v][slot]);
+                    }
+                } else {
+                    // Two tiles at a time: lane = row, half of the warp a group of 32 columns each.  Reads of eight rows touch all banks once, and so do writes of 16 bytes of
+                    // eight rows.  One fence for both: it waits for the writes.
+                    const int rg = warp - kPtWarpLoad4, row = rg * 16 + (lane & 15);
+                    // Loops that are not unrolled: the warps' instructions come from one small cache, and what is large here stops the softmax's (unrolled, 442 us where this took 360).
+                    for (int x = 0; x < tiles && ok; ++x) {
+                        const int is_v = two_rows ? 0 : x & 1, n = ring / 2 + (two_rows ? x : (x >> 1) * 2), i = ring + 2 * x;   // of the first of the two
+#pragma unroll 1
+                        for (int t = 0; t < 2; ++t) {
+                            const int v = two_rows ? t : is_v, it = two_rows ? n : n + t, raw = it % C::kRaw, slot = (i + t) % C::kRing;
+                            ok = ok && pt_wait(&raw_full[v][raw], (uint32_t)(it / C::kRaw) & 1u, s_abort, err, 0x5b00 + v);
+                            if (i + t >= C::kRing) ok = ok && pt_wait(&empty[slot], (uint32_t)((i + t) / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
+                            if (!ok) break;
+                            const uint8_t* from = smem + C::kRawOff + (v * C::kRaw + raw) * C::kCodes + row * (5 * kChunk);
+                            uint8_t* to = smem + C::kRingOff + slot * C::kTile + row * 128;
+#pragma unroll 1
+                            for (int u = 0; u < D / 64; ++u) {
+                                const int g = 2 * u + (lane >> 4);
+                                uint32_t w[4], step, low;
+                                if constexpr (D == 128) {
+                                    const uint4 y = *reinterpret_cast<const uint4*>(from + g * 16);
+                                    w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
+                                } else {
+                                    const uint2 y = *reinterpret_cast<const uint2*>(from + g * 16), z = *reinterpret_cast<const uint2*>(from + g * 16 + 8);
+                                    w[0] = y.x, w[1] = y.y, w[2] = z.x, w[3] = z.y;
+                                }
+                                int4_meta<T>(*reinterpret_cast<const uint32_t*>(from + D / 2 + g * 4), step, low);
+#pragma unroll
+                                for (int y = 0; y < 4; ++y)
+                                    *reinterpret_cast<uint4*>(to + u * (kPtHalf * 128) + ((((lane >> 4) * 4 + y) ^ (row & 7)) << 4)) = int4_eight<T>(w[y], step, low);
+                            }
+                        }
+                        if (!ok) break;
                         pa_fence_async();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&full[slot]);
+                        if (lane == 0) {
+#pragma unroll
+                            for (int t = 0; t < 2; ++t)
+                                mbar_arrive(&raw_empty[two_rows ? t : is_v][(two_rows ? n : n + t) % C::kRaw]), mbar_arrive(&full[(i + t) % C::kRing]);
+                        }
                     }
                 }
             } else if (box) {
