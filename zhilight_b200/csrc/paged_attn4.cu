@@ -39,12 +39,31 @@ static Paged4Plan paged4_plan(int rows, int max_new, int seqs, int max_keys, int
     return s;
 }
 
+// Boxes of 16 rows of K and of V, as words of 32 bits: whole rows of 80 bytes, or (rows of 40, which are no multiple of 16) what 16 rows hold where those lie behind one another
+template <int D>
+static bool p4_maps(CUtensorMap (&maps)[2], const PagedAttn& p, const PagedCache& c) {
+    constexpr int kRow = int4_row_bytes(D);
+    if (D == 64 && c.row_stride != kRow && c.page_size > 1) return false;
+    auto step = [](long long bytes, bool more) { return more ? (uint64_t)bytes : 16u; };   // of one alone none is taken
+    const uint64_t dims[4] = {(uint64_t)(D == 128 ? kRow / 4 : c.page_size * (kRow / 4)), (uint64_t)(D == 128 ? c.page_size : 1), (uint64_t)p.kv_heads, (uint64_t)c.num_pages};
+    const uint64_t strides[3] = {step(c.row_stride, D == 128 && c.page_size > 1), step(c.head_stride, p.kv_heads > 1), step(c.page_stride, c.num_pages > 1)};
+    const uint32_t box[4] = {D == 128 ? kRow / 4 : 16 * (kRow / 4), D == 128 ? 16 : 1, 1, 1};
+    for (int i = 0; i < 2; ++i)
+        if (!tc_make_map_nd(&maps[i], i ? c.v : c.k, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return false;
+    return true;
+}
+
 template <typename T, int D, int NT>
 static int paged4_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pdl, zl_stream_t stream) {
     using C = P4Cfg<D, NT>;
     static bool done[64] = {};
+    ZL_CHECK_WAITS();
+    unsigned* words = wait_words();
+    ZL_CHECK_CUDA(words ? cudaSuccess : cudaErrorMemoryAllocation);
     ZL_CHECK_CUDA(allow_smem(k_paged_attn4_few<T, D, NT>, C::kBytes, done));
-    ZL_CHECK_CUDA(launch(k_paged_attn4_few<T, D, NT>, dim3(ctas), dim3(kP4Warps * 32), C::kBytes, stream, pdl, p, c));
+    CUtensorMap maps[2] = {};
+    const int tma = c.page_size % 16 == 0 && p4_maps<D>(maps, p, c);
+    ZL_CHECK_CUDA(launch(k_paged_attn4_few<T, D, NT>, dim3(ctas), dim3(kP4Warps * 32), C::kBytes, stream, pdl, p, c, maps[0], maps[1], tma, words + kWaitAttnPaged));
     if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 8 * NT>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p));
     return ZL_OK;
 }

@@ -1,7 +1,7 @@
 // Attention of few (token, head) rows of a kv head over pages of 4 bits (int4_cache.cuh).  Work is shared out as in paged_attn_few.cuh: tiles of 64 keys of all
 // blocks stand in one line, a CTA takes an equal stretch, a warp has 16 keys of a tile and a ring of its own.
 //
-// What 4 bits take off the memory they put on the instructions: a key and its value are 160 bytes instead of 512, and every code costs two to three of them.
+// What 4 bits take off the memory they put on the instructions: a key and its value are 160 bytes instead of 512, and every code costs more than one of them.
 // So the products are turned around, S^T = K Q^T and O^T += V^T P^T by mma.sync with the keys' and values' 16 rows as the first operand and 8 rows of queries as the
 // second: blocks of 8 rows (one token of a group of 8, two of 4) take half the products, exponentials and registers that 16 rows would.
 //   K: columns may be summed in any order as long as Q's are in the same one, so lane (g, t) takes a quarter of the columns of keys g and g + 8 in one piece,
@@ -10,9 +10,13 @@
 //      that this costs an eighth of an instruction a value.  Output columns may lie anywhere: lane g takes D / 8 neighbouring ones.
 //   P: the scores' accumulators, rounded to 16 bits, are the second operand once 8 x 8 of them are transposed (movmatrix).
 // Probabilities are rounded to the rows' type once (half a step each, of random sign: beside the output's own rounding), sums are in 32 bits.
+//
+// Codes of bf16 rows become numbers by one `and` and one fma for two (P4Codes).  16 rows of a head come by one TMA box where a page holds whole 16s of them and its map can be made
+// (heads of 128; heads of 64 where the rows of a head lie behind one another), else by copies of D / 8 bytes.
 #pragma once
 #include "int4_cache.cuh"
 #include "paged_attn_few.cuh"
+#include "paged_attn_tc.cuh"
 
 namespace zl {
 
@@ -20,14 +24,55 @@ constexpr int kP4Warps = 4, kP4Keys = 16 * kP4Warps, kP4Stages = 4;
 
 template <int D, int NT>
 struct P4Cfg {
-    static constexpr int kChunk = D / 8;                             // bytes copied at once; a row is four of codes and one of pairs
-    static constexpr int kVc = 8 * D, kKm = 16 * D, kVm = 18 * D;    // of a stage: codes of K, of V, pairs of K, of V
-    static constexpr int kStage = 20 * D;
+    static constexpr int kChunk = D / 8, kRow = 5 * kChunk;          // bytes copied at once; of a row, four chunks of codes and one of pairs
+    static constexpr int kV = 16 * kRow, kStage = 2 * kV;            // 16 rows of K, then of V
     static constexpr int kWarp = kP4Stages * kStage;
     static constexpr int kBytes = kP4Warps * kWarp;
     static constexpr int kPitch = D + 8;                             // floats; of a row of a warp's output in its ring
     static_assert(8 * NT * kPitch * 4 <= kWarp, "a warp's output, where its ring was");
     static constexpr int kPerSm = NT == 1 ? 4 : 3;
+};
+
+// Codes as numbers.  fp16: exactly what they stand for.  bf16: that times 2^-20, from a multiplication and a sum that are rounded together, like those of int4_two.  A code
+// at bits 0 - 3 or 4 - 7 is, taken as a bf16 number, c * 2^-133 or 16 c * 2^-133 (also where it reaches the exponent's lowest bit), so the step is multiplied by 2^113 and
+// the lowest value by 2^-20 beforehand.  That overflows for steps from 2^15 on; whoever calls keeps the largest pair in sight (track) and goes over such keys with SLOW.
+template <typename T, bool SLOW>
+struct P4Codes {
+    static constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;
+    static constexpr float kScale = kScaled ? 1048576.f : 1.f;       // what the numbers are to be multiplied by
+    // pairs (step, lowest) of two groups in, steps and lowest values as operands out: a step for codes at bits 0 - 3 and one for those at bits 4 - 7
+    uint32_t step, step16, low;
+    __device__ __forceinline__ void set(uint32_t s, uint32_t l) {
+        step = s, low = l;
+        if constexpr (kScaled && !SLOW) step16 = times(s, 0x3d803d80u);   // 1 / 16
+    }
+    static __device__ __forceinline__ uint32_t times(uint32_t x, uint32_t y) {
+        using P = typename Int4Pair<T>::type;
+        const P z = __hmul2(*reinterpret_cast<const P*>(&x), *reinterpret_cast<const P*>(&y));
+        return *reinterpret_cast<const uint32_t*>(&z);
+    }
+    // a pair as it is stored
+    static __device__ __forceinline__ uint32_t pair(uint32_t meta, uint32_t& track) {
+        if constexpr (kScaled && !SLOW) {
+            meta = times(meta, 0x35807800u);                              // 2^113 below, 2^-20 above
+            const __nv_bfloat162 x = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&meta)), *reinterpret_cast<const __nv_bfloat162*>(&track));
+            track = *reinterpret_cast<const uint32_t*>(&x);
+        }
+        return meta;
+    }
+    template <int J>
+    __device__ __forceinline__ uint32_t two(uint32_t x) const {
+        if constexpr (!kScaled) {
+            return int4_two<T, J>(x, step, low);
+        } else if constexpr (SLOW) {
+            return times(int4_two<T, J>(x, step, low), 0x35803580u);
+        } else {
+            const uint32_t c = (J & 2 ? x >> 8 : x) & (J & 1 ? 0x00f000f0u : 0x000f000fu);
+            const __nv_bfloat162 y = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&c), *reinterpret_cast<const __nv_bfloat162*>(J & 1 ? &step16 : &step),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&low));
+            return *reinterpret_cast<const uint32_t*>(&y);
+        }
+    }
 };
 
 // tiles of 64 keys; at least one: a block that sees nothing is written too
@@ -60,31 +105,32 @@ __device__ __forceinline__ void p4_words(uint32_t (&w)[N], const uint8_t* at) {
     }
 }
 
-// grid: CTAs that share the line; blocks of up to 8 NT rows
+// grid: CTAs that share the line; blocks of up to 8 NT rows.  tma: 16 rows come as a box of k_map and v_map
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged_attn4_few(const PagedAttn p, const PagedCache c) {
+__global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm))
+k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, int tma, unsigned* err) {
     using C = P4Cfg<D, NT>;
-    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr bool kHalf = std::is_same<T, __half>::value, kScaled = P4Codes<T, false>::kScaled;
     constexpr int R = 8 * NT, KS = D / 16, MT = D / 16, KW = D / 32, VW = D / 64;
-    constexpr float kTau = PagedExp<kHalf>::kTau, kUp = PagedExp<kHalf>::kUp;
+    // Values times 2^-20 take probabilities of 2^20 more: products and the sums that become parts are those of PagedExp, and the probabilities' sum follows at the end.
+    constexpr float kTau = PagedExp<kHalf>::kTau, kUp = PagedExp<kHalf>::kUp + (kScaled ? 20.f : 0.f);
     extern __shared__ __align__(128) uint8_t p4_smem[];
     __shared__ float2 s_ml[kP4Warps][R];
+    __shared__ uint64_t full[kP4Warps][kP4Stages];
+    __shared__ int s_gave_up;
+    volatile int* s_abort = &s_gave_up;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     uint8_t* ring = p4_smem + warp * C::kWarp;
     const uint32_t ring_at = smem_u32(ring);
-    // This lane's five chunks of a stage's 160: the chunk of which row, where in the stage.  V's rows stand as the lanes read them, 2t + {0, 1, 8, 9} four behind one
-    // another, and (D = 128) every second pair of them with the halves of its codes changed: reads of four rows touch all banks once.
-    int place[5];
-#pragma unroll
-    for (int i = 0; i < 5; ++i) {
-        const int x = lane + 32 * i, is_v = x >= 80, r = (x - 80 * is_v) / 5, ch = (x - 80 * is_v) % 5;
-        const int slot = is_v ? (r & 8) + (r & 1) * 4 + ((r & 7) >> 1) : r;
-        place[i] = r | is_v << 4 | ch << 5 | (ch == 4 ? (is_v ? C::kVm : C::kKm) + slot * C::kChunk
-                                                      : (is_v ? C::kVc : 0) + slot * (D / 2) + (ch ^ (is_v && D == 128 ? slot & 2 : 0)) * C::kChunk) << 8;
-    }
+    if (lane == 0)
+        for (int i = 0; i < kP4Stages; ++i) mbar_init(&full[warp][i], 1);
+    if (tid == 0) s_gave_up = 0;
+    mbar_fence_init();
+    __syncthreads();
     pdl_wait();
     pdl_trigger();
     if (tid == 0) p.cuts[blockIdx.x].parts = 0;
+    int used = 0;   // tiles of this warp so far: of its ring
     PagedWalk<P4Kind> walk;
     const PagedBlock& k = walk.k;
     const PagedPlace& at = walk.place;
@@ -94,26 +140,33 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
         walk.share(first, count);
         if (count == 0) continue;
         const int key0 = ((k.hi >= 0 ? k.lo / kP4Keys : 0) + first) * kP4Keys + warp * 16;
-        const long long head = (long long)at.hk * c.head_stride;
         // Lanes 0 - 15 ask for the page numbers of the 16 rows a stage ahead; where pages hold whole 16s these are one page
-        const bool one_page = c.page_size % 16 == 0;
         auto find = [&](int j) {
-            const int row = key0 + j * kP4Keys + (lane & 15), pg = c.by_page(row);
+            const int row = key0 + j * kP4Keys + (tma ? 0 : lane & 15), pg = c.by_page(row);
             return j < count && row <= k.hi && pg < c.max_pages ? c.table[(size_t)k.seq * c.ld_table + pg] : -1;
         };
         auto copy = [&](int j, int id) {
-            const uint32_t to = ring_at + (uint32_t)(j % kP4Stages) * C::kStage;
-            const int row0 = key0 + j * kP4Keys, mine = row0 + (one_page ? 0 : lane & 15);
-            long long off = id >= 0 && id < c.num_pages ? (long long)id * c.page_stride + (long long)(mine - c.by_page(mine) * c.page_size) * c.row_stride + head : -1;
-            if (one_page) off = __shfl_sync(0xffffffffu, off, 0);
+            const int stage = (used + j) % kP4Stages, row0 = key0 + j * kP4Keys;
+            if (tma) {
+                if (lane == 0) {
+                    mbar_expect_tx(&full[warp][stage], C::kStage);
+                    const int row = row0 - c.by_page(row0) * c.page_size, page = id >= 0 && id < c.num_pages ? id : -1;   // -1: reads as zeros
 #pragma unroll
-            for (int i = 0; i < 5; ++i) {
-                const int r = place[i] & 15;
-                long long o = one_page ? off : __shfl_sync(0xffffffffu, off, r);
-                const bool in = o >= 0 && row0 + r <= k.hi;
-                if (one_page) o += r * c.row_stride;
-                o += (place[i] >> 5 & 7) * C::kChunk;
-                p4_copy<C::kChunk>(to + (uint32_t)(place[i] >> 8), static_cast<const uint8_t*>(place[i] & 16 ? c.v : c.k) + (in ? o : 0), in ? C::kChunk : 0);
+                    for (int v = 0; v < 2; ++v)
+                        pt_load_4d(ring_at + (uint32_t)(stage * C::kStage + v * C::kV), v ? &v_map : &k_map, D == 128 ? 0 : row * (C::kRow / 4), D == 128 ? row : 0, at.hk, page,
+                                   &full[warp][stage]);
+                }
+            } else {
+                const int mine = row0 + (lane & 15);
+                const long long off = id >= 0 && id < c.num_pages
+                                          ? (long long)id * c.page_stride + (long long)(mine - c.by_page(mine) * c.page_size) * c.row_stride + (long long)at.hk * c.head_stride : -1;
+#pragma unroll 1
+                for (int x = lane; x < 160; x += 32) {
+                    const int is_v = x >= 80, r = (x - 80 * is_v) / 5, ch = (x - 80 * is_v) % 5;
+                    const long long o = __shfl_sync(0xffffffffu, off, r);
+                    p4_copy<C::kChunk>(ring_at + (uint32_t)(stage * C::kStage + x * C::kChunk), static_cast<const uint8_t*>(is_v ? c.v : c.k) + (o < 0 ? 0 : o + ch * C::kChunk),
+                                       o < 0 ? 0 : C::kChunk);
+                }
             }
         };
         // rows of q: row g of each 8, as the columns of the second operand; what rows 2t and 2t + 1 see
@@ -140,16 +193,20 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
                 lo[n][e] = paged_from(p, at_place);
             }
         }
+        // keys that all rows of the block see; rows that are none may see them too
+        const int all_hi = min(k.place0 + p.by_group(k.row0), k.have - 1), all_lo = paged_from(p, k.place0 + p.by_group(k.row0 + k.rows - 1));
         float o[MT][NT][4], l[NT][2], m_ref[NT][2];
-        // Once, mostly.  A masked probability is exactly zero, but zero times NaN, which a broken group of a row's values reads as, is NaN in its sum.  Where the warp's sums hold
-        // a NaN that no score explains, it goes over its keys once more: of 16 keys with a broken group it takes the product key by key, of those that a row sees.
-        for (bool again = false;; again = true) {
+        uint32_t track = 0;
+        // The block's keys, one way or the other: -> whether there was a pair that the fast one does not serve.  A masked probability is exactly zero, but zero times NaN, which a
+        // broken group of a row's values reads as, is NaN in its sum: of 16 keys with such a group SLOW takes the product key by key, of those that a row sees.
+        auto pass = [&](auto slow) {
+            constexpr bool SLOW = decltype(slow)::value;
             int id = find(0);
 #pragma unroll 1
             for (int j = 0; j < kP4Stages - 1; ++j) {
                 const int next = find(j + 1);
                 if (j < count) copy(j, id);
-                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (!tma) asm volatile("cp.async.commit_group;" ::: "memory");
                 id = next;
             }
 #pragma unroll
@@ -158,31 +215,40 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
                 for (int m = 0; m < MT; ++m) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
                 l[n][0] = l[n][1] = 0.f, m_ref[n][0] = m_ref[n][1] = kPagedNone;
             }
+#pragma unroll 1
             for (int j = 0; j < count; ++j) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kP4Stages - 2) : "memory");
+                const int stage = (used + j) % kP4Stages, kb = key0 + j * kP4Keys;
+                uint8_t* st = ring + stage * C::kStage;
+                if (tma) pt_wait(&full[warp][stage], (uint32_t)((used + j) / kP4Stages) & 1u, s_abort, err, 0x5c00 + warp);
+                else asm volatile("cp.async.wait_group %0;" ::"n"(kP4Stages - 2) : "memory");
                 __syncwarp();
                 const int next = find(j + kP4Stages);
                 if (j + kP4Stages - 1 < count) copy(j + kP4Stages - 1, id);
-                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (!tma) asm volatile("cp.async.commit_group;" ::: "memory");
                 id = next;
-                const int kb = key0 + j * kP4Keys;
                 if (kb > k.hi || kb + 15 < k.lo) continue;
-                const uint8_t* st = ring + (j % kP4Stages) * C::kStage;
+                if (tma && kb + 15 > k.hi) {   // what a page holds behind the last key may be anything
+                    if (kb + (lane & 15) > k.hi)
+#pragma unroll
+                        for (int i = 0; i < D / kInt4Group; ++i) *reinterpret_cast<uint32_t*>(st + lane * C::kRow + D / 2 + i * 4) = 0;
+                    pa_fence_async();
+                    __syncwarp();
+                }
                 float s[NT][4] = {};
                 {
-                    uint32_t x[2][KW], step[2], low[2];
+                    uint32_t x[2][KW];
+                    P4Codes<T, SLOW> k_code[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const int r = g + u * 8;
-                        p4_words<KW>(x[u], st + r * (D / 2) + t4 * C::kChunk);
-                        int4_meta<T>(*reinterpret_cast<const uint32_t*>(st + C::kKm + r * C::kChunk + t4 * (D / 4) / kInt4Group * 4), step[u], low[u]);
+                        const uint8_t* row = st + (g + u * 8) * C::kRow;
+                        p4_words<KW>(x[u], row + t4 * C::kChunk);
+                        const uint32_t pair = P4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + t4 * (D / 4) / kInt4Group * 4), track);
+                        k_code[u].set(__byte_perm(pair, 0, 0x1010), __byte_perm(pair, 0, 0x3232));
                     }
 #pragma unroll
                     for (int w = 0; w < KW; ++w) {
-                        const uint32_t a[4] = {int4_two<T, 0>(x[0][w], step[0], low[0]), int4_two<T, 0>(x[1][w], step[1], low[1]),
-                                               int4_two<T, 1>(x[0][w], step[0], low[0]), int4_two<T, 1>(x[1][w], step[1], low[1])};
-                        const uint32_t b[4] = {int4_two<T, 2>(x[0][w], step[0], low[0]), int4_two<T, 2>(x[1][w], step[1], low[1]),
-                                               int4_two<T, 3>(x[0][w], step[0], low[0]), int4_two<T, 3>(x[1][w], step[1], low[1])};
+                        const uint32_t a[4] = {k_code[0].template two<0>(x[0][w]), k_code[1].template two<0>(x[1][w]), k_code[0].template two<1>(x[0][w]), k_code[1].template two<1>(x[1][w])};
+                        const uint32_t b[4] = {k_code[0].template two<2>(x[0][w]), k_code[1].template two<2>(x[1][w]), k_code[0].template two<3>(x[0][w]), k_code[1].template two<3>(x[1][w])};
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             pf_mma<T>(s[n], a, qb[n][2 * w][0], qb[n][2 * w][1]);
@@ -190,17 +256,18 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
                         }
                     }
                 }
+                const float scale = p.scale * P4Codes<T, SLOW>::kScale;
+                const bool masks = kb + 15 > all_hi || kb < all_lo;
                 bool up = false;
                 float top[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const int key = kb + g + u * 8;
-                            float& x = s[n][2 * u + e];
-                            x = key <= hi[n][e] && key >= lo[n][e] ? x * p.scale : -INFINITY;
+                        s[n][e] *= scale, s[n][2 + e] *= scale;
+                        if (masks) {
+                            if (kb + g > hi[n][e] || kb + g < lo[n][e]) s[n][e] = -INFINITY;
+                            if (kb + g + 8 > hi[n][e] || kb + g + 8 < lo[n][e]) s[n][2 + e] = -INFINITY;
                         }
                         top[n][e] = fmaxf(s[n][e], s[n][2 + e]);
                         up |= top[n][e] - m_ref[n][e] > kTau;
@@ -230,23 +297,24 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
                         pb[n][u] = p4_transpose(pf_pack<T>(x, y));
                     }
                 bool apart = false;   // the product key by key
-                if (again) {
+                if constexpr (SLOW) {
                     bool whole = true;
-                    for (int x = lane; x < D / 2; x += 32) whole = whole && int4_finite<T>(*reinterpret_cast<const uint32_t*>(st + C::kVm + x * 4));
+                    for (int x = lane; x < D / 2; x += 32) whole = whole && int4_finite<T>(*reinterpret_cast<const uint32_t*>(st + C::kV + x % 16 * C::kRow + D / 2 + x / 16 * 4));
                     apart = __any_sync(0xffffffffu, !whole);
                 }
                 if (apart) {
+                    if constexpr (SLOW) {
 #pragma unroll 1
                     for (int key = 0; key < 16; ++key) {
-                        const int slot = (key & 8) + (key & 1) * 4 + ((key & 7) >> 1);
-                        const uint32_t meta = *reinterpret_cast<const uint32_t*>(st + C::kVm + slot * C::kChunk + g * (D / 8) / kInt4Group * 4);
+                        const uint8_t* row = st + C::kV + key * C::kRow;
+                        const uint32_t meta = *reinterpret_cast<const uint32_t*>(row + D / 2 + g * (D / 8) / kInt4Group * 4);
                         uint32_t x[VW];
-                        p4_words<VW>(x, st + C::kVc + slot * (D / 2) + (D == 128 ? ((g >> 1) ^ (slot & 2)) * 16 + (g & 1) * 8 : g * 4));
+                        p4_words<VW>(x, row + g * (D / 16));
                         const T* two = reinterpret_cast<const T*>(&meta);
                         float v[D / 8];
 #pragma unroll
                         for (int i = 0; i < D / 8; ++i)
-                            v[i] = round_to<T>(fmaf((float)(x[i >> 3] >> ((i & 1) * 16 + (i & 6) * 2) & 15u), to_f32<T>(two[0]), to_f32<T>(two[1])));
+                            v[i] = round_to<T>(fmaf((float)(x[i >> 3] >> ((i & 1) * 16 + (i & 6) * 2) & 15u), to_f32<T>(two[0]), to_f32<T>(two[1]))) / P4Codes<T, SLOW>::kScale;
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -257,16 +325,18 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
                                     for (int i = 0; i < D / 8; ++i) o[i >> 1][n][(i & 1) * 2 + e] = fmaf(w, v[i], o[i >> 1][n][(i & 1) * 2 + e]);
                             }
                     }
-                } else {
-                    uint32_t x[4][VW], meta[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int slot = 4 * u + t4;
-                        p4_words<VW>(x[u], st + C::kVc + slot * (D / 2) + (D == 128 ? ((g >> 1) ^ (t4 & 2)) * 16 + (g & 1) * 8 : g * 4));
-                        meta[u] = *reinterpret_cast<const uint32_t*>(st + C::kVm + slot * C::kChunk + g * (D / 8) / kInt4Group * 4);
                     }
-                    const uint32_t step[2] = {__byte_perm(meta[0], meta[1], 0x5410), __byte_perm(meta[2], meta[3], 0x5410)};
-                    const uint32_t low[2] = {__byte_perm(meta[0], meta[1], 0x7632), __byte_perm(meta[2], meta[3], 0x7632)};
+                } else {
+                    uint32_t x[4][VW], pair[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {   // keys 2t + {0, 1, 8, 9}
+                        const uint8_t* row = st + C::kV + (2 * t4 + (u & 1) + (u >> 1) * 8) * C::kRow;
+                        p4_words<VW>(x[u], row + g * (D / 16));
+                        pair[u] = P4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + g * (D / 8) / kInt4Group * 4), track);
+                    }
+                    P4Codes<T, SLOW> v_code[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) v_code[u].set(__byte_perm(pair[2 * u], pair[2 * u + 1], 0x5410), __byte_perm(pair[2 * u], pair[2 * u + 1], 0x7632));
 #pragma unroll
                     for (int w = 0; w < VW; ++w) {
                         uint32_t even[2], odd[2];   // columns 0 2 4 6 and 1 3 5 7 of two keys
@@ -274,8 +344,7 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
                         for (int u = 0; u < 2; ++u) even[u] = __byte_perm(x[2 * u][w], x[2 * u + 1][w], 0x5410), odd[u] = __byte_perm(x[2 * u][w], x[2 * u + 1][w], 0x7632);
                         auto product = [&](auto index) {
                             constexpr int J = decltype(index)::value;
-                            const uint32_t a[4] = {int4_two<T, J>(even[0], step[0], low[0]), int4_two<T, J>(odd[0], step[0], low[0]),
-                                                   int4_two<T, J>(even[1], step[1], low[1]), int4_two<T, J>(odd[1], step[1], low[1])};
+                            const uint32_t a[4] = {v_code[0].template two<J>(even[0]), v_code[0].template two<J>(odd[0]), v_code[1].template two<J>(even[1]), v_code[1].template two<J>(odd[1])};
 #pragma unroll
                             for (int n = 0; n < NT; ++n) pf_mma<T>(o[w * 4 + J][n], a, pb[n][0], pb[n][1]);
                         };
@@ -284,13 +353,19 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
                     }
                 }
             }
+            used += count;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], x);
-            if (again) break;
+        };
+        pass(std::false_type{});
+        bool again = false;
+        if constexpr (kScaled) {
+            again = (track & 0x7fffu) >= 0x7f80u || (track >> 16 & 0x7fffu) >= 0x7f80u;
+        } else {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -300,11 +375,13 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
                     for (int m = 0; m < MT; ++m) none |= o[m][n][e] != o[m][n][e] || o[m][n][2 + e] != o[m][n][2 + e];
                     again |= none && l[n][e] == l[n][e] && n * 8 + t4 * 2 + e < k.rows;
                 }
-            if (!__any_sync(0xffffffffu, again)) break;
+        }
+        if (__any_sync(0xffffffffu, again)) {
             __syncwarp();
+            pass(std::true_type{});
         }
         // the warps' parts, in their rings
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (!tma) asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncwarp();
         float* mine = reinterpret_cast<float*>(ring);
 #pragma unroll
@@ -312,7 +389,7 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = n * 8 + t4 * 2 + e;
-                if (g == 0) s_ml[warp][r] = make_float2(m_ref[n][e], l[n][e]);
+                if (g == 0) s_ml[warp][r] = make_float2(m_ref[n][e], l[n][e] / P4Codes<T, false>::kScale);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) *reinterpret_cast<float2*>(mine + r * C::kPitch + g * (D / 8) + 2 * m) = make_float2(o[m][n][e], o[m][n][2 + e]);
             }
@@ -342,8 +419,10 @@ __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm)) k_paged
             }
         }
         if (tid == 0) walk.cut(p, first, count);
-        __syncthreads();   // the rings are the next block's
+        pa_fence_async();   // TMA writes where the parts were
+        __syncthreads();    // the rings are the next block's
     }
+    tc2_drain(s_abort);
 }
 
 }  // namespace zl
