@@ -64,7 +64,7 @@ static int paged4_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pd
     CUtensorMap maps[2] = {};
     const int tma = c.page_size % 16 == 0 && p4_maps<D>(maps, p, c);
     ZL_CHECK_CUDA(launch(k_paged_attn4_few<T, D, NT>, dim3(ctas), dim3(kP4Warps * 32), C::kBytes, stream, pdl, p, c, maps[0], maps[1], tma, words + kWaitAttnPaged));
-    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 8 * NT>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p));
+    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 8 * NT, 8>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p));
     return ZL_OK;
 }
 

@@ -1,5 +1,5 @@
-// Attention of few (token, head) rows of a kv head over pages of 4 bits (int4_cache.cuh).  Work is shared out as in paged_attn_few.cuh: tiles of 64 keys of all
-// blocks stand in one line, a CTA takes an equal stretch, a warp has 16 keys of a tile and a ring of its own.
+// Attention of few (token, head) rows of a kv head over pages of 4 bits (int4_cache.cuh).  Work is shared out as in paged_attn_few.cuh: tiles of 128 keys of all
+// blocks stand in one line, a CTA takes an equal stretch, a warp has 32 keys of a tile and a ring of its own.
 //
 // What 4 bits take off the memory they put on the instructions: a key and its value are 160 bytes instead of 512, and every code costs more than one of them.
 // So the products are turned around, S^T = K Q^T and O^T += V^T P^T by mma.sync with the keys' and values' 16 rows as the first operand and 8 rows of queries as the
@@ -20,12 +20,12 @@
 
 namespace zl {
 
-constexpr int kP4Warps = 4, kP4Keys = 16 * kP4Warps, kP4Stages = 4;
+constexpr int kP4Warps = 4, kP4Each = 32, kP4Keys = kP4Each * kP4Warps, kP4Stages = 2;
 
 template <int D, int NT>
 struct P4Cfg {
     static constexpr int kChunk = D / 8, kRow = 5 * kChunk;          // bytes copied at once; of a row, four chunks of codes and one of pairs
-    static constexpr int kV = 16 * kRow, kStage = 2 * kV;            // 16 rows of K, then of V
+    static constexpr int kV = kP4Each * kRow, kStage = 2 * kV;       // rows of K, then of V
     static constexpr int kWarp = kP4Stages * kStage;
     static constexpr int kBytes = kP4Warps * kWarp;
     static constexpr int kPitch = D + 8;                             // floats; of a row of a warp's output in its ring
@@ -75,7 +75,7 @@ struct P4Codes {
     }
 };
 
-// tiles of 64 keys; at least one: a block that sees nothing is written too
+// tiles of 128 keys; at least one: a block that sees nothing is written too
 struct P4Kind {
     static constexpr int kSetup = 2;
     static __device__ __forceinline__ int turns(const PagedAttn&, const PagedBlock& k) { return k.hi >= 0 ? k.hi / kP4Keys - k.lo / kP4Keys + 1 : 1; }
@@ -139,30 +139,30 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
         int first, count;
         walk.share(first, count);
         if (count == 0) continue;
-        const int key0 = ((k.hi >= 0 ? k.lo / kP4Keys : 0) + first) * kP4Keys + warp * 16;
-        // Lanes 0 - 15 ask for the page numbers of the 16 rows a stage ahead; where pages hold whole 16s these are one page
+        const int key0 = ((k.hi >= 0 ? k.lo / kP4Keys : 0) + first) * kP4Keys + warp * kP4Each;
+        // The lanes ask for the page numbers of the rows a stage ahead; where pages hold whole 16s lanes 0 and 1 do
         auto find = [&](int j) {
-            const int row = key0 + j * kP4Keys + (tma ? 0 : lane & 15), pg = c.by_page(row);
+            const int row = key0 + j * kP4Keys + (tma ? (lane & 1) * 16 : lane), pg = c.by_page(row);
             return j < count && row <= k.hi && pg < c.max_pages ? c.table[(size_t)k.seq * c.ld_table + pg] : -1;
         };
         auto copy = [&](int j, int id) {
             const int stage = (used + j) % kP4Stages, row0 = key0 + j * kP4Keys;
             if (tma) {
-                if (lane == 0) {
-                    mbar_expect_tx(&full[warp][stage], C::kStage);
-                    const int row = row0 - c.by_page(row0) * c.page_size, page = id >= 0 && id < c.num_pages ? id : -1;   // -1: reads as zeros
-#pragma unroll
-                    for (int v = 0; v < 2; ++v)
-                        pt_load_4d(ring_at + (uint32_t)(stage * C::kStage + v * C::kV), v ? &v_map : &k_map, D == 128 ? 0 : row * (C::kRow / 4), D == 128 ? row : 0, at.hk, page,
-                                   &full[warp][stage]);
+                if (lane == 0) mbar_expect_tx(&full[warp][stage], C::kStage);
+                __syncwarp();
+                if (lane < 2) {
+                    const int row16 = row0 + lane * 16, row = row16 - c.by_page(row16) * c.page_size, page = id >= 0 && id < c.num_pages ? id : -1;   // -1: reads as zeros
+                    const uint32_t to = ring_at + (uint32_t)(stage * C::kStage + lane * (16 * C::kRow));
+                    pt_load_4d(to, &k_map, D == 128 ? 0 : row * (C::kRow / 4), D == 128 ? row : 0, at.hk, page, &full[warp][stage]);
+                    pt_load_4d(to + C::kV, &v_map, D == 128 ? 0 : row * (C::kRow / 4), D == 128 ? row : 0, at.hk, page, &full[warp][stage]);
                 }
             } else {
-                const int mine = row0 + (lane & 15);
+                const int mine = row0 + lane;
                 const long long off = id >= 0 && id < c.num_pages
                                           ? (long long)id * c.page_stride + (long long)(mine - c.by_page(mine) * c.page_size) * c.row_stride + (long long)at.hk * c.head_stride : -1;
 #pragma unroll 1
-                for (int x = lane; x < 160; x += 32) {
-                    const int is_v = x >= 80, r = (x - 80 * is_v) / 5, ch = (x - 80 * is_v) % 5;
+                for (int x = lane; x < 10 * kP4Each; x += 32) {
+                    const int is_v = x >= 5 * kP4Each, r = (x - 5 * kP4Each * is_v) / 5, ch = (x - 5 * kP4Each * is_v) % 5;
                     const long long o = __shfl_sync(0xffffffffu, off, r);
                     p4_copy<C::kChunk>(ring_at + (uint32_t)(stage * C::kStage + x * C::kChunk), static_cast<const uint8_t*>(is_v ? c.v : c.k) + (o < 0 ? 0 : o + ch * C::kChunk),
                                        o < 0 ? 0 : C::kChunk);
@@ -226,21 +226,25 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                 if (j + kP4Stages - 1 < count) copy(j + kP4Stages - 1, id);
                 if (!tma) asm volatile("cp.async.commit_group;" ::: "memory");
                 id = next;
-                if (kb > k.hi || kb + 15 < k.lo) continue;
-                if (tma && kb + 15 > k.hi) {   // what a page holds behind the last key may be anything
-                    if (kb + (lane & 15) > k.hi)
+                if (kb > k.hi || kb + kP4Each - 1 < k.lo) continue;
+                if (tma && kb + kP4Each - 1 > k.hi) {   // what a page holds behind the last key may be anything
+                    if (kb + lane > k.hi)
 #pragma unroll
-                        for (int i = 0; i < D / kInt4Group; ++i) *reinterpret_cast<uint32_t*>(st + lane * C::kRow + D / 2 + i * 4) = 0;
+                        for (int i = 0; i < D / kInt4Group; ++i) {
+                            *reinterpret_cast<uint32_t*>(st + lane * C::kRow + D / 2 + i * 4) = 0;
+                            *reinterpret_cast<uint32_t*>(st + C::kV + lane * C::kRow + D / 2 + i * 4) = 0;
+                        }
                     pa_fence_async();
                     __syncwarp();
                 }
-                float s[NT][4] = {};
-                {
+                float s[2][NT][4] = {};   // keys kb + 16 h + {g, g + 8}, rows 8 n + 2t + {0, 1}
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
                     uint32_t x[2][KW];
                     P4Codes<T, SLOW> k_code[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint8_t* row = st + (g + u * 8) * C::kRow;
+                        const uint8_t* row = st + (16 * h + g + u * 8) * C::kRow;
                         p4_words<KW>(x[u], row + t4 * C::kChunk);
                         const uint32_t pair = P4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + t4 * (D / 4) / kInt4Group * 4), track);
                         k_code[u].set(__byte_perm(pair, 0, 0x1010), __byte_perm(pair, 0, 0x3232));
@@ -251,25 +255,27 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                         const uint32_t b[4] = {k_code[0].template two<2>(x[0][w]), k_code[1].template two<2>(x[1][w]), k_code[0].template two<3>(x[0][w]), k_code[1].template two<3>(x[1][w])};
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            pf_mma<T>(s[n], a, qb[n][2 * w][0], qb[n][2 * w][1]);
-                            pf_mma<T>(s[n], b, qb[n][2 * w + 1][0], qb[n][2 * w + 1][1]);
+                            pf_mma<T>(s[h][n], a, qb[n][2 * w][0], qb[n][2 * w][1]);
+                            pf_mma<T>(s[h][n], b, qb[n][2 * w + 1][0], qb[n][2 * w + 1][1]);
                         }
                     }
                 }
                 const float scale = p.scale * P4Codes<T, SLOW>::kScale;
-                const bool masks = kb + 15 > all_hi || kb < all_lo;
+                const bool masks = kb + kP4Each - 1 > all_hi || kb < all_lo;
                 bool up = false;
                 float top[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        s[n][e] *= scale, s[n][2 + e] *= scale;
-                        if (masks) {
-                            if (kb + g > hi[n][e] || kb + g < lo[n][e]) s[n][e] = -INFINITY;
-                            if (kb + g + 8 > hi[n][e] || kb + g + 8 < lo[n][e]) s[n][2 + e] = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float& x = s[i >> 1][n][(i & 1) * 2 + e];
+                            x *= scale;
+                            const int key = kb + g + 8 * i;
+                            if (masks && (key > hi[n][e] || key < lo[n][e])) x = -INFINITY;
                         }
-                        top[n][e] = fmaxf(s[n][e], s[n][2 + e]);
+                        top[n][e] = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
                         up |= top[n][e] - m_ref[n][e] > kTau;
                     }
                 if (__any_sync(0xffffffffu, up)) {
@@ -286,51 +292,51 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                             for (int m = 0; m < MT; ++m) o[m][n][e] *= f, o[m][n][2 + e] *= f;
                         }
                 }
-                uint32_t pb[NT][2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int h = 0; h < 2; ++h) {
+                    const uint8_t* values = st + C::kV + 16 * h * C::kRow;
+                    uint32_t pb[NT][2];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {   // the difference first: it is as exact as the scores, whatever their size is
-                        float &x = s[n][2 * u], &y = s[n][2 * u + 1];
-                        x = pa_exp2((x - m_ref[n][0]) + kUp), y = pa_exp2((y - m_ref[n][1]) + kUp);
-                        l[n][0] += x, l[n][1] += y;
-                        pb[n][u] = p4_transpose(pf_pack<T>(x, y));
-                    }
-                bool apart = false;   // the product key by key
-                if constexpr (SLOW) {
-                    bool whole = true;
-                    for (int x = lane; x < D / 2; x += 32) whole = whole && int4_finite<T>(*reinterpret_cast<const uint32_t*>(st + C::kV + x % 16 * C::kRow + D / 2 + x / 16 * 4));
-                    apart = __any_sync(0xffffffffu, !whole);
-                }
-                if (apart) {
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {   // the difference first: it is as exact as the scores, whatever their size is
+                            float &x = s[h][n][2 * u], &y = s[h][n][2 * u + 1];
+                            x = pa_exp2((x - m_ref[n][0]) + kUp), y = pa_exp2((y - m_ref[n][1]) + kUp);
+                            l[n][0] += x, l[n][1] += y;
+                            pb[n][u] = p4_transpose(pf_pack<T>(x, y));
+                        }
                     if constexpr (SLOW) {
+                        bool whole = true;
+                        for (int x = lane; x < D / 2; x += 32) whole = whole && int4_finite<T>(*reinterpret_cast<const uint32_t*>(values + x % 16 * C::kRow + D / 2 + x / 16 * 4));
+                        if (__any_sync(0xffffffffu, !whole)) {   // the product key by key
 #pragma unroll 1
-                    for (int key = 0; key < 16; ++key) {
-                        const uint8_t* row = st + C::kV + key * C::kRow;
-                        const uint32_t meta = *reinterpret_cast<const uint32_t*>(row + D / 2 + g * (D / 8) / kInt4Group * 4);
-                        uint32_t x[VW];
-                        p4_words<VW>(x, row + g * (D / 16));
-                        const T* two = reinterpret_cast<const T*>(&meta);
-                        float v[D / 8];
+                            for (int key = 0; key < 16; ++key) {
+                                const uint8_t* row = values + key * C::kRow;
+                                const uint32_t meta = *reinterpret_cast<const uint32_t*>(row + D / 2 + g * (D / 8) / kInt4Group * 4);
+                                uint32_t x[VW];
+                                p4_words<VW>(x, row + g * (D / 16));
+                                const T* two = reinterpret_cast<const T*>(&meta);
+                                float v[D / 8];
 #pragma unroll
-                        for (int i = 0; i < D / 8; ++i)
-                            v[i] = round_to<T>(fmaf((float)(x[i >> 3] >> ((i & 1) * 16 + (i & 6) * 2) & 15u), to_f32<T>(two[0]), to_f32<T>(two[1]))) / P4Codes<T, SLOW>::kScale;
+                                for (int i = 0; i < D / 8; ++i)
+                                    v[i] = round_to<T>(fmaf((float)(x[i >> 3] >> ((i & 1) * 16 + (i & 6) * 2) & 15u), to_f32<T>(two[0]), to_f32<T>(two[1]))) / P4Codes<T, SLOW>::kScale;
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float w = __shfl_sync(0xffffffffu, key & 8 ? s[n][2 + e] : s[n][e], (key & 7) << 2 | t4);
-                                if (kb + key <= hi[n][e] && kb + key >= lo[n][e])
+                                    for (int e = 0; e < 2; ++e) {
+                                        const float w = __shfl_sync(0xffffffffu, key & 8 ? s[h][n][2 + e] : s[h][n][e], (key & 7) << 2 | t4);
+                                        if (kb + 16 * h + key <= hi[n][e] && kb + 16 * h + key >= lo[n][e])
 #pragma unroll
-                                    for (int i = 0; i < D / 8; ++i) o[i >> 1][n][(i & 1) * 2 + e] = fmaf(w, v[i], o[i >> 1][n][(i & 1) * 2 + e]);
+                                            for (int i = 0; i < D / 8; ++i) o[i >> 1][n][(i & 1) * 2 + e] = fmaf(w, v[i], o[i >> 1][n][(i & 1) * 2 + e]);
+                                    }
                             }
+                            continue;
+                        }
                     }
-                    }
-                } else {
                     uint32_t x[4][VW], pair[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {   // keys 2t + {0, 1, 8, 9}
-                        const uint8_t* row = st + C::kV + (2 * t4 + (u & 1) + (u >> 1) * 8) * C::kRow;
+                        const uint8_t* row = values + (2 * t4 + (u & 1) + (u >> 1) * 8) * C::kRow;
                         p4_words<VW>(x[u], row + g * (D / 16));
                         pair[u] = P4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + g * (D / 8) / kInt4Group * 4), track);
                     }
