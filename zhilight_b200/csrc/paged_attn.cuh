@@ -29,6 +29,7 @@ struct PagedAttn {
     float2* ml;                       // parts of blocks that were cut, two places for every CTA: {maximum, sum} of their rows, and the rows
     float* part;
     struct PagedCut* cuts;            // for every CTA
+    int split;                        // of kernels that share a call's sequences (KIND::takes): (token, head) rows of a kv head up to which one of them takes a sequence
 };
 
 // Exponentials carry 2^up, and a row's reference follows its maximum once that is more than `tau` above it.  fp16 probabilities are at most 2^15, and with 2^10 the
@@ -70,7 +71,7 @@ struct PagedCut {
     int hk, parts;   // its kv head; stretches that have a part, 0: there is no such block
 };
 
-// A warp's view of the line that the blocks of a kernel's work stand in: sequence by sequence, in it kv head by kv head, in that block by block, each
+// A warp's view of the line that the blocks of a kernel's work stand in: sequence by sequence of those that KIND::takes(), in it kv head by kv head, in that block by block, each
 // KIND::kSetup + KIND::turns() long.  A CTA of the grid takes an equal stretch of the line.  128 sequences are in view at a time, four to a lane; the blocks of a
 // sequence that has many are looked at by the whole warp.  Everything fits 32 bits, which the entry point sees to, for sequences that have no more rows together
 // than q: where they have, their rows overlap, and the line is empty.  No loop here goes by the lengths alone: one that changes under the kernel cannot keep it running.
@@ -102,6 +103,7 @@ struct PagedLine {
             k.n = b + u < c.seqs ? max(min(at[u + 1], p.rows) - k.first, 0) : 0;
             low += k.n & 0xffff, high += k.n >> 16;
             k.n *= p.group;
+            if (!KIND::takes(p, k.n)) k.n = 0;
             k.place0 = len[u] - at[u + 1] + k.first;
             k.have = min(max(len[u], 0), c.room());
             const bool many = k.n > kAlone * p.block_rows;

@@ -6,36 +6,53 @@
 
 namespace zl {
 
-// Calls whose sequences bring at most so many (token, head) rows of a kv head each go to the kernel for few rows, as do groups that no tile holds a token of.
-constexpr int kFewRows4 = 16;
+// Calls whose sequences bring at most so many (token, head) rows of a kv head go to the kernel for few rows, and all where groups have more heads than a tile has rows.
+// Drafts of 16 sequences, 48 rows, up to 6000 keys: 49 us there, in three blocks, 87 on the tiles, whose blocks of up to 128 rows cost the same.
+// Of other calls, those sequences go there that bring a token or two of a group of up to 8 heads, or up to 16 rows: portions of prompts beside 20 single tokens (24 sequences, keys in a
+// window of 1024) 71 us, 95 with all on the tiles.
+constexpr int kFewRows4 = 64, kFewBeside = 16;
 
+// what lies where in the workspace, for one of the two kernels
 struct Paged4Plan {
-    bool tiles;                     // on the 5th-generation tensor cores
-    int ctas, block_rows, tile_rows;
-    size_t ml, part, cuts, bytes;   // what lies where in the workspace
+    int ctas, block_rows, tile_rows;   // ctas 0: it is not launched
+    size_t ml, part, cuts;
+};
+struct Paged4Plans {
+    Paged4Plan few, tiles;
+    int split;                         // rows of a sequence for the kernel for few
+    size_t bytes;
 };
 
 template <int D>
 static int paged4_few_ctas(bool eight) { return device_sm_count() * (eight ? P4Cfg<D, 1>::kPerSm : P4Cfg<D, 2>::kPerSm); }
 
-static Paged4Plan paged4_plan(int rows, int max_new, int seqs, int max_keys, int heads, int kv_heads, int dim) {
-    Paged4Plan s = {};
+static Paged4Plans paged4_plan(int rows, int max_new, int seqs, int max_keys, int heads, int kv_heads, int dim) {
+    Paged4Plans s = {};
     const int group = heads / kv_heads;
     const long long all = (long long)rows * group, most = (long long)max_new * group;
-    s.tiles = most > kFewRows4 && group <= kPaRows;
-    s.tile_rows = s.tiles ? kPaRows / group * group : 0;
-    s.block_rows = s.tiles ? 2 * s.tile_rows : most <= 8 ? 8 : 16;
-    // no more CTAs than the line can be long: every sequence adds less than one block to those of the rows, each of all the keys there is room for
-    const long long units = (all / s.block_rows + seqs) * (s.tiles ? PtKind::kSetup + cdiv(max_keys, kPtKeys) : P4Kind::kSetup + cdiv(max_keys, kP4Keys)) * kv_heads;
-    const int most_ctas = s.tiles ? device_sm_count() : dim == 64 ? paged4_few_ctas<64>(s.block_rows == 8) : paged4_few_ctas<128>(s.block_rows == 8);
-    s.ctas = (int)(units < most_ctas ? units : most_ctas);
-    const size_t parts = (size_t)s.ctas * 2 * (s.tiles ? kPtRows : s.block_rows);
+    const bool tiles = most > kFewRows4 && group <= kPaRows;
     auto take = [&](size_t bytes) {
         const size_t at = s.bytes;
         s.bytes += (bytes + 255) / 256 * 256;
         return at;
     };
-    s.ml = take(parts * sizeof(float2)), s.part = take(parts * dim * sizeof(float)), s.cuts = take((size_t)s.ctas * sizeof(PagedCut));
+    auto plan = [&](Paged4Plan& p, int block_rows, int places, int block_units, int most_ctas) {
+        // no more CTAs than the line can be long: every sequence adds less than one block to those of the rows, each of all the keys there is room for
+        const long long units = (all / block_rows + seqs) * block_units * kv_heads;
+        p.block_rows = block_rows;
+        p.ctas = (int)(units < most_ctas ? units : most_ctas);
+        const size_t parts = (size_t)p.ctas * 2 * places;
+        p.ml = take(parts * sizeof(float2)), p.part = take(parts * dim * sizeof(float)), p.cuts = take((size_t)p.ctas * sizeof(PagedCut));
+    };
+    if (tiles) {
+        s.tiles.tile_rows = kPaRows / group * group;
+        plan(s.tiles, 2 * s.tiles.tile_rows, kPtRows, PtKind::kSetup + cdiv(max_keys, kPtKeys), device_sm_count());
+    }
+    if (!tiles || (seqs > 1 && group <= kFewBeside)) {   // one sequence alone has the rows that the bound says; wider groups are no few rows
+        const bool eight = (tiles ? group : most) <= 8;   // beside the tiles: single tokens, mostly
+        s.split = !tiles ? INT_MAX : eight ? 8 : kFewBeside;
+        plan(s.few, eight ? 8 : 16, eight ? 8 : 16, P4Kind::kSetup + cdiv(max_keys, kP4Keys), dim == 64 ? paged4_few_ctas<64>(eight) : paged4_few_ctas<128>(eight));
+    }
     return s;
 }
 
@@ -57,14 +74,11 @@ template <typename T, int D, int NT>
 static int paged4_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pdl, zl_stream_t stream) {
     using C = P4Cfg<D, NT>;
     static bool done[64] = {};
-    ZL_CHECK_WAITS();
-    unsigned* words = wait_words();
-    ZL_CHECK_CUDA(words ? cudaSuccess : cudaErrorMemoryAllocation);
     ZL_CHECK_CUDA(allow_smem(k_paged_attn4_few<T, D, NT>, C::kBytes, done));
     CUtensorMap maps[2] = {};
     const int tma = c.page_size % 16 == 0 && p4_maps<D>(maps, p, c);
-    ZL_CHECK_CUDA(launch(k_paged_attn4_few<T, D, NT>, dim3(ctas), dim3(kP4Warps * 32), C::kBytes, stream, pdl, p, c, maps[0], maps[1], tma, words + kWaitAttnPaged));
-    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 8 * NT, 8>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p));
+    ZL_CHECK_CUDA(launch(k_paged_attn4_few<T, D, NT>, dim3(ctas), dim3(kP4Warps * 32), C::kBytes, stream, pdl, p, c, maps[0], maps[1], tma, wait_words() + kWaitAttnPaged));
+    if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 8 * NT>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p));
     return ZL_OK;
 }
 
@@ -72,22 +86,32 @@ template <typename T, int D>
 static int paged4_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool pdl, zl_stream_t stream) {
     using C = PtCfg<D, true>;
     static bool done[64] = {};
-    ZL_CHECK_WAITS();
-    unsigned* words = wait_words();
-    ZL_CHECK_CUDA(words ? cudaSuccess : cudaErrorMemoryAllocation);
     ZL_CHECK_CUDA(allow_smem(k_paged_attn_tiles<T, D, true>, C::kBytes, done));
     CUtensorMap q_map = {};
     const CUtensorMapDataType dt = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     ZL_CHECK_CUDA(pt_q_map<D>(&q_map, p, dt) ? cudaSuccess : cudaErrorInvalidValue);
-    ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D, true>, dim3(ctas), dim3(kPtThreads<true>), C::kBytes, stream, pdl, p, c, q_map, q_map, q_map, 0, words + kWaitAttnPaged));
+    ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D, true>, dim3(ctas), dim3(kPtThreads<true>), C::kBytes, stream, pdl, p, c, q_map, q_map, q_map, 0, wait_words() + kWaitAttnPaged));
     if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join_tiles<T, D>, dim3(ctas, kPtRows / 32), dim3(256), 0, stream, true, p));
     return ZL_OK;
 }
 
 template <typename T, int D>
-static int paged4(const PagedAttn& p, const PagedCache& c, const Paged4Plan& s, bool pdl, zl_stream_t stream) {
-    if (s.tiles) return paged4_tiles<T, D>(p, c, s.ctas, pdl, stream);
-    return s.block_rows == 8 ? paged4_few<T, D, 1>(p, c, s.ctas, pdl, stream) : paged4_few<T, D, 2>(p, c, s.ctas, pdl, stream);
+static int paged4(PagedAttn p, const PagedCache& c, const Paged4Plans& s, uint8_t* ws, bool pdl, zl_stream_t stream) {
+    ZL_CHECK_WAITS();
+    ZL_CHECK_CUDA(wait_words() ? cudaSuccess : cudaErrorMemoryAllocation);
+    auto with = [&](const Paged4Plan& plan) {
+        p.block_rows = plan.block_rows, p.tile_rows = plan.tile_rows;
+        p.ml = reinterpret_cast<float2*>(ws + plan.ml), p.part = reinterpret_cast<float*>(ws + plan.part), p.cuts = reinterpret_cast<PagedCut*>(ws + plan.cuts);
+    };
+    const bool both = s.few.ctas && s.tiles.ctas;
+    p.split = s.split;
+    if (s.few.ctas) {
+        with(s.few);
+        const int rc = s.few.block_rows == 8 ? paged4_few<T, D, 1>(p, c, s.few.ctas, pdl, stream) : paged4_few<T, D, 2>(p, c, s.few.ctas, pdl, stream);
+        if (rc || !both) return rc;
+    }
+    with(s.tiles);
+    return paged4_tiles<T, D>(p, c, s.tiles.ctas, pdl || both, stream);
 }
 
 }  // namespace zl
@@ -111,15 +135,15 @@ extern "C" int zl_paged_attention_int4(const void* q, const void* k_cache, const
     ZL_CHECK_SUPPORTED(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0);
     ZL_CHECK_SUPPORTED(heads <= 65535 && (long long)rows * heads < INT_MAX);
     const long long room = (long long)max_pages * page_size;
-    const Paged4Plan s = paged4_plan(rows, max_new, seqs, (int)(room < INT_MAX - 255 ? room : INT_MAX - 255), heads, kv_heads, dim);
+    const Paged4Plans s = paged4_plan(rows, max_new, seqs, (int)(room < INT_MAX - 255 ? room : INT_MAX - 255), heads, kv_heads, dim);
     // the kernels count tiles in 32 bits
-    ZL_CHECK_SUPPORTED(((long long)rows * (heads / kv_heads) / (s.tiles ? kPaRows / 2 : s.block_rows) + seqs) * (room / kP4Keys + 2 + P4Kind::kSetup) < (INT_MAX - (1 << 16)) / kv_heads);
+    const int least_rows = s.few.ctas ? s.few.block_rows : kPaRows / 2;   // of a block
+    ZL_CHECK_SUPPORTED(((long long)rows * (heads / kv_heads) / least_rows + seqs) * (room / kP4Keys + 2 + P4Kind::kSetup) < (INT_MAX - (1 << 16)) / kv_heads);
     ZL_CHECK_ARG(workspace && workspace_bytes >= s.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
     const PagedCache c = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), num_pages, page_stride, row_stride, head_stride, page_table, ld_table, max_pages,
                           page_size, seqs, paged_divisor(page_size)};
+    const PagedAttn p = {q, out, seq_lens, q_starts, rows, heads, heads / kv_heads, window, paged_divisor(heads / kv_heads), scale * 1.4426950408889634f, kv_heads};
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    const PagedAttn p = {q, out, seq_lens, q_starts, rows, heads, heads / kv_heads, window, paged_divisor(heads / kv_heads), scale * 1.4426950408889634f, kv_heads,
-                         s.block_rows, s.tile_rows, reinterpret_cast<float2*>(ws + s.ml), reinterpret_cast<float*>(ws + s.part), reinterpret_cast<PagedCut*>(ws + s.cuts)};
-    if (dtype == ZL_F16) return dim == 64 ? paged4<__half, 64>(p, c, s, pdl != 0, stream) : paged4<__half, 128>(p, c, s, pdl != 0, stream);
-    return dim == 64 ? paged4<__nv_bfloat16, 64>(p, c, s, pdl != 0, stream) : paged4<__nv_bfloat16, 128>(p, c, s, pdl != 0, stream);
+    if (dtype == ZL_F16) return dim == 64 ? paged4<__half, 64>(p, c, s, ws, pdl != 0, stream) : paged4<__half, 128>(p, c, s, ws, pdl != 0, stream);
+    return dim == 64 ? paged4<__nv_bfloat16, 64>(p, c, s, ws, pdl != 0, stream) : paged4<__nv_bfloat16, 128>(p, c, s, ws, pdl != 0, stream);
 }

@@ -78,6 +78,7 @@ struct P4Codes {
 // tiles of 128 keys; at least one: a block that sees nothing is written too
 struct P4Kind {
     static constexpr int kSetup = 2;
+    static __device__ __forceinline__ bool takes(const PagedAttn& p, int rows) { return rows <= p.split; }
     static __device__ __forceinline__ int turns(const PagedAttn&, const PagedBlock& k) { return k.hi >= 0 ? k.hi / kP4Keys - k.lo / kP4Keys + 1 : 1; }
 };
 

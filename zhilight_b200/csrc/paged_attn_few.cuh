@@ -33,6 +33,7 @@ struct PfCfg {
 // tiles of 64 keys; at least one: a block that sees nothing is written too
 struct PfKind {
     static constexpr int kSetup = 2;
+    static __device__ __forceinline__ bool takes(const PagedAttn&, int) { return true; }
     static __device__ __forceinline__ int turns(const PagedAttn&, const PagedBlock& k) { return k.hi >= 0 ? k.hi / kPfKeys - k.lo / kPfKeys + 1 : 1; }
 };
 
