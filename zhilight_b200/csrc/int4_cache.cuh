@@ -18,6 +18,16 @@ namespace zl {
 constexpr int kInt4Group = 32;
 constexpr int int4_row_bytes(int dim) { return dim / 8 * 5; }
 
+// How 16 rows of a head of a 4-bit cache come to shared memory, and lie there.  Heads of 128: as a box of whole rows of 80 bytes.  Heads of 64, whose 40 bytes are no multiple of 16: as
+// one piece where they lie behind one another (kRun), else 48 bytes of each row, from the 16-byte border at or before it, where a row has its heads behind one another (kWide).
+// None of these, or pages that do not hold whole 16s: by copies of D / 8 bytes.
+enum { kInt4Copies, kInt4Run, kInt4Wide };
+template <int D>
+constexpr int kInt4Pitch = D == 128 ? 80 : 48;   // most
+template <int D>
+__device__ __forceinline__ int int4_pitch(int form) { return D == 128 ? 80 : form == kInt4Wide ? 48 : 40; }
+template <int D>
+__device__ __forceinline__ int int4_skip(int form, int hk) { return D == 64 && form == kInt4Wide ? (hk & 1) * 8 : 0; }
 template <typename T>
 struct Int4Pair {
     using type = __half2;

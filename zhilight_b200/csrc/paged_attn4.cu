@@ -56,18 +56,22 @@ static Paged4Plans paged4_plan(int rows, int max_new, int seqs, int max_keys, in
     return s;
 }
 
-// Boxes of 16 rows of K and of V, as words of 32 bits: whole rows of 80 bytes, or (rows of 40, which are no multiple of 16) what 16 rows hold where those lie behind one another
+// Boxes of 16 rows of K and of V (int4_box), as words of 32 bits: -> kInt4Copies where there are none
 template <int D>
-static bool p4_maps(CUtensorMap (&maps)[2], const PagedAttn& p, const PagedCache& c) {
-    constexpr int kRow = int4_row_bytes(D);
-    if (D == 64 && c.row_stride != kRow && c.page_size > 1) return false;
+static int p4_maps(CUtensorMap (&maps)[2], const PagedAttn& p, const PagedCache& c) {
+    constexpr int kRow = int4_row_bytes(D), kWords = kRow / 4;
+    if (c.page_size % 16 != 0) return kInt4Copies;
+    const bool run = D == 128 || c.row_stride == kRow, wide = !run && (p.kv_heads == 1 || c.head_stride == kRow);
+    if (!run && !wide) return kInt4Copies;
     auto step = [](long long bytes, bool more) { return more ? (uint64_t)bytes : 16u; };   // of one alone none is taken
-    const uint64_t dims[4] = {(uint64_t)(D == 128 ? kRow / 4 : c.page_size * (kRow / 4)), (uint64_t)(D == 128 ? c.page_size : 1), (uint64_t)p.kv_heads, (uint64_t)c.num_pages};
-    const uint64_t strides[3] = {step(c.row_stride, D == 128 && c.page_size > 1), step(c.head_stride, p.kv_heads > 1), step(c.page_stride, c.num_pages > 1)};
-    const uint32_t box[4] = {D == 128 ? kRow / 4 : 16 * (kRow / 4), D == 128 ? 16 : 1, 1, 1};
+    const bool rows = D == 128 || wide;
+    const uint64_t dims[4] = {(uint64_t)(D == 128 ? kWords : wide ? p.kv_heads * kWords : c.page_size * kWords), (uint64_t)(rows ? c.page_size : 1), (uint64_t)(wide ? 1 : p.kv_heads),
+                              (uint64_t)c.num_pages};
+    const uint64_t strides[3] = {step(c.row_stride, rows), step(c.head_stride, !wide && p.kv_heads > 1), step(c.page_stride, c.num_pages > 1)};
+    const uint32_t box[4] = {(uint32_t)(D == 128 ? kWords : wide ? 12 : 16 * kWords), rows ? 16u : 1u, 1, 1};
     for (int i = 0; i < 2; ++i)
-        if (!tc_make_map_nd(&maps[i], i ? c.v : c.k, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return false;
-    return true;
+        if (!tc_make_map_nd(&maps[i], i ? c.v : c.k, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return kInt4Copies;
+    return wide ? kInt4Wide : kInt4Run;
 }
 
 template <typename T, int D, int NT>
@@ -76,8 +80,8 @@ static int paged4_few(const PagedAttn& p, const PagedCache& c, int ctas, bool pd
     static bool done[64] = {};
     ZL_CHECK_CUDA(allow_smem(k_paged_attn4_few<T, D, NT>, C::kBytes, done));
     CUtensorMap maps[2] = {};
-    const int tma = c.page_size % 16 == 0 && p4_maps<D>(maps, p, c);
-    ZL_CHECK_CUDA(launch(k_paged_attn4_few<T, D, NT>, dim3(ctas), dim3(kP4Warps * 32), C::kBytes, stream, pdl, p, c, maps[0], maps[1], tma, wait_words() + kWaitAttnPaged));
+    const int form = p4_maps<D>(maps, p, c);
+    ZL_CHECK_CUDA(launch(k_paged_attn4_few<T, D, NT>, dim3(ctas), dim3(kP4Warps * 32), C::kBytes, stream, pdl, p, c, maps[0], maps[1], form, wait_words() + kWaitAttnPaged));
     if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join<T, D, 8 * NT>, dim3(ctas), dim3(kJoinWarps * 32), 0, stream, true, p));
     return ZL_OK;
 }
@@ -87,10 +91,11 @@ static int paged4_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool 
     using C = PtCfg<D, true>;
     static bool done[64] = {};
     ZL_CHECK_CUDA(allow_smem(k_paged_attn_tiles<T, D, true>, C::kBytes, done));
-    CUtensorMap q_map = {};
+    CUtensorMap q_map = {}, maps[2] = {};
+    const int form = p4_maps<D>(maps, p, c);
     const CUtensorMapDataType dt = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     ZL_CHECK_CUDA(pt_q_map<D>(&q_map, p, dt) ? cudaSuccess : cudaErrorInvalidValue);
-    ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D, true>, dim3(ctas), dim3(kPtThreads<true>), C::kBytes, stream, pdl, p, c, q_map, q_map, q_map, 0, wait_words() + kWaitAttnPaged));
+    ZL_CHECK_CUDA(launch(k_paged_attn_tiles<T, D, true>, dim3(ctas), dim3(kPtThreads<true>), C::kBytes, stream, pdl, p, c, q_map, maps[0], maps[1], form, wait_words() + kWaitAttnPaged));
     if (ctas > 1) ZL_CHECK_CUDA(launch(k_paged_join_tiles<T, D>, dim3(ctas, kPtRows / 32), dim3(256), 0, stream, true, p));
     return ZL_OK;
 }

@@ -11,8 +11,8 @@
 //   P: the scores' accumulators, rounded to 16 bits, are the second operand once 8 x 8 of them are transposed (movmatrix).
 // Probabilities are rounded to the rows' type once (half a step each, of random sign: beside the output's own rounding), sums are in 32 bits.
 //
-// Codes of bf16 rows become numbers by one `and` and one fma for two (P4Codes).  16 rows of a head come by one TMA box where a page holds whole 16s of them and its map can be made
-// (heads of 128; heads of 64 where the rows of a head lie behind one another), else by copies of D / 8 bytes.
+// Codes of bf16 rows become numbers by one `and` and one fma for two (P4Codes).  16 rows of a head come by one TMA box where a page holds whole 16s of them, else by copies
+// (kInt4Copies ...).
 #pragma once
 #include "int4_cache.cuh"
 #include "paged_attn_few.cuh"
@@ -24,8 +24,8 @@ constexpr int kP4Warps = 4, kP4Each = 32, kP4Keys = kP4Each * kP4Warps, kP4Stage
 
 template <int D, int NT>
 struct P4Cfg {
-    static constexpr int kChunk = D / 8, kRow = 5 * kChunk;          // bytes copied at once; of a row, four chunks of codes and one of pairs
-    static constexpr int kV = kP4Each * kRow, kStage = 2 * kV;       // rows of K, then of V
+    static constexpr int kChunk = D / 8;                             // bytes copied at once; of a row, four chunks of codes and one of pairs
+    static constexpr int kV = kP4Each * kInt4Pitch<D>, kStage = 2 * kV;   // rows of K, then of V
     static constexpr int kWarp = kP4Stages * kStage;
     static constexpr int kBytes = kP4Warps * kWarp;
     static constexpr int kPitch = D + 8;                             // floats; of a row of a warp's output in its ring
@@ -106,7 +106,7 @@ __device__ __forceinline__ void p4_words(uint32_t (&w)[N], const uint8_t* at) {
     }
 }
 
-// grid: CTAs that share the line; blocks of up to 8 NT rows.  tma: 16 rows come as a box of k_map and v_map
+// grid: CTAs that share the line; blocks of up to 8 NT rows.  tma: one of kInt4Copies ...
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm))
 k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, int tma, unsigned* err) {
@@ -140,6 +140,7 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
         int first, count;
         walk.share(first, count);
         if (count == 0) continue;
+        const int pitch = int4_pitch<D>(tma), skip = int4_skip<D>(tma, at.hk);
         const int key0 = ((k.hi >= 0 ? k.lo / kP4Keys : 0) + first) * kP4Keys + warp * kP4Each;
         // The lanes ask for the page numbers of the rows a stage ahead; where pages hold whole 16s lanes 0 and 1 do
         auto find = [&](int j) {
@@ -149,13 +150,13 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
         auto copy = [&](int j, int id) {
             const int stage = (used + j) % kP4Stages, row0 = key0 + j * kP4Keys;
             if (tma) {
-                if (lane == 0) mbar_expect_tx(&full[warp][stage], C::kStage);
+                if (lane == 0) mbar_expect_tx(&full[warp][stage], 2 * kP4Each * pitch);
                 __syncwarp();
                 if (lane < 2) {
                     const int row16 = row0 + lane * 16, row = row16 - c.by_page(row16) * c.page_size, page = id >= 0 && id < c.num_pages ? id : -1;   // -1: reads as zeros
-                    const uint32_t to = ring_at + (uint32_t)(stage * C::kStage + lane * (16 * C::kRow));
-                    pt_load_4d(to, &k_map, D == 128 ? 0 : row * (C::kRow / 4), D == 128 ? row : 0, at.hk, page, &full[warp][stage]);
-                    pt_load_4d(to + C::kV, &v_map, D == 128 ? 0 : row * (C::kRow / 4), D == 128 ? row : 0, at.hk, page, &full[warp][stage]);
+                    const uint32_t to = ring_at + (uint32_t)(stage * C::kStage + lane * 16 * pitch);
+                    int4_box<D>(to, &k_map, tma, at.hk, row, page, &full[warp][stage]);
+                    int4_box<D>(to + C::kV, &v_map, tma, at.hk, row, page, &full[warp][stage]);
                 }
             } else {
                 const int mine = row0 + lane;
@@ -165,7 +166,7 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                 for (int x = lane; x < 10 * kP4Each; x += 32) {
                     const int is_v = x >= 5 * kP4Each, r = (x - 5 * kP4Each * is_v) / 5, ch = (x - 5 * kP4Each * is_v) % 5;
                     const long long o = __shfl_sync(0xffffffffu, off, r);
-                    p4_copy<C::kChunk>(ring_at + (uint32_t)(stage * C::kStage + x * C::kChunk), static_cast<const uint8_t*>(is_v ? c.v : c.k) + (o < 0 ? 0 : o + ch * C::kChunk),
+                    p4_copy<C::kChunk>(ring_at + (uint32_t)(stage * C::kStage + is_v * C::kV + (x - 5 * kP4Each * is_v) * C::kChunk), static_cast<const uint8_t*>(is_v ? c.v : c.k) + (o < 0 ? 0 : o + ch * C::kChunk),
                                        o < 0 ? 0 : C::kChunk);
                 }
             }
@@ -232,8 +233,8 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                     if (kb + lane > k.hi)
 #pragma unroll
                         for (int i = 0; i < D / kInt4Group; ++i) {
-                            *reinterpret_cast<uint32_t*>(st + lane * C::kRow + D / 2 + i * 4) = 0;
-                            *reinterpret_cast<uint32_t*>(st + C::kV + lane * C::kRow + D / 2 + i * 4) = 0;
+                            *reinterpret_cast<uint32_t*>(st + lane * pitch + skip + D / 2 + i * 4) = 0;
+                            *reinterpret_cast<uint32_t*>(st + C::kV + lane * pitch + skip + D / 2 + i * 4) = 0;
                         }
                     pa_fence_async();
                     __syncwarp();
@@ -245,7 +246,7 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                     P4Codes<T, SLOW> k_code[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint8_t* row = st + (16 * h + g + u * 8) * C::kRow;
+                        const uint8_t* row = st + (16 * h + g + u * 8) * pitch + skip;
                         p4_words<KW>(x[u], row + t4 * C::kChunk);
                         const uint32_t pair = P4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + t4 * (D / 4) / kInt4Group * 4), track);
                         k_code[u].set(__byte_perm(pair, 0, 0x1010), __byte_perm(pair, 0, 0x3232));
@@ -295,7 +296,7 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint8_t* values = st + C::kV + 16 * h * C::kRow;
+                    const uint8_t* values = st + C::kV + 16 * h * pitch + skip;
                     uint32_t pb[NT][2];
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -308,11 +309,11 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                         }
                     if constexpr (SLOW) {
                         bool whole = true;
-                        for (int x = lane; x < D / 2; x += 32) whole = whole && int4_finite<T>(*reinterpret_cast<const uint32_t*>(values + x % 16 * C::kRow + D / 2 + x / 16 * 4));
+                        for (int x = lane; x < D / 2; x += 32) whole = whole && int4_finite<T>(*reinterpret_cast<const uint32_t*>(values + x % 16 * pitch + D / 2 + x / 16 * 4));
                         if (__any_sync(0xffffffffu, !whole)) {   // the product key by key
 #pragma unroll 1
                             for (int key = 0; key < 16; ++key) {
-                                const uint8_t* row = values + key * C::kRow;
+                                const uint8_t* row = values + key * pitch;
                                 const uint32_t meta = *reinterpret_cast<const uint32_t*>(row + D / 2 + g * (D / 8) / kInt4Group * 4);
                                 uint32_t x[VW];
                                 p4_words<VW>(x, row + g * (D / 16));
@@ -337,7 +338,7 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                     uint32_t x[4][VW], pair[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {   // keys 2t + {0, 1, 8, 9}
-                        const uint8_t* row = values + (2 * t4 + (u & 1) + (u >> 1) * 8) * C::kRow;
+                        const uint8_t* row = values + (2 * t4 + (u & 1) + (u >> 1) * 8) * pitch;
                         p4_words<VW>(x[u], row + g * (D / 16));
                         pair[u] = P4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + g * (D / 8) / kInt4Group * 4), track);
                     }

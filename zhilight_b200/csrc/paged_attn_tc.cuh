@@ -99,7 +99,7 @@ struct PtCfg {
     static constexpr int kTile = kAtoms * kPtHalf * 128;    // K or V: [64 of d][64 keys][128 B]
     static constexpr int kRing = D == 64 ? 16 : INT4 ? 8 : 10;
     static constexpr int kRaw = D == 64 ? 6 : 3;            // tiles of codes, of keys and as many of values
-    static constexpr int kCodes = kPtHalf * (D / 8 * 5);    // a tile's codes and pairs
+    static constexpr int kCodes = kPtHalf * kInt4Pitch<D>;  // a tile's codes and pairs
     static constexpr int kRingOff = 2 * kQ, kRawOff = kRingOff + kRing * kTile;
     static constexpr int kBytes = kRawOff + (INT4 ? 2 * kRaw * kCodes : 0) + 1024;   // + slack for the manual 1024-byte alignment
     static_assert(tmem_alone(kBytes) && kBytes + 1024 <= 227 * 1024, "all of tensor memory, an SM to itself");
@@ -123,6 +123,12 @@ __device__ __forceinline__ void pt_load_3d(uint32_t dst, const CUtensorMap* map,
 // tc2_wait for a barrier whose phase has mostly ended by now: all lanes look once
 __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile int* s_abort, unsigned* err, unsigned code) {
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || tc2_wait(bar, parity, s_abort, err, code);
+}
+
+template <int D>
+__device__ __forceinline__ void int4_box(uint32_t dst, const CUtensorMap* map, int form, int hk, int row, int page, uint64_t* bar) {
+    const bool wide = D == 64 && form == kInt4Wide;
+    pt_load_4d(dst, map, D == 128 ? 0 : wide ? hk * 10 - (hk & 1) * 2 : row * 10, D == 128 || wide ? row : 0, wide ? 0 : hk, page, bar);
 }
 
 template <typename T>
@@ -215,7 +221,7 @@ __device__ __noinline__ void pt_add_broken4(const PagedCache& c, int seq, long l
     }
 }
 
-// grid: CTAs that share the line.  box: rows of a TMA box of K and V, 0: no TMA.  INT4: k_map and v_map are not looked at
+// grid: CTAs that share the line.  box: rows of a TMA box of K and V, 0: no TMA.  INT4: one of kInt4Copies ..., for boxes of 16 rows
 template <typename T, int D, bool INT4 = false>
 __global__ void __launch_bounds__(kPtThreads<INT4>, 1)
 k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -237,7 +243,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
         for (int i = 0; i < C::kRing; ++i) mbar_init(&full[i], INT4 ? kPtHalf / 16 : box ? 1 : kPtLoaders), mbar_init(&empty[i], 1);
         for (int i = 0; i < 4; ++i) mbar_init(&s_full[i >> 1][i & 1], 1), mbar_init(&p_full[i >> 1][i & 1], 4), mbar_init(&o_done[i >> 1][i & 1], 1);
         if constexpr (INT4)
-            for (int i = 0; i < 2 * C::kRaw; ++i) mbar_init(&raw_full[i & 1][i >> 1], 32), mbar_init(&raw_empty[i & 1][i >> 1], 4);
+            for (int i = 0; i < 2 * C::kRaw; ++i) mbar_init(&raw_full[i & 1][i >> 1], box ? 1 : 32), mbar_init(&raw_empty[i & 1][i >> 1], 4);
         mbar_init(&q_full, 1), mbar_init(&q_free, 1), mbar_init(&o_free, 8), mbar_init(&joined, 4);
         s_gave_up = s_blocks[0] = s_blocks[1] = 0;
         mbar_fence_init();
@@ -360,7 +366,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                 // have been used.
                 if (m == 0 || !two_rows) {
                     const int behind = min(k.hi + 1 - base, kPtHalf);   // rows that hold keys
-                    const bool look = behind > 0 && (base + behind - 1 > all_hi || base < all_lo), cut = box && behind > 0 && behind % box != 0;
+                    const bool look = behind > 0 && (base + behind - 1 > all_hi || base < all_lo), cut = !INT4 && box && behind > 0 && behind % box != 0;
                     if (look || cut) {
                         const int it = ring + j * items + (two_rows ? 1 : 2 + m), slot = it % C::kRing;
                         if (!tc2_wait(&full[slot], (uint32_t)(it / C::kRing) & 1u, s_abort, err, 0x5800 + slot)) break;
@@ -539,7 +545,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             };
             if constexpr (INT4) {
                 constexpr int kChunk = D / 8, kEach = 5 * kPtHalf / 32;
-                const int tiles = count * items;   // of keys, and as many of values
+                const int tiles = count * items, pitch = int4_pitch<D>(box), skip = int4_skip<D>(box, at.hk);   // of keys, and as many of values
                 if (warp < kPtWarpLoad4) {
                     // A lane looks up rows lane and lane + 32 of the tile, a tile ahead, and copies ten of its 320 chunks
                     const int is_v = warp - kPtWarpLoad;
@@ -549,7 +555,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                     auto ask = [&](int n) {
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
-                            const int row = first_row(n) + u * 32 + lane, pg = c.by_page(row);
+                            const int row = first_row(n) + (box ? (lane & 3) * 16 : u * 32 + lane), pg = c.by_page(row);
                             ids[u] = n < tiles && row <= k.hi && pg < c.max_pages ? c.table[(size_t)k.seq * c.ld_table + pg] : -1;
                         }
                     };
@@ -557,6 +563,18 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                     for (int n = 0; n < tiles && ok; ++n) {
                         if (n == 1) load_q();
                         const int it = ring / 2 + n, slot = it % C::kRaw;
+                        if (box) {   // four boxes of 16 rows, a lane each
+                            const int id = ids[0] >= 0 && ids[0] < c.num_pages ? ids[0] : -1, row = first_row(n) + (lane & 3) * 16;   // -1: reads as zeros
+                            ask(n + 1);
+                            if (it >= C::kRaw) ok = ok && pt_wait(&raw_empty[is_v][slot], (uint32_t)(it / C::kRaw - 1) & 1u, s_abort, err, 0x5a00 + is_v);
+                            if (!ok) break;
+                            if (lane == 0) mbar_expect_tx(&raw_full[is_v][slot], kPtHalf * pitch);
+                            __syncwarp();
+                            if (lane < 4)
+                                int4_box<D>(smem_u32(smem) + (uint32_t)(C::kRawOff + (is_v * C::kRaw + slot) * C::kCodes + lane * 16 * pitch), is_v ? &v_map : &k_map, box, at.hk,
+                                            row - c.by_page(row) * c.page_size, id, &raw_full[is_v][slot]);
+                            continue;
+                        }
                         long long offs[2];
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
@@ -590,8 +608,9 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                             ok = ok && pt_wait(&raw_full[v][raw], (uint32_t)(it / C::kRaw) & 1u, s_abort, err, 0x5b00 + v);
                             if (i + t >= C::kRing) ok = ok && pt_wait(&empty[slot], (uint32_t)((i + t) / C::kRing - 1) & 1u, s_abort, err, 0x5500 + slot);
                             if (!ok) break;
-                            const uint8_t* from = smem + C::kRawOff + (v * C::kRaw + raw) * C::kCodes + row * (5 * kChunk);
+                            const uint8_t* from = smem + C::kRawOff + (v * C::kRaw + raw) * C::kCodes + row * pitch + skip;
                             uint8_t* to = smem + C::kRingOff + slot * C::kTile + row * 128;
+                            const int first = row_of(2 * x + t);
 #pragma unroll 1
                             for (int u = 0; u < D / 64; ++u) {
                                 const int g = 2 * u + (lane >> 4);
@@ -603,7 +622,8 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                                     const uint2 y = *reinterpret_cast<const uint2*>(from + g * 16), z = *reinterpret_cast<const uint2*>(from + g * 16 + 8);
                                     w[0] = y.x, w[1] = y.y, w[2] = z.x, w[3] = z.y;
                                 }
-                                int4_meta<T>(*reinterpret_cast<const uint32_t*>(from + D / 2 + g * 4), step, low);
+                                const uint32_t pair = *reinterpret_cast<const uint32_t*>(from + D / 2 + g * 4);
+                                int4_meta<T>(first + row > k.hi ? 0u : pair, step, low);   // what a page holds behind the last key may be anything
 #pragma unroll
                                 for (int y = 0; y < 4; ++y)
                                     *reinterpret_cast<uint4*>(to + u * (kPtHalf * 128) + ((((lane >> 4) * 4 + y) ^ (row & 7)) << 4)) = int4_eight<T>(w[y], step, low);
