@@ -83,6 +83,50 @@ __device__ __forceinline__ bool int4_finite(uint32_t meta) {
     return (meta & 0x7fffu) < kInf && (meta >> 16 & 0x7fffu) < kInf;
 }
 
+// Codes as numbers.  fp16: exactly what they stand for.  bf16: that times 2^-20, from a multiplication and a sum that are rounded together, like those of int4_two.  A code
+// at bits 0 - 3 or 4 - 7 is, taken as a bf16 number, c * 2^-133 or 16 c * 2^-133 (also where it reaches the exponent's lowest bit), so the step is multiplied by 2^113 and
+// the lowest value by 2^-20 beforehand.  That overflows for steps from 2^15 on; whoever calls keeps the largest pair in sight (track) and goes over such keys with SLOW.
+template <typename T, bool SLOW>
+struct Int4Codes {
+    static constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;
+    static constexpr float kScale = kScaled ? 1048576.f : 1.f;       // what the numbers are to be multiplied by
+    // pairs (step, lowest) of two groups in, steps and lowest values as operands out: a step for codes at bits 0 - 3 and one for those at bits 4 - 7
+    uint32_t step, step16, low;
+    __device__ __forceinline__ void set(uint32_t s, uint32_t l) {
+        step = s, low = l;
+        if constexpr (kScaled && !SLOW) step16 = times(s, 0x3d803d80u);   // 1 / 16
+    }
+    static __device__ __forceinline__ uint32_t times(uint32_t x, uint32_t y) {
+        using P = typename Int4Pair<T>::type;
+        const P z = __hmul2(*reinterpret_cast<const P*>(&x), *reinterpret_cast<const P*>(&y));
+        return *reinterpret_cast<const uint32_t*>(&z);
+    }
+    // a pair (step, lowest) as it is stored
+    static __device__ __forceinline__ uint32_t pair(uint32_t meta, uint32_t& track) {
+        if constexpr (kScaled && !SLOW) {
+            meta = times(meta, 0x35807800u);                              // 2^113 below, 2^-20 above
+            const __nv_bfloat162 x = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&meta)), *reinterpret_cast<const __nv_bfloat162*>(&track));
+            track = *reinterpret_cast<const uint32_t*>(&x);
+        }
+        return meta;
+    }
+    static __device__ __forceinline__ bool served(uint32_t track) { return (track & 0x7fffu) < 0x7f80u && (track >> 16 & 0x7fffu) < 0x7f80u; }
+    template <int J>
+    __device__ __forceinline__ uint32_t two(uint32_t x) const {
+        if constexpr (!kScaled) {
+            return int4_two<T, J>(x, step, low);
+        } else if constexpr (SLOW) {
+            return times(int4_two<T, J>(x, step, low), 0x35803580u);
+        } else {
+            const uint32_t c = (J & 2 ? x >> 8 : x) & (J & 1 ? 0x00f000f0u : 0x000f000fu);
+            const __nv_bfloat162 y = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&c), *reinterpret_cast<const __nv_bfloat162*>(J & 1 ? &step16 : &step),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&low));
+            return *reinterpret_cast<const uint32_t*>(&y);
+        }
+    }
+    __device__ __forceinline__ uint4 eight(uint32_t x) const { return make_uint4(two<0>(x), two<1>(x), two<2>(x), two<3>(x)); }   // neighbouring columns
+};
+
 template <typename T>
 __device__ __forceinline__ T int4_round_down(float x);
 template <>

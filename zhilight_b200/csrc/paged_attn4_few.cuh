@@ -11,7 +11,7 @@
 //   P: the scores' accumulators, rounded to 16 bits, are the second operand once 8 x 8 of them are transposed (movmatrix).
 // Probabilities are rounded to the rows' type once (half a step each, of random sign: beside the output's own rounding), sums are in 32 bits.
 //
-// Codes of bf16 rows become numbers by one `and` and one fma for two (P4Codes).  16 rows of a head come by one TMA box where a page holds whole 16s of them, else by copies
+// Codes of bf16 rows become numbers by one `and` and one fma for two (Int4Codes).  16 rows of a head come by one TMA box where a page holds whole 16s of them, else by copies
 // (kInt4Copies ...).
 #pragma once
 #include "int4_cache.cuh"
@@ -31,48 +31,6 @@ struct P4Cfg {
     static constexpr int kPitch = D + 8;                             // floats; of a row of a warp's output in its ring
     static_assert(8 * NT * kPitch * 4 <= kWarp, "a warp's output, where its ring was");
     static constexpr int kPerSm = NT == 1 ? 4 : 3;
-};
-
-// Codes as numbers.  fp16: exactly what they stand for.  bf16: that times 2^-20, from a multiplication and a sum that are rounded together, like those of int4_two.  A code
-// at bits 0 - 3 or 4 - 7 is, taken as a bf16 number, c * 2^-133 or 16 c * 2^-133 (also where it reaches the exponent's lowest bit), so the step is multiplied by 2^113 and
-// the lowest value by 2^-20 beforehand.  That overflows for steps from 2^15 on; whoever calls keeps the largest pair in sight (track) and goes over such keys with SLOW.
-template <typename T, bool SLOW>
-struct P4Codes {
-    static constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;
-    static constexpr float kScale = kScaled ? 1048576.f : 1.f;       // what the numbers are to be multiplied by
-    // pairs (step, lowest) of two groups in, steps and lowest values as operands out: a step for codes at bits 0 - 3 and one for those at bits 4 - 7
-    uint32_t step, step16, low;
-    __device__ __forceinline__ void set(uint32_t s, uint32_t l) {
-        step = s, low = l;
-        if constexpr (kScaled && !SLOW) step16 = times(s, 0x3d803d80u);   // 1 / 16
-    }
-    static __device__ __forceinline__ uint32_t times(uint32_t x, uint32_t y) {
-        using P = typename Int4Pair<T>::type;
-        const P z = __hmul2(*reinterpret_cast<const P*>(&x), *reinterpret_cast<const P*>(&y));
-        return *reinterpret_cast<const uint32_t*>(&z);
-    }
-    // a pair as it is stored
-    static __device__ __forceinline__ uint32_t pair(uint32_t meta, uint32_t& track) {
-        if constexpr (kScaled && !SLOW) {
-            meta = times(meta, 0x35807800u);                              // 2^113 below, 2^-20 above
-            const __nv_bfloat162 x = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&meta)), *reinterpret_cast<const __nv_bfloat162*>(&track));
-            track = *reinterpret_cast<const uint32_t*>(&x);
-        }
-        return meta;
-    }
-    template <int J>
-    __device__ __forceinline__ uint32_t two(uint32_t x) const {
-        if constexpr (!kScaled) {
-            return int4_two<T, J>(x, step, low);
-        } else if constexpr (SLOW) {
-            return times(int4_two<T, J>(x, step, low), 0x35803580u);
-        } else {
-            const uint32_t c = (J & 2 ? x >> 8 : x) & (J & 1 ? 0x00f000f0u : 0x000f000fu);
-            const __nv_bfloat162 y = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&c), *reinterpret_cast<const __nv_bfloat162*>(J & 1 ? &step16 : &step),
-                                             *reinterpret_cast<const __nv_bfloat162*>(&low));
-            return *reinterpret_cast<const uint32_t*>(&y);
-        }
-    }
 };
 
 // tiles of 128 keys; at least one: a block that sees nothing is written too
@@ -111,7 +69,7 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm))
 k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, int tma, unsigned* err) {
     using C = P4Cfg<D, NT>;
-    constexpr bool kHalf = std::is_same<T, __half>::value, kScaled = P4Codes<T, false>::kScaled;
+    constexpr bool kHalf = std::is_same<T, __half>::value, kScaled = Int4Codes<T, false>::kScaled;
     constexpr int R = 8 * NT, KS = D / 16, MT = D / 16, KW = D / 32, VW = D / 64;
     // Values times 2^-20 take probabilities of 2^20 more: products and the sums that become parts are those of PagedExp, and the probabilities' sum follows at the end.
     constexpr float kTau = PagedExp<kHalf>::kTau, kUp = PagedExp<kHalf>::kUp + (kScaled ? 20.f : 0.f);
@@ -243,12 +201,12 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t x[2][KW];
-                    P4Codes<T, SLOW> k_code[2];
+                    Int4Codes<T, SLOW> k_code[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const uint8_t* row = st + (16 * h + g + u * 8) * pitch + skip;
                         p4_words<KW>(x[u], row + t4 * C::kChunk);
-                        const uint32_t pair = P4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + t4 * (D / 4) / kInt4Group * 4), track);
+                        const uint32_t pair = Int4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + t4 * (D / 4) / kInt4Group * 4), track);
                         k_code[u].set(__byte_perm(pair, 0, 0x1010), __byte_perm(pair, 0, 0x3232));
                     }
 #pragma unroll
@@ -262,7 +220,7 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                         }
                     }
                 }
-                const float scale = p.scale * P4Codes<T, SLOW>::kScale;
+                const float scale = p.scale * Int4Codes<T, SLOW>::kScale;
                 const bool masks = kb + kP4Each - 1 > all_hi || kb < all_lo;
                 bool up = false;
                 float top[NT][2];
@@ -321,7 +279,7 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                                 float v[D / 8];
 #pragma unroll
                                 for (int i = 0; i < D / 8; ++i)
-                                    v[i] = round_to<T>(fmaf((float)(x[i >> 3] >> ((i & 1) * 16 + (i & 6) * 2) & 15u), to_f32<T>(two[0]), to_f32<T>(two[1]))) / P4Codes<T, SLOW>::kScale;
+                                    v[i] = round_to<T>(fmaf((float)(x[i >> 3] >> ((i & 1) * 16 + (i & 6) * 2) & 15u), to_f32<T>(two[0]), to_f32<T>(two[1]))) / Int4Codes<T, SLOW>::kScale;
 #pragma unroll
                                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -340,9 +298,9 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
                     for (int u = 0; u < 4; ++u) {   // keys 2t + {0, 1, 8, 9}
                         const uint8_t* row = values + (2 * t4 + (u & 1) + (u >> 1) * 8) * pitch;
                         p4_words<VW>(x[u], row + g * (D / 16));
-                        pair[u] = P4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + g * (D / 8) / kInt4Group * 4), track);
+                        pair[u] = Int4Codes<T, SLOW>::pair(*reinterpret_cast<const uint32_t*>(row + D / 2 + g * (D / 8) / kInt4Group * 4), track);
                     }
-                    P4Codes<T, SLOW> v_code[2];
+                    Int4Codes<T, SLOW> v_code[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) v_code[u].set(__byte_perm(pair[2 * u], pair[2 * u + 1], 0x5410), __byte_perm(pair[2 * u], pair[2 * u + 1], 0x7632));
 #pragma unroll
@@ -372,7 +330,7 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
         pass(std::false_type{});
         bool again = false;
         if constexpr (kScaled) {
-            again = (track & 0x7fffu) >= 0x7f80u || (track >> 16 & 0x7fffu) >= 0x7f80u;
+            again = !Int4Codes<T, false>::served(track);
         } else {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -397,7 +355,7 @@ k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = n * 8 + t4 * 2 + e;
-                if (g == 0) s_ml[warp][r] = make_float2(m_ref[n][e], l[n][e] / P4Codes<T, false>::kScale);
+                if (g == 0) s_ml[warp][r] = make_float2(m_ref[n][e], l[n][e] / Int4Codes<T, false>::kScale);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) *reinterpret_cast<float2*>(mine + r * C::kPitch + g * (D / 8) + 2 * m) = make_float2(o[m][n][e], o[m][n][2 + e]);
             }

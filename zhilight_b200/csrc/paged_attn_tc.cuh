@@ -228,6 +228,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                    const __grid_constant__ CUtensorMap v_map, int box, unsigned* err) {
     using C = PtCfg<D, INT4>;
     constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr float kScale = INT4 ? Int4Codes<T, false>::kScale : 1.f;   // of keys and values: probabilities carry it too, the scores' scale and the sums take it away
     constexpr int CH = D / 8;
     extern __shared__ uint8_t pt_smem[];
     uint8_t* smem = pt_smem + ((1024u - (smem_u32(pt_smem) & 1023u)) & 1023u);
@@ -282,8 +283,8 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             const int m = warp >> 2, rt = tid & (kPaRows - 1), r = two_rows ? m * p.tile_rows + rt : rt;   // tile; row of it and of the block
             const bool mine = rt < p.tile_rows && r < k.rows;
             const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = taddr + (uint32_t)(m * 128), to = taddr + (uint32_t)(C::kO + m * D);
-            constexpr float kTau = PagedExp<kHalf>::kTau, kUp = PagedExp<kHalf>::kUp;
-            const float cs = p.scale;
+            constexpr float kTau = PagedExp<kHalf>::kTau, kUp = PagedExp<kHalf>::kUp + (kScale > 1.f ? 20.f : 0.f);
+            const float cs = p.scale * kScale;
             const int row = k.row0 + (mine ? r : 0), t = p.by_group(row), place = k.place0 + t;
             const int hi = mine ? min(place, k.have - 1) : -1, lo = mine ? paged_from(p, place) : 0;
             const int key0 = (t0 + (two_rows ? 0 : m)) * kPtKeys, step = two_rows ? kPtKeys : 2 * kPtKeys;
@@ -390,6 +391,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
             }
             for (int b = 0; b < 2; ++b) tc2_wait(&o_done[m][b], (uint32_t)(turn + count - 1) & 1u, s_abort, err, 0x5700 + m);
             tc_fence_after();
+            l /= kScale;
             // noted before the tile's probabilities were handed on, whose product has ended
             if (__any_sync(0xffffffffu, s_broken[blocks & 1] == blocks + 1))
                 (INT4 ? pt_add_broken4<T, D> : pt_add_broken<T, D>)(c, k.seq, (long long)at.hk * c.head_stride, to, lo, hi, key0, min(t0 * kPtKeys + count * step - 1, k.hi), all_lo, all_hi, step / kPtKeys);
@@ -611,10 +613,10 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                             const uint8_t* from = smem + C::kRawOff + (v * C::kRaw + raw) * C::kCodes + row * pitch + skip;
                             uint8_t* to = smem + C::kRingOff + slot * C::kTile + row * 128;
                             const int first = row_of(2 * x + t);
-#pragma unroll 1
+#pragma unroll
                             for (int u = 0; u < D / 64; ++u) {
                                 const int g = 2 * u + (lane >> 4);
-                                uint32_t w[4], step, low;
+                                uint32_t w[4];
                                 if constexpr (D == 128) {
                                     const uint4 y = *reinterpret_cast<const uint4*>(from + g * 16);
                                     w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
@@ -623,10 +625,18 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                                     w[0] = y.x, w[1] = y.y, w[2] = z.x, w[3] = z.y;
                                 }
                                 const uint32_t pair = *reinterpret_cast<const uint32_t*>(from + D / 2 + g * 4);
-                                int4_meta<T>(first + row > k.hi ? 0u : pair, step, low);   // what a page holds behind the last key may be anything
+                                const uint32_t stored = first + row > k.hi ? 0u : pair;   // what a page holds behind the last key may be anything
+                                auto write = [&](auto codes, uint32_t track) {
+                                    const uint32_t two = decltype(codes)::pair(stored, track);
+                                    codes.set(__byte_perm(two, 0, 0x1010), __byte_perm(two, 0, 0x3232));
 #pragma unroll
-                                for (int y = 0; y < 4; ++y)
-                                    *reinterpret_cast<uint4*>(to + u * (kPtHalf * 128) + ((((lane >> 4) * 4 + y) ^ (row & 7)) << 4)) = int4_eight<T>(w[y], step, low);
+                                    for (int y = 0; y < 4; ++y)
+                                        *reinterpret_cast<uint4*>(to + u * (kPtHalf * 128) + ((((lane >> 4) * 4 + y) ^ (row & 7)) << 4)) = codes.eight(w[y]);
+                                    return decltype(codes)::served(track);
+                                };
+                                const bool served = write(Int4Codes<T, false>{}, 0u);
+                                if constexpr (kScale > 1.f)
+                                    if (__any_sync(0xffffffffu, !served)) write(Int4Codes<T, true>{}, 0u);
                             }
                         }
                         if (!ok) break;
