@@ -63,7 +63,7 @@ HISTORY = dict(tokens=P, ld_tokens=10, seqs=4, longest=10, token_lens=P)
     (dict(HISTORY, token_lens=None), -1), (dict(HISTORY, seqs=3), -1), (dict(HISTORY, ld_tokens=9), -1), (dict(HISTORY, longest=-1), -1),
     (dict(bias_starts=P, n_bias=3), -1), (dict(bias_starts=P, n_bias=-1), -1), (dict(mask=P, ld_mask=3, masks=4), -1), (dict(mask=P, ld_mask=4, masks=3), -1),
     (dict(mask=P, ld_mask=4, masks=0, mask_row=P), -1), (dict(out_dtype=ops.F16), -2), (dict(dtype=ops.F32, out_dtype=ops.BF16), -2), (dict(dtype=9, out_dtype=9), -2),
-    (dict(vocab=1 << 25, ld_logits=1 << 25, ld_out=1 << 25), -2), (dict(rows=(1 << 31) - 1, vocab=4097, ld_logits=5000, ld_out=5000), -2)])
+    (dict(vocab=1 << 25, ld_logits=1 << 25, ld_out=1 << 25), -2), (dict(rows=(1 << 31) - 1, vocab=1 << 24, ld_logits=1 << 24, ld_out=1 << 24), -2)])
 def test_adjust_refuses(lib, kw, code):
     assert lib.zl_adjust_logits(*adjust_args(**kw)) == code, lib.zl_last_error()
 
