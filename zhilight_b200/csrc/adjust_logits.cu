@@ -6,26 +6,30 @@
 //
 // A CTA has a piece of a row's vocabulary, with a counter in shared memory for each word: how often it came, whether it is in the history, whether there is a bias.  Every CTA goes
 // over the whole history and counts the words of its piece by atomics of its own shared memory: whole numbers, which add up the same in every order.  (With the history
-// shared out among the CTAs of a cluster, and counts sent to the piece's owner: 52 us where this takes %s, 117 rows behind 9000 words, of which most are
-// frequent ones that one CTA owns.)  A warp whose 32 words are one counts it once, so that a history of one word does not queue up.  The logits' first loads are
+// shared out among the CTAs of a cluster, and counts sent to the piece's owner: 52 us where this takes %s, 117 rows behind up to 9000 words, of which most are
+// frequent ones that one CTA owns.)  Where 256 words are one it is counted once, so that a history of one word does not queue up.  The logits' first loads are
 // on their way meanwhile.
 //
-// Biases of a piece stand in a list, in their order, with their words' logits as they were; once the piece is written a thread for each word writes those
-// again.  (A search of the list at every marked word took most of the time: 300 biases a row.)  Of a list that is too long for this, each marked word
-// goes over the row's own list.
+// Few words of a piece are marked, mostly.  Whoever marks a word first puts it on a list; the piece is written as if there were none, and the marked words once more behind that.
+// (With penalties worked out at every word, which costs three times the instructions of the rest, 64 rows of 128256 took 20 us instead of %s.)  Where
+// the list is too long, or out is in, that is done all the same.  Biases of a piece stand in a second list, in their order; of one that is too long for it the words go over the
+// row's own.
 #include "paged.cuh"
+
+#include <type_traits>
 
 namespace zl {
 
-constexpr int kAlThreads = 512, kAlAhead = 4;
+constexpr int kAlAhead = 4, kAlList = 512;
 
-// A counter: whether the word is in the history, whether there is a bias, how often it came behind the prompt.  16 bits where histories are short enough.
+// A counter: whether the word is in the history, whether there is a bias, how often it came behind the prompt.  16 bits where histories are short enough, two to a word of 32.
 template <typename C>
 struct AlCounter {
-    static constexpr int kBits = 8 * sizeof(C);
-    static constexpr uint32_t kSeen = 1u << (kBits - 1), kBias = 1u << (kBits - 2), kCount = kBias - 1, kEach = 32 / kBits;   // of 32 bits
-    static __device__ __forceinline__ uint32_t* at(uint32_t* words, int i) { return words + i / kEach; }
-    static __device__ __forceinline__ uint32_t shifted(uint32_t x, int i) { return x << (i % kEach * kBits); }
+    static constexpr int kBits = 8 * sizeof(C), kEach = 32 / kBits;
+    static constexpr uint32_t kSeen = 1u << (kBits - 1), kBias = 1u << (kBits - 2), kCount = kBias - 1;
+    // before the change
+    static __device__ __forceinline__ uint32_t add(uint32_t* c, int i, uint32_t n) { return (C)(atomicAdd(c + i / kEach, n << (i % kEach * kBits)) >> (i % kEach * kBits)); }
+    static __device__ __forceinline__ uint32_t mark(uint32_t* c, int i, uint32_t bit) { return (C)(atomicOr(c + i / kEach, bit << (i % kEach * kBits)) >> (i % kEach * kBits)); }
 };
 constexpr int kAlShort = 0x3fff;
 
@@ -36,7 +40,7 @@ struct AdjustLogits {
     const int32_t *tokens, *token_seq, *token_lens, *prompt_lens, *bias_starts, *bias_words, *mask, *mask_row;
     const float *repetition, *frequency, *presence, *bias, *temperature;
     long long ld_tokens, ld_mask;
-    int seqs, longest, n_bias, masks, vocab, pieces, piece;
+    int seqs, longest, n_bias, masks, vocab, pieces, piece, in_place, room;   // room: of the list of marked words
     PagedDivisor by_pieces;
 };
 
@@ -49,164 +53,235 @@ __device__ __forceinline__ void al_load(TI (&v)[VEC], const TI* at) {
 }
 
 // grid: pieces of rows; dynamic shared memory: a counter for each of the piece's words, where there is a history or a bias
-template <typename TI, typename TO, typename C, int VEC>
-__global__ void __launch_bounds__(kAlThreads) k_adjust_logits(const AdjustLogits p) {
+template <typename TI, typename TO, typename C, int VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p) {
     using Counter = AlCounter<C>;
-    constexpr int kAhead = VEC == 1 ? 8 : 2, kStep = kAlThreads * VEC;
+    constexpr int kAhead = VEC == 1 ? 8 : 4, kStep = THREADS * VEC, kEach = (kAlList + THREADS - 1) / THREADS;
     extern __shared__ __align__(16) uint32_t al_count[];
-    __shared__ int s_words[kAlThreads], s_have[kAlThreads / 32];
-    __shared__ float s_bias[kAlThreads], s_logit[kAlThreads];
+    constexpr int kHave = kEach * THREADS / 32;
+    __shared__ int s_words[kAlList], s_have[kHave];
+    __shared__ float s_bias[kAlList];
+    __shared__ int s_marks;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r = p.by_pieces((int)blockIdx.x), lo = min(((int)blockIdx.x - r * p.pieces) * p.piece, p.vocab), hi = min(lo + p.piece, p.vocab);
+    uint16_t* s_marked = reinterpret_cast<uint16_t*>(al_count + (p.piece + 8) / Counter::kEach);
+    TI* s_was = reinterpret_cast<TI*>(s_marked + p.room);   // their logits, where out is in
     const bool counts = p.tokens != nullptr, marks = counts || p.bias_starts;
+    const TI* in = static_cast<const TI*>(p.in) + (long long)r * p.ld_in;
+    TO* out = static_cast<TO*>(p.out) + (long long)r * p.ld_out;
+    // Vectors stand on borders of 16 bytes: the first one begins up to VEC - 1 words before the piece
+    const int base = lo - (int)(reinterpret_cast<uintptr_t>(in + lo) / sizeof(TI) % VEC);
     if (marks) {
-        for (int i = tid * 4; i < (hi - lo + (int)Counter::kEach - 1) / (int)Counter::kEach; i += kAlThreads * 4) *reinterpret_cast<uint4*>(al_count + i) = make_uint4(0, 0, 0, 0);
+        if (tid == 0) s_marks = 0;
+        for (int i = tid * 4; i < (hi - base + Counter::kEach - 1) / Counter::kEach; i += THREADS * 4) *reinterpret_cast<uint4*>(al_count + i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
     }
     pdl_trigger();
     pdl_wait();
-    const TI* in = static_cast<const TI*>(p.in) + (long long)r * p.ld_in;
-    TO* out = static_cast<TO*>(p.out) + (long long)r * p.ld_out;
     TI x[kAhead][VEC];
     auto fetch = [&](int i0) {
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (i0 + u * kStep < hi) al_load(x[u], in + i0 + u * kStep);
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + u * kStep;
+            if (i >= lo && i + VEC <= hi) al_load(x[u], in + i);
+            else
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (i + e >= lo && i + e < hi) x[u][e] = in[i + e];
+        }
     };
-    const int start = lo + tid * VEC;
+    const int start = base + tid * VEC;
     fetch(start);
     int first = 0, last = 0;   // of the biases
     if (p.bias_starts) first = max(p.bias_starts[r], 0), last = min(p.bias_starts[r + 1], p.n_bias);
-    const int mine = first + tid < last ? p.bias_words[first + tid] : -1;   // this thread's of the first ones
+    int mine[kEach];   // this thread's of the first ones
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) mine[u] = first + u * THREADS + tid < last ? p.bias_words[first + u * THREADS + tid] : -1;
     const float rep = p.repetition ? p.repetition[r] : 1.f, up = 1.f / rep, freq = p.frequency ? p.frequency[r] : 0.f, pres = p.presence ? p.presence[r] : 0.f;
     const float heat = p.temperature ? p.temperature[r] : 0.f, inv = heat >= 1.17549435e-38f ? 1.f / heat : 1.f;
     const int mask_row = !p.mask ? -1 : p.mask_row ? p.mask_row[r] : r;
     const int32_t* mask = mask_row >= 0 && mask_row < p.masks ? p.mask + (long long)mask_row * p.ld_mask : nullptr;
+    // a counter before it was changed: a word that had no mark goes on the list
+    auto note = [&](bool is_first, int off) {
+        const unsigned firsts = __ballot_sync(0xffffffffu, is_first);
+        if (firsts == 0) return;
+        int to = 0;
+        if (lane == 0) to = atomicAdd(&s_marks, __popc(firsts));
+        to = __shfl_sync(0xffffffffu, to, 0) + __popc(firsts & ((1u << lane) - 1u));
+        if (is_first && to < p.room) s_marked[to] = (uint16_t)off;
+    };
     if (counts) {
         const int seq = p.token_seq ? p.token_seq[r] : r, n = seq >= 0 && seq < p.seqs ? min(p.token_lens[r], p.longest) : 0, prompt = p.prompt_lens ? p.prompt_lens[r] : 0;
         const int32_t* words = p.tokens + (long long)max(seq, 0) * p.ld_tokens;
-        for (int i0 = tid; i0 - lane < n; i0 += kAlAhead * kAlThreads) {
-            int word[kAlAhead];
+        const unsigned from = (unsigned)(lo - base), size = (unsigned)(hi - lo);
+        auto go = [&](int i, const int end, auto behind) {   // words i .. end - 1
+            constexpr bool kBehind = decltype(behind)::value;
+            for (i += tid; i - lane < end; i += kAlAhead * THREADS) {
+                int off[kAlAhead];
 #pragma unroll
-            for (int u = 0; u < kAlAhead; ++u) word[u] = i0 + u * kAlThreads < n ? words[i0 + u * kAlThreads] : -1;
+                for (int u = 0; u < kAlAhead; ++u) off[u] = i + u * THREADS < end ? words[i + u * THREADS] - base : -1 - base;
+                const int of_first = __shfl_sync(0xffffffffu, off[0], 0);
+                bool one = true;
 #pragma unroll
-            for (int u = 0; u < kAlAhead; ++u) {
-                const int off = word[u] - lo;
-                const bool is = word[u] >= lo && word[u] < hi, behind = i0 + u * kAlThreads >= prompt;
-                if (!__any_sync(0xffffffffu, is)) continue;
-                const int key = is ? off << 1 | (int)behind : -1;
-                const bool one = __all_sync(0xffffffffu, key == __shfl_sync(0xffffffffu, key, 0));
-                if (is && (!one || lane == 0)) {
-                    if (behind) atomicAdd(Counter::at(al_count, off), Counter::shifted(one ? 32u : 1u, off));
-                    else atomicOr(Counter::at(al_count, off), Counter::shifted(Counter::kSeen, off));
+                for (int u = 0; u < kAlAhead; ++u) one &= off[u] == of_first;
+                if (__all_sync(0xffffffffu, one)) {
+                    uint32_t before = 1;
+                    if (lane == 0 && (unsigned)off[0] - from < size) before = kBehind ? Counter::add(al_count, off[0], 32u * kAlAhead) : Counter::mark(al_count, off[0], Counter::kSeen);
+                    note(before == 0, off[0]);
+                    continue;
+                }
+#pragma unroll
+                for (int u = 0; u < kAlAhead; ++u) {
+                    uint32_t before = 1;
+                    if ((unsigned)off[u] - from < size) before = kBehind ? Counter::add(al_count, off[u], 1u) : Counter::mark(al_count, off[u], Counter::kSeen);
+                    note(before == 0, off[u]);
                 }
             }
+        };
+        const int middle = min(max(prompt, 0), n);
+        if (middle > 0) go(0, middle, std::false_type{});
+        if (n > middle) go(middle, n, std::true_type{});
+    }
+    int listed = -1;   // -1: the row's own list
+    if (last - first <= kAlList) {
+        listed = 0;
+        if (first < last) {
+            unsigned here[kEach];
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) {
+                here[u] = __ballot_sync(0xffffffffu, mine[u] >= lo && mine[u] < hi);
+                if (lane == 0) s_have[u * (THREADS / 32) + warp] = __popc(here[u]);
+            }
+            __syncthreads();
+            int at[kEach] = {};
+            for (int w = 0; w < kHave; ++w) {
+                const int n = s_have[w];
+#pragma unroll
+                for (int u = 0; u < kEach; ++u)
+                    if (w < u * (THREADS / 32) + warp) at[u] += n;
+                listed += n;
+            }
+#pragma unroll
+            for (int u = 0; u < kEach; ++u)
+                if (here[u] >> lane & 1u) {
+                    const int to = at[u] + __popc(here[u] & ((1u << lane) - 1u));
+                    s_words[to] = mine[u], s_bias[to] = p.bias[first + u * THREADS + tid];
+                }
         }
     }
-    int listed = 0;
-    if (first < last && last - first <= kAlThreads) {
-        const bool is = mine >= lo && mine < hi;
-        const unsigned here = __ballot_sync(0xffffffffu, is);
-        if (lane == 0) s_have[warp] = __popc(here);
-        __syncthreads();
-        int at = __popc(here & ((1u << lane) - 1u));
-        for (int w = 0; w < kAlThreads / 32; ++w) {
-            const int n = s_have[w];
-            if (w < warp) at += n;
-            listed += n;
-        }
-        if (is) s_words[at] = mine, s_bias[at] = p.bias[first + tid], s_logit[at] = to_f32<TI>(in[mine]);
-    } else {
-        for (int i = first + tid; i < last; i += kAlThreads) {
-            const int off = p.bias_words[i] - lo;
-            if (off >= 0 && off < hi - lo) atomicOr(Counter::at(al_count, off), Counter::shifted(Counter::kBias, off));
-        }
+    for (int i0 = first + warp * 32; i0 < last; i0 += THREADS) {
+        const int word = i0 + lane < last ? p.bias_words[i0 + lane] : -1, off = word - base;
+        const bool is = word >= lo && word < hi;
+        uint32_t before = 1;
+        if (is) before = Counter::mark(al_count, off, Counter::kBias);
+        note(before == 0, off);
     }
     if (marks) __syncthreads();
     const C* marked = reinterpret_cast<const C*>(al_count);
-    auto penalised = [&](float z, uint32_t mark) {
+    auto adjusted = [&](float z, uint32_t mark, int word) {
         const uint32_t n = mark & Counter::kCount;
         if (mark & (Counter::kCount | Counter::kSeen)) z *= z > 0.f ? up : rep;
-        return n ? z - fmaf(freq, (float)n, pres) : z;
+        if (n) z -= fmaf(freq, (float)n, pres);
+        if (mark & Counter::kBias) {
+            if (listed >= 0) {
+                for (int b = 0; b < listed; ++b)
+                    if (s_words[b] == word) z += s_bias[b];
+            } else {
+                for (int b = first; b < last; ++b)
+                    if (p.bias_words[b] == word) z += p.bias[b];
+            }
+        }
+        return z;
     };
+    const int some = marks ? s_marks : 0;
+    auto ends = [&](float z, int word) { return from_f32<TO>(!mask || ((uint32_t)mask[word >> 5] >> (word & 31) & 1u) ? z * inv : -INFINITY); };
+    if (some > p.room) {   // word by word
+        for (int i = lo + tid; i < hi; i += THREADS) {
+            const float z = to_f32<TI>(in[i]);
+            const uint32_t mark = marked[i - base];
+            out[i] = ends(mark ? adjusted(z, mark, i) : z, i);
+        }
+        return;
+    }
+    if (p.in_place && some) {
+        for (int i = tid; i < some; i += THREADS) s_was[i] = in[base + s_marked[i]];
+        __syncthreads();
+    }
     for (int i0 = start; i0 < hi; i0 += kAhead * kStep) {
         if (i0 != start) fetch(i0);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const int i = i0 + u * kStep;
             if (i >= hi) break;
-            const uint32_t allowed = mask ? (uint32_t)mask[i >> 5] >> (i & 31) : 0xffffffffu;
+            uint32_t allowed = 0xffffffffu;
+            if (mask) {   // bits of words i .. i + VEC - 1; behind the row's end there may be none
+                const int w = max(i, 0) >> 5;
+                allowed = i < 0 ? (uint32_t)mask[0] << -i : (uint32_t)mask[w] >> (i & 31);
+                if (VEC > 1 && (i & 31) + VEC > 32 && i > 0 && (w + 1) * 32 < hi) allowed |= (uint32_t)mask[w + 1] << (32 - (i & 31));
+            }
             float z[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) z[e] = to_f32<TI>(x[u][e]);
-            if (marks) {
-                C mark[VEC];
-                bool any = true;
-                if constexpr (VEC * sizeof(C) >= 8) {
-                    uint2 w[VEC * sizeof(C) / 8];
-                    any = false;
-#pragma unroll
-                    for (int e = 0; e < VEC * (int)sizeof(C) / 8; ++e) {
-                        w[e] = *reinterpret_cast<const uint2*>(marked + (i - lo) + e * 8 / (int)sizeof(C));
-                        any |= (w[e].x | w[e].y) != 0;
-                        *reinterpret_cast<uint2*>(mark + e * 8 / (int)sizeof(C)) = w[e];
-                    }
-                } else {
-                    mark[0] = marked[i - lo];
-                }
-                if (any)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        z[e] = penalised(z[e], mark[e]);
-                        if (mark[e] & Counter::kBias)
-                            for (int b = first; b < last; ++b)
-                                if (p.bias_words[b] == i + e) z[e] += p.bias[b];
-                    }
-            }
             TO y[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) y[e] = from_f32<TO>(allowed >> e & 1u ? z[e] * inv : -INFINITY);
             if constexpr (VEC == 1) out[i] = y[0];
+            else if (i < lo || i + VEC > hi)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    if (i + e >= lo && i + e < hi) out[i + e] = y[e];
+                }
             else
 #pragma unroll
                 for (int e = 0; e < VEC * (int)sizeof(TO); e += 16) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out + i) + e) = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(y) + e);
         }
     }
-    if (listed == 0) return;
+    if (some == 0) return;
     __syncthreads();
-    if (tid >= listed) return;
-    const int word = s_words[tid];
-    bool again = false;
-    for (int b = 0; b < tid; ++b) again |= s_words[b] == word;
-    if (again) return;   // the first one sees to it
-    float z = penalised(s_logit[tid], marked[word - lo]) + s_bias[tid];
-    for (int b = tid + 1; b < listed; ++b)
-        if (s_words[b] == word) z += s_bias[b];
-    const bool allowed = !mask || ((uint32_t)mask[word >> 5] >> (word & 31) & 1u);
-    out[word] = from_f32<TO>(allowed ? z * inv : -INFINITY);
+#pragma unroll 2
+    for (int i = tid; i < some; i += THREADS) {
+        const int off = s_marked[i], word = base + off;
+        out[word] = ends(adjusted(to_f32<TI>(p.in_place ? s_was[i] : in[word]), marked[off], word), word);
+    }
 }
 
-template <typename TI, typename TO, typename C>
-static int adjust_logits(const AdjustLogits& p, int rows, bool pdl, zl_stream_t stream) {
-    // whole 16 bytes where rows and pitches allow it
-    constexpr int kVec = 16 / sizeof(TI);
-    const uintptr_t at = reinterpret_cast<uintptr_t>(p.in) | reinterpret_cast<uintptr_t>(p.out);
-    const bool wide = at % 16 == 0 && p.vocab % kVec == 0 && p.ld_in * sizeof(TI) % 16 == 0 && p.ld_out * sizeof(TO) % 16 == 0;
-    const size_t smem = p.tokens || p.bias_starts ? (size_t)p.piece * sizeof(C) : 0;
-    ZL_CHECK_CUDA(launch(wide ? k_adjust_logits<TI, TO, C, kVec> : k_adjust_logits<TI, TO, C, 1>, dim3((unsigned)rows * p.pieces), dim3(kAlThreads), smem, stream, pdl, p));
+constexpr int kAlMaxBytes = 128 * 1024, kAlMaxList = 32 * 1024;   // of a piece's counters, of words that are marked
+
+template <typename TI, typename TO, typename C, int THREADS>
+static int adjust_logits(AdjustLogits p, int rows, bool pdl, zl_stream_t stream) {
+    // 16 bytes at a time where the borders of 16 bytes of a row lie at the same words in both; 117 rows of 50257 30 us word by word, %s so
+    constexpr int kVec = 16 / sizeof(TI), kOut = 16 / sizeof(TO);
+    const long long ahead = (long long)(reinterpret_cast<uintptr_t>(p.in) / sizeof(TI) % kVec) - (long long)(reinterpret_cast<uintptr_t>(p.out) / sizeof(TO) % kOut);
+    const bool wide = ahead % kOut == 0 && (p.ld_in - p.ld_out) % kOut == 0 && reinterpret_cast<uintptr_t>(p.in) % sizeof(TI) == 0 && reinterpret_cast<uintptr_t>(p.out) % sizeof(TO) == 0;
+    // counters, with words before the piece; no more marked words than the piece has, or the history and the biases
+    const long long marks = (long long)p.longest + p.n_bias;
+    p.room = (int)(marks < p.piece ? marks : p.piece);
+    if (p.room > kAlMaxList / (p.in_place ? 3 : 1)) p.room = kAlMaxList / (p.in_place ? 3 : 1);
+    p.room = (p.room + 7) / 8 * 8;
+    const size_t smem = p.tokens || p.bias_starts ? (size_t)(p.piece + 8) * sizeof(C) + p.room * (2 + (p.in_place ? sizeof(TI) : 0)) : 0;
+    const auto kernel = wide ? k_adjust_logits<TI, TO, C, kVec, THREADS> : k_adjust_logits<TI, TO, C, 1, THREADS>;
+    if (smem > 32 * 1024) {
+        static bool done[2][64] = {};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64 || !done[wide][dev]) {
+            ZL_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kAlMaxBytes + 2 * kAlMaxList + 256));
+            if (dev >= 0 && dev < 64) done[wide][dev] = true;
+        }
+    }
+    ZL_CHECK_CUDA(launch(kernel, dim3((unsigned)rows * p.pieces), dim3(THREADS), smem, stream, pdl, p));
     return ZL_OK;
 }
 
-// The number of pieces: the fewest cycles of the SM that has the most, of 26 for 100 words (the bytes), 12 for 100 words of history and 300 for a CTA.  A piece has up to 40 KB of counters,
-// so that an SM holds four, and 1024 words or more.  117 rows of 50257 behind 9000: 5, 64 rows of 128256 behind 4000: 9, one row of 32000: 31.
+// The number of pieces: the fewest cycles of the SM that has the most, of 26 for 100 words (the bytes), 20 for 100 words of history and 3200 for a CTA.  A piece has 1024 words or more, and
+// counters that fit.  117 rows of 50257 behind 9000: one, 64 rows of 128256 behind 4000: two, one row of 32000: 31.
 static int al_pieces(int rows, int vocab, int longest, int counter) {
-    const int least = (int)(((long long)vocab * counter - 1) / (40 * 1024 - 64)) + 1, most = vocab / 1024 > least ? vocab / 1024 : least, sms = device_sm_count();
+    const int least = (int)(((long long)vocab * counter - 1) / (kAlMaxBytes - 128)) + 1, most = vocab / 1024 > least ? vocab / 1024 : least, sms = device_sm_count();
     int best = least;
     double cost = 0.0;
     for (int n = least; n <= most && n <= least + 256; ++n) {
         const long long ctas = ((long long)rows * n + sms - 1) / sms;
-        if (ctas < 3 && n < most) continue;   // for what an SM has in flight
-        const double x = (double)ctas * (0.26 * vocab / n + 0.12 * longest + 300.0);
+        const double x = (double)ctas * (0.26 * vocab / n + 0.2 * longest + 3200.0);
         if (cost == 0.0 || x < cost) cost = x, best = n;
     }
     return best;
@@ -225,21 +300,29 @@ extern "C" int zl_adjust_logits(const void* logits, long long ld_logits, int dty
     ZL_CHECK_ARG(!tokens || (token_lens && seqs > 0 && longest >= 0 && ld_tokens >= longest && (token_seq || seqs >= rows)));
     ZL_CHECK_ARG(!bias_starts || (n_bias >= 0 && (n_bias == 0 || (bias_words && bias))));
     ZL_CHECK_ARG(!mask || (masks > 0 && ld_mask >= (vocab - 1) / 32 + 1 && (mask_row || masks >= rows)));
-    ZL_CHECK_SUPPORTED(vocab <= 1 << 24 && longest <= 1 << 29 && (out_dtype == dtype || out_dtype == ZL_F32) && (dtype == ZL_F32 || dtype == ZL_F16 || dtype == ZL_BF16));
+    ZL_CHECK_SUPPORTED(vocab <= 1 << 24 && longest < 1 << 23 && (out_dtype == dtype || out_dtype == ZL_F32) && (dtype == ZL_F32 || dtype == ZL_F16 || dtype == ZL_BF16));
     AdjustLogits p = {logits, out, ld_logits, ld_out, tokens, token_seq, token_lens, prompt_lens, bias_starts, bias_words, mask, mask_row,
-                      repetition, frequency, presence, bias, temperature, ld_tokens, ld_mask, seqs, tokens ? longest : 0, n_bias, masks, vocab};
+                      repetition, frequency, presence, bias, temperature, ld_tokens, ld_mask, seqs, tokens ? longest : 0, bias_starts ? n_bias : 0, masks, vocab};
+    // anything of the one in the other
+    const uintptr_t in0 = reinterpret_cast<uintptr_t>(logits), out0 = reinterpret_cast<uintptr_t>(out);
+    const uintptr_t in1 = in0 + ((rows - 1) * (uintptr_t)ld_logits + vocab) * (dtype == ZL_F32 ? 4 : 2), out1 = out0 + ((rows - 1) * (uintptr_t)ld_out + vocab) * (out_dtype == ZL_F32 ? 4 : 2);
+    p.in_place = in0 < out1 && out0 < in1;
     const bool counts16 = p.longest <= kAlShort;
     p.pieces = al_pieces(rows, vocab, p.longest, counts16 ? 2 : 4);
     p.piece = (((vocab - 1) / p.pieces + 1) + 31) / 32 * 32;
     p.by_pieces = paged_divisor(p.pieces);
     ZL_CHECK_SUPPORTED((long long)rows * p.pieces < 1ll << 31);
     const bool dep = pdl != 0;
-    auto with = [&](auto counter) {
+    auto with = [&](auto counter, auto threads) {
         using C = decltype(counter);
-        if (dtype == ZL_F32) return adjust_logits<float, float, C>(p, rows, dep, stream);
-        if (dtype == ZL_F16) return out_dtype == ZL_F32 ? adjust_logits<__half, float, C>(p, rows, dep, stream) : adjust_logits<__half, __half, C>(p, rows, dep, stream);
-        return out_dtype == ZL_F32 ? adjust_logits<__nv_bfloat16, float, C>(p, rows, dep, stream)
-                                   : adjust_logits<__nv_bfloat16, __nv_bfloat16, C>(p, rows, dep, stream);
+        constexpr int N = decltype(threads)::value;
+        if (dtype == ZL_F32) return adjust_logits<float, float, C, N>(p, rows, dep, stream);
+        if (dtype == ZL_F16) return out_dtype == ZL_F32 ? adjust_logits<__half, float, C, N>(p, rows, dep, stream) : adjust_logits<__half, __half, C, N>(p, rows, dep, stream);
+        return out_dtype == ZL_F32 ? adjust_logits<__nv_bfloat16, float, C, N>(p, rows, dep, stream)
+                                   : adjust_logits<__nv_bfloat16, __nv_bfloat16, C, N>(p, rows, dep, stream);
     };
-    return counts16 ? with(uint16_t{}) : with(uint32_t{});
+    using Few = std::integral_constant<int, 256>;
+    using Many = std::integral_constant<int, 1024>;
+    if (p.piece <= 8192) return counts16 ? with(uint16_t{}, Few{}) : with(uint32_t{}, Few{});
+    return counts16 ? with(uint16_t{}, Many{}) : with(uint32_t{}, Many{});
 }

@@ -465,7 +465,7 @@ PyObject* adjust_logits(PyObject*, PyObject* const* a, Py_ssize_t na) {
         };
         auto table = [&](PyObject* o) -> Table {   // (rows, columns) int32
             const at::Tensor& t = here(o, false);
-            must(t.scalar_type() == at::kInt && t.dim() == 2 && t.numel() > 0 && t.size(0) < 1 << 30 && t.size(1) <= 1 << 29 && (t.stride(1) == 1 || t.size(1) == 1));
+            must(t.scalar_type() == at::kInt && t.dim() == 2 && t.numel() > 0 && t.size(0) < 1 << 30 && t.size(1) < 1 << 23 && (t.stride(1) == 1 || t.size(1) == 1));
             const long long step = t.size(0) > 1 ? t.stride(0) : t.size(1);
             must(step >= t.size(1));
             return {static_cast<const int32_t*>(t.data_ptr()), step, (int)t.size(0), (int)t.size(1)};
