@@ -6,13 +6,13 @@
 //
 // A CTA has a piece of a row's vocabulary, with a counter in shared memory for each word: how often it came, whether it is in the history, whether there is a bias.  Every CTA goes
 // over the whole history and counts the words of its piece by atomics of its own shared memory: whole numbers, which add up the same in every order.  (With the history
-// shared out among the CTAs of a cluster, and counts sent to the piece's owner: 52 us where this takes %s, 117 rows behind up to 9000 words, of which most are
-// frequent ones that one CTA owns.)  Where 256 words are one it is counted once, so that a history of one word does not queue up.  The logits' first loads are
+// shared out among the CTAs of a cluster, and counts sent to the piece's owner: 52 us where this takes 28, 117 rows behind up to 9000 words, of which most are
+// frequent ones that one CTA owns.)  Where 128 words are one it is counted once, so that a history of one word does not queue up.  The logits' first loads are
 // on their way meanwhile.
 //
 // Few words of a piece are marked, mostly.  Whoever marks a word first puts it on a list; the piece is written as if there were none, and the marked words once more behind that.
-// (With penalties worked out at every word, which costs three times the instructions of the rest, 64 rows of 128256 took 20 us instead of %s.)  Where
-// the list is too long, or out is in, that is done all the same.  Biases of a piece stand in a second list, in their order; of one that is too long for it the words go over the
+// (With penalties worked out at every word, which costs three times the instructions of the rest, 64 rows of 128256 took 20 us instead of 18.)  Where
+// the list is too long for shared memory that is done all the same.  Biases of a piece stand in a second list, in their order; of one that is too long for it the words go over the
 // row's own.
 #include "paged.cuh"
 
@@ -20,7 +20,7 @@
 
 namespace zl {
 
-constexpr int kAlAhead = 4, kAlList = 512;
+constexpr int kAlThreads = 256, kAlAhead = 4, kAlList = 512;
 
 // A counter: whether the word is in the history, whether there is a bias, how often it came behind the prompt.  16 bits where histories are short enough, two to a word of 32.
 template <typename C>
@@ -53,12 +53,12 @@ __device__ __forceinline__ void al_load(TI (&v)[VEC], const TI* at) {
 }
 
 // grid: pieces of rows; dynamic shared memory: a counter for each of the piece's words, where there is a history or a bias
-template <typename TI, typename TO, typename C, int VEC, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p) {
+template <typename TI, typename TO, typename C, int VEC>
+__global__ void __launch_bounds__(kAlThreads, 4) k_adjust_logits(const AdjustLogits p) {
     using Counter = AlCounter<C>;
-    constexpr int kAhead = VEC == 1 ? 8 : 4, kStep = THREADS * VEC, kEach = (kAlList + THREADS - 1) / THREADS;
+    constexpr int kAhead = VEC == 1 ? 8 : 4, kStep = kAlThreads * VEC, kEach = kAlList / kAlThreads;
     extern __shared__ __align__(16) uint32_t al_count[];
-    constexpr int kHave = kEach * THREADS / 32;
+    constexpr int kHave = kEach * kAlThreads / 32;
     __shared__ int s_words[kAlList], s_have[kHave];
     __shared__ float s_bias[kAlList];
     __shared__ int s_marks;
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p)
     const int base = lo - (int)(reinterpret_cast<uintptr_t>(in + lo) / sizeof(TI) % VEC);
     if (marks) {
         if (tid == 0) s_marks = 0;
-        for (int i = tid * 4; i < (hi - base + Counter::kEach - 1) / Counter::kEach; i += THREADS * 4) *reinterpret_cast<uint4*>(al_count + i) = make_uint4(0, 0, 0, 0);
+        for (int i = tid * 4; i < (hi - base + Counter::kEach - 1) / Counter::kEach; i += kAlThreads * 4) *reinterpret_cast<uint4*>(al_count + i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
     }
     pdl_trigger();
@@ -94,9 +94,15 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p)
     fetch(start);
     int first = 0, last = 0;   // of the biases
     if (p.bias_starts) first = max(p.bias_starts[r], 0), last = min(p.bias_starts[r + 1], p.n_bias);
-    int mine[kEach];   // this thread's of the first ones
+    const int seq = !counts ? -1 : p.token_seq ? p.token_seq[r] : r, length = counts ? p.token_lens[r] : 0, prompt = p.prompt_lens ? p.prompt_lens[r] : 0;
+    int mine[kEach];   // this thread's of the first ones, and what they are
+    float mine_bias[kEach];
 #pragma unroll
-    for (int u = 0; u < kEach; ++u) mine[u] = first + u * THREADS + tid < last ? p.bias_words[first + u * THREADS + tid] : -1;
+    for (int u = 0; u < kEach; ++u) {
+        const int i = first + u * kAlThreads + tid;
+        mine[u] = -1, mine_bias[u] = 0.f;
+        if (i < last) mine[u] = p.bias_words[i], mine_bias[u] = p.bias[i];
+    }
     const float rep = p.repetition ? p.repetition[r] : 1.f, up = 1.f / rep, freq = p.frequency ? p.frequency[r] : 0.f, pres = p.presence ? p.presence[r] : 0.f;
     const float heat = p.temperature ? p.temperature[r] : 0.f, inv = heat >= 1.17549435e-38f ? 1.f / heat : 1.f;
     const int mask_row = !p.mask ? -1 : p.mask_row ? p.mask_row[r] : r;
@@ -111,15 +117,15 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p)
         if (is_first && to < p.room) s_marked[to] = (uint16_t)off;
     };
     if (counts) {
-        const int seq = p.token_seq ? p.token_seq[r] : r, n = seq >= 0 && seq < p.seqs ? min(p.token_lens[r], p.longest) : 0, prompt = p.prompt_lens ? p.prompt_lens[r] : 0;
+        const int n = seq >= 0 && seq < p.seqs ? min(length, p.longest) : 0;
         const int32_t* words = p.tokens + (long long)max(seq, 0) * p.ld_tokens;
         const unsigned from = (unsigned)(lo - base), size = (unsigned)(hi - lo);
         auto go = [&](int i, const int end, auto behind) {   // words i .. end - 1
             constexpr bool kBehind = decltype(behind)::value;
-            for (i += tid; i - lane < end; i += kAlAhead * THREADS) {
+            for (i += tid; i - lane < end; i += kAlAhead * kAlThreads) {
                 int off[kAlAhead];
 #pragma unroll
-                for (int u = 0; u < kAlAhead; ++u) off[u] = i + u * THREADS < end ? words[i + u * THREADS] - base : -1 - base;
+                for (int u = 0; u < kAlAhead; ++u) off[u] = i + u * kAlThreads < end ? words[i + u * kAlThreads] - base : -1 - base;
                 const int of_first = __shfl_sync(0xffffffffu, off[0], 0);
                 bool one = true;
 #pragma unroll
@@ -150,7 +156,7 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p)
 #pragma unroll
             for (int u = 0; u < kEach; ++u) {
                 here[u] = __ballot_sync(0xffffffffu, mine[u] >= lo && mine[u] < hi);
-                if (lane == 0) s_have[u * (THREADS / 32) + warp] = __popc(here[u]);
+                if (lane == 0) s_have[u * (kAlThreads / 32) + warp] = __popc(here[u]);
             }
             __syncthreads();
             int at[kEach] = {};
@@ -158,19 +164,19 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p)
                 const int n = s_have[w];
 #pragma unroll
                 for (int u = 0; u < kEach; ++u)
-                    if (w < u * (THREADS / 32) + warp) at[u] += n;
+                    if (w < u * (kAlThreads / 32) + warp) at[u] += n;
                 listed += n;
             }
 #pragma unroll
             for (int u = 0; u < kEach; ++u)
                 if (here[u] >> lane & 1u) {
                     const int to = at[u] + __popc(here[u] & ((1u << lane) - 1u));
-                    s_words[to] = mine[u], s_bias[to] = p.bias[first + u * THREADS + tid];
+                    s_words[to] = mine[u], s_bias[to] = mine_bias[u];
                 }
         }
     }
-    for (int i0 = first + warp * 32; i0 < last; i0 += THREADS) {
-        const int word = i0 + lane < last ? p.bias_words[i0 + lane] : -1, off = word - base;
+    for (int i0 = first + warp * 32, u = 0; i0 < last; i0 += kAlThreads, ++u) {
+        const int word = u == 0 ? mine[0] : i0 + lane < last ? p.bias_words[i0 + lane] : -1, off = word - base;
         const bool is = word >= lo && word < hi;
         uint32_t before = 1;
         if (is) before = Counter::mark(al_count, off, Counter::kBias);
@@ -184,6 +190,7 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p)
         if (n) z -= fmaf(freq, (float)n, pres);
         if (mark & Counter::kBias) {
             if (listed >= 0) {
+#pragma unroll 8
                 for (int b = 0; b < listed; ++b)
                     if (s_words[b] == word) z += s_bias[b];
             } else {
@@ -196,15 +203,21 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p)
     const int some = marks ? s_marks : 0;
     auto ends = [&](float z, int word) { return from_f32<TO>(!mask || ((uint32_t)mask[word >> 5] >> (word & 31) & 1u) ? z * inv : -INFINITY); };
     if (some > p.room) {   // word by word
-        for (int i = lo + tid; i < hi; i += THREADS) {
+        for (int i = lo + tid; i < hi; i += kAlThreads) {
             const float z = to_f32<TI>(in[i]);
             const uint32_t mark = marked[i - base];
             out[i] = ends(mark ? adjusted(z, mark, i) : z, i);
         }
         return;
     }
+    // Logits of marked words as they are: the first of each thread's in registers, on their way while the piece is written
+    constexpr int kWas = 6;
+    TI was[kWas];
+#pragma unroll
+    for (int u = 0; u < kWas; ++u)
+        if (u * kAlThreads + tid < some) was[u] = in[base + s_marked[u * kAlThreads + tid]];
     if (p.in_place && some) {
-        for (int i = tid; i < some; i += THREADS) s_was[i] = in[base + s_marked[i]];
+        for (int i = kWas * kAlThreads + tid; i < some; i += kAlThreads) s_was[i] = in[base + s_marked[i]];
         __syncthreads();
     }
     for (int i0 = start; i0 < hi; i0 += kAhead * kStep) {
@@ -238,18 +251,21 @@ __global__ void __launch_bounds__(THREADS) k_adjust_logits(const AdjustLogits p)
     }
     if (some == 0) return;
     __syncthreads();
-#pragma unroll 2
-    for (int i = tid; i < some; i += THREADS) {
+    auto again = [&](int i, TI x) {
         const int off = s_marked[i], word = base + off;
-        out[word] = ends(adjusted(to_f32<TI>(p.in_place ? s_was[i] : in[word]), marked[off], word), word);
-    }
+        out[word] = ends(adjusted(to_f32<TI>(x), marked[off], word), word);
+    };
+#pragma unroll
+    for (int u = 0; u < kWas; ++u)
+        if (u * kAlThreads + tid < some) again(u * kAlThreads + tid, was[u]);
+    for (int i = kWas * kAlThreads + tid; i < some; i += kAlThreads) again(i, p.in_place ? s_was[i] : in[base + s_marked[i]]);
 }
 
-constexpr int kAlMaxBytes = 128 * 1024, kAlMaxList = 32 * 1024;   // of a piece's counters, of words that are marked
+constexpr int kAlMaxBytes = 34 * 1024, kAlMaxList = 16 * 1024;   // of a piece's counters, of words that are marked
 
-template <typename TI, typename TO, typename C, int THREADS>
+template <typename TI, typename TO, typename C>
 static int adjust_logits(AdjustLogits p, int rows, bool pdl, zl_stream_t stream) {
-    // 16 bytes at a time where the borders of 16 bytes of a row lie at the same words in both; 117 rows of 50257 30 us word by word, %s so
+    // 16 bytes at a time where the borders of 16 bytes of a row lie at the same words in both; 117 rows of 50257 30 us word by word, 26 so, when the rest was otherwise
     constexpr int kVec = 16 / sizeof(TI), kOut = 16 / sizeof(TO);
     const long long ahead = (long long)(reinterpret_cast<uintptr_t>(p.in) / sizeof(TI) % kVec) - (long long)(reinterpret_cast<uintptr_t>(p.out) / sizeof(TO) % kOut);
     const bool wide = ahead % kOut == 0 && (p.ld_in - p.ld_out) % kOut == 0 && reinterpret_cast<uintptr_t>(p.in) % sizeof(TI) == 0 && reinterpret_cast<uintptr_t>(p.out) % sizeof(TO) == 0;
@@ -259,7 +275,7 @@ static int adjust_logits(AdjustLogits p, int rows, bool pdl, zl_stream_t stream)
     if (p.room > kAlMaxList / (p.in_place ? 3 : 1)) p.room = kAlMaxList / (p.in_place ? 3 : 1);
     p.room = (p.room + 7) / 8 * 8;
     const size_t smem = p.tokens || p.bias_starts ? (size_t)(p.piece + 8) * sizeof(C) + p.room * (2 + (p.in_place ? sizeof(TI) : 0)) : 0;
-    const auto kernel = wide ? k_adjust_logits<TI, TO, C, kVec, THREADS> : k_adjust_logits<TI, TO, C, 1, THREADS>;
+    const auto kernel = wide ? k_adjust_logits<TI, TO, C, kVec> : k_adjust_logits<TI, TO, C, 1>;
     if (smem > 32 * 1024) {
         static bool done[2][64] = {};
         int dev = 0;
@@ -269,19 +285,21 @@ static int adjust_logits(AdjustLogits p, int rows, bool pdl, zl_stream_t stream)
             if (dev >= 0 && dev < 64) done[wide][dev] = true;
         }
     }
-    ZL_CHECK_CUDA(launch(kernel, dim3((unsigned)rows * p.pieces), dim3(THREADS), smem, stream, pdl, p));
+    ZL_CHECK_CUDA(launch(kernel, dim3((unsigned)rows * p.pieces), dim3(kAlThreads), smem, stream, pdl, p));
     return ZL_OK;
 }
 
-// The number of pieces: the fewest cycles of the SM that has the most, of 26 for 100 words (the bytes), 20 for 100 words of history and 3200 for a CTA.  A piece has 1024 words or more, and
-// counters that fit.  117 rows of 50257 behind 9000: one, 64 rows of 128256 behind 4000: two, one row of 32000: 31.
+// The number of pieces: the fewest cycles of the SM that has the most, of 26 for 100 words (the bytes), 12 for 100 words of history and 300 for a CTA, from three CTAs an SM on.  A piece
+// has 1024 words or more, and counters that leave room for four CTAs.  us by the number of pieces, 117 rows of 50257 behind up to 9000 words: 3 37, 4 43, 5 28 (taken), 6 32, 9 36;
+// 64 rows of 128256 behind up to 4000: 4 21, 6 20, 9 18 (taken).  CTAs of 1024 threads, of which one piece a row is best: 32 and 19.
 static int al_pieces(int rows, int vocab, int longest, int counter) {
     const int least = (int)(((long long)vocab * counter - 1) / (kAlMaxBytes - 128)) + 1, most = vocab / 1024 > least ? vocab / 1024 : least, sms = device_sm_count();
     int best = least;
     double cost = 0.0;
     for (int n = least; n <= most && n <= least + 256; ++n) {
         const long long ctas = ((long long)rows * n + sms - 1) / sms;
-        const double x = (double)ctas * (0.26 * vocab / n + 0.2 * longest + 3200.0);
+        if (ctas < 3 && n < most) continue;
+        const double x = (double)ctas * (0.26 * vocab / n + 0.12 * longest + 300.0);
         if (cost == 0.0 || x < cost) cost = x, best = n;
     }
     return best;
@@ -313,16 +331,12 @@ extern "C" int zl_adjust_logits(const void* logits, long long ld_logits, int dty
     p.by_pieces = paged_divisor(p.pieces);
     ZL_CHECK_SUPPORTED((long long)rows * p.pieces < 1ll << 31);
     const bool dep = pdl != 0;
-    auto with = [&](auto counter, auto threads) {
+    auto with = [&](auto counter) {
         using C = decltype(counter);
-        constexpr int N = decltype(threads)::value;
-        if (dtype == ZL_F32) return adjust_logits<float, float, C, N>(p, rows, dep, stream);
-        if (dtype == ZL_F16) return out_dtype == ZL_F32 ? adjust_logits<__half, float, C, N>(p, rows, dep, stream) : adjust_logits<__half, __half, C, N>(p, rows, dep, stream);
-        return out_dtype == ZL_F32 ? adjust_logits<__nv_bfloat16, float, C, N>(p, rows, dep, stream)
-                                   : adjust_logits<__nv_bfloat16, __nv_bfloat16, C, N>(p, rows, dep, stream);
+        if (dtype == ZL_F32) return adjust_logits<float, float, C>(p, rows, dep, stream);
+        if (dtype == ZL_F16) return out_dtype == ZL_F32 ? adjust_logits<__half, float, C>(p, rows, dep, stream) : adjust_logits<__half, __half, C>(p, rows, dep, stream);
+        return out_dtype == ZL_F32 ? adjust_logits<__nv_bfloat16, float, C>(p, rows, dep, stream)
+                                   : adjust_logits<__nv_bfloat16, __nv_bfloat16, C>(p, rows, dep, stream);
     };
-    using Few = std::integral_constant<int, 256>;
-    using Many = std::integral_constant<int, 1024>;
-    if (p.piece <= 8192) return counts16 ? with(uint16_t{}, Few{}) : with(uint32_t{}, Few{});
-    return counts16 ? with(uint16_t{}, Many{}) : with(uint32_t{}, Many{});
+    return counts16 ? with(uint16_t{}) : with(uint32_t{});
 }

@@ -153,10 +153,17 @@ __device__ __forceinline__ uint32_t int4_encode(const uint4& x, uint32_t& meta) 
     const float step = to_f32<T>(two[0]);
     uint32_t codes = 0;
     if (numbers == 15u && step >= 1.17549435e-38f) {
+        // Quotients by the reciprocal and one correction of what is left over (Markstein 1990), a quarter of a division's instructions.  x and lo are numbers of T: where the quotient lies
+        // on the border between two codes it comes out exactly, as the correction's error is 2^-46 of it, elsewhere it is 2^-17 away from one.  Far down the products would lose bits.
+        const float inv = __fdiv_rn(1.f, step);
+        const bool far = step < 1e-30f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float n = rintf(2.f * __fdiv_rn(__fsub_rn(__fmul_rn(f[i], 0.5f), half), step));
-            codes |= (uint32_t)(int)fminf(n, 15.f) << ((i & 1) * 16 + (i & 6) * 2);
+            const float d = __fsub_rn(__fmul_rn(f[i], 0.5f), half);
+            float q = __fmul_rn(d, inv);
+            q = __fmaf_rn(__fmaf_rn(-q, step, d), inv, q);
+            if (far) q = __fdiv_rn(d, step);
+            codes |= (uint32_t)__float2int_rn(fminf(2.f * q, 15.f)) << ((i & 1) * 16 + (i & 6) * 2);
         }
     }
     return codes;

@@ -61,6 +61,7 @@ struct AxesRope {
     int axes, half, heads, kv_heads, dim;
     float mscale;
     int rows, stages, row_bytes;
+    PagedDivisor by_half;
 };
 
 __device__ __forceinline__ void rope_s2g(void* dst, const void* src, uint32_t bytes) {
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(256, INT4 ? kRopeThreads4 / 256 : kRopeThreads
             // x less whole turns, 2 pi in two parts (Cody and Waite 1980): the products are not rounded, what is left is within 2^-53 of its size
             const double n = rint(x * 0.15915494309189533577);
             double sn, cs;
-            sincos(fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586477, x)), &sn, &cs);
+            sincospi(0.31830988618379067154 * fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586477, x)), &sn, &cs);
             sn *= (double)p.mscale, cs *= (double)p.mscale;
             exact[b * p.half + i] = make_double2(cs, sn);
             to[0] = (float)cs, to[2] = (float)sn;
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(256, INT4 ? kRopeThreads4 / 256 : kRopeThreads
                 const double2* w = exact + (i & 1) * p.half;
                 const int second = FORM == kRopeAdjacent ? 1 : p.half, each = FORM == kRopeAdjacent ? 2 : 1;
                 for (int it = tid; it < p.kv_heads * p.half; it += threads) {
-                    const int head = it / p.half, k = it - head * p.half;
+                    const int head = p.by_half(it), k = it - head * p.half;
                     T* x = reinterpret_cast<T*>(row) + (p.heads + head) * p.dim + k * each;
                     const double2 cs = w[k];
                     const double f = (double)to_f32<T>(x[0]), g = (double)to_f32<T>(x[second]);
@@ -218,9 +219,9 @@ __global__ void __launch_bounds__(256, INT4 ? kRopeThreads4 / 256 : kRopeThreads
         if (INT4 && ok && id >= 0 && id < c.num_pages) {
             const long long at = (long long)id * c.page_stride + (long long)in_page * c.row_stride;
             const uint4* from = reinterpret_cast<const uint4*>(row) + p.heads * (p.dim >> 3);
-            const int d8 = p.dim >> 3, all = 2 * p.kv_heads * d8;
+            const int d8 = p.dim >> 3, all = 2 * p.kv_heads * d8, by = p.dim == 64 ? 3 : 4;
             for (int i0 = warp * 32; i0 < all; i0 += threads) {   // whole groups of 4 lanes are in or out
-                const int it = i0 + lane, head = it / d8, col8 = it - head * d8;
+                const int it = i0 + lane, head = it >> by, col8 = it & (d8 - 1);
                 uint32_t meta;
                 const uint32_t codes = int4_encode<T>(from[min(it, all - 1)], meta);
                 if (it < all) {
@@ -288,13 +289,13 @@ static int axes_rope_append(const void* qkv, long long ldq, const int32_t* pos, 
     // a thread for every two pieces to turn; as many CTAs as the SMs hold threads and rows in shared memory
     const int row_bytes = (heads + 2 * kv_heads) * dim * 2, turns = 2 * 8 * (half + 7) + (INT4 ? 16 + 2 * 16 * half : 0);
     const int items = (heads + kv_heads) * (form == kRopePairs ? half / 8 : form == kRopeAdjacent ? (half + 3) / 4 : half), two = cdiv(items, 2 * 32) * 32;
-    const int threads = two < 64 ? 64 : two < 256 ? two : 256;
+    const int threads = INT4 ? 256 : two < 64 ? 64 : two < 256 ? two : 256;   // 4 bits: most of the work is behind the turns
     int stages = kRopeMaxStages;
     while (stages > (INT4 ? 2 : 1) && stages * row_bytes + turns > kRopeSmem) --stages;
     const int smem = stages * row_bytes + turns;
     ZL_CHECK_SUPPORTED(smem <= kRopeSmem);
     const int by_smem = kSmSmem / (smem + kCtaSmem + 256), by_threads = (INT4 ? kRopeThreads4 : kRopeThreads) / threads, most = device_sm_count() * (by_smem < by_threads ? by_smem : by_threads);
-    const AxesRope p = {qkv, q_out, pos, axis, token_seq, placement, inv_freq, ldq, ld_pos, axes, half, heads, kv_heads, dim, mscale, T, stages, row_bytes};
+    const AxesRope p = {qkv, q_out, pos, axis, token_seq, placement, inv_freq, ldq, ld_pos, axes, half, heads, kv_heads, dim, mscale, T, stages, row_bytes, paged_divisor(half > 0 ? half : 1)};
     if (dtype == ZL_F16) return form == kRopePairs ? axes_rope<__half, kRopePairs, INT4>(p, c, T < most ? T : most, threads, smem, pdl, stream)
                                 : form == kRopeAdjacent ? axes_rope<__half, kRopeAdjacent, INT4>(p, c, T < most ? T : most, threads, smem, pdl, stream)
                                                         : axes_rope<__half, kRopeAny, INT4>(p, c, T < most ? T : most, threads, smem, pdl, stream);
