@@ -137,34 +137,47 @@ __device__ __forceinline__ __nv_bfloat16 int4_round_down<__nv_bfloat16>(float x)
 // 8 columns of a group whose other columns are in the neighbouring lanes of this group of four; all lanes of the warp call it.  -> the codes; the group's pair
 template <typename T>
 __device__ __forceinline__ uint32_t int4_encode(const uint4& x, uint32_t& meta) {
+    using P = typename Int4Pair<T>::type;
     constexpr unsigned kAll = 0xffffffffu;
+    constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00 : 0x7f80, kAbs = 0x7fff7fffu;
+    const uint32_t size = __vmaxu2(__vmaxu2(x.x & kAbs, x.y & kAbs), __vmaxu2(x.z & kAbs, x.w & kAbs));
+    const unsigned numbers = __ballot_sync(kAll, (size & 0xffffu) < kInf && size >> 16 < kInf) >> (threadIdx.x & 28) & 15u;
+    // the highest value and the lowest one's opposite, in T
+    const P* two = reinterpret_cast<const P*>(&x);
+    const P high = __hmax2(__hmax2(two[0], two[1]), __hmax2(two[2], two[3])), less = __hmin2(__hmin2(two[0], two[1]), __hmin2(two[2], two[3]));
+    const uint32_t h = *reinterpret_cast<const uint32_t*>(&high), l = *reinterpret_cast<const uint32_t*>(&less) ^ 0x80008000u, a = __byte_perm(h, l, 0x5410), b = __byte_perm(h, l, 0x7632);
+    P ends = __hmax2(*reinterpret_cast<const P*>(&a), *reinterpret_cast<const P*>(&b));
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        const uint32_t other = __shfl_xor_sync(kAll, *reinterpret_cast<const uint32_t*>(&ends), o);
+        ends = __hmax2(ends, *reinterpret_cast<const P*>(&other));
+    }
+    const T* of = reinterpret_cast<const T*>(&ends);
+    const float half = -0.5f * to_f32<T>(of[1]);   // of the lowest
+    const T pair[2] = {int4_round_down<T>(__fdiv_rn(__fmaf_rn(to_f32<T>(of[0]), 0.5f, -half), 7.5f)), from_f32<T>(half * 2.f)};
+    meta = numbers == 15u ? *reinterpret_cast<const uint32_t*>(pair) : 0x7fff7fffu;
+    const float step = to_f32<T>(pair[0]);
+    if (numbers != 15u || !(step >= 1.17549435e-38f)) return 0;
     float f[8];
     unpack8<T>(x, f);
-    float lo = f[0], hi = f[0];
-    bool number = fabsf(f[0]) < INFINITY;
-#pragma unroll
-    for (int i = 1; i < 8; ++i) lo = fminf(lo, f[i]), hi = fmaxf(hi, f[i]), number = number && fabsf(f[i]) < INFINITY;
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) lo = fminf(lo, __shfl_xor_sync(kAll, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(kAll, hi, o));
-    const unsigned numbers = __ballot_sync(kAll, number) >> (threadIdx.x & 28) & 15u;
-    const float half = __fmul_rn(lo, 0.5f);
-    T two[2] = {int4_round_down<T>(__fdiv_rn(__fsub_rn(__fmul_rn(hi, 0.5f), half), 7.5f)), from_f32<T>(lo)};
-    meta = numbers == 15u ? *reinterpret_cast<const uint32_t*>(two) : 0x7fff7fffu;
-    const float step = to_f32<T>(two[0]);
     uint32_t codes = 0;
-    if (numbers == 15u && step >= 1.17549435e-38f) {
+    if (step >= 1e-30f) {
         // Quotients by the reciprocal and one correction of what is left over (Markstein 1990), a quarter of a division's instructions.  x and lo are numbers of T: where the quotient lies
-        // on the border between two codes it comes out exactly, as the correction's error is 2^-46 of it, elsewhere it is 2^-17 away from one.  Far down the products would lose bits.
+        // on the border between two codes it comes out exactly, as the correction's error is 2^-46 of it, elsewhere it is 2^-17 away from one.  Codes are whole numbers at the
+        // end of 1.5 * 2^23 + c, each multiplied into its place; what that number adds there is taken away beforehand.
         const float inv = __fdiv_rn(1.f, step);
-        const bool far = step < 1e-30f;
+        constexpr uint32_t kWhole = 0x4b400000u;
+        codes = 0u - kWhole * 0x11111111u;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float d = __fsub_rn(__fmul_rn(f[i], 0.5f), half);
+            const float d = __fmaf_rn(f[i], 0.5f, -half);
             float q = __fmul_rn(d, inv);
             q = __fmaf_rn(__fmaf_rn(-q, step, d), inv, q);
-            if (far) q = __fdiv_rn(d, step);
-            codes |= (uint32_t)__float2int_rn(fminf(2.f * q, 15.f)) << ((i & 1) * 16 + (i & 6) * 2);
+            codes += __float_as_uint(__fmaf_rn(fminf(q, 7.5f), 2.f, 12582912.f)) << ((i & 1) * 16 + (i & 6) * 2);
         }
+    } else {   // far down those products would lose bits
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) codes |= (uint32_t)__float2int_rn(fminf(2.f * __fdiv_rn(__fmaf_rn(f[i], 0.5f, -half), step), 15.f)) << ((i & 1) * 16 + (i & 6) * 2);
     }
     return codes;
 }
