@@ -150,12 +150,12 @@ def test_append_takes_pages_of_the_table_only(cuda):
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------------
-def check_attention(dtype, heads, kv_heads, dim, page, order, window, seqs, seed=0, max_new=None, break_pages=False, behind=3, scale=None):
+def check_attention(dtype, heads, kv_heads, dim, page, order, window, seqs, seed=0, max_new=None, break_pages=False, behind=3, scale=None, extra=1):
     """seqs: [(keys, new tokens)]."""
     g = torch.Generator().manual_seed(seed)
     lens, new = [n for n, _ in seqs], [m for _, m in seqs]
     pages = sum(-(-n // page) for n in lens) + 2
-    table = tables(g, lens, page, pages)
+    table = tables(g, lens, page, pages, extra)
     k, v = pool(g, pages, page, kv_heads, dim, dtype, order)
     if break_pages:
         table[0, 0], table[-1, 1] = pages, -1
@@ -203,6 +203,34 @@ def test_attention_portions(cuda, dtype, heads, kv_heads, dim, page, order, wind
 def test_attention_of_long_stretches(cuda, dtype, heads, kv_heads, dim, page, window, seqs):
     """Enough keys for every CTA to go round its buffers several times, blocks whole and cut."""
     check_attention(dtype, heads, kv_heads, dim, page, "rows", window, seqs, max_new=max(n for _, n in seqs))
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,order", [(BF16, 8, 2, 128, 16, "rows"), (F16, 8, 2, 64, 64, "heads"), (BF16, 4, 4, 128, 20, "wide"), (F16, 24, 8, 64, 32, "rows"),
+                                                                 (F16, 7, 1, 128, 128, "rows"), (BF16, 16, 1, 64, 8, "rows"), (F16, 5, 5, 64, 1, "rows"), (BF16, 12, 3, 64, 16, "wide")])
+@pytest.mark.parametrize("window", [0, 100, 300])
+@pytest.mark.parametrize("seqs", [[(700, 700)], [(700, 130), (1, 1), (129, 129), (513, 257), (40, 0)], [(1000 + 131 * i, 1 + i % 90) for i in range(6)]])
+def test_attention_behind_wide_tables(cuda, dtype, heads, kv_heads, dim, page, order, window, seqs):
+    """Tables with room for far more keys than a workspace has: the tiles make codes numbers by themselves."""
+    check_attention(dtype, heads, kv_heads, dim, page, order, window, seqs, extra=(1 << 30) // (page * kv_heads * dim * 4) // len(seqs))
+
+
+def test_attention_behind_wide_tables_elsewhere(cuda):
+    """Bad pages, rows before the first key and broken tokens on that way."""
+    wide = (1 << 30) // (16 * 2 * 64 * 4)
+    check_attention(F16, 8, 2, 128, 16, "rows", 0, [(200, 150), (220, 150)], break_pages=True, extra=wide)
+    check_attention(BF16, 8, 2, 64, 16, "rows", 3, [(100, 200), (0, 200), (200, 200)], extra=wide)
+    check_attention(BF16, 8, 2, 64, 16, "heads", 0, [(100, 200), (0, 200), (200, 200)], extra=wide)
+    g = torch.Generator().manual_seed(5)
+    table = tables(g, [400], 16, 40, extra=wide)
+    q = torch.randn(150, 8, 64, generator=g).to(BF16)
+    for where, which in ((399, 1), (300, 1), (220, 0), (399, 0)):
+        k, v = pool(g, 40, 16, 2, 64, BF16, "rows")
+        (k, v)[which][int(table[0, where // 16]), where % 16, 1, 36:40] = 0xff   # columns 32 to 63
+        got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), torch.tensor([400], dtype=torch.int32).cuda(), starts_of([150]).cuda(), 0.125).cpu().double()
+        want, off = oracle.attention(q, codes.decode(k, BF16), codes.decode(v, BF16), table, [400], starts_of([150]), 0.125, 0)
+        fine = torch.ones(150, 8, 64, dtype=torch.bool)
+        fine[torch.arange(250, 400) >= where, 4:, 32 if which else 0:] = False
+        assert ((got - want).abs() <= off)[fine].all() and torch.isnan(got[~fine]).all()
 
 
 @pytest.mark.parametrize("max_new", [1, 3, 20, 200, None])

@@ -25,6 +25,7 @@ struct PagedCache {
     const int32_t* table;
     int ld_table, max_pages, page_size, seqs;
     PagedDivisor by_page;
+    int limit;   // rows of a sequence, where its last page has more than there are; 0: whole pages
     // element offset of row i >= 0 of sequence b, -1: nowhere
     __device__ __forceinline__ long long row_at(int b, int i) const {
         const int pg = by_page(i);
@@ -34,7 +35,7 @@ struct PagedCache {
         return (long long)id * page_stride + (long long)(i - pg * page_size) * row_stride;
     }
     // rows that the table has room for, as far as tiles of them are counted in 32 bits
-    __device__ __forceinline__ int room() const { return (int)min((long long)max_pages * page_size, 0x7fff0000ll); }
+    __device__ __forceinline__ int room() const { return limit ? limit : (int)min((long long)max_pages * page_size, 0x7fff0000ll); }
 };
 
 }  // namespace zl

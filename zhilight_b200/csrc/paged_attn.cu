@@ -79,6 +79,11 @@ static int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool p
     return ZL_OK;
 }
 
+int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, int dim, int dtype, bool pdl, zl_stream_t stream) {
+    if (dtype == ZL_F16) return dim == 64 ? paged_tiles<__half, 64>(p, c, ctas, pdl, stream) : paged_tiles<__half, 128>(p, c, ctas, pdl, stream);
+    return dim == 64 ? paged_tiles<__nv_bfloat16, 64>(p, c, ctas, pdl, stream) : paged_tiles<__nv_bfloat16, 128>(p, c, ctas, pdl, stream);
+}
+
 template <typename T, int D>
 static int paged_attention(const PagedAttn& p, const PagedCache& c, const PagedPlan& s, bool pdl, zl_stream_t stream) {
     return s.tiles ? paged_tiles<T, D>(p, c, s.ctas, pdl, stream) : paged_few<T, D>(p, c, s.ctas, pdl, stream);

@@ -29,7 +29,7 @@ struct PagedAttn {
     float2* ml;                       // parts of blocks that were cut, two places for every CTA: {maximum, sum} of their rows, and the rows
     float* part;
     struct PagedCut* cuts;            // for every CTA
-    int split;                        // of kernels that share a call's sequences (KIND::takes): (token, head) rows of a kv head up to which one of them takes a sequence
+    int split;                        // of kernels that share a call's sequences (KIND::takes): (token, head) rows of a kv head up to which one of them takes a sequence; 0 where one has all
 };
 
 // Exponentials carry 2^up, and a row's reference follows its maximum once that is more than `tau` above it.  fp16 probabilities are at most 2^15, and with 2^10 the
@@ -328,5 +328,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_join(const PagedAttn 
     }
     if (group == 0 && mine) paged_row_out<T, D>(p, x.k, x.hk, r, l, v);
 }
+
+// The kernel for tiles and its join, over a cache of 16 bits (paged_attn.cu): checked arguments
+int paged_tiles(const PagedAttn& p, const PagedCache& c, int ctas, int dim, int dtype, bool pdl, zl_stream_t stream);
 
 }  // namespace zl

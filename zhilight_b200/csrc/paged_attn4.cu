@@ -20,8 +20,15 @@ struct Paged4Plan {
 struct Paged4Plans {
     Paged4Plan few, tiles;
     int split;                         // rows of a sequence for the kernel for few
-    size_t bytes;
+    int wide_pages;                    // pages of 64 rows a sequence, of keys and values in 16 bits for the tiles; 0: the tiles make codes numbers by themselves
+    size_t k, v, table, bytes;
 };
+
+// The tiles make every key's codes numbers once for each block of rows, which bounds them: 2048 tokens of 32 heads on 8 behind 6000 299 us.  Made numbers once, beforehand, in the workspace, they
+// are read like a cache of 16 bits: 242.  The workspace has room for all that the page table has room for, so that is done up to this size of it; what is
+// written there are only the keys that portions see.
+constexpr size_t kWideBytes = 256u << 20;
+constexpr int kWidePage = 64, kWideShares = 4;
 
 template <int D>
 static int paged4_few_ctas(bool eight) { return device_sm_count() * (eight ? P4Cfg<D, 1>::kPerSm : P4Cfg<D, 2>::kPerSm); }
@@ -47,6 +54,14 @@ static Paged4Plans paged4_plan(int rows, int max_new, int seqs, int max_keys, in
     if (tiles) {
         s.tiles.tile_rows = kPaRows / group * group;
         plan(s.tiles, 2 * s.tiles.tile_rows, kPtRows, PtKind::kSetup + cdiv(max_keys, kPtKeys), device_sm_count());
+    }
+    if (tiles) {
+        const long long pages = ((long long)max_keys + kWidePage - 1) / kWidePage;
+        const size_t each = (size_t)kv_heads * kWidePage * dim * 2;
+        if ((unsigned long long)seqs * pages * each * 2 <= kWideBytes) {
+            s.wide_pages = (int)pages;
+            s.k = take(seqs * pages * each), s.v = take(seqs * pages * each), s.table = take(seqs * pages * sizeof(int32_t));
+        }
     }
     if (!tiles || (seqs > 1 && group <= kFewBeside)) {   // one sequence alone has the rows that the bound says; wider groups are no few rows
         const bool eight = (tiles ? group : most) <= 8;   // beside the tiles: single tokens, mostly
@@ -100,6 +115,48 @@ static int paged4_tiles(const PagedAttn& p, const PagedCache& c, int ctas, bool 
     return ZL_OK;
 }
 
+// Keys and values of a tile of 64 rows of a sequence as numbers: grid (tiles, sequences, shares of the work).  Tiles that no row of the kernel for tiles sees, and sequences of few rows, are left out.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_paged4_wide(const PagedAttn p, const PagedCache c, T* __restrict__ k_out, T* __restrict__ v_out, int32_t* table) {
+    constexpr int kPieces = D / 16, kAhead = 4;
+    __shared__ long long s_off[kWidePage];
+    const int tid = threadIdx.x, b = blockIdx.y, row0 = blockIdx.x * kWidePage, page = b * gridDim.x + blockIdx.x;
+    pdl_trigger();
+    pdl_wait();
+    if (tid == 0 && blockIdx.z == 0) table[page] = page;
+    const int from = max(p.starts[b], 0), tokens = max(min(p.starts[b + 1], p.rows) - from, 0), len = p.lens[b], place0 = len - p.starts[b + 1] + from, have = min(max(len, 0), c.room());
+    const int hi = min(place0 + tokens - 1, have - 1), lo = paged_from(p, place0) / kPtKeys * kPtKeys;
+    if (!PtKind::takes(p, tokens * p.group) || row0 > hi || row0 + kWidePage <= lo) return;
+    if (tid < kWidePage) s_off[tid] = row0 + tid <= hi ? c.row_at(b, row0 + tid) : -1;
+    __syncthreads();
+    const int half = p.kv_heads * kWidePage * kPieces, items = 2 * half;   // a cache's page; both
+    for (int i0 = (int)blockIdx.z * (kAhead * 256) + tid; i0 < items; i0 += (int)gridDim.z * (kAhead * 256)) {
+        uint2 codes[kAhead];
+        uint32_t meta[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + u * 256, piece = i % kPieces, row = i / kPieces % kWidePage, head = i / (kPieces * kWidePage), is_v = head >= p.kv_heads;
+            codes[u] = make_uint2(0u, 0u), meta[u] = 0;
+            if (i >= items || s_off[row] < 0) continue;
+            const uint8_t* at = static_cast<const uint8_t*>(is_v ? c.v : c.k) + s_off[row] + (long long)(head - (is_v ? p.kv_heads : 0)) * c.head_stride;
+            codes[u] = *reinterpret_cast<const uint2*>(at + piece * 8);
+            meta[u] = *reinterpret_cast<const uint32_t*>(at + D / 2 + piece / 2 * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + u * 256;
+            const bool odd = i & 1, is_v = i >= half;
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? codes[u].x : codes[u].y, 1);   // two lanes have a group of 32 columns (int4 values)
+            if (i >= items) continue;
+            uint32_t step, low;
+            int4_meta<T>(meta[u], step, low);
+            uint4* to = reinterpret_cast<uint4*>(is_v ? v_out : k_out) + ((size_t)page * half + i - (is_v ? half : 0)) * 2 - odd;
+            to[0] = int4_eight<T>(odd ? other : codes[u].x, step, low);
+            to[2] = int4_eight<T>(odd ? codes[u].y : other, step, low);
+        }
+    }
+}
+
 template <typename T, int D>
 static int paged4(PagedAttn p, const PagedCache& c, const Paged4Plans& s, uint8_t* ws, bool pdl, zl_stream_t stream) {
     ZL_CHECK_WAITS();
@@ -116,7 +173,15 @@ static int paged4(PagedAttn p, const PagedCache& c, const Paged4Plans& s, uint8_
         if (rc || !both) return rc;
     }
     with(s.tiles);
-    return paged4_tiles<T, D>(p, c, s.tiles.ctas, pdl || both, stream);
+    if (!both) p.split = 0;
+    if (s.wide_pages == 0) return paged4_tiles<T, D>(p, c, s.tiles.ctas, pdl || both, stream);
+    T *k = reinterpret_cast<T*>(ws + s.k), *v = reinterpret_cast<T*>(ws + s.v);
+    int32_t* table = reinterpret_cast<int32_t*>(ws + s.table);
+    ZL_CHECK_CUDA(launch(k_paged4_wide<T, D>, dim3(s.wide_pages, c.seqs, kWideShares), dim3(256), 0, stream, pdl || both, p, c, k, v, table));
+    const long long rows = (long long)c.max_pages * c.page_size;   // below 2^31, or the workspace would be larger
+    const PagedCache wide = {k, v, (long long)c.seqs * s.wide_pages, (long long)p.kv_heads * kWidePage * D, D, kWidePage * D, table, s.wide_pages, s.wide_pages, kWidePage, c.seqs,
+                             paged_divisor(kWidePage), (int)rows};
+    return paged_tiles(p, wide, s.tiles.ctas, D, std::is_same<T, __half>::value ? ZL_F16 : ZL_BF16, true, stream);
 }
 
 }  // namespace zl

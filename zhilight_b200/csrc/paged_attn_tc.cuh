@@ -86,9 +86,6 @@ struct PtKind {
         const int tiles = k.hi >= 0 ? k.hi / kPtKeys - k.lo / kPtKeys + 1 : 1;
         return k.rows > p.tile_rows ? tiles : (tiles + 1) >> 1;
     }
-    static __device__ __forceinline__ bool takes(const PagedAttn&, int) { return true; }
-};
-struct Pt4Kind : PtKind {   // beside the kernel for few rows
     static __device__ __forceinline__ bool takes(const PagedAttn& p, int rows) { return rows > p.split; }
 };
 
@@ -264,7 +261,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
     // later one cannot end before the waiter has gone on: a phase is told from its neighbours by its parity alone.
     int blocks = 0, turn = 0, ring = 0;   // ring / 2: of keys, and of values
     bool ok = true;           // no wait has given up
-    PagedWalk<std::conditional_t<INT4, Pt4Kind, PtKind>> walk;
+    PagedWalk<PtKind> walk;
     const PagedBlock& k = walk.k;
     const PagedPlace& at = walk.place;
     walk.find(p, c, -1);
