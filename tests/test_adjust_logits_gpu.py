@@ -104,6 +104,23 @@ def test_adjust_strided_and_in_place(cuda, vocab):
             assert torch.equal(dz._base[:, :first].cpu(), wide[:, :first]) and torch.equal(dz._base[:, first + vocab:].cpu(), wide[:, first + vocab:])
 
 
+def test_adjust_beside_itself(cuda):
+    """Out in the same rows as the logits, or in them: refused where a word of one is another one's of the other."""
+    g = torch.Generator().manual_seed(14)
+    wide = (torch.randn(4, 2100, generator=g) * 3).to(BF16)
+    kw = settings(g, 4, 1000, 3, 60, 5, 2)
+    dev, dwide = on_gpu(kw), wide.cuda()
+    check(wide[:, :1000], kw, got=ops.adjust_logits(dwide[:, :1000], out=dwide[:, 1000:2000], **dev))
+    assert torch.equal(dwide[:, :1000].cpu(), wide[:, :1000]) and torch.equal(dwide[:, 2000:].cpu(), wide[:, 2000:])
+    flat = torch.zeros(9000, dtype=BF16, device="cuda")
+    for x, y in ((flat[:4000].view(4, 1000), flat[8:4008].view(4, 1000)), (flat[:4000].view(4, 1000), flat[3000:7000].view(4, 1000)), (dwide[:, 600:1600], dwide[:, :1000]),
+                 (flat[:4000].view(4, 1000), flat[:8000].view(4, 2000)[:, :1000]), (flat[:1000].view(1, 1000), flat[999:1999].view(1, 1000)),
+                 (flat[:1000].view(1, 1000), flat[:2000].view(torch.float32).view(1, 1000))):
+        with pytest.raises(RuntimeError, match="beside"):
+            ops.adjust_logits(x, out=y, out_dtype=y.dtype)
+    check(torch.zeros(4, 1000, dtype=BF16), {}, got=ops.adjust_logits(flat[:4000].view(4, 1000), out=flat[4000:8000].view(4, 1000)))
+
+
 def test_adjust_of_special_numbers(cuda):
     """Infinities and NaN in logits, biases and settings; masks that leave nothing or hide them; empty histories and lists."""
     vocab = 300

@@ -177,7 +177,7 @@ def check_attention(dtype, heads, kv_heads, dim, page, order, window, seqs, seed
 
 @pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(BF16, 32, 8, 128), (F16, 32, 8, 128), (BF16, 16, 16, 64), (F16, 8, 1, 64), (BF16, 28, 4, 128),
                                                       (F16, 20, 1, 128), (BF16, 3, 1, 64), (F16, 40, 1, 128), (F16, 12, 1, 64)])
-@pytest.mark.parametrize("page,order", [(16, "rows"), (64, "heads"), (20, "wide"), (1, "rows"), (256, "rows")])
+@pytest.mark.parametrize("page,order", [(16, "rows"), (64, "heads"), (20, "wide"), (1, "rows"), (256, "rows"), (32, "wide"), (48, "heads")])
 def test_attention_single_tokens(cuda, dtype, heads, kv_heads, dim, page, order):
     check_attention(dtype, heads, kv_heads, dim, page, order, 0, [(1, 1), (17, 1), (300, 1), (64, 1), (0, 0), (129, 1), (5, 0), (1025, 1)], max_new=1)
 
@@ -346,6 +346,64 @@ def test_attention_of_large_and_small_values(cuda, dtype, size, new, heads, dim)
     assert ((got - want).abs() <= off + lost).all()
 
 
+@pytest.mark.parametrize("dtype,size", [(BF16, 2.0 ** 19), (BF16, 2.0 ** 100), (F16, 2.0 ** 12)])
+@pytest.mark.parametrize("new,heads,extra", [(1, 4, 1), (4, 8, 1), (150, 8, 1), (150, 8, 400000)])
+def test_attention_of_large_keys(cuda, dtype, size, new, heads, extra):
+    """Keys whose steps are beyond 2^15 behind ones whose steps are not, queries to match."""
+    g = torch.Generator().manual_seed(33)
+    lens, page = [300, new + 7], 16
+    table, starts = tables(g, lens, page, 50, extra), starts_of([new, new])
+    x = torch.randn(50, page, 2, 64, generator=g)
+    x[:, ::3] *= 1.0 / 1024
+    k, v = rows_in((x.clamp(-3.9, 3.9) * size).to(dtype), "rows", dtype), pool(g, 50, page, 2, 64, dtype, "rows")[1]
+    q = (torch.randn(2 * new, heads, 64, generator=g) / size).to(dtype)
+    got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), starts.cuda(), 0.125, max_new=new).cpu().double()
+    want, off = oracle.attention(q, codes.decode(k, dtype), codes.decode(v, dtype), table, lens, starts, 0.125, 0)
+    assert ((got - want).abs() <= off).all()
+
+
+STEEP = {"one": [(300, 1), (77, 1), (1000, 1)], "drafts": [(300, 4), (80, 3), (4, 4)], "portion": [(300, 150), (150, 150), (700, 33)],
+         "many": [(90 + 7 * (i % 5), 1 + i % 20) for i in range(60)]}
+
+
+@pytest.mark.parametrize("dtype,q_size,k_size", [(F16, 2.0 ** 8, 2.0 ** 8), (F16, 2.0 ** 13, 2.0 ** 13), (F16, 2.0 ** 15, 2.0 ** 15), (BF16, 2.0 ** 12, 2.0 ** 14), (BF16, 2.0 ** 27, 2.0 ** 27),
+                                                 (BF16, 2.0 ** 34, 2.0 ** 34), (BF16, 2.0 ** 50, 2.0 ** 58)])
+@pytest.mark.parametrize("seqs", list(STEEP))
+@pytest.mark.parametrize("extra", [1, 400000])
+def test_attention_of_large_scores(cuda, dtype, q_size, k_size, seqs, extra):
+    """Queries of +-q_size in every column, key j k_size * (1 + (j * 37 % 7) / 128) in every column, which 4 bits hold exactly (a step of zero): products and sums of powers of two times whole
+    numbers below 2^8 are exact in 32 bits, and two scores are the same number or 2^9 apart at least: a row is the mean of the values of its highest scores.  2^-21 covers the
+    exponentials' own error, a half step of the type the rounding of equal ones where it is not theirs; sums add a unit for each key, the result is rounded once."""
+    g = torch.Generator().manual_seed(21)
+    seqs = STEEP[seqs]
+    lens, new = [n for n, _ in seqs], [m for _, m in seqs]
+    table, starts = tables(g, lens, 16, sum(-(-n // 16) for n in lens) + 2, extra // len(seqs)), starts_of(new)
+    k = torch.zeros(sum(-(-n // 16) for n in lens) + 2, 16, 2, 64, dtype=dtype)
+    step = lambda j: 1.0 + (j * 37 % 7) / 128.0  # noqa: E731
+    for b, n in enumerate(lens):
+        for j in range(n):
+            k[int(table[b, j // 16]), j % 16] = k_size * step(j)
+    v = rows_in(torch.randn(k.shape, generator=g).to(dtype), "rows", dtype)
+    k = rows_in(k, "rows", dtype)
+    hide(k, table, lens)
+    hide(v, table, lens)
+    sign = torch.tensor([1.0, -1.0] * 4)
+    q = (sign[:, None] * q_size).expand(sum(new), 8, 64).contiguous().to(dtype)
+    got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), starts.cuda(), 1.0, max_new=max(new)).cpu().double()
+    vv = codes.decode(v, dtype)
+    for b, (n, m) in enumerate(seqs):
+        x = oracle.rows_of(vv, table, b, n)
+        c = torch.tensor([step(j) for j in range(n)], dtype=torch.float64)
+        seen = torch.arange(n)[None] <= torch.arange(n - m, n)[:, None]
+        for h in range(8):
+            s = torch.where(seen, c * float(sign[h]), -math.inf)
+            p = (s == s.amax(1, keepdim=True)).double()
+            p /= p.sum(1, keepdim=True)
+            o, spread = p @ x[:, h // 4], p @ x[:, h // 4].abs()
+            err = spread * (2.0 ** -21 + oracle.EPS[dtype] / 2 + 2 * (n + 64) * 2.0 ** -24)
+            assert ((got[int(starts[b]):int(starts[b + 1]), h] - o).abs() <= err + oracle.half_step(o.abs() + err, dtype)).all(), (b, h)
+
+
 @pytest.mark.parametrize("new", [1, 5, 150])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_attention_with_equal_rows_and_large_scores(cuda, dtype, new):
@@ -430,8 +488,38 @@ def test_attention_in_place(cuda, heads, kv_heads, new):
     table, lens, starts = tables(g, [200, 300], 16, 40).cuda(), torch.tensor([200, 300], dtype=torch.int32).cuda(), starts_of([new, new]).cuda()
     q = torch.randn(2 * new, heads, 64, generator=g).to(BF16).cuda()
     want = ops.paged_attention_int4(q, k.cuda(), v.cuda(), table, lens, starts, 0.125, max_new=new)
+    mixed = starts_of([1, new]).cuda()
+    both = ops.paged_attention_int4(q, k.cuda(), v.cuda(), table, lens, mixed, 0.125)
+    x = q.clone()
     got = ops.paged_attention_int4(q, k.cuda(), v.cuda(), table, lens, starts, 0.125, max_new=new, out=q)
     assert got is q and torch.equal(got, want)
+    assert torch.equal(ops.paged_attention_int4(x, k.cuda(), v.cuda(), table, lens, mixed, 0.125, out=x)[:1 + new], both[:1 + new])
+
+
+def test_attention_replayed_with_other_lengths(cuda):
+    """A graph takes lengths, starts and pages as they are when it is replayed, whichever kernels the sequences' rows go to."""
+    g = torch.Generator().manual_seed(12)
+    k, v = pool(g, 120, 16, 2, 64, BF16, "rows")
+    kd, vd, kk, vv = to_gpu(k), to_gpu(v), codes.decode(k, BF16), codes.decode(v, BF16)
+    q = torch.randn(260, 4, 64, generator=g).to(BF16)
+    for width in (50, 200000):
+        table, lens, starts = torch.full((4, width), -1, dtype=torch.int32).cuda(), torch.zeros(4, dtype=torch.int32).cuda(), torch.zeros(5, dtype=torch.int32).cuda()
+        out, dq, graph = torch.zeros_like(q).cuda(), q.cuda(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.paged_attention_int4(dq, kd, vd, table, lens, starts, 0.125, out=out)
+        for shares in ((65, 65, 65, 65), (1, 257, 0, 2), (0, 0, 3, 1), (260, 0, 0, 0)):
+            n = [m + 100 * (i + 1) for i, m in enumerate(shares)]
+            t, s = tables(g, n, 16, 120, extra=0), starts_of(shares)
+            table[:, :t.shape[1]].copy_(t)
+            lens.copy_(torch.tensor(n, dtype=torch.int32))
+            starts.copy_(s)
+            out.fill_(7.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            used = int(s[-1])
+            want, off = oracle.attention(q, kk, vv, t, n, s, 0.125, 0)
+            got = out.cpu().double()
+            assert ((got - want).abs() <= off)[:used].all() and (got[used:] == 7.0).all()
 
 
 # ---- as a program uses them ----------------------------------------------------------------------------------------------------

@@ -321,10 +321,16 @@ extern "C" int zl_adjust_logits(const void* logits, long long ld_logits, int dty
     ZL_CHECK_SUPPORTED(vocab <= 1 << 24 && longest < 1 << 23 && (out_dtype == dtype || out_dtype == ZL_F32) && (dtype == ZL_F32 || dtype == ZL_F16 || dtype == ZL_BF16));
     AdjustLogits p = {logits, out, ld_logits, ld_out, tokens, token_seq, token_lens, prompt_lens, bias_starts, bias_words, mask, mask_row,
                       repetition, frequency, presence, bias, temperature, ld_tokens, ld_mask, seqs, tokens ? longest : 0, bias_starts ? n_bias : 0, masks, vocab};
-    // anything of the one in the other
-    const uintptr_t in0 = reinterpret_cast<uintptr_t>(logits), out0 = reinterpret_cast<uintptr_t>(out);
-    const uintptr_t in1 = in0 + ((rows - 1) * (uintptr_t)ld_logits + vocab) * (dtype == ZL_F32 ? 4 : 2), out1 = out0 + ((rows - 1) * (uintptr_t)ld_out + vocab) * (out_dtype == ZL_F32 ? 4 : 2);
-    p.in_place = in0 < out1 && out0 < in1;
+    // Out may be logits itself, or lie beside it in the same rows; else a word could be read after another one was written over it
+    const long long size = dtype == ZL_F32 ? 4 : 2, out_size = out_dtype == ZL_F32 ? 4 : 2, ahead = (long long)(reinterpret_cast<uintptr_t>(out) - reinterpret_cast<uintptr_t>(logits));
+    const long long step = rows > 1 ? ld_logits * size : 0, out_step = rows > 1 ? ld_out * out_size : 0;
+    const bool apart = ahead >= (rows - 1) * step + vocab * size || -ahead >= (rows - 1) * out_step + vocab * out_size;
+    if (!apart) {
+        const bool same = ahead == 0 && step == out_step && size == out_size && dtype == out_dtype;
+        const long long beside = step > 0 && step == out_step ? (ahead % step + step) % step : 0;
+        ZL_CHECK_SUPPORTED(same || (beside >= vocab * size && step - beside >= vocab * out_size));
+    }
+    p.in_place = !apart;
     const bool counts16 = p.longest <= kAlShort;
     p.pieces = al_pieces(rows, vocab, p.longest, counts16 ? 2 : 4);
     p.piece = (((vocab - 1) / p.pieces + 1) + 31) / 32 * 32;

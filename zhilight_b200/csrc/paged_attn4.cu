@@ -24,11 +24,12 @@ struct Paged4Plans {
     size_t k, v, table, bytes;
 };
 
-// The tiles make every key's codes numbers once for each block of rows, which bounds them: 2048 tokens of 32 heads on 8 behind 6000 299 us.  Made numbers once, beforehand, in the workspace, they
+// The tiles make every key's codes numbers once for each block of rows, which bounds them: 2048 tokens of 32 heads on 8 behind 6000 302 us.  Made numbers once, beforehand, in the workspace, they
 // are read like a cache of 16 bits: 242.  The workspace has room for all that the page table has room for, so that is done up to this size of it; what is
-// written there are only the keys that portions see.
+// written there are only the keys that portions see.  And only from some blocks of rows on, by the rows / beforehand: 64 tokens behind 4000 27 / 30 us, 300 behind 300 23 / 25,
+// 100 of four sequences behind 1000 40 / 39, 1000 behind 1000 61 / 53, 200 behind 30000 242 / 192.
 constexpr size_t kWideBytes = 256u << 20;
-constexpr int kWidePage = 64, kWideShares = 4;
+constexpr int kWidePage = 64, kWideShares = 4, kWideRows = 512;
 
 template <int D>
 static int paged4_few_ctas(bool eight) { return device_sm_count() * (eight ? P4Cfg<D, 1>::kPerSm : P4Cfg<D, 2>::kPerSm); }
@@ -58,7 +59,7 @@ static Paged4Plans paged4_plan(int rows, int max_new, int seqs, int max_keys, in
     if (tiles) {
         const long long pages = ((long long)max_keys + kWidePage - 1) / kWidePage;
         const size_t each = (size_t)kv_heads * kWidePage * dim * 2;
-        if ((unsigned long long)seqs * pages * each * 2 <= kWideBytes) {
+        if (most > kWideRows && (unsigned long long)seqs * pages * each * 2 <= kWideBytes) {
             s.wide_pages = (int)pages;
             s.k = take(seqs * pages * each), s.v = take(seqs * pages * each), s.table = take(seqs * pages * sizeof(int32_t));
         }

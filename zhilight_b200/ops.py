@@ -1267,7 +1267,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
 
 def paged_attention_int4(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window=0, max_new=None, out=None, pdl=False):
     """paged_attention over caches of 4 bits (pages, page_size, kv_heads, int4_row_bytes(dim)) uint8 whose rows were written from q's type
-    (qkv_axes_rope_append_int4): the attention over what they stand for, int4_cache_values.  -> out, like q."""
+    (qkv_axes_rope_append_int4): the attention over what they stand for, int4_cache_values.  A broken group (NaN) of a key or value reaches the rows that see
+    it and no others.  Portions of prompts take a workspace of up to 256 MB, by the room that page_table has.  -> out, like q."""
     if _lib.host is not None:
         y = _lib.host.paged_attention_int4(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl)
         if y is not None:
@@ -1346,7 +1347,7 @@ def adjust_logits(logits, tokens=None, token_seq=None, token_lens=None, prompt_l
     mask (M, W >= vocab / 32) int32, rows of any pitch, mask_row (R) int32 (None: row r has mask r; outside [0, M): no mask): words w whose bit w % 32 of
     mask[., w // 32] is clear get -inf.  A row whose mask leaves nothing is -inf throughout.
 
-    Arithmetic in 32 bits.  -> out (R, vocab) in out_dtype (logits' own or fp32; None: logits' own), which may be logits itself."""
+    Arithmetic in 32 bits.  -> out (R, vocab) in out_dtype (logits' own or fp32; None: logits' own), which may be logits itself, or lie beside it in wider rows."""
     if _lib.host is not None:
         y = _lib.host.adjust_logits(logits, tokens, token_seq, token_lens, prompt_lens, repetition, frequency, presence, bias_starts, bias_words, bias, temperature,
                                     mask, mask_row, out_dtype, out, pdl)
