@@ -31,9 +31,6 @@ struct Paged4Plans {
 constexpr size_t kWideBytes = 256u << 20;
 constexpr int kWidePage = 64, kWideShares = 4, kWideRows = 512;
 
-template <int D>
-static int paged4_few_ctas(bool eight) { return device_sm_count() * (eight ? P4Cfg<D, 1>::kPerSm : P4Cfg<D, 2>::kPerSm); }
-
 static Paged4Plans paged4_plan(int rows, int max_new, int seqs, int max_keys, int heads, int kv_heads, int dim) {
     Paged4Plans s = {};
     const int group = heads / kv_heads;
@@ -67,7 +64,7 @@ static Paged4Plans paged4_plan(int rows, int max_new, int seqs, int max_keys, in
     if (!tiles || (seqs > 1 && group <= kFewBeside)) {   // one sequence alone has the rows that the bound says; wider groups are no few rows
         const bool eight = (tiles ? group : most) <= 8;   // beside the tiles: single tokens, mostly
         s.split = !tiles ? INT_MAX : eight ? 8 : kFewBeside;
-        plan(s.few, eight ? 8 : 16, eight ? 8 : 16, P4Kind::kSetup + cdiv(max_keys, kP4Keys), dim == 64 ? paged4_few_ctas<64>(eight) : paged4_few_ctas<128>(eight));
+        plan(s.few, eight ? 8 : 16, eight ? 8 : 16, P4Kind::kSetup + cdiv(max_keys, kP4Keys), kP4PerSm * device_sm_count());
     }
     return s;
 }

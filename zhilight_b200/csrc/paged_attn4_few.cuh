@@ -20,7 +20,7 @@
 
 namespace zl {
 
-constexpr int kP4Warps = 4, kP4Each = 32, kP4Keys = kP4Each * kP4Warps, kP4Stages = 2;
+constexpr int kP4Warps = 4, kP4Each = 32, kP4Keys = kP4Each * kP4Warps, kP4Stages = 2, kP4PerSm = 3;   // four CTAs of 128 registers an SM: decoding 28.2 us, a long sequence 48.8; three 26.9 and 48.0
 
 template <int D, int NT>
 struct P4Cfg {
@@ -30,7 +30,6 @@ struct P4Cfg {
     static constexpr int kBytes = kP4Warps * kWarp;
     static constexpr int kPitch = D + 8;                             // floats; of a row of a warp's output in its ring
     static_assert(8 * NT * kPitch * 4 <= kWarp, "a warp's output, where its ring was");
-    static constexpr int kPerSm = NT == 1 ? 4 : 3;
 };
 
 // tiles of 128 keys; at least one: a block that sees nothing is written too
@@ -66,7 +65,7 @@ __device__ __forceinline__ void p4_words(uint32_t (&w)[N], const uint8_t* at) {
 
 // grid: CTAs that share the line; blocks of up to 8 NT rows.  tma: one of kInt4Copies ...
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kP4Warps * 32, (P4Cfg<D, NT>::kPerSm))
+__global__ void __launch_bounds__(kP4Warps * 32, kP4PerSm)
 k_paged_attn4_few(const PagedAttn p, const PagedCache c, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, int tma, unsigned* err) {
     using C = P4Cfg<D, NT>;
     constexpr bool kHalf = std::is_same<T, __half>::value, kScaled = Int4Codes<T, false>::kScaled;

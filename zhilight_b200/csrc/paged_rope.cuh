@@ -289,7 +289,8 @@ static int axes_rope_append(const void* qkv, long long ldq, const int32_t* pos, 
     // a thread for every two pieces to turn; as many CTAs as the SMs hold threads and rows in shared memory
     const int row_bytes = (heads + 2 * kv_heads) * dim * 2, turns = 2 * 8 * (half + 7) + (INT4 ? 16 + 2 * 16 * half : 0);
     const int items = (heads + kv_heads) * (form == kRopePairs ? half / 8 : form == kRopeAdjacent ? (half + 3) / 4 : half), two = cdiv(items, 2 * 32) * 32;
-    const int threads = INT4 ? 256 : two < 64 ? 64 : two < 256 ? two : 256;   // 4 bits: most of the work is behind the turns
+    // 4 bits: most of the work is behind the turns; fewer warps repeat less for each token once there are tokens for all SMs (4525 tokens 29 us instead of 31), more are done sooner with one
+    const int threads = INT4 ? (T > 3 * device_sm_count() ? 128 : 256) : two < 64 ? 64 : two < 256 ? two : 256;
     int stages = kRopeMaxStages;
     while (stages > (INT4 ? 2 : 1) && stages * row_bytes + turns > kRopeSmem) --stages;
     const int smem = stages * row_bytes + turns;
