@@ -41,6 +41,8 @@ namespace zl {
 constexpr int kPtRows = 256, kPtKeys = 128, kPtHalf = 64, kPtWarpS = 8, kPtWarpO = 9, kPtWarpLoad = 10, kPtLoaders = 64;
 // Of a cache of 4 bits: warps 10 and 11 bring codes of keys and of values, a ring of tiles each, as they are; warps 12 to 15 make them numbers of T on the way into the ring
 // of tiles, 16 rows of every tile each (all four in every tile: a warp that passed over some could take one phase of their barriers for another).
+// 2048 tokens of 32 heads on 8 behind 6000: 302 us, bound by these four warps, one on each scheduler beside two of the softmax (when it took 309, 1900 of the 2700 cycles
+// for 64 keys went by in them).  More threads would leave the softmax too few registers.
 constexpr int kPtWarpLoad4 = 12;
 template <bool INT4>
 constexpr int kPtThreads = INT4 ? 512 : 384;
@@ -598,7 +600,7 @@ k_paged_attn_tiles(const PagedAttn p, const PagedCache c, const __grid_constant_
                     // Two tiles at a time: lane = row, half of the warp a group of 32 columns each.  Reads of eight rows touch all banks once, and so do writes of 16 bytes of
                     // eight rows.  One fence for both: it waits for the writes.
                     const int rg = warp - kPtWarpLoad4, row = rg * 16 + (lane & 15);
-                    // Loops that are not unrolled: the warps' instructions come from one small cache, and what is large here stops the softmax's (unrolled, 442 us where this took 360).
+                    // Loops that are not unrolled: the warps' instructions come from one small cache, and what is large here stops the softmax's (at a time unrolled 442 us, as it stands 309).
                     for (int x = 0; x < tiles && ok; ++x) {
                         const int is_v = two_rows ? 0 : x & 1, n = ring / 2 + (two_rows ? x : (x >> 1) * 2), i = ring + 2 * x;   // of the first of the two
 #pragma unroll 1
