@@ -293,10 +293,11 @@ static int adjust_logits(AdjustLogits p, int rows, bool pdl, zl_stream_t stream)
 // has 1024 words or more, and counters that leave room for four CTAs.  us by the number of pieces, 117 rows of 50257 behind up to 9000 words: 3 37, 4 43, 5 28 (taken), 6 32, 9 36;
 // 64 rows of 128256 behind up to 4000: 4 21, 6 20, 9 18 (taken).  CTAs of 1024 threads, of which one piece a row is best: 32 and 19.
 static int al_pieces(int rows, int vocab, int longest, int counter) {
-    const int least = (int)(((long long)vocab * counter - 1) / (kAlMaxBytes - 128)) + 1, most = vocab / 1024 > least ? vocab / 1024 : least, sms = device_sm_count();
+    const int least = (int)(((long long)vocab * counter - 1) / (kAlMaxBytes - 128)) + 1, sms = device_sm_count();
+    const int most = vocab / 1024 < least ? least : vocab / 1024 < least + 256 ? vocab / 1024 : least + 256;
     int best = least;
     double cost = 0.0;
-    for (int n = least; n <= most && n <= least + 256; ++n) {
+    for (int n = least; n <= most; ++n) {
         const long long ctas = ((long long)rows * n + sms - 1) / sms;
         if (ctas < 3 && n < most) continue;
         const double x = (double)ctas * (0.26 * vocab / n + 0.12 * longest + 300.0);

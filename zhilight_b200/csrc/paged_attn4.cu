@@ -10,8 +10,9 @@ namespace zl {
 // Drafts of 16 sequences, 48 rows, up to 6000 keys: 49 us there, in three blocks, 87 on the tiles, whose blocks of up to 128 rows cost the same.
 // Of other calls, those sequences go there that bring a token or two of a group of up to 8 heads, or up to 16 rows: portions of prompts beside 20 single tokens (24 sequences, keys in a
 // window of 1024) 71 us, 95 with all on the tiles.
-// Few sequences are not worth two launches more: two with 141 tokens together, 28 heads on 4, 34 us with them and 30 without.
-constexpr int kFewRows4 = 64, kFewBeside = 16, kBesideSeqs = 8;
+// Few keys are not worth two launches more.  By the room that the page table has (lengths are the device's), us with both kernels / the tiles alone, a portion beside single tokens: two
+// sequences of 740 keys 29 / 21, four of 2000 36 / 35, eight of 1000 28 / 28, eight of 4500 51 / 77, two of 30000 47 / 81, eight of 30000 97 / 249.
+constexpr int kFewRows4 = 64, kFewBeside = 16, kBesideKeys = 8192;
 
 // what lies where in the workspace, for one of the two kernels
 struct Paged4Plan {
@@ -62,7 +63,7 @@ static Paged4Plans paged4_plan(int rows, int max_new, int seqs, int max_keys, in
             s.k = take(seqs * pages * each), s.v = take(seqs * pages * each), s.table = take(seqs * pages * sizeof(int32_t));
         }
     }
-    if (!tiles || (seqs > kBesideSeqs && group <= kFewBeside)) {   // wider groups are no few rows
+    if (!tiles || (seqs > 1 && (long long)seqs * max_keys >= kBesideKeys && group <= kFewBeside)) {   // wider groups are no few rows
         const bool eight = (tiles ? group : most) <= 8;   // beside the tiles: single tokens, mostly
         s.split = !tiles ? INT_MAX : eight ? 8 : kFewBeside;
         plan(s.few, eight ? 8 : 16, eight ? 8 : 16, P4Kind::kSetup + cdiv(max_keys, kP4Keys), kP4PerSm * device_sm_count());
