@@ -233,6 +233,41 @@ def test_attention_behind_wide_tables_elsewhere(cuda):
         assert ((got - want).abs() <= off)[fine].all() and torch.isnan(got[~fine]).all()
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page,order", [(BF16, 8, 2, 128, 16, "rows"), (F16, 8, 2, 64, 64, "heads"), (BF16, 16, 1, 128, 20, "wide"), (F16, 32, 2, 64, 32, "rows"),
+                                                                 (BF16, 5, 5, 64, 1, "rows"), (F16, 17, 1, 128, 16, "rows"), (BF16, 160, 1, 64, 16, "rows")])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("room", [2500, 20000])
+@pytest.mark.parametrize("seqs", [[(700, 1), (1300, 300)], [(700, 130), (1, 1), (129, 129), (513, 257), (40, 0), (1300, 4), (300, 1)]])
+def test_attention_of_few_rows_beside_portions(cuda, dtype, heads, kv_heads, dim, page, order, window, room, seqs):
+    """A table with room for few keys and for more; groups of heads that count as few rows and wider ones."""
+    check_attention(dtype, heads, kv_heads, dim, page, order, window, seqs, extra=room // page)
+
+
+@pytest.mark.parametrize("max_new", [1, 5, 100, None])
+@pytest.mark.parametrize("wide", [400, 60000])
+def test_attention_of_lengths_out_of_range_behind_wide_tables(cuda, max_new, wide):
+    """Lengths that the table has no room for, starts out of order: rows of q alone are touched, and the sequences in range are right."""
+    g = torch.Generator().manual_seed(15)
+    page, dim = 16, 64
+    table = torch.full((4, wide), -1, dtype=torch.int32)
+    table[:, :20] = torch.randperm(80, generator=g).view(4, 20).to(torch.int32)
+    k, v = pool(g, 80, page, 2, dim, BF16, "rows")
+    q = torch.randn(310, 8, dim, generator=g).to(BF16)
+    kk, vv = codes.decode(k, BF16), codes.decode(v, BF16)
+    for starts, lens in (((0, 300, 301, 302, 303), (320, 300, 2 ** 31 - 1, -4)), ((0, 300, 301, 301, 2 ** 31 - 1), (320, 300, 5, -2 ** 31)),
+                         ((0, 300, 301, 280, 280), (320, 1, 7, 2 ** 31 - 1)), ((0, 300, 301, -2 ** 31, -2 ** 31), (320, 0, 2 ** 31 - 1, -2 ** 31)), ((0, 300, 301, 301, -2 ** 31), (320, 300, 2 ** 31 - 1, 5))):
+        out = torch.full((330, 8, dim), 7.0, dtype=BF16, device="cuda")
+        ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor(starts, dtype=torch.int32).cuda(),
+                                 0.125, max_new=max_new, out=out[:310])
+        out = out.cpu().double()
+        assert (out[310:] == 7.0).all()
+        want, off = oracle.attention(q[:301], kk, vv, table[:2], lens[:2], starts[:3], 0.125, 0)
+        assert ((out[:301] - want).abs() <= off).all()
+        k16, v16 = (x.cuda() for x in (kk, vv))                       # the same over a cache of 16 bits
+        got = ops.paged_attention(q.cuda(), k16, v16, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), torch.tensor(starts, dtype=torch.int32).cuda(), 0.125, max_new=max_new)
+        assert ((got[:301].cpu().double() - want).abs() <= off).all()
+
+
 @pytest.mark.parametrize("max_new", [1, 3, 20, 200, None])
 def test_attention_does_not_depend_on_the_bound_of_new_tokens(cuda, max_new):
     check_attention(BF16, 8, 2, 128, 16, "rows", 0, [(300, 200), (40, 1), (90, 3), (600, 18)], max_new=max_new)

@@ -100,7 +100,7 @@ struct PagedLine {
         for (int u = 0; u < 4; ++u) {
             PagedBlock k;
             k.first = max(at[u], 0);
-            k.n = b + u < c.seqs ? max(min(at[u + 1], p.rows) - k.first, 0) : 0;
+            k.n = b + u < c.seqs ? max(min(at[u + 1], p.rows), k.first) - k.first : 0;
             low += k.n & 0xffff, high += k.n >> 16;
             k.n *= p.group;
             if (!KIND::takes(p, k.n)) k.n = 0;
@@ -167,7 +167,7 @@ struct PagedLine {
         rem -= place.hk * each;
         k.seq = b0 + src * 4 + u;
         k.first = max(p.starts[k.seq], 0);
-        k.n = max(min(p.starts[k.seq + 1], p.rows) - k.first, 0) * p.group;
+        k.n = (max(min(p.starts[k.seq + 1], p.rows), k.first) - k.first) * p.group;
         const int len = p.lens[k.seq];
         k.place0 = len - p.starts[k.seq + 1] + k.first;
         k.have = min(max(len, 0), c.room());

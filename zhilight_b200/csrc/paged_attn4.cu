@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(256) k_paged4_wide(const PagedAttn p, const Pa
     pdl_trigger();
     pdl_wait();
     if (tid == 0 && blockIdx.z == 0) table[page] = page;
-    const int from = max(p.starts[b], 0), tokens = max(min(p.starts[b + 1], p.rows) - from, 0), len = p.lens[b], place0 = len - p.starts[b + 1] + from, have = min(max(len, 0), c.room());
+    const int from = max(p.starts[b], 0), tokens = max(min(p.starts[b + 1], p.rows), from) - from, len = p.lens[b], place0 = len - p.starts[b + 1] + from, have = min(max(len, 0), c.room());
     const int hi = min(place0 + tokens - 1, have - 1), lo = paged_from(p, place0) / kPtKeys * kPtKeys;
     if (!PtKind::takes(p, tokens * p.group) || row0 > hi || row0 + kWidePage <= lo) return;
     if (tid < kWidePage) s_off[tid] = row0 + tid <= hi ? c.row_at(b, row0 + tid) : -1;
