@@ -1185,7 +1185,7 @@ int zl_paged_attention_int4(const void* q, const void* k_cache, const void* v_ca
  *   biases bias_starts[r] .. bias_starts[r + 1] - 1 (clamped to 0 .. n_bias): z = z + bias[i] for the word bias_words[i], in the list's order
  *   temperature[r] >= 2^-126:      z = z * (1 / temperature[r]); else z stays
  *   mask row mask_row[r] (NULL: r; outside [0, masks): none), bit w % 32 of word w / 32 is clear: z = -inf.  A mask may leave nothing.
- * Arrays that are NULL take no part.  Whole numbers are counted: the same result in every run.  vocab up to 2^24, longest below 2^23. */
+ * Arrays that are NULL take no part.  Whole numbers are counted: the same result in every run.  vocab up to 2^24, longest below 2^23, n_bias up to 2^31 - 1025. */
 int zl_adjust_logits(const void* logits, long long ld_logits, int dtype, void* out, long long ld_out, int out_dtype, int rows, int vocab,
                      const int32_t* tokens, long long ld_tokens, int seqs, int longest, const int32_t* token_seq, const int32_t* token_lens,
                      const int32_t* prompt_lens, const float* repetition, const float* frequency, const float* presence, const int32_t* bias_starts,

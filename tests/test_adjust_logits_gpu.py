@@ -165,6 +165,17 @@ def test_adjust_of_long_bias_lists(cuda):
     check(torch.randn(3, vocab, generator=g), kw)
 
 
+@pytest.mark.parametrize("vocab", [1000, 20000])
+def test_adjust_of_bias_lists_at_the_ends_of_whole_numbers(cuda, vocab):
+    """Starts near the largest and the least whole number count as the list's end and its beginning: none wraps around to a place outside of it."""
+    g = torch.Generator().manual_seed(15)
+    top, least, n = 2 ** 31 - 1, -2 ** 31, 700
+    bias_words, bias = torch.randint(0, vocab, (n,), generator=g, dtype=torch.int32), torch.randn(n, generator=g)
+    z = torch.randn(5, vocab, generator=g)
+    for starts in ([top] * 6, [least] * 6, [0, top, top, least, least, top], [top - 255, top, 40, n, top - 512, least], [least, top, least + 1, 300, top - 31, n]):
+        check(z, dict(bias_starts=torch.tensor(starts, dtype=torch.int32), bias_words=bias_words, bias=bias))
+
+
 def test_adjust_without_rows_or_histories(cuda):
     z = torch.randn(3, 40, device="cuda")
     none = torch.zeros(3, 0, dtype=torch.int32, device="cuda")

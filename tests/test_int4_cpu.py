@@ -154,6 +154,23 @@ def test_oracle_rows_come_back(dtype, dim):
     assert torch.equal(y.unflatten(-1, (-1, 32)).amin(-1)[2:], low[2:])
 
 
+@pytest.mark.parametrize("n_bias,code", [((1 << 31) - 1, -2), ((1 << 31) - 1024, -2), (-1, -1)])
+def test_adjust_refuses_lists_whose_places_do_not_fit(lib, n_bias, code):
+    assert lib.zl_adjust_logits(*adjust_args(bias_starts=P, bias_words=P, bias=P, n_bias=n_bias)) == code, lib.zl_last_error()
+
+
+def test_adjust_front_end_refuses_sizes_beyond_32_bits(lib):
+    """Sizes that would come around as small ones, of tensors without memory."""
+    def many(*shape, dtype=torch.int32):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    n = (1 << 32) + 5
+    for bad in (dict(bias_starts=i32(4), bias_words=many(n), bias=many(n, dtype=torch.float32)), dict(tokens=many(3, n), token_lens=i32(3)),
+                dict(tokens=many(n, 3), token_lens=i32(3)), dict(mask=many(n, 3)), dict(logits=many(n, 70, dtype=torch.float16))):
+        with pytest.raises(_lib.ZLError, match="32 bits"):
+            ops.adjust_logits(**dict(dict(logits=torch.zeros(3, 70)), **bad))
+
+
 def test_oracle_adjusts_logits():
     z = torch.tensor([[1.0, -2.0, 3.0, 4.0, 0.5], [1.0, 1.0, 1.0, 1.0, 1.0]])
     tokens = torch.tensor([[0, 1, 2, 2, 7, -1]], dtype=torch.int32)

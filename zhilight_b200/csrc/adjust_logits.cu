@@ -16,6 +16,7 @@
 // row's own.
 #include "paged.cuh"
 
+#include <climits>
 #include <type_traits>
 
 namespace zl {
@@ -93,7 +94,8 @@ __global__ void __launch_bounds__(kAlThreads, 4) k_adjust_logits(const AdjustLog
     const int start = base + tid * VEC;
     fetch(start);
     int first = 0, last = 0;   // of the biases
-    if (p.bias_starts) first = max(p.bias_starts[r], 0), last = min(p.bias_starts[r + 1], p.n_bias);
+    // Clamped at both ends before anything is added to them: a start near the largest integer would wrap around, to places before the list.
+    if (p.bias_starts) first = min(max(p.bias_starts[r], 0), p.n_bias), last = max(min(p.bias_starts[r + 1], p.n_bias), first);
     const int seq = !counts ? -1 : p.token_seq ? p.token_seq[r] : r, length = counts ? p.token_lens[r] : 0, prompt = p.prompt_lens ? p.prompt_lens[r] : 0;
     int mine[kEach];   // this thread's of the first ones, and what they are
     float mine_bias[kEach];
@@ -318,6 +320,7 @@ extern "C" int zl_adjust_logits(const void* logits, long long ld_logits, int dty
     ZL_CHECK_ARG(logits && out && rows > 0 && vocab > 0 && ld_logits >= vocab && ld_out >= vocab);
     ZL_CHECK_ARG(!tokens || (token_lens && seqs > 0 && longest >= 0 && ld_tokens >= longest && (token_seq || seqs >= rows)));
     ZL_CHECK_ARG(!bias_starts || (n_bias >= 0 && (n_bias == 0 || (bias_words && bias))));
+    ZL_CHECK_SUPPORTED(!bias_starts || n_bias <= INT_MAX - 1024);   // a CTA's look ahead from the list's end is counted in 32 bits
     ZL_CHECK_ARG(!mask || (masks > 0 && ld_mask >= (vocab - 1) / 32 + 1 && (mask_row || masks >= rows)));
     ZL_CHECK_SUPPORTED(vocab <= 1 << 24 && longest < 1 << 23 && (out_dtype == dtype || out_dtype == ZL_F32) && (dtype == ZL_F32 || dtype == ZL_F16 || dtype == ZL_BF16));
     AdjustLogits p = {logits, out, ld_logits, ld_out, tokens, token_seq, token_lens, prompt_lens, bias_starts, bias_words, mask, mask_row,

@@ -1389,6 +1389,7 @@ def adjust_logits(logits, tokens=None, token_seq=None, token_lens=None, prompt_l
               "mask must be (M, vocab / 32 or more) int32, its rows in one piece")
         _need(mask_row is not None or mask.shape[0] >= r, "a mask of fewer rows than the logits' needs mask_row")
         _need(mask.shape[0] < 2 or mask.stride(0) >= mask.shape[1], "rows of mask must not share memory")
+    _need(max([r, n] + [s for x in (tokens, mask) if x is not None for s in x.shape]) < 2 ** 31 - 1024, "rows, words and biases are counted in 32 bits", -2)
     _here(logits, tokens, token_seq, token_lens, prompt_lens, repetition, frequency, presence, bias_starts, bias_words, bias, temperature, mask, mask_row, out)
     if out is None:
         out = torch.empty((r, vocab), dtype=want, device=logits.device)
