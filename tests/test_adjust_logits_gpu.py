@@ -176,6 +176,53 @@ def test_adjust_of_bias_lists_at_the_ends_of_whole_numbers(cuda, vocab):
         check(z, dict(bias_starts=torch.tensor(starts, dtype=torch.int32), bias_words=bias_words, bias=bias))
 
 
+def some_rows(z, kw, rows):
+    """The same call for some of its rows, on the host."""
+    each = ("token_seq", "token_lens", "prompt_lens", "repetition", "frequency", "presence", "temperature", "mask_row")
+    kw = {n: x[rows] if n in each else x for n, x in kw.items()}
+    lists = [slice(int(kw["bias_starts"][r]), int(kw["bias_starts"][r + 1])) for r in rows]
+    counts = torch.tensor([0] + [x.stop - x.start for x in lists])
+    kw.update(bias_words=torch.cat([kw["bias_words"][x] for x in lists]), bias=torch.cat([kw["bias"][x] for x in lists]), bias_starts=counts.cumsum(0).to(torch.int32))
+    return z[rows], kw
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(BF16, None), (BF16, F32), (F16, None), (F32, None)])
+@pytest.mark.parametrize("rows,vocab,longest,first,different,biases", [
+    (128, 32000, 9000, 200, 1400, 9), (128, 32000, 9000, 0, 2500, 9), (160, 50257, 9000, 16000, 5300, 9), (128, 32000, 9000, 21400, 5470, 9), (130, 33001, 12000, 10900, 9000, 40),
+    (200, 32000, 16000, 0, 16000, 3), (400, 17000, 16000, 5, 16000, 1100), (300, 16384, 20000, 1, 16000, 9)])
+def test_adjust_of_many_rows(cuda, dtype, out_dtype, rows, vocab, longest, first, different, biases):
+    """Rows enough for wide pieces, histories of thousands of different words side by side: lists of marked words that a thread's registers do not hold, that fill their room,
+    and that are too long for it, with counters of 16 and of 32 bits; beside the logits, over them, and from rows that begin anywhere."""
+    g = torch.Generator().manual_seed(vocab + different)
+    kw = settings(g, rows, vocab, 4, longest, 2, 3)
+    for s in range(3):                                               # each of the words once, then some of them again; the last history is as it was
+        words = first + torch.randperm(different, generator=g)
+        again = words[torch.randint(0, different, (longest - different,), generator=g)]
+        kw["tokens"][s] = torch.cat([words, again])[torch.randperm(longest, generator=g)]
+    kw["token_seq"] = torch.arange(rows, dtype=torch.int32) % 4
+    kw["token_lens"] = torch.where(torch.arange(rows) % 5 == 4, kw["token_lens"], longest).to(torch.int32)
+    counts = torch.randint(0, 2 * biases + 1, (rows,), generator=g) * (torch.arange(rows) % 3 > 0)
+    counts[1], counts[2] = 2 * biases, biases                        # of words behind the others, where there are any
+    kw["bias_starts"][1:] = counts.cumsum(0)
+    n = int(counts.sum())
+    kw["bias_words"], kw["bias"] = torch.randint(min(first + different, vocab - 9), vocab, (n,), generator=g, dtype=torch.int32), torch.randn(n, generator=g)
+    wide = (torch.randn(rows, vocab + 8, generator=g) * 3).to(dtype)
+    sample = torch.tensor([0, 1, 2, 3, 4, rows // 2, rows - 2, rows - 1])
+    dev, dwide = on_gpu(kw), wide.cuda()
+    for at in (0, 3):
+        z = wide[:, at:at + vocab]
+        z_some, kw_some = some_rows(z, kw, sample)
+        dz = dwide[:, at:at + vocab]
+        check(z_some, kw_some, out_dtype, got=ops.adjust_logits(dz, out_dtype=out_dtype, **dev)[sample])
+        assert torch.equal(dz.cpu(), z)
+        if out_dtype is None:
+            other, room = ops.adjust_logits(dz, **dev), dwide.clone()
+            got = ops.adjust_logits(room[:, at:at + vocab], out=room[:, at:at + vocab], **dev)
+            check(z_some, kw_some, got=got[sample])
+            assert torch.equal(got.view(torch.int16 if dtype != F32 else torch.int32), other.view(torch.int16 if dtype != F32 else torch.int32))   # every row, NaN or not
+            assert torch.equal(room[:, :at], dwide[:, :at]) and torch.equal(room[:, at + vocab:], dwide[:, at + vocab:])
+
+
 def test_adjust_without_rows_or_histories(cuda):
     z = torch.randn(3, 40, device="cuda")
     none = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
