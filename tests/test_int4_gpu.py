@@ -362,6 +362,36 @@ def test_attention_blocks_with_broken_tokens(cuda, new, heads):
     assert torch.isnan(got[~fine]).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("page,order", [(16, "rows"), (32, "heads"), (20, "rows"), (16, "wide")])
+@pytest.mark.parametrize("new,heads,dim,extra", [(1, 8, 128, 1), (1, 8, 64, 1), (2, 8, 64, 1), (3, 8, 128, 1), (6, 8, 64, 1), (16, 8, 128, 1), (40, 8, 64, 1), (140, 8, 128, 1),
+                                                 (140, 8, 128, 1 << 30), (150, 8, 64, 1), (150, 8, 64, 1 << 30), (17, 40, 64, 1)])
+@pytest.mark.parametrize("window", [0, 3, 40])
+def test_attention_beside_broken_groups(cuda, dtype, page, order, new, heads, dim, extra, window):
+    """Broken groups of keys or values, several of them and in two pages, also behind the last key of a sequence and before the windows: rows that must not see them are what they are without.
+    Blocks of 8 and of 16 rows, tiles that make numbers of codes and tiles that read them made, pages that boxes serve and others."""
+    g = torch.Generator().manual_seed(new * 7 + dim + page)
+    kv_heads, n, pages = 2, 400, 60
+    table = tables(g, [n, n - 77], page, pages, 1 if extra == 1 else extra // (page * kv_heads * dim * 4) // 2)
+    q = torch.randn(2 * new, heads, dim, generator=g).to(dtype)
+    starts, lens = starts_of([new, new]), torch.tensor([n, n - 77], dtype=torch.int32)
+    for wheres in ((n - new // 2 - 1,), (n - 1, n - new - 30), (n - new - 41, n - new - 42, n - 3), (n - new, n - new // 3 - 1)):
+        for which in range(2):
+            k, v = pool(g, pages, page, kv_heads, dim, dtype, order)
+            hide(k, table, lens.tolist()), hide(v, table, lens.tolist())
+            for where in wheres:
+                (k, v)[which][int(table[0, where // page]), where % page, 1, dim // 2 + 4:dim // 2 + 8] = 0xff   # columns 32 to 63
+            got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), lens.cuda(), starts.cuda(), dim ** -0.5, window=window, max_new=new).cpu().double()
+            want, off = oracle.attention(q, codes.decode(k, dtype), codes.decode(v, dtype), table, lens.tolist(), starts, dim ** -0.5, window)
+            at = torch.arange(n - new, n)[:, None]
+            broken = torch.tensor(wheres)
+            sees = ((at >= broken) & ((at < broken + window) if window else torch.ones((), dtype=torch.bool))).any(1)
+            fine = torch.ones(2 * new, heads, dim, dtype=torch.bool)
+            fine[:new][sees, heads // 2:, 32 if which else 0:64 if which else dim] = False
+            assert ((got - want).abs() <= off)[fine].all(), (wheres, which)
+            assert torch.isnan(got[~fine]).all(), (wheres, which)
+
+
 @pytest.mark.parametrize("dtype,size", [(BF16, 2.0 ** 124), (BF16, 2.0 ** -100), (BF16, 2.0 ** -70), (F16, 2.0 ** 13), (F16, 2.0 ** -14)])
 @pytest.mark.parametrize("new,heads", [(1, 4), (4, 8), (150, 8)])
 @pytest.mark.parametrize("dim", [64, 128])
