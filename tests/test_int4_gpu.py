@@ -1,5 +1,6 @@
 """Operators over a paged cache of 4 bits on a GPU, against their formulas in 64 bits (paged_oracle, int4_oracle)."""
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -126,6 +127,57 @@ def test_append_at_the_ends_of_the_type(cuda, dtype, dim):
         for y in ops.int4_cache_values(kd, vd, dtype):
             y = y.cpu()
             assert torch.equal(torch.isnan(y), broken) and torch.equal(y[~broken], want[~broken])
+
+
+def formula_row(x, dtype):
+    """A row of numbers of dtype -> its bytes, by fractions: nothing is rounded but what the formula rounds."""
+    v, (bits, least), words, pairs = [Fraction(float(y)) for y in x], codes.BITS[dtype], [], []
+    for i in range(0, len(v), 32):
+        low, high = min(v[i:i + 32]), max(v[i:i + 32])
+        part = (high - low) / 15
+        power = least
+        while part >= Fraction(2) ** (power + 1):
+            power += 1
+        unit = Fraction(2) ** (power - bits + 1)
+        step = part // unit * unit
+        code = [min(round((y - low) / step), 15) if step >= Fraction(2) ** -126 else 0 for y in v[i:i + 32]]   # to the nearest, ties to even
+        words += [sum(c << codes.PLACE[j] for j, c in enumerate(code[k:k + 8])) for k in range(0, 32, 8)]
+        pairs.append(torch.tensor([float(step), min(float(y) for y in x[i:i + 32])], dtype=dtype))   # -0 is a lowest value too
+    return torch.cat([torch.tensor([w - (w >> 31 << 32) for w in words], dtype=torch.int32).view(torch.uint8), torch.cat(pairs).view(torch.uint8)])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_append_of_numbers_far_apart(cuda, dtype):
+    """Groups whose numbers have more bits between them than 32-bit numbers: lowest values so small that the range is just below or above 15 steps of the type, values beside the
+    border between two codes by as little, and any numbers of the type in one group.  Steps and codes are the formula's."""
+    g = torch.Generator().manual_seed(41)
+    dim, (bits, least) = 64, codes.BITS[dtype]
+    tiny = 2.0 ** (least - bits + 1)                                 # the smallest number of the type
+    x = torch.zeros(400, dim)
+    for i in range(200):
+        scale = 2.0 ** (i % 9 if dtype == F16 else i % 50 - 20)
+        low = (-1.0) ** i * max(2.0 ** -(10 + i // 4 % 40), tiny)
+        x[i] = torch.randint(0, 31, (dim,), generator=g) * 0.5 * scale   # whole steps and halves of them
+        x[i, ::32], x[i, 1::32] = low, 15.0 * scale
+        if low > 0:
+            x[i].clamp_(min=low)
+        elif i % 3 == 0:
+            x[i, 2:9], x[i, 34:41] = -low, -low * 2
+    any_bits = torch.randint(-2 ** 15, 2 ** 15, (400, dim), generator=g, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = x.to(dtype)
+    x[200:] = torch.where(torch.isfinite(any_bits[200:]), any_bits[200:], torch.ones((), dtype=dtype))
+    x[300:] = torch.where(torch.rand(100, dim, generator=g) < 0.7, (x[300:].double().abs() ** 0.25).to(dtype), x[300:])
+    x[0], x[1] = x[2], x[3]
+    x[0, :3], x[1, :3] = torch.tensor([-2.0 ** -25, 15.0, 2.5]), torch.tensor([2.0 ** -25, 15.0, 2.5])
+    x[0, 3:32], x[1, 3:32] = 7.5, 7.5
+    kd = torch.zeros(25, 16, 1, 40, dtype=torch.uint8, device="cuda")
+    vd, one = torch.zeros_like(kd), torch.zeros(400, dtype=torch.int32, device="cuda")
+    ops.qkv_axes_rope_append_int4(torch.cat([x, x, x.flip(1)], 1).cuda(), one[None], torch.ones(1, dtype=torch.float64).cuda(), one[:1] - 1, one,
+                                  torch.arange(400, dtype=torch.int32).cuda(), torch.arange(25, dtype=torch.int32)[None].cuda(), kd, vd, 1)
+    for got, rows in ((kd, x), (vd, x.flip(1))):
+        want = torch.stack([formula_row(r, dtype) for r in rows.double().tolist()])
+        off = torch.nonzero((got.cpu().view(400, 40) != want).any(1)).flatten()
+        assert off.numel() == 0, (off.tolist(), rows[off[0]].tolist())
 
 
 def test_append_takes_pages_of_the_table_only(cuda):

@@ -134,6 +134,10 @@ __device__ __forceinline__ __half int4_round_down<__half>(float x) { return __fl
 template <>
 __device__ __forceinline__ __nv_bfloat16 int4_round_down<__nv_bfloat16>(float x) { return __float2bfloat16_rz(x); }
 
+// the number above one that is at least zero
+__device__ __forceinline__ __half int4_next(__half x) { return __ushort_as_half((unsigned short)(__half_as_ushort(x) + 1)); }
+__device__ __forceinline__ __nv_bfloat16 int4_next(__nv_bfloat16 x) { return __ushort_as_bfloat16((unsigned short)(__bfloat16_as_ushort(x) + 1)); }
+
 // 8 columns of a group whose other columns are in the neighbouring lanes of this group of four; all lanes of the warp call it.  -> the codes; the group's pair
 template <typename T>
 __device__ __forceinline__ uint32_t int4_encode(const uint4& x, uint32_t& meta) {
@@ -154,30 +158,41 @@ __device__ __forceinline__ uint32_t int4_encode(const uint4& x, uint32_t& meta) 
     }
     const T* of = reinterpret_cast<const T*>(&ends);
     const float half = -0.5f * to_f32<T>(of[1]);   // of the lowest
-    const T pair[2] = {int4_round_down<T>(__fdiv_rn(__fmaf_rn(to_f32<T>(of[0]), 0.5f, -half), 7.5f)), from_f32<T>(half * 2.f)};
+    // The step: the largest number of T that 7.5 times is at most half the range, all exactly: 32 bits hold 7.5 times a number of T, and rounding the range towards zero moves it
+    // past none of them.  A product with 1 / 7.5, both rounded down, gives that number or the one below it.
+    const float part = __fmaf_rz(to_f32<T>(of[0]), 0.5f, -half);
+    T pair[2] = {int4_round_down<T>(__fmul_rz(part, 0x1.111110p-3f)), from_f32<T>(half * 2.f)};
+    const T next = int4_next(pair[0]);
+    if (__fmul_rn(to_f32<T>(next), 7.5f) <= part) pair[0] = next;
     meta = numbers == 15u ? *reinterpret_cast<const uint32_t*>(pair) : 0x7fff7fffu;
     const float step = to_f32<T>(pair[0]);
     if (numbers != 15u || !(step >= 1.17549435e-38f)) return 0;
     float f[8];
     unpack8<T>(x, f);
     uint32_t codes = 0;
+    // half of x - lo, of which 32 bits may not hold all: what is lost leaves the last bit set, so that a difference beside the border between two codes, (c + 1/2) step, which
+    // has 16 bits, does not become it
+    auto above = [&](float x) {
+        const uint32_t down = __float_as_uint(__fmaf_rz(x, 0.5f, -half)), up = __float_as_uint(__fmaf_ru(x, 0.5f, -half));   // the same number or neighbours
+        return __uint_as_float(down | ((down ^ up) & 1u));
+    };
     if (step >= 1e-30f) {
-        // Quotients by the reciprocal and one correction of what is left over (Markstein 1990), a quarter of a division's instructions.  x and lo are numbers of T: where the quotient lies
-        // on the border between two codes it comes out exactly, as the correction's error is 2^-46 of it, elsewhere it is 2^-17 away from one.  Codes are whole numbers at the
+        // Quotients by the reciprocal and one correction of what is left over (Markstein 1990), a quarter of a division's instructions: rounded once.  One on the border between two
+        // codes comes out exactly, and one beside it does not come out as the border: it is more than half a unit of 32 bits away from it.  Codes are whole numbers at the
         // end of 1.5 * 2^23 + c, each multiplied into its place; what that number adds there is taken away beforehand.
         const float inv = __fdiv_rn(1.f, step);
         constexpr uint32_t kWhole = 0x4b400000u;
         codes = 0u - kWhole * 0x11111111u;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float d = __fmaf_rn(f[i], 0.5f, -half);
+            const float d = above(f[i]);
             float q = __fmul_rn(d, inv);
             q = __fmaf_rn(__fmaf_rn(-q, step, d), inv, q);
             codes += __float_as_uint(__fmaf_rn(fminf(q, 7.5f), 2.f, 12582912.f)) << ((i & 1) * 16 + (i & 6) * 2);
         }
     } else {   // far down those products would lose bits
 #pragma unroll 1
-        for (int i = 0; i < 8; ++i) codes |= (uint32_t)__float2int_rn(fminf(2.f * __fdiv_rn(__fmaf_rn(f[i], 0.5f, -half), step), 15.f)) << ((i & 1) * 16 + (i & 6) * 2);
+        for (int i = 0; i < 8; ++i) codes |= (uint32_t)__float2int_rn(fminf(2.f * __fdiv_rn(above(f[i]), step), 15.f)) << ((i & 1) * 16 + (i & 6) * 2);
     }
     return codes;
 }
