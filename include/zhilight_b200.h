@@ -1180,10 +1180,10 @@ int zl_paged_attention_int4(const void* q, const void* k_cache, const void* v_ca
 /* Penalties, biases, temperature and grammar masks on logits (rows, ld_logits >= vocab) in `dtype` -> out (rows, ld_out) in the same type or fp32; out may be logits.
  * History of row r: the first token_lens[r] (clamped to 0 .. longest) words of row token_seq[r] (NULL: r; outside [0, seqs): no history) of tokens (seqs, ld_tokens), the
  * first prompt_lens[r] (NULL: 0) of them a prompt; words outside the vocabulary are passed over.  In this order, each in 32 bits:
- *   a word of the history:         z = z > 0 ? z * (1 / repetition[r]) : z * repetition[r]
+ *   a word of the history:         z = z > 0 ? z / repetition[r] : z * repetition[r]
  *   n > 0 times behind the prompt: z = z - (frequency[r] * n + presence[r])
  *   biases bias_starts[r] .. bias_starts[r + 1] - 1 (clamped to 0 .. n_bias): z = z + bias[i] for the word bias_words[i], in the list's order
- *   temperature[r] >= 2^-126:      z = z * (1 / temperature[r]); else z stays
+ *   temperature[r] >= 2^-126:      z = z / temperature[r]; else z stays
  *   mask row mask_row[r] (NULL: r; outside [0, masks): none), bit w % 32 of word w / 32 is clear: z = -inf.  A mask may leave nothing.
  * Arrays that are NULL take no part.  Whole numbers are counted: the same result in every run.  vocab up to 2^24, longest below 2^23, n_bias up to 2^31 - 1025. */
 int zl_adjust_logits(const void* logits, long long ld_logits, int dtype, void* out, long long ld_out, int out_dtype, int rows, int vocab,

@@ -223,6 +223,23 @@ def test_adjust_of_many_rows(cuda, dtype, out_dtype, rows, vocab, longest, first
             assert torch.equal(room[:, :at], dwide[:, :at]) and torch.equal(room[:, at + vocab:], dwide[:, at + vocab:])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("vocab", [1003, 40000])
+def test_adjust_divides(cuda, dtype, vocab):
+    """Quotients by repetition and temperature are 32-bit quotients, rounded once: what torch's division on the host gives, bit by bit."""
+    g = torch.Generator().manual_seed(16)
+    z = torch.randn(24, vocab, generator=g) * torch.exp2(torch.randint(-3, 6, (24, vocab), generator=g).float())
+    z[:, ::50], z[:, 1::50] = math.inf, -math.inf
+    z, by = z.to(dtype), 0.05 + torch.rand(24, generator=g) * 2.5
+    by[0], by[1], by[2], by[3] = 1.0, 2.0 ** -20, 3.0e20, 1.0 + 2.0 ** -23
+    want = z.float() / by[:, None]
+    assert torch.equal(ops.adjust_logits(z.cuda(), temperature=by.cuda(), out_dtype=F32).cpu(), want)
+    words = torch.arange(vocab, dtype=torch.int32)[None]
+    kw = dict(tokens=words, token_seq=torch.zeros(24, dtype=torch.int32), token_lens=torch.full((24,), vocab, dtype=torch.int32), repetition=by)
+    want = torch.where(z.float() > 0, want, z.float() * by[:, None])
+    assert torch.equal(ops.adjust_logits(z.cuda(), out_dtype=F32, **on_gpu(kw)).cpu(), want)
+
+
 def test_adjust_without_rows_or_histories(cuda):
     z = torch.randn(3, 40, device="cuda")
     none = torch.zeros(3, 0, dtype=torch.int32, device="cuda")

@@ -1,8 +1,8 @@
 // What stands between a model's logits and the probabilities that words are drawn from or drafts verified against: penalties for repeated words, biases, temperature,
 // a grammar's mask.  Of a row with history h (the first of it a prompt), word w, n(w) its times behind the prompt:
 //
-//   z = z * (1 / repetition) (z > 0) or z * repetition, where w is in h;   z -= frequency * n(w) + presence, where n(w) > 0
-//   z += its biases, one after the other;   z *= 1 / temperature;   -inf, where the mask has no bit for w
+//   z = z / repetition (z > 0) or z * repetition, where w is in h;   z -= frequency * n(w) + presence, where n(w) > 0
+//   z += its biases, one after the other;   z /= temperature;   -inf, where the mask has no bit for w
 //
 // A CTA has a piece of a row's vocabulary, with a counter in shared memory for each word: how often it came, whether it is in the history, whether there is a bias.  Every CTA goes
 // over the whole history and counts the words of its piece by atomics of its own shared memory: whole numbers, which add up the same in every order.  (With the history
@@ -106,7 +106,13 @@ __global__ void __launch_bounds__(kAlThreads, 4) k_adjust_logits(const AdjustLog
         if (i < last) mine[u] = p.bias_words[i], mine_bias[u] = p.bias[i];
     }
     const float rep = p.repetition ? p.repetition[r] : 1.f, up = 1.f / rep, freq = p.frequency ? p.frequency[r] : 0.f, pres = p.presence ? p.presence[r] : 0.f;
-    const float heat = p.temperature ? p.temperature[r] : 0.f, inv = heat >= 1.17549435e-38f ? 1.f / heat : 1.f;
+    const float given = p.temperature ? p.temperature[r] : 0.f, heat = given >= 1.17549435e-38f ? given : 1.f, inv = 1.f / heat;
+    // z / by: by the reciprocal and one correction of what is left over (Markstein 1990), which is a number where z, the divisor and the quotient are
+    auto quotient = [](float z, float by, float inverse) {
+        const float q = z * inverse, left = fmaf(-q, by, z);
+        return fabsf(left) < INFINITY ? fmaf(left, inverse, q) : q;
+    };
+    auto cooled = [&](float z) { return quotient(z, heat, inv); };
     const int mask_row = !p.mask ? -1 : p.mask_row ? p.mask_row[r] : r;
     const int32_t* mask = mask_row >= 0 && mask_row < p.masks ? p.mask + (long long)mask_row * p.ld_mask : nullptr;
     // a counter before it was changed: a word that had no mark goes on the list
@@ -188,7 +194,7 @@ __global__ void __launch_bounds__(kAlThreads, 4) k_adjust_logits(const AdjustLog
     const C* marked = reinterpret_cast<const C*>(al_count);
     auto adjusted = [&](float z, uint32_t mark, int word) {
         const uint32_t n = mark & Counter::kCount;
-        if (mark & (Counter::kCount | Counter::kSeen)) z *= z > 0.f ? up : rep;
+        if (mark & (Counter::kCount | Counter::kSeen)) z = z > 0.f ? (fabsf(up) < INFINITY ? quotient(z, rep, up) : z / rep) : z * rep;
         if (n) z -= fmaf(freq, (float)n, pres);
         if (mark & Counter::kBias) {
             if (listed >= 0) {
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(kAlThreads, 4) k_adjust_logits(const AdjustLog
         return z;
     };
     const int some = marks ? s_marks : 0;
-    auto ends = [&](float z, int word) { return from_f32<TO>(!mask || ((uint32_t)mask[word >> 5] >> (word & 31) & 1u) ? z * inv : -INFINITY); };
+    auto ends = [&](float z, int word) { return from_f32<TO>(!mask || ((uint32_t)mask[word >> 5] >> (word & 31) & 1u) ? cooled(z) : -INFINITY); };
     if (some > p.room) {   // word by word
         for (int i = lo + tid; i < hi; i += kAlThreads) {
             const float z = to_f32<TI>(in[i]);
@@ -239,7 +245,7 @@ __global__ void __launch_bounds__(kAlThreads, 4) k_adjust_logits(const AdjustLog
             for (int e = 0; e < VEC; ++e) z[e] = to_f32<TI>(x[u][e]);
             TO y[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) y[e] = from_f32<TO>(allowed >> e & 1u ? z[e] * inv : -INFINITY);
+            for (int e = 0; e < VEC; ++e) y[e] = from_f32<TO>(allowed >> e & 1u ? cooled(z[e]) : -INFINITY);
             if constexpr (VEC == 1) out[i] = y[0];
             else if (i < lo || i + VEC > hi)
 #pragma unroll
