@@ -68,14 +68,6 @@ template <typename T>
 __device__ __forceinline__ uint4 int4_eight(uint32_t x, uint32_t step, uint32_t low) {
     return make_uint4(int4_two<T, 0>(x, step, low), int4_two<T, 1>(x, step, low), int4_two<T, 2>(x, step, low), int4_two<T, 3>(x, step, low));
 }
-// one column
-template <typename T>
-__device__ __forceinline__ float int4_value(const uint8_t* row, int dim, int col) {
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(row + (col >> 3) * 4), meta = *reinterpret_cast<const uint32_t*>(row + dim / 2 + (col / kInt4Group) * 4);
-    const T* two = reinterpret_cast<const T*>(&meta);
-    const float c = (float)(word >> ((col & 1) * 16 + (col & 6) * 2) & 15u);
-    return round_to<T>(fmaf(c, to_f32<T>(two[0]), to_f32<T>(two[1])));
-}
 // whether a group's pair is one of numbers
 template <typename T>
 __device__ __forceinline__ bool int4_finite(uint32_t meta) {

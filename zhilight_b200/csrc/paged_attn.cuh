@@ -260,8 +260,8 @@ __device__ __forceinline__ void paged_row_out(const PagedAttn& p, const PagedBlo
 // Blocks that were cut, of the kernel for few rows.  grid (its CTAs): the first part of a block lies in its CTA's place 1, the others in the place 0 of theirs,
 // R rows each.  A chain of three loads bounds it, so the warps share out the rows and, where there are fewer, the parts of a row too, and ask for many at
 // once; more CTAs, a row each, cost more than they give (37 blocks that nothing cuts: 13.4 -> 22.5 us a call).
-constexpr int kJoinWarps = 16;   // not fewer warps than rows
-template <typename T, int D, int R, int kJoinAhead = 4>
+constexpr int kJoinWarps = 16, kJoinAhead = 4;   // not fewer warps than rows
+template <typename T, int D, int R>
 __global__ void __launch_bounds__(kJoinWarps * 32) k_paged_join(const PagedAttn p) {
     constexpr int E = D / 32;
     static_assert(R <= kJoinWarps, "a warp for every row");
