@@ -1171,7 +1171,8 @@ int zl_qkv_axes_rope_append_int4(const void* qkv, long long ldq, const int32_t* 
 int zl_int4_cache_values(const void* k_cache, const void* v_cache, long long num_pages, int page_size, long long page_stride, long long row_stride,
                          long long head_stride, const int32_t* pages, long long n, void* k_out, void* v_out, int kv_heads, int dim, int dtype, int pdl,
                          zl_stream_t stream);
-/* zl_paged_attention over such a cache.  A broken group (NaN) of a key or value reaches the rows that see it and no others. */
+/* zl_paged_attention over such a cache.  A broken group (NaN) of a key or value reaches the rows that see it and no others.  Over a bf16 cache scale is up to 2^64, keys are taken to
+ * multiples of 2^-113, and values below 2^-86 are lost. */
 size_t zl_paged_attention_int4_workspace_bytes(int rows, int max_new, int seqs, int max_keys /* max_pages * page_size */, int heads, int kv_heads, int dim);
 int zl_paged_attention_int4(const void* q, const void* k_cache, const void* v_cache, long long num_pages, int page_size, long long page_stride,
                             long long row_stride, long long head_stride, const int32_t* page_table, int ld_table, int max_pages,

@@ -34,6 +34,11 @@ def test_attention_refuses(lib, kw, code):
     assert lib.zl_paged_attention_int4(*attention_args(**dict(BYTES, **kw))) == code, lib.zl_last_error()
 
 
+@pytest.mark.parametrize("scale", [2.0 ** 65, 3.0e38])
+def test_attention_refuses_scales_beyond_its_sums(lib, scale):
+    assert lib.zl_paged_attention_int4(*attention_args(**dict(BYTES, scale=scale))) == -2, lib.zl_last_error()
+
+
 def values_args(**kw):
     a = dict(k_cache=P, v_cache=P, num_pages=8, page_size=16, page_stride=1280, row_stride=80, head_stride=80, pages=None, n=8, k_out=P, v_out=P, kv_heads=1,
              dim=128, dtype=ops.BF16, pdl=0, stream=None)

@@ -479,6 +479,20 @@ def test_attention_of_large_keys(cuda, dtype, size, new, heads, extra):
     assert ((got - want).abs() <= off).all()
 
 
+@pytest.mark.parametrize("dtype,scale", [(BF16, 2.0 ** 64), (BF16, 2.0 ** -60), (F16, 2.0 ** 10)])
+@pytest.mark.parametrize("new,extra", [(1, 1), (9, 1), (150, 1), (150, 400000)])
+def test_attention_of_large_and_small_scales(cuda, dtype, scale, new, extra):
+    """Queries that the scale makes ordinary ones."""
+    g = torch.Generator().manual_seed(35)
+    lens, page = [300, new + 7], 16
+    table, starts = tables(g, lens, page, 50, extra), starts_of([new, new])
+    k, v = pool(g, 50, page, 2, 64, dtype, "rows")
+    q = (torch.randn(2 * new, 8, 64, generator=g) / scale / 8).to(dtype)
+    got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), starts.cuda(), scale, max_new=new).cpu().double()
+    want, off = oracle.attention(q, codes.decode(k, dtype), codes.decode(v, dtype), table, lens, starts, scale, 0)
+    assert ((got - want).abs() <= off).all()
+
+
 STEEP = {"one": [(300, 1), (77, 1), (1000, 1)], "drafts": [(300, 4), (80, 3), (4, 4)], "portion": [(300, 150), (150, 150), (700, 33)],
          "many": [(90 + 7 * (i % 5), 1 + i % 20) for i in range(60)]}
 

@@ -203,6 +203,7 @@ extern "C" int zl_paged_attention_int4(const void* q, const void* k_cache, const
     ZL_CHECK_ARG(page_table && max_pages > 0 && ld_table >= max_pages && seqs > 0);
     ZL_CHECK_SUPPORTED(dtype == ZL_F16 || dtype == ZL_BF16);
     ZL_CHECK_SUPPORTED(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0);
+    ZL_CHECK_SUPPORTED(dtype == ZL_F16 || scale <= 0x1p64f);   // products with bf16 keys carry 2^-20 (Int4Codes), which the scale takes away: neither that nor the smallest sums may leave 32 bits
     ZL_CHECK_SUPPORTED(heads <= 65535 && (long long)rows * heads < INT_MAX);
     const long long room = (long long)max_pages * page_size;
     const Paged4Plans s = paged4_plan(rows, max_new, seqs, (int)(room < INT_MAX - 255 ? room : INT_MAX - 255), heads, kv_heads, dim);

@@ -1268,7 +1268,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
 def paged_attention_int4(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window=0, max_new=None, out=None, pdl=False):
     """paged_attention over caches of 4 bits (pages, page_size, kv_heads, int4_row_bytes(dim)) uint8 whose rows were written from q's type
     (qkv_axes_rope_append_int4): the attention over what they stand for, int4_cache_values.  A broken group (NaN) of a key or value reaches the rows that see
-    it and no others.  Portions of prompts take a workspace of up to 256 MB, by the room that page_table has.  -> out, like q."""
+    it and no others.  scale up to 2^64 for bf16.  Portions of prompts take a workspace of up to 256 MB, by the room that page_table has.  -> out, like q."""
     if _lib.host is not None:
         y = _lib.host.paged_attention_int4(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl)
         if y is not None:
