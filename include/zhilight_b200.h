@@ -1160,7 +1160,8 @@ int zl_verify_drafts(const float* target, long long target_seq, long long target
  * heads of 128, 40 for 64; no other dim).  A code c stands for lowest + step * c, rounded to that type; the step is a 15th of the range of the 32 values, rounded down, a
  * value becomes the nearest whole number of steps, at most 15.  32 values with an infinity or NaN among them read as NaN.  Columns 8i .. 8i + 7 lie in bits
  * 0 16 4 20 8 24 12 28 of word i.  Strides are bytes here, multiples of dim / 8, as both bases are.
- * zl_qkv_axes_rope_append_int4 is zl_qkv_axes_rope_append into such a cache: two rows of qkv have to fit shared memory (56000 elements). */
+ * zl_qkv_axes_rope_append_int4 is zl_qkv_axes_rope_append into such a cache: two rows of qkv have to fit shared memory beside
+ * cosines and sines: (heads + 2 kv_heads) * dim up to 56288 - 12 half elements. */
 int zl_qkv_axes_rope_append_int4(const void* qkv, long long ldq, const int32_t* pos, long long ld_pos, int axes, const double* inv_freq,
                                  const int32_t* axis, int half, int layout, float mscale, const int32_t* token_seq, const int32_t* placement,
                                  const int32_t* page_table, int ld_table, int max_pages, int seqs, void* k_cache, void* v_cache, long long num_pages,

@@ -34,6 +34,13 @@ def test_attention_refuses(lib, kw, code):
     assert lib.zl_paged_attention_int4(*attention_args(**dict(BYTES, **kw))) == code, lib.zl_last_error()
 
 
+def test_append_refuses_rows_beyond_shared_memory(lib):
+    """Two rows of 434 heads of 128, and cosines and sines of 64 frequencies: 32 elements more than there is room for."""
+    assert 434 * 128 == 56288 - 12 * 64 + 32
+    args = dict(BYTES, heads=432, kv_heads=1, half=64, ldq=434 * 128)
+    assert lib.zl_qkv_axes_rope_append_int4(*append_args(**args)) == -2, lib.zl_last_error()
+
+
 @pytest.mark.parametrize("scale", [2.0 ** 65, 3.0e38])
 def test_attention_refuses_scales_beyond_its_sums(lib, scale):
     assert lib.zl_paged_attention_int4(*attention_args(**dict(BYTES, scale=scale))) == -2, lib.zl_last_error()

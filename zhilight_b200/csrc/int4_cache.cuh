@@ -2,7 +2,9 @@
 // T of the rows that it was written from, 5 dim / 8 bytes in all.  A code c stands for T(lowest + step * c), rounded once.
 //
 // Of a group with lowest and highest value lo and hi, the step is (hi - lo) / 15 rounded down to T, so that no code stands for more than hi, and x becomes
-// the nearest whole number of steps above lo, at most 15 (ties to even): off by half a step, and by at most 15 * eps(T) / 2 of one more at the upper end, which the step's rounding leaves.  lo
+// the nearest whole number of steps above lo, at most 15 (ties to even).  What is read is off by half a step; at the upper end by what the step's rounding leaves too, up to 15 units
+// of T at the step (15 eps(T) of it; of fp16 steps below 2^-14, which are multiples of 2^-24, more: ranges below 15 * 2^-24 have a step of zero); and by its own rounding to T, half a
+// unit of the value, which may be the largest part: bf16 values of 3 +- 0.15 are off by up to 0.94 steps.  lo
 // is one of the values, so T holds it as it is.  Differences are taken of halves: a range may be beyond the largest 32-bit number.  A step below the normal
 // 32-bit numbers counts as none.  A group with an infinity or NaN reads as NaN.
 //

@@ -8,6 +8,12 @@ namespace zl {
 
 // Calls whose sequences bring at most so many (token, head) rows of a kv head go to the kernel for few rows, and all where groups have more heads than a tile has rows.
 // Drafts of 16 sequences, 48 rows, up to 6000 keys: 49 us there, in three blocks, 87 on the tiles, whose blocks of up to 128 rows cost the same.
+// Few rows / tiles in us, by the rows of a kv head (groups of 8, bf16, heads of 128, 8 kv heads; fp16 and heads of 64 have their borders within 16 rows of these):
+//   keys        1 x 1000   1 x 8000   1 x 60000   4 x 6000   16 x 1000   16 x 6000   64 x 300   64 x 2000
+//   32 rows     12 / 17    22 / 30    58 / 85     32 / 48    26 / 35      84 / 136   39 / 76    113 / 213
+//   48          13 / 18    24 / 30    79 / 90     41 / 50    35 / 36     119 / 138   51 / 78    163 / 217
+//   64          15 / 18    26 / 30    97 / 86     50 / 50    41 / 36     151 / 138   66 / 76    213 / 213
+//   80          15 / 19    28 / 30   118 / 91     56 / 51    52 / 36     188 / 138   95 / 78    279 / 221
 // Of other calls, those sequences go there that bring a token or two of a group of up to 8 heads, or up to 16 rows: portions of prompts beside 20 single tokens (24 sequences, keys in a
 // window of 1024) 71 us, 95 with all on the tiles.
 // Few keys are not worth two launches more.  By the room that the page table has (lengths are the device's), us with both kernels / the tiles alone, a portion beside single tokens: two

@@ -75,7 +75,7 @@ extern "C" int zl_qkv_axes_rope_append_int4(const void* qkv, long long ldq, cons
     ZL_CHECK_SUPPORTED(dtype == ZL_F16 || dtype == ZL_BF16);
     ZL_CHECK_ARG(ldq >= (long long)(heads + 2 * kv_heads) * dim);
     ZL_CHECK_SUPPORTED(ldq % 8 == 0 && ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out)) & 15) == 0);
-    ZL_CHECK_SUPPORTED((heads + 2ll * kv_heads) * dim <= kRopeSmem / 4);   // two rows in shared memory
+    ZL_CHECK_SUPPORTED((heads + 2ll * kv_heads) * dim <= kRopeSmem / 4);   // two rows in shared memory; what stands beside them there is seen to in axes_rope_append
     const PagedCache c = {k_cache, v_cache, num_pages, page_stride, row_stride, head_stride, page_table, ld_table, max_pages, page_size, seqs, paged_divisor(page_size)};
     return axes_rope_append<true>(qkv, ldq, pos, ld_pos, axes, inv_freq, axis, half, layout, mscale, token_seq, placement, c, q_out, T, heads, kv_heads, dim, dtype,
                                   pdl != 0, stream);

@@ -1186,7 +1186,8 @@ def qkv_axes_rope_append(qkv, pos, inv_freq, axis, token_seq, placement, page_ta
 def qkv_axes_rope_append_int4(qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout=ROT_HALVES, mscale=1.0, pdl=False):
     """qkv_axes_rope_append into caches of 4 bits: (pages, page_size, kv_heads, int4_row_bytes(dim)) uint8, dim 64 or 128, read by paged_attention_int4 and
     int4_cache_values.  Keys, turned in 64 bits and rounded to 32 and then to qkv's type, and values are held as 16 equal steps between the lowest and the highest of every 32
-    columns: off by up to half a step, a 30th of that range; 32 columns with an infinity or NaN read as NaN.  Decoding is fastest where a page has the rows of
+    columns: off by up to half a step, a 30th of that range, and by two roundings to the type, the step's (down, 15 times at the upper end) and that of what is read: values close
+    together far from zero, and fp16 ranges below 2^-10, lose more.  32 columns with an infinity or NaN read as NaN.  Decoding is fastest where a page has the rows of
     a head one behind another: caches made as (pages, kv_heads, page_size, bytes) and passed with .transpose(1, 2).  -> q (T, heads * dim)."""
     if _lib.host is not None:
         y = _lib.host.qkv_axes_rope_append_int4(qkv, pos, inv_freq, axis, token_seq, placement, page_table, k_cache, v_cache, heads, layout, mscale, pdl)
@@ -1268,7 +1269,8 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, 
 def paged_attention_int4(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window=0, max_new=None, out=None, pdl=False):
     """paged_attention over caches of 4 bits (pages, page_size, kv_heads, int4_row_bytes(dim)) uint8 whose rows were written from q's type
     (qkv_axes_rope_append_int4): the attention over what they stand for, int4_cache_values.  A broken group (NaN) of a key or value reaches the rows that see
-    it and no others.  scale up to 2^64 for bf16.  Portions of prompts take a workspace of up to 256 MB, by the room that page_table has.  -> out, like q."""
+    it and no others.  scale up to 2^64 for bf16.  Portions of prompts take a workspace of up to 256 MB, by the room that page_table has,
+    beside up to 48 MB for the parts of what CTAs share.  -> out, like q."""
     if _lib.host is not None:
         y = _lib.host.paged_attention_int4(q, k_cache, v_cache, page_table, seq_lens, q_starts, scale, window, max_new, out, pdl)
         if y is not None:
