@@ -320,6 +320,25 @@ def test_attention_of_lengths_out_of_range_behind_wide_tables(cuda, max_new, wid
         assert ((got[:301].cpu().double() - want).abs() <= off).all()
 
 
+@pytest.mark.parametrize("page,dim", [(20, 64), (48, 128), (16, 64), (1, 64)])
+@pytest.mark.parametrize("new", [(1, 1, 1), (150, 200, 1), (9, 3, 160), (30, 20, 8)])
+@pytest.mark.parametrize("window", [0, 130])
+def test_attention_of_sequences_longer_than_the_table(cuda, page, dim, new, window):
+    """Keys that the table has no room for do not count, wherever its room ends in a tile: whole rows of q see what is left, or nothing of it in a window."""
+    g = torch.Generator().manual_seed(page + new[0])
+    columns = 613 // page
+    lens = [columns * page + 7, columns * page + 190, 400]
+    table = tables(g, lens, page, sum(-(-n // page) for n in lens) + 2)[:, :columns].contiguous()
+    k, v = pool(g, sum(-(-n // page) for n in lens) + 2, page, 2, dim, BF16, "rows")
+    used = [min(n, columns * page) for n in lens]
+    hide(k, table, used), hide(v, table, used)
+    q, starts = torch.randn(sum(new), 16, dim, generator=g).to(BF16), starts_of(new)
+    got = ops.paged_attention_int4(q.cuda(), to_gpu(k), to_gpu(v), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), starts.cuda(), dim ** -0.5, window=window,
+                                   max_new=max(new)).cpu().double()
+    want, off = oracle.attention(q, codes.decode(k, BF16), codes.decode(v, BF16), table, lens, starts, dim ** -0.5, window)
+    assert ((got - want).abs() <= off).all()
+
+
 @pytest.mark.parametrize("max_new", [1, 3, 20, 200, None])
 def test_attention_does_not_depend_on_the_bound_of_new_tokens(cuda, max_new):
     check_attention(BF16, 8, 2, 128, 16, "rows", 0, [(300, 200), (40, 1), (90, 3), (600, 18)], max_new=max_new)
