@@ -240,6 +240,17 @@ def test_adjust_divides(cuda, dtype, vocab):
     assert torch.equal(ops.adjust_logits(z.cuda(), out_dtype=F32, **on_gpu(kw)).cpu(), want)
 
 
+def test_adjust_leaves_signs_of_zeros(cuda):
+    """Logits that nothing applies to are what they were to the last bit, and a quotient of zero has its sign."""
+    g = torch.Generator().manual_seed(17)
+    z = torch.randn(4, 1000, generator=g)
+    z[:, ::7], z[:, 3::7] = 0.0, -0.0
+    assert torch.equal(ops.adjust_logits(z.cuda()).cpu().view(torch.int32), z.view(torch.int32))
+    by = torch.tensor([0.0, 0.3, 1.0, 7.0])
+    want = torch.where(by[:, None] > 0, z / by[:, None], z)
+    assert torch.equal(ops.adjust_logits(z.cuda(), temperature=by.cuda()).cpu().view(torch.int32), want.view(torch.int32))
+
+
 def test_adjust_without_rows_or_histories(cuda):
     z = torch.randn(3, 40, device="cuda")
     none = torch.zeros(3, 0, dtype=torch.int32, device="cuda")

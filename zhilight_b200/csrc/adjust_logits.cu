@@ -107,10 +107,10 @@ __global__ void __launch_bounds__(kAlThreads, 4) k_adjust_logits(const AdjustLog
     }
     const float rep = p.repetition ? p.repetition[r] : 1.f, up = 1.f / rep, freq = p.frequency ? p.frequency[r] : 0.f, pres = p.presence ? p.presence[r] : 0.f;
     const float given = p.temperature ? p.temperature[r] : 0.f, heat = given >= 1.17549435e-38f ? given : 1.f, inv = 1.f / heat;
-    // z / by: by the reciprocal and one correction of what is left over (Markstein 1990), which is a number where z, the divisor and the quotient are
+    // z / by: by the reciprocal and one correction of what is too much (Markstein 1990), which is a number where z, the divisor and the quotient are; -0 stays -0
     auto quotient = [](float z, float by, float inverse) {
-        const float q = z * inverse, left = fmaf(-q, by, z);
-        return fabsf(left) < INFINITY ? fmaf(left, inverse, q) : q;
+        const float q = z * inverse, over = fmaf(q, by, -z);
+        return fabsf(over) < INFINITY ? fmaf(-over, inverse, q) : q;
     };
     auto cooled = [&](float z) { return quotient(z, heat, inv); };
     const int mask_row = !p.mask ? -1 : p.mask_row ? p.mask_row[r] : r;
